@@ -19,7 +19,7 @@ from typing import Optional
 _HERE = pathlib.Path(__file__).resolve().parent
 LIB_NAME = "libdetkernels.so"
 LIB_PATH = _HERE / LIB_NAME
-ABI_VERSION = 21
+ABI_VERSION = 22
 
 _lock = threading.Lock()
 _lib = None  # type: Optional[ctypes.CDLL]
@@ -252,6 +252,14 @@ _SIGNATURES = {
     "det_embed_ws_floats": ([c_int, c_int, c_int], ctypes.c_int64),
     "det_embed_bwd": ([c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
                        c_int, ctypes.c_int64, c_void_p, c_int], c_int),
+    # det_vocab.hip: losses over a vocabulary.  stream, const DetVocabHead* / DetVocabLogits* (vocab_loss._HeadParams,
+    # _LogitParams)
+    "det_vocab_head_ws_bytes": ([c_void_p, c_int], c_i64),
+    "det_vocab_head_forward": ([c_void_p, c_void_p], c_int),
+    "det_vocab_head_backward": ([c_void_p, c_void_p], c_int),
+    "det_vocab_logits_ws_bytes": ([c_void_p], c_i64),
+    "det_vocab_logits_forward": ([c_void_p, c_void_p], c_int),
+    "det_vocab_logits_backward": ([c_void_p, c_void_p], c_int),
 }
 
 

@@ -1,0 +1,1469 @@
+// det_vocab: losses of a language model's last layer over a vocabulary of V words, without its logits.
+//
+// A row n (token) has a hidden state h_n [D]; word v has a weight row w_v [D] and a bias b_v.
+//     z_nv = (h_n . w_v + b_v) / T        lse_n = log sum_v exp z_nv        p_nv = exp(z_nv - lse_n)
+// Both losses compare p_n with a sparse distribution s_n over K words (index a_nk, share s_nk):
+//     cross entropy  K = 1, s = 1 - eps, T = 1, and eps / V on every word (label smoothing):
+//                    loss_n = lse_n - (1 - eps) z_n,target - eps / V sum_v z_nv
+//     distillation   s_n = softmax of the teacher's K top logits / T, in the same units:
+//                    loss_n = T^2 sum_k s_nk (log s_nk - z_n,a_nk + lse_n)
+// and have one derivative, G_nv = c_n (p_nv - eps / V - sum_k s_nk [a_nk = v]), from which
+//     dh_n = sum_v G_nv w_v        dw_v = sum_n G_nv h_n        db_v = sum_n G_nv.
+//
+// Forward: one product [rows x D] . [D x V] whose epilogue reduces each 256 x 256 tile of logits to a
+// maximum and a sum of exponentials per row; a joining pass per row adds the K picked logits (dot
+// products of their own).  Backward: the vocabulary is walked in chunks; per chunk the product runs
+// again, its epilogue writes G (16 bits) to a workspace, and two more products read it.  Four products
+// of 2 N V D operations in all, for the three that a program with the logits in memory needs.
+//
+// Rows without a target are dropped before the products (an ordered list of the kept ones, made on the
+// device; tiles past its end return), so a masked-language-model step with 15 % targets costs 15 %.
+//
+// fp32 operands become two fp16 planes each, x s = hi + lo with s a power of two that puts the tensor's
+// largest finite magnitude at 2^14..2^15, and a product is hi hi + hi lo + lo hi in fp32 accumulators:
+// each operand is held to 2^-23 of itself (2^-39 of the tensor's largest value at worst) and the
+// dropped lo lo is below 2^-22 of its product, the size of one fp32 rounding, at a third of the matrix
+// units' 16-bit rate instead of the sixteenth that their fp32 instructions have.
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+namespace {
+
+typedef unsigned short u16;
+typedef __attribute__((ext_vector_type(8))) short s16x8;
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef __attribute__((ext_vector_type(8))) u16 us8;
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+enum { kF32 = 0, kBF16 = 1, kF16 = 2 };  // element types, as in _lib.py
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kNegInf = -__builtin_huge_valf();
+
+template <int DT> struct Elem;
+template <> struct Elem<kF32> { typedef float type; };
+template <> struct Elem<kBF16> { typedef u16 type; };
+template <> struct Elem<kF16> { typedef u16 type; };
+
+__device__ __forceinline__ float bf2f(u16 u) { return __uint_as_float(static_cast<uint32_t>(u) << 16); }
+__device__ __forceinline__ u16 f2bf(float f) { return __builtin_bit_cast(u16, static_cast<__bf16>(f)); }
+__device__ __forceinline__ float h2f(u16 u) { return static_cast<float>(__builtin_bit_cast(_Float16, u)); }
+__device__ __forceinline__ u16 f2h(float f) { return __builtin_bit_cast(u16, static_cast<_Float16>(f)); }
+
+template <int DT>
+__device__ __forceinline__ float to_f(typename Elem<DT>::type v) {
+  if constexpr (DT == kF32) return v;
+  else if constexpr (DT == kBF16) return bf2f(v);
+  else return h2f(v);
+}
+template <int DT>
+__device__ __forceinline__ typename Elem<DT>::type from_f(float f) {
+  if constexpr (DT == kF32) return f;
+  else if constexpr (DT == kBF16) return f2bf(f);
+  else return f2h(f);
+}
+__device__ __forceinline__ float load_any(const void* p, int64_t i, int dt) {
+  return dt == kF32 ? static_cast<const float*>(p)[i] : dt == kBF16 ? bf2f(static_cast<const u16*>(p)[i])
+                                                                    : h2f(static_cast<const u16*>(p)[i]);
+}
+__device__ __forceinline__ void store_any(void* p, int64_t i, int dt, float f) {
+  if (dt == kF32) static_cast<float*>(p)[i] = f;
+  else static_cast<u16*>(p)[i] = dt == kBF16 ? f2bf(f) : f2h(f);
+}
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// The running maximum m and sum s of 2^(c (z - m)), c = log2(e) / T: (m, s) + (m2, s2).  A maximum of -inf
+// stands for nothing yet.  Maximum and sum stay apart up to the end (no m + log s): logits masked with the
+// type's lowest value would absorb the logarithm, and times log2(e) they would be out of range.
+__device__ __forceinline__ void join(float& m, float& s, float m2, float s2, float c) {
+  const float hi = fmaxf(m, m2);
+  const float ref = hi == kNegInf ? 0.f : hi;
+  s = s * exp2_((m - ref) * c) + s2 * exp2_((m2 - ref) * c);
+  m = hi;
+}
+__device__ __forceinline__ void join_lanes(float& m, float& s, int width, float c) {
+  for (int o = 1; o < width; o <<= 1) {
+    const float m2 = __shfl_xor(m, o, 64), s2 = __shfl_xor(s, o, 64);
+    join(m, s, m2, s2, c);
+  }
+}
+__device__ __forceinline__ float sum_lanes(float v) {
+  for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+__device__ __forceinline__ float max_lanes(float v) {
+  for (int o = 1; o < 64; o <<= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+  return v;
+}
+
+// the power of two that brings a tensor's largest finite magnitude (its bits) to [2^14, 2^15), and its inverse
+__device__ __forceinline__ int scale_exp(uint32_t bits) {
+  if (bits == 0) return 0;
+  int e = 14 - (static_cast<int>(bits >> 23) - 127);
+  return e > 60 ? 60 : e < -100 ? -100 : e;
+}
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
+
+__device__ __forceinline__ int64_t load_index(const void* p, int64_t i, int wide) {
+  return wide ? static_cast<const int64_t*>(p)[i] : static_cast<const int32_t*>(p)[i];
+}
+
+constexpr int kGExp = 14;  // fp16 G is held times 2^14: |G| <= 1 stays below 65504, its smallest step is 2^-38
+
+// ------------------------------------------------------------------------------------------------
+// Rows: the ordered list of the rows that count.  info[0] = how many, info[1], info[2] = the largest
+// finite magnitudes (as bits) of the hidden states and the weights, cleared here for absmax_kernel.
+// ------------------------------------------------------------------------------------------------
+struct RowArgs {
+  const void* target;   // cross entropy: [N] words, else null
+  const void* index;    // distillation: [N, K] words (< 0: no entry)
+  const void* teacher;  // [N, K] logits (-inf: no entry)
+  uint8_t* flag;        // [N], distillation
+  int* info;
+  int* list;
+  int64_t ignore, index_ld, teacher_ld;
+  int N, K, wide, teacher_dt;
+};
+
+__global__ void __launch_bounds__(256) list_flags_kernel(RowArgs a) {
+  const int n = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (n >= a.N) return;
+  bool any = false;
+  for (int k = lane; k < a.K; k += 64)
+    any |= load_index(a.index, n * a.index_ld + k, a.wide) >= 0 && load_any(a.teacher, n * a.teacher_ld + k, a.teacher_dt) != kNegInf;
+  const uint64_t votes = __ballot(any);
+  if (lane == 0) a.flag[n] = votes != 0;
+}
+
+__global__ void __launch_bounds__(1024) rows_kernel(RowArgs a) {
+  __shared__ int wave_n[16];
+  __shared__ int base_n;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  if (tid == 0) base_n = 0;
+  __syncthreads();
+  for (int n0 = 0; n0 < a.N; n0 += 1024) {
+    const int n = n0 + tid;
+    const bool keep = n < a.N && (a.target != nullptr ? load_index(a.target, n, a.wide) != a.ignore : a.flag[n] != 0);
+    const uint64_t votes = __ballot(keep);
+    if (lane == 0) wave_n[w] = __popcll(votes);
+    __syncthreads();
+    int before = base_n;
+    for (int i = 0; i < w; ++i) before += wave_n[i];
+    if (keep) a.list[before + __popcll(votes & ((uint64_t(1) << lane) - 1))] = n;
+    __syncthreads();
+    if (tid == 0)
+      for (int i = 0; i < 16; ++i) base_n += wave_n[i];
+    __syncthreads();
+  }
+  if (tid == 0) {
+    a.info[0] = base_n;
+    a.info[1] = 0;
+    a.info[2] = 0;
+  }
+}
+
+// the largest finite magnitude of a [rows, cols] fp32 matrix into *out (bits; a maximum has no order)
+__global__ void __launch_bounds__(256) absmax_kernel(const float* x, int64_t ld, int rows, int cols, int* out) {
+  uint32_t m = 0;
+  for (int r = blockIdx.x; r < rows; r += gridDim.x)
+    for (int c = threadIdx.x; c < cols; c += 256) {
+      const uint32_t b = __float_as_uint(x[r * ld + c]) & 0x7FFFFFFFu;
+      if (b < 0x7F800000u && b > m) m = b;
+    }
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t v = __shfl_xor(m, o, 64);
+    m = v > m ? v : m;
+  }
+  if ((threadIdx.x & 63) == 0) atomicMax(reinterpret_cast<unsigned int*>(out), m);
+}
+
+// ------------------------------------------------------------------------------------------------
+// Operands of the products: 16-bit rows, 16-byte aligned, columns past the width zero.  Copies the
+// rows of `list` (or all), and splits fp32 into two fp16 planes.
+// ------------------------------------------------------------------------------------------------
+struct PackArgs {
+  const void* src;
+  int64_t src_ld;
+  const int* list;   // null: rows as they are
+  const int* count;  // null: `rows`
+  const int* absmax; // fp32
+  u16* dst;
+  int64_t plane;     // elements between the planes
+  int rows, cols, ld;  // ld % 8 == 0
+};
+
+template <int DT>
+__global__ void __launch_bounds__(256) pack_kernel(PackArgs a) {
+  const int rows = a.count != nullptr ? *a.count : a.rows;
+  const int chunks = a.ld >> 3;
+  const float s = DT == kF32 ? pow2(scale_exp(static_cast<uint32_t>(*a.absmax))) : 1.f;
+  for (int r = blockIdx.x; r < rows; r += gridDim.x) {
+    const int64_t from = static_cast<int64_t>(a.list != nullptr ? a.list[r] : r) * a.src_ld;
+    for (int c = threadIdx.x; c < chunks; c += 256) {
+      us8 hi, lo;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int col = c * 8 + e;
+        if constexpr (DT == kF32) {
+          const float x = col < a.cols ? static_cast<const float*>(a.src)[from + col] * s : 0.f;
+          hi[e] = f2h(x);
+          lo[e] = f2h(x - h2f(hi[e]));
+        } else {
+          hi[e] = col < a.cols ? static_cast<const u16*>(a.src)[from + col] : u16(0);
+        }
+      }
+      u16* d = a.dst + static_cast<int64_t>(r) * a.ld + c * 8;
+      *reinterpret_cast<us8*>(d) = hi;
+      if constexpr (DT == kF32) *reinterpret_cast<us8*>(d + a.plane) = lo;
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
+// The products.  C tile 256 x 256, 8 waves as 2 (rows) x 4 (columns) of 128 x 64, v_mfma 16x16x32.
+// An operand lies with its k contiguous ("row": element (i, k) at i * ld + k) or strided ("col":
+// (i, k) at k * ld + i, read back from LDS transposed).  LDS holds two stages of four 16 KiB half
+// tiles (A rows 0-127, 128-255, B 0-127, 128-255), each two 8 KiB images: k 0-31 and 32-63 of one
+// plane, or k 0-31 of the two planes of a split fp32 operand (three products a stage then).
+// Everything outside an operand's extents is fetched out of the buffer's range, which gives zeros.
+// ------------------------------------------------------------------------------------------------
+struct Operand {
+  const u16* p;
+  int64_t plane, ld;
+};
+
+enum { kStats, kGrad, kPartial, kOut };
+
+struct GemmArgs {
+  Operand A, B;
+  const int* m_dyn;  // rows of A that count (null: M)
+  const int* k_dyn;  // length of the sum (null: K)
+  int M, N, K;
+  int splits, k_per_split;  // kPartial: blocks of one tile, each over k_per_split (a multiple of 64) of K
+  const int* info;          // scales of fp32 operands
+  // kStats, kGrad: z = acc / scales + bias, c = log2(e) / T
+  const void* bias;
+  int bias_dt;
+  float c;
+  float2* part;   // kStats [M][tiles of N]: maximum and sum
+  float* part_z;  // sum of z / V, or null
+  float inv_v;
+  int tile0, ntiles;
+  // kGrad: p = 2^(c (z - top) - log2 sum)
+  const float *top, *log_s;  // [M]
+  const float* row_w;        // [M]
+  float smooth_v;      // eps / V
+  u16* G;              // [M][ldg]
+  int64_t g_plane;
+  int ldg;
+  // kPartial: out[split][M][ldo] fp32, added to what is there if `add`
+  float* out32;
+  int64_t ldo, split_stride;
+  int add;
+  // kOut: out[m][n] of type out_dt, times *alpha and the scale of B
+  void* out;
+  int out_dt;
+  const float* alpha;
+};
+
+constexpr int kTile = 256, kThreads = 512;
+constexpr int kHalf = 16384, kStage = 4 * kHalf;
+constexpr int kLdc = kTile + 16;
+constexpr int kGemmSmem = (2 * kStage > kTile * kLdc * 2) ? 2 * kStage : kTile * kLdc * 2;
+constexpr unsigned kOOB = 0x80000000u;     // past kRange: the load returns zeros
+constexpr unsigned kRange = 0x7FFFFFF0u;
+
+template <int N>
+__device__ __forceinline__ void wait_vmcnt() {  // all but the wave's last N loads and stores are done
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ int xcd_remap(int bid, int nwg) {  // consecutive tiles on one XCD
+  const int q = nwg >> 3, r = nwg & 7, x = bid & 7;
+  return (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (bid >> 3);
+}
+// "row" images: 64-byte rows, chunk ch of row r at ch ^ f(r)
+__device__ __forceinline__ int swz64(int row, int ch) { return row * 64 + ((ch ^ ((-(row >> 2)) & 3)) << 4); }
+// "col" images: [32 k][64 columns], 128-byte rows
+__device__ __forceinline__ int swz128_ch(int row, int ch) { return ch ^ ((((row >> 1) & 1) << 1) | (((row >> 3) & 1) << 2)); }
+
+// columns c0..c0+15 x 32 k of a [32][64] image: lane (g = lane >> 4, i = lane & 15) gets k 8g..8g+7 of column c0 + i
+__device__ __forceinline__ s16x8 tr_frag(const unsigned char* sub, int c0, int lane) {
+  const int g = lane >> 4, q = (lane >> 2) & 3, p = lane & 3;
+  const int col = c0 + 4 * p;
+  const int r0 = 8 * g + q, r1 = r0 + 4;
+  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(sub + r0 * 128 + (swz128_ch(r0, col >> 3) << 4) + ((col & 4) << 1)));
+  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(sub + r1 * 128 + (swz128_ch(r1, col >> 3) << 4) + ((col & 4) << 1)));
+  return s16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+}
+
+template <bool F16>
+__device__ __forceinline__ f32x4 mfma16(s16x8 a, s16x8 b, f32x4 c) {
+  if constexpr (F16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+template <bool F16, int PL, bool ACOL, bool BCOL, int EPI>
+__global__ void __launch_bounds__(kThreads, 1) gemm_kernel(GemmArgs g) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  constexpr int KT = PL == 1 ? 64 : 32;  // k per stage
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wr = wid >> 2, wc = wid & 3;
+  const int M = g.m_dyn != nullptr ? *g.m_dyn : g.M;
+  const int K = g.k_dyn != nullptr ? *g.k_dyn : g.K;
+  const int ntm = (M + kTile - 1) / kTile, ntn = (g.N + kTile - 1) / kTile;
+  const int total = ntm * ntn;
+  int split = 0, bid = blockIdx.x;
+  if (EPI == kPartial) {
+    split = bid % g.splits;
+    bid /= g.splits;
+  }
+  if (bid >= total) return;  // the grid is sized for every row
+  bid = xcd_remap(bid, total);
+  // tiles go down eight row tiles before they go on to the next column tile: what runs at one time
+  // on an XCD then shares both operands
+  const int per = 8 * ntn, band = bid / per, left = ntm - band * 8;
+  const int high = left < 8 ? left : 8;
+  const int in = bid - band * per;
+  const int mt = band * 8 + in % high, nt = in / high;
+  const int m0 = mt * kTile, n0 = nt * kTile;
+  const int kbeg = EPI == kPartial ? split * g.k_per_split : 0;
+  int kend = EPI == kPartial ? kbeg + g.k_per_split : K;
+  if (kend > K) kend = K;
+  const int nk = kend > kbeg ? (kend - kbeg + KT - 1) / KT : 0;
+
+  // this lane's 16-byte pieces of the four half tiles: "row" operands 16 rows a wave, 4 lanes a row;
+  // "col" operands 8 k rows of a 64-column image a wave, 8 lanes a row; chunks swizzled at the source
+  const int rrow = lane >> 2, rch = (lane & 3) ^ ((-(rrow >> 2)) & 3);
+  const int crow = (wid & 3) * 8 + (lane >> 3), csub = wid >> 2, cch = swz128_ch(crow, lane & 7);
+  unsigned voff[4];
+  bool vok[4];
+#pragma unroll
+  for (int h = 0; h < 4; ++h) {
+    const bool isa = h < 2, col = isa ? ACOL : BCOL;
+    const int64_t ld = isa ? g.A.ld : g.B.ld;
+    const int origin = isa ? m0 : n0, extent = isa ? M : g.N;
+    if (!col) {
+      const int r = (h & 1) * 128 + wid * 16 + rrow;
+      vok[h] = origin + r < extent;
+      voff[h] = static_cast<unsigned>(r * ld * 2 + rch * 16);
+    } else {
+      const int c = (h & 1) * 128 + csub * 64 + cch * 8;
+      vok[h] = origin + c < extent;
+      voff[h] = static_cast<unsigned>(crow * ld * 2 + c * 2);
+    }
+  }
+  auto stage1 = [&](const Operand& op, bool col, int origin, int h, int t) {
+    unsigned char* dst = smem + (t & 1) * kStage + h * kHalf + wid * 1024;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const u16* base = op.p + (PL == 2 ? s * op.plane : 0);
+      const int k0 = kbeg + t * KT + (PL == 1 ? s * 32 : 0);
+      bool ok;
+      unsigned off = voff[h];
+      if (!col) {
+        base += origin * op.ld;
+        ok = vok[h] && k0 + rch * 8 < kend;
+        off += static_cast<unsigned>(k0) * 2u;
+      } else {
+        base += k0 * op.ld + origin;
+        ok = vok[h] && k0 + crow < kend;
+      }
+      const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<u16*>(base), 0, kRange, 0x00020000);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(dst + s * 8192), 16, ok ? off : kOOB, 0, 0, 0);
+    }
+  };
+  auto stage = [&](int t) {
+    stage1(g.A, ACOL, m0, 0, t);
+    stage1(g.A, ACOL, m0, 1, t);
+    stage1(g.B, BCOL, n0, 2, t);
+    stage1(g.B, BCOL, n0, 3, t);
+  };
+
+  f32x4 acc[8][4];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  s16x8 af[8][2], bf[4][2];
+  const int fr = lane & 15, fch = lane >> 4;
+  auto read_a = [&](int t, int i0) {
+    const unsigned char* base = smem + (t & 1) * kStage + wr * kHalf;
+#pragma unroll
+    for (int i = i0; i < i0 + 4; ++i)
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        af[i][s] = ACOL ? tr_frag(base + s * 8192 + (i >> 2) * 4096, (i * 16) & 63, lane)
+                        : *reinterpret_cast<const s16x8*>(base + s * 8192 + swz64(i * 16 + fr, fch));
+  };
+  auto read_b = [&](int t, int j0) {
+    const unsigned char* base = smem + (t & 1) * kStage + (2 + (wc >> 1)) * kHalf;
+#pragma unroll
+    for (int j = j0; j < j0 + 2; ++j)
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        bf[j][s] = BCOL ? tr_frag(base + s * 8192 + (wc & 1) * 4096, j * 16, lane)
+                        : *reinterpret_cast<const s16x8*>(base + s * 8192 + swz64((wc & 1) * 64 + j * 16 + fr, fch));
+  };
+  auto mfma = [&](int i0, int j0) {
+#pragma unroll
+    for (int s = 0; s < (PL == 1 ? 2 : 3); ++s)
+#pragma unroll
+      for (int i = i0; i < i0 + 4; ++i)
+#pragma unroll
+        for (int j = j0; j < j0 + 2; ++j)  // one plane: k halves 0, 1; two: hi hi, hi lo, lo hi
+          acc[i][j] = mfma16<F16>(af[i][PL == 1 ? s : s >> 1], bf[j][PL == 1 ? s : s & 1], acc[i][j]);
+  };
+
+  if (nk > 0) stage(0);
+  for (int t = 0; t < nk; ++t) {
+    wait_vmcnt<0>();  // this wave's pieces of stage t (a barrier alone does not wait for them)
+    __syncthreads();  // ... and every other wave's; stage t - 1 is read
+    if (t + 1 < nk) stage(t + 1);
+    read_a(t, 0);
+    read_a(t, 4);
+    read_b(t, 0);
+    read_b(t, 2);
+    mfma(0, 0);
+    mfma(0, 2);
+    mfma(4, 2);
+    mfma(4, 0);
+  }
+  __syncthreads();
+
+  // acc[i][j][r]: row wr * 128 + i * 16 + fch * 4 + r, column wc * 64 + j * 16 + fr
+  if constexpr (EPI == kStats || EPI == kGrad) {
+    const float zs = PL == 1 ? 1.f : pow2(-scale_exp(static_cast<uint32_t>(g.info[1]))) * pow2(-scale_exp(static_cast<uint32_t>(g.info[2])));
+    const float c = g.c;
+    float bias[4];
+    bool cok[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int col = n0 + wc * 64 + j * 16 + fr;
+      cok[j] = col < g.N;
+      bias[j] = g.bias != nullptr && cok[j] ? load_any(g.bias, col, g.bias_dt) : 0.f;
+    }
+    if constexpr (EPI == kStats) {
+      float* red = reinterpret_cast<float*>(smem);  // [3][4 column waves][256 rows]
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float z[4], m = kNegInf, s = 0.f, sz = 0.f;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            z[j] = acc[i][j][r] * zs + bias[j];
+            if (cok[j]) {
+              m = fmaxf(m, z[j]);
+              sz = fmaf(z[j], g.inv_v, sz);
+            }
+          }
+          const float ref = m == kNegInf ? 0.f : m;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s += cok[j] ? exp2_((z[j] - ref) * c) : 0.f;
+          join_lanes(m, s, 16, c);
+          if (g.part_z != nullptr)
+            for (int o = 1; o < 16; o <<= 1) sz += __shfl_xor(sz, o, 64);
+          if (fr == 0) {
+            const int row = wr * 128 + i * 16 + fch * 4 + r;
+            red[wc * 256 + row] = m;
+            red[1024 + wc * 256 + row] = s;
+            red[2048 + wc * 256 + row] = sz;
+          }
+        }
+      __syncthreads();
+      if (tid < 256 && m0 + tid < M) {
+        float m = red[tid], s = red[1024 + tid], sz = red[2048 + tid];
+#pragma unroll
+        for (int w = 1; w < 4; ++w) {
+          join(m, s, red[w * 256 + tid], red[1024 + w * 256 + tid], c);
+          sz += red[2048 + w * 256 + tid];
+        }
+        const int64_t at = static_cast<int64_t>(m0 + tid) * g.ntiles + g.tile0 + nt;
+        g.part[at] = make_float2(m, s);
+        if (g.part_z != nullptr) g.part_z[at] = sz;
+      }
+    } else {
+      u16* ct = reinterpret_cast<u16*>(smem);
+      // G once into the accumulators: both planes have to come from the same bits of it
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int row = m0 + wr * 128 + i * 16 + fch * 4 + r;
+          const bool ok = row < M;
+          const float top = ok ? g.top[row] : 0.f, l = ok ? g.log_s[row] : 0.f, w = ok ? g.row_w[row] : 0.f;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float p = exp2_(fmaf(acc[i][j][r] * zs + bias[j] - top, c, -l));
+            acc[i][j][r] = cok[j] && ok ? w * (p - g.smooth_v) : 0.f;
+          }
+        }
+#pragma unroll
+      for (int pl = 0; pl < PL; ++pl) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const u16 o = F16 ? f2h(acc[i][j][r]) : f2bf(acc[i][j][r]);
+              acc[i][j][r] -= F16 ? h2f(o) : 0.f;  // what is left, for the second plane
+              ct[(wr * 128 + i * 16 + fch * 4 + r) * kLdc + wc * 64 + j * 16 + fr] = o;
+            }
+        __syncthreads();
+        for (int q = tid; q < kTile * (kTile / 8); q += kThreads) {
+          const int row = q >> 5, cc = (q & 31) * 8;
+          if (m0 + row < M && n0 + cc < g.ldg)
+            *reinterpret_cast<us8*>(g.G + pl * g.g_plane + static_cast<int64_t>(m0 + row) * g.ldg + n0 + cc) =
+                *reinterpret_cast<const us8*>(ct + row * kLdc + cc);
+        }
+        __syncthreads();
+      }
+    }
+  } else if constexpr (EPI == kPartial) {
+    float* out = g.out32 + split * g.split_stride;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int row = m0 + wr * 128 + i * 16 + fch * 4 + r;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int col = n0 + wc * 64 + j * 16 + fr;
+          if (row < M && col < g.N) {
+            float* o = out + row * g.ldo + col;
+            *o = g.add ? *o + acc[i][j][r] : acc[i][j][r];
+          }
+        }
+      }
+  } else {
+    float alpha = *g.alpha;
+    if (PL == 2) alpha *= pow2(-scale_exp(static_cast<uint32_t>(g.info[1])));
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int row = m0 + wr * 128 + i * 16 + fch * 4 + r;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int col = n0 + wc * 64 + j * 16 + fr;
+          if (row < M && col < g.N) store_any(g.out, row * g.ldo + col, g.out_dt, acc[i][j][r] * alpha);
+        }
+      }
+  }
+#endif
+}
+
+// ------------------------------------------------------------------------------------------------
+// Joining a row's tiles, its K picked logits, its loss.  One wave a row (cross entropy) or four (lists).
+// ------------------------------------------------------------------------------------------------
+struct FinishArgs {
+  const void *x, *w, *bias;
+  int64_t x_ld, w_ld;
+  int dt, bias_dt, D, V, K, ntiles, N;
+  const int *info, *list;
+  const float2* part;
+  const float* part_z;
+  const void *target, *index, *teacher;
+  int64_t index_ld, teacher_ld;
+  int wide, teacher_dt;
+  float inv_t, smooth;
+  float *top, *log_s;  // [kept]
+  float* picked;       // [kept][K] logits of the picked words
+  float* share;        // [kept][K]
+  double* rows;        // losses [kept], for a mean or a sum (a row's may be past fp32 where their mean is not)
+  float* each;         // losses [N], or null
+};
+
+template <int DT>
+__device__ __forceinline__ float dot_wave(const void* x, const void* w, int D, int lane) {
+  typedef typename Elem<DT>::type T;
+  const T *a = static_cast<const T*>(x), *b = static_cast<const T*>(w);
+  float s = 0.f;
+  for (int d = lane; d < D; d += 64) s = fmaf(to_f<DT>(a[d]), to_f<DT>(b[d]), s);
+  return sum_lanes(s);
+}
+
+// an entry of a teacher's list: absent if its word is negative or its logit -inf
+__device__ __forceinline__ bool list_entry(const void* index, int64_t at, int wide, const void* teacher, int64_t t_at, int t_dt,
+                                           int64_t& word, float& t) {
+  word = load_index(index, at, wide);
+  t = load_any(teacher, t_at, t_dt);
+  return word >= 0 && t != kNegInf;
+}
+// one entry's part of the divergence / T^2: q (log q - log p), q = 2^(c (t - tt) - tl), log p = (z - top) / T - ln 2 log_s
+__device__ __forceinline__ float diverge(float q, float t, float tt, float tl, float z, float top, float log_s, float inv_t) {
+  if (q == 0.f) return 0.f;
+  return q * (((t - tt) * inv_t - tl * kLn2) - ((z - top) * inv_t - log_s * kLn2));
+}
+
+template <int DT>
+__global__ void __launch_bounds__(256) finish_kernel(FinishArgs a) {
+  __shared__ float red[4][4];
+  typedef typename Elem<DT>::type T;
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+  const int count = a.info[0];
+  const float c = a.inv_t * kLog2e;
+  for (int row = blockIdx.x; row < count; row += gridDim.x) {
+    const int n = a.list[row];
+    float m = kNegInf, s = 0.f, sz = 0.f;
+    for (int t = tid; t < a.ntiles; t += 256) {
+      const float2 v = a.part[static_cast<int64_t>(row) * a.ntiles + t];
+      join(m, s, v.x, v.y, c);
+      if (a.part_z != nullptr) sz += a.part_z[static_cast<int64_t>(row) * a.ntiles + t];
+    }
+    join_lanes(m, s, 64, c);
+    sz = sum_lanes(sz);
+    __syncthreads();
+    if (lane == 0) {
+      red[wv][0] = m;
+      red[wv][1] = s;
+      red[wv][2] = sz;
+    }
+    __syncthreads();
+    m = red[0][0];
+    s = red[0][1];
+    sz = red[0][2];
+    for (int w = 1; w < 4; ++w) {
+      join(m, s, red[w][0], red[w][1], c);
+      sz += red[w][2];
+    }
+    const float log_s = log2f(s);
+    const T* x = static_cast<const T*>(a.x) + n * a.x_ld;
+    auto logit = [&](int64_t word) {
+      const float z = dot_wave<DT>(x, static_cast<const T*>(a.w) + word * a.w_ld, a.D, lane);
+      return a.bias != nullptr ? z + load_any(a.bias, word, a.bias_dt) : z;
+    };
+    float loss = 0.f;  // this wave's part
+    // a word outside the vocabulary: the row's loss and gradients are NaN
+    if (a.target != nullptr) {
+      if (wv == 0) {
+        const int64_t word = load_index(a.target, n, a.wide);
+        float z = __builtin_nanf("");
+        if (word >= 0 && word < a.V) z = logit(word);
+        if (lane == 0) {
+          a.picked[row] = z;
+          a.share[row] = 1.f - a.smooth;
+        }
+        // T = 1; with eps = 1 the target does not count, not even one of logit -inf
+        loss = log_s * kLn2;
+        if (a.smooth != 1.f || z != z) loss += (1.f - a.smooth) * (m - z);
+        if (a.smooth != 0.f) loss += a.smooth * (m - sz);
+      }
+    } else {
+      float tt = kNegInf, ts = 0.f;
+      const int64_t i0 = n * a.index_ld, t0 = n * a.teacher_ld;
+      for (int k = lane; k < a.K; k += 64) {  // every wave goes over the whole list
+        int64_t word;
+        float t;
+        if (list_entry(a.index, i0 + k, a.wide, a.teacher, t0 + k, a.teacher_dt, word, t)) join(tt, ts, t, 1.f, c);
+      }
+      join_lanes(tt, ts, 64, c);
+      const float tl = log2f(ts);
+      for (int k = wv; k < a.K; k += 4) {
+        int64_t word;
+        float t, z = 0.f, q = 0.f;
+        if (list_entry(a.index, i0 + k, a.wide, a.teacher, t0 + k, a.teacher_dt, word, t)) {
+          q = exp2_(fmaf(t - tt, c, -tl));
+          if (word >= a.V) loss = __builtin_nanf("");
+          else z = logit(word);
+          loss += diverge(q, t, tt, tl, z, m, log_s, a.inv_t);
+        }
+        if (lane == 0) {
+          a.picked[static_cast<int64_t>(row) * a.K + k] = z;
+          a.share[static_cast<int64_t>(row) * a.K + k] = q;
+        }
+      }
+    }
+    if (lane == 0) red[wv][3] = loss;
+    __syncthreads();
+    if (tid == 0) {
+      const float t = (red[0][3] + red[1][3]) + (red[2][3] + red[3][3]);
+      a.top[row] = m;
+      a.log_s[row] = t != t ? t : log_s;
+      const double all = static_cast<double>(t) / (static_cast<double>(a.inv_t) * a.inv_t);
+      if (a.each != nullptr) a.each[n] = static_cast<float>(all);
+      else a.rows[row] = all;
+    }
+  }
+}
+
+// sum of the kept rows' losses, or their mean (nothing kept: 0)
+__global__ void __launch_bounds__(1024) reduce_kernel(const double* rows, const int* info, int mean, float* out) {
+  __shared__ double part[16];
+  const int count = info[0];
+  double s = 0.0;
+  for (int i = threadIdx.x; i < count; i += 1024) s += rows[i];
+  for (int o = 1; o < 64; o <<= 1) s += __shfl_xor(s, o, 64);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s = 0.0;
+    for (int w = 0; w < 16; ++w) s += part[w];
+    *out = static_cast<float>(mean && count > 0 ? s / count : s);
+  }
+}
+
+__global__ void __launch_bounds__(256) zero_kernel(float* p, int64_t n) {
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) p[i] = 0.f;
+}
+
+// ------------------------------------------------------------------------------------------------
+// Backward: what each row weighs.  row_w[c] = g_n / max |g| (1 for one g) times 2^kGExp for fp16 G,
+// *alpha = max |g| T / (2^kGExp) (/ rows for a mean): G itself stays within [-1, 1] 2^kGExp.
+// ------------------------------------------------------------------------------------------------
+struct WeightArgs {
+  const float* g;  // [1], or [N] (each)
+  const int *info, *list;
+  float* row_w;
+  float* alpha;
+  float heat, g_scale;
+  int each, mean;
+};
+
+__global__ void __launch_bounds__(1024) weights_kernel(WeightArgs a) {
+  __shared__ float part[16];
+  const int count = a.info[0];
+  float top = 0.f;
+  bool nan = false;
+  if (a.each) {
+    for (int c = threadIdx.x; c < count; c += 1024) {
+      const float g = fabsf(a.g[a.list[c]]);
+      nan |= g != g;
+      top = fmaxf(top, g);
+    }
+    if (nan) top = __builtin_huge_valf();
+    top = max_lanes(top);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
+    __syncthreads();
+    top = part[0];
+    for (int w = 1; w < 16; ++w) top = fmaxf(top, part[w]);
+  } else {
+    top = a.g[0];
+  }
+  for (int c = threadIdx.x; c < count; c += 1024)
+    a.row_w[c] = (a.each ? (top == 0.f ? 0.f : a.g[a.list[c]] / top) : 1.f) * a.g_scale;
+  if (threadIdx.x == 0) *a.alpha = top * a.heat / a.g_scale / (a.mean && count > 0 ? static_cast<float>(count) : 1.f);
+}
+
+// the picked words' entries of a chunk's G, from the fp32 logits of the forward pass (a word twice in
+// a list: its entries add up, and each of them writes the same value)
+struct ScatterArgs {
+  const int *info, *list;
+  const void *target, *index;
+  int64_t index_ld;
+  int wide, K, v0, nv, f16, planes, ldg;
+  const float *picked, *share, *top, *log_s, *row_w;
+  float smooth_v, c;
+  u16* G;
+  int64_t g_plane;
+};
+
+__global__ void __launch_bounds__(256) scatter_kernel(ScatterArgs a) {
+  const int count = a.info[0];
+  const int64_t all = static_cast<int64_t>(count) * a.K;
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < all; i += gridDim.x * 256ll) {
+    const int c = static_cast<int>(i / a.K), k = static_cast<int>(i - static_cast<int64_t>(c) * a.K);
+    const int n = a.list[c];
+    const int64_t word = a.target != nullptr ? load_index(a.target, n, a.wide) : load_index(a.index, n * a.index_ld + k, a.wide);
+    if (word < a.v0 || word >= a.v0 + a.nv) continue;
+    const float* share = a.share + static_cast<int64_t>(c) * a.K;
+    float s = share[k];
+    if (a.target == nullptr) {
+      s = 0.f;
+      for (int j = 0; j < a.K; ++j)
+        if (load_index(a.index, n * a.index_ld + j, a.wide) == word) s += share[j];
+      if (share[k] == 0.f) continue;  // G has p already, or another entry writes it
+    }
+    const float v = a.row_w[c] * ((exp2_(fmaf(a.picked[i] - a.top[c], a.c, -a.log_s[c])) - a.smooth_v) - s);
+    u16* o = a.G + static_cast<int64_t>(c) * a.ldg + (word - a.v0);
+    const u16 hi = a.f16 ? f2h(v) : f2bf(v);
+    *o = hi;
+    if (a.planes == 2) o[a.g_plane] = f2h(v - h2f(hi));
+  }
+}
+
+// column sums of a chunk's G (rows split over blockIdx.y), then the bias gradient
+__global__ void __launch_bounds__(256) colsum_kernel(const u16* G, int64_t g_plane, int planes, int f16, int ldg, const int* info,
+                                                     float* part) {
+  __shared__ float red[8][256 + 8];
+  const int tid = threadIdx.x, cg = tid & 31, rg = tid >> 5;
+  const int col = blockIdx.x * 256 + cg * 8;
+  const int count = info[0];
+  float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (col < ldg)
+    for (int r = blockIdx.y * 8 + rg; r < count; r += gridDim.y * 8)
+      for (int pl = 0; pl < planes; ++pl) {
+        const us8 v = *reinterpret_cast<const us8*>(G + pl * g_plane + static_cast<int64_t>(r) * ldg + col);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] += f16 ? h2f(v[e]) : bf2f(v[e]);
+      }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) red[rg][cg * 8 + e] = s[e];
+  __syncthreads();
+  float t = 0.f;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) t += red[w][tid];
+  if (blockIdx.x * 256 + tid < ldg) part[static_cast<int64_t>(blockIdx.y) * ldg + blockIdx.x * 256 + tid] = t;
+}
+
+__global__ void __launch_bounds__(256) dbias_kernel(const float* part, int splits, int ldg, int nv, const float* alpha, void* db,
+                                                    int64_t at, int dt) {
+  const int v = blockIdx.x * 256 + threadIdx.x;
+  if (v >= nv) return;
+  float t = 0.f;
+  for (int s = 0; s < splits; ++s) t += part[static_cast<int64_t>(s) * ldg + v];
+  store_any(db, at + v, dt, t * *alpha);
+}
+
+// dh: the sum of a kept row's partials, zeros for the others.  pos: binary search in the ordered list
+__global__ void __launch_bounds__(256) dx_kernel(const float* part, int splits, int64_t split_stride, int64_t ldo, const int* info,
+                                                 const int* list, const float* alpha, int planes, void* dx, int dt, int D) {
+  const int n = blockIdx.x;
+  int lo = 0, hi = info[0];
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (list[mid] < n) lo = mid + 1;
+    else hi = mid;
+  }
+  const bool kept = lo < info[0] && list[lo] == n;
+  float a = *alpha;
+  if (planes == 2) a *= pow2(-scale_exp(static_cast<uint32_t>(info[2])));
+  for (int d = threadIdx.x; d < D; d += 256) {
+    float t = 0.f;
+    if (kept)
+      for (int s = 0; s < splits; ++s) t += part[s * split_stride + lo * ldo + d];
+    store_any(dx, static_cast<int64_t>(n) * D + d, dt, t * a);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
+// A teacher's top logits against logits in memory: reads them once forward, once backward.
+// ------------------------------------------------------------------------------------------------
+struct LogitArgs {
+  const void* z;
+  int64_t z_ld;
+  int dt, N, V, K, segs, seg_len;  // seg_len % 8 == 0
+  const void *index, *teacher;
+  int64_t index_ld, teacher_ld;
+  int wide, teacher_dt;
+  float inv_t;
+  int each, mean;
+  float2* part;        // [N][segs]
+  float *top, *log_s;  // [N]; a log_s of +inf marks a row without a list (every p 0)
+  float* share;        // [N][K]
+  double* rows;        // [N]
+  float* loss_each;    // [N], or null
+  int* info;     // [0]: rows with a list
+  // backward
+  const float* g;
+  void* dz;
+  int64_t dz_ld;
+};
+
+// elements of a segment in 16-byte pieces: f(column, value) for the ragged ends, and for whole pieces
+template <int DT, class F>
+__device__ __forceinline__ void walk(const typename Elem<DT>::type* p, int lo, int hi, int tid, int nthr, F&& f) {
+  typedef typename Elem<DT>::type T;
+  constexpr int W = 16 / sizeof(T);
+  typedef __attribute__((ext_vector_type(W))) T V;
+  const int mis = static_cast<int>((reinterpret_cast<uintptr_t>(p + lo) & 15) / sizeof(T));
+  int start = lo + (mis ? W - mis : 0);
+  if (start > hi) start = hi;
+  const int whole = (hi - start) / W;
+  if (tid < start - lo) f(lo + tid, to_f<DT>(p[lo + tid]));
+  for (int i = tid; i < whole; i += nthr) {
+    const V v = *reinterpret_cast<const V*>(p + start + i * W);
+#pragma unroll
+    for (int e = 0; e < W; ++e) f(start + i * W + e, to_f<DT>(v[e]));
+  }
+  const int rest = start + whole * W;
+  if (tid < hi - rest) f(rest + tid, to_f<DT>(p[rest + tid]));
+}
+
+template <int DT>
+__global__ void __launch_bounds__(256) logit_stats_kernel(LogitArgs a) {
+  __shared__ float red[2][4];
+  typedef typename Elem<DT>::type T;
+  const int n = blockIdx.x / a.segs, seg = blockIdx.x - n * a.segs, tid = threadIdx.x;
+  const T* z = static_cast<const T*>(a.z) + n * a.z_ld;
+  const int lo = seg * a.seg_len;
+  int hi = lo + a.seg_len;
+  if (hi > a.V) hi = a.V;
+  const float c = a.inv_t * kLog2e;
+  float m = kNegInf, s = 0.f;
+  if (lo < hi) walk<DT>(z, lo, hi, tid, 256, [&](int, float v) { join(m, s, v, 1.f, c); });
+  join_lanes(m, s, 64, c);
+  if ((tid & 63) == 0) {
+    red[0][tid >> 6] = m;
+    red[1][tid >> 6] = s;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    for (int w = 1; w < 4; ++w) join(m, s, red[0][w], red[1][w], c);
+    a.part[static_cast<int64_t>(n) * a.segs + seg] = make_float2(m, s);
+  }
+}
+
+__global__ void __launch_bounds__(256) logit_finish_kernel(LogitArgs a) {
+  const int n = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (n >= a.N) return;
+  const float c = a.inv_t * kLog2e;
+  float m = kNegInf, s = 0.f, tt = kNegInf, ts = 0.f;
+  for (int t = lane; t < a.segs; t += 64) {
+    const float2 v = a.part[static_cast<int64_t>(n) * a.segs + t];
+    join(m, s, v.x, v.y, c);
+  }
+  join_lanes(m, s, 64, c);
+  const float log_s = log2f(s);
+  const int64_t i0 = n * a.index_ld, t0 = n * a.teacher_ld;
+  int64_t word;
+  float t;
+  for (int k = lane; k < a.K; k += 64)
+    if (list_entry(a.index, i0 + k, a.wide, a.teacher, t0 + k, a.teacher_dt, word, t)) join(tt, ts, t, 1.f, c);
+  join_lanes(tt, ts, 64, c);
+  const bool kept = !(ts == 0.f);  // no entry: (-inf, 0); a NaN among them: NaN
+  const float tl = log2f(ts);
+  float loss = 0.f;
+  for (int k = lane; k < a.K; k += 64) {
+    float q = 0.f, z = 0.f;
+    if (list_entry(a.index, i0 + k, a.wide, a.teacher, t0 + k, a.teacher_dt, word, t)) {
+      q = exp2_(fmaf(t - tt, c, -tl));
+      if (word >= a.V) loss = __builtin_nanf("");
+      else z = load_any(a.z, n * a.z_ld + word, a.dt);
+      loss += diverge(q, t, tt, tl, z, m, log_s, a.inv_t);
+    }
+    a.share[static_cast<int64_t>(n) * a.K + k] = q;
+  }
+  loss = sum_lanes(loss);
+  if (lane == 0) {
+    const double all = kept ? static_cast<double>(loss) / (static_cast<double>(a.inv_t) * a.inv_t) : 0.0;
+    if (a.loss_each != nullptr) a.loss_each[n] = static_cast<float>(all);
+    else a.rows[n] = all;
+    a.top[n] = m;
+    a.log_s[n] = kept ? (loss != loss ? loss : log_s) : __builtin_huge_valf();
+  }
+}
+
+// the kept rows, and the sum or mean of their losses
+__global__ void __launch_bounds__(1024) logit_reduce_kernel(const double* rows, const float* log_s, int N, int mean, int* info, float* out) {
+  __shared__ double part[16];
+  __shared__ int cnt[16];
+  double s = 0.0;
+  int c = 0;
+  for (int i = threadIdx.x; i < N; i += 1024) {
+    if (out != nullptr) s += rows[i];
+    c += log_s[i] != __builtin_huge_valf();
+  }
+  for (int o = 1; o < 64; o <<= 1) {
+    s += __shfl_xor(s, o, 64);
+    c += __shfl_xor(c, o, 64);
+  }
+  if ((threadIdx.x & 63) == 0) {
+    part[threadIdx.x >> 6] = s;
+    cnt[threadIdx.x >> 6] = c;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s = 0.0;
+    c = 0;
+    for (int w = 0; w < 16; ++w) {
+      s += part[w];
+      c += cnt[w];
+    }
+    info[0] = c;
+    if (out != nullptr) *out = static_cast<float>(mean && c > 0 ? s / c : s);
+  }
+}
+
+template <int DT>
+__global__ void __launch_bounds__(256) logit_grad_kernel(LogitArgs a) {
+  typedef typename Elem<DT>::type T;
+  const int n = blockIdx.x / a.segs, seg = blockIdx.x - n * a.segs, tid = threadIdx.x;
+  const T* z = static_cast<const T*>(a.z) + n * a.z_ld;
+  T* dz = static_cast<T*>(a.dz) + n * a.dz_ld;
+  const int lo = seg * a.seg_len;
+  int hi = lo + a.seg_len;
+  if (hi > a.V) hi = a.V;
+  if (lo >= hi) return;
+  const float top = a.top[n], log_s = a.log_s[n], c = a.inv_t * kLog2e;
+  if (log_s == __builtin_huge_valf()) {  // a row without a list
+    for (int v = lo + tid; v < hi; v += 256) dz[v] = from_f<DT>(0.f);
+    return;
+  }
+  const int count = a.info[0];
+  const float g = a.g[a.each ? n : 0] / a.inv_t / (a.mean && count > 0 ? static_cast<float>(count) : 1.f);
+  walk<DT>(z, lo, hi, tid, 256, [&](int v, float x) { dz[v] = from_f<DT>(g * exp2_(fmaf(x - top, c, -log_s))); });
+  wait_vmcnt<0>();
+  __syncthreads();  // every p is written; the picked words are written over
+  for (int k = tid; k < a.K; k += 256) {
+    const int64_t word = load_index(a.index, n * a.index_ld + k, a.wide);
+    if (word < lo || word >= hi) continue;
+    float s = 0.f;
+    for (int j = 0; j < a.K; ++j)
+      if (load_index(a.index, n * a.index_ld + j, a.wide) == word) s += a.share[static_cast<int64_t>(n) * a.K + j];
+    dz[word] = from_f<DT>(g * (exp2_(fmaf(to_f<DT>(z[word]) - top, c, -log_s)) - s));
+  }
+}
+
+// ------------------------------------------------------------------------------------------------
+// Host side
+// ------------------------------------------------------------------------------------------------
+int64_t up(int64_t x, int64_t a) { return (x + a - 1) / a * a; }
+int ceil_div(int64_t x, int64_t a) { return static_cast<int>((x + a - 1) / a); }
+
+template <bool F16, int PL, bool ACOL, bool BCOL, int EPI>
+int launch_gemm(hipStream_t st, const GemmArgs& a) {
+  const void* fn = reinterpret_cast<const void*>(&gemm_kernel<F16, PL, ACOL, BCOL, EPI>);
+  const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, kGemmSmem);
+  if (e != hipSuccess) return static_cast<int>(e);
+  const int64_t tiles = static_cast<int64_t>(ceil_div(a.M, kTile)) * ceil_div(a.N, kTile) * (EPI == kPartial ? a.splits : 1);
+  if (tiles >= (int64_t(1) << 31)) return -4;
+  hipLaunchKernelGGL((gemm_kernel<F16, PL, ACOL, BCOL, EPI>), dim3(static_cast<unsigned>(tiles)), dim3(kThreads), kGemmSmem, st, a);
+  return static_cast<int>(hipGetLastError());
+}
+template <bool ACOL, bool BCOL, int EPI>
+int gemm(hipStream_t st, int dt, const GemmArgs& a) {
+  if (dt == kBF16) return launch_gemm<false, 1, ACOL, BCOL, EPI>(st, a);
+  if (dt == kF16) return launch_gemm<true, 1, ACOL, BCOL, EPI>(st, a);
+  return launch_gemm<true, 2, ACOL, BCOL, EPI>(st, a);
+}
+
+}  // namespace
+
+// Mirrored by vocab_loss._HeadParams.
+struct DetVocabHead {
+  const void *x, *w, *bias, *target, *index, *teacher;
+  void *dx, *dw, *db;             // backward: null where not wanted
+  const void* gout;               // backward: fp32 [1] or [N]
+  float* loss;                    // forward: [1] or [N]
+  float *stats;                   // [2, N] maxima and log2 of sums, [N, K] picked logits, [N, K] shares: forward writes, backward reads
+  int* rows;                      // [4 + N]: info, then the list of kept rows
+  void* ws;
+  int64_t ws_bytes, x_ld, w_ld, index_ld, teacher_ld, ignore;
+  int N, D, V, K, dtype, bias_dt, wide, teacher_dt, reduction;  // reduction 0 each row, 1 mean, 2 sum
+  float inv_t, smooth;
+};
+
+namespace {
+
+// What both directions lay out in the workspace.
+struct Plan {
+  int planes, ldh, chunk, nchunks, ntiles, splits, k_per_split, csplits;
+  bool pack_w;
+  int64_t off_h, off_w, off_flag, off_part, off_partz, off_rows, off_roww, off_alpha, off_g, off_dx, off_cs, total;
+};
+
+constexpr int64_t kChunkBytes = int64_t(256) << 20;  // G of one chunk, and the packed weights of one
+
+Plan plan(const DetVocabHead& p, bool backward) {
+  Plan q = {};
+  q.planes = p.dtype == kF32 ? 2 : 1;
+  q.ldh = static_cast<int>(up(p.D, 8));
+  q.pack_w = p.dtype == kF32 || p.D % 8 != 0 || p.w_ld % 8 != 0 || (reinterpret_cast<uintptr_t>(p.w) & 15) != 0;
+  int64_t chunk = up(p.V, kTile);
+  if (backward) {
+    const int64_t fit = kChunkBytes / (int64_t(2) * q.planes * p.N) / kTile * kTile;
+    if (chunk > fit) chunk = fit;
+  }
+  if (q.pack_w) {
+    const int64_t fit = kChunkBytes / (int64_t(2) * q.planes * q.ldh) / kTile * kTile;
+    if (chunk > fit) chunk = fit;
+  }
+  if (chunk > (1 << 20)) chunk = 1 << 20;  // 256 rows of G stay within 32-bit offsets
+  if (chunk < kTile) chunk = kTile;
+  q.nchunks = ceil_div(p.V, chunk);
+  q.chunk = static_cast<int>(up(ceil_div(p.V, q.nchunks), kTile));  // even chunks
+  q.nchunks = ceil_div(p.V, q.chunk);
+  q.ntiles = ceil_div(p.V, kTile);
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t o = at;
+    at += up(bytes, 256);
+    return o;
+  };
+  q.off_h = take(int64_t(2) * q.planes * p.N * q.ldh);
+  q.off_w = q.pack_w ? take(int64_t(2) * q.planes * q.chunk * q.ldh) : 0;
+  if (!backward) {
+    q.off_flag = take(p.N);
+    q.off_part = take(int64_t(8) * p.N * q.ntiles);
+    q.off_partz = p.smooth != 0.f ? take(int64_t(4) * p.N * q.ntiles) : 0;
+    q.off_rows = take(int64_t(8) * p.N);
+  } else {
+    // few tiles: the sum over the chunk is split until about two blocks a CU run, none under 512 long
+    const int64_t tiles = int64_t(ceil_div(p.N, kTile)) * ceil_div(p.D, kTile);
+    int64_t splits = tiles < 512 ? 512 / tiles : 1;
+    const int64_t most = q.chunk / 512 > 0 ? q.chunk / 512 : 1;
+    if (splits > most) splits = most;
+    q.k_per_split = static_cast<int>(up(ceil_div(q.chunk, splits), 64));
+    q.splits = ceil_div(q.chunk, q.k_per_split);
+    q.off_roww = take(int64_t(4) * p.N);
+    q.off_alpha = take(4);
+    q.off_g = take(int64_t(2) * q.planes * p.N * q.chunk);
+    q.off_dx = p.dx != nullptr ? take(int64_t(4) * q.splits * p.N * q.ldh) : 0;
+    q.csplits = p.N > 2048 ? 32 : ceil_div(p.N, 64);
+    q.off_cs = p.db != nullptr ? take(int64_t(4) * q.csplits * q.chunk) : 0;
+  }
+  q.total = at;
+  return q;
+}
+
+int check_head(const DetVocabHead& p) {
+  if (p.N < 1 || p.D < 1 || p.V < 1 || p.K < 1) return -1;
+  if (p.dtype < 0 || p.dtype > 2 || p.reduction < 0 || p.reduction > 2) return -2;
+  if ((p.target == nullptr) == (p.index == nullptr)) return -3;
+  // offsets inside a tile are 32-bit: 256 rows of an operand, 64 rows of G
+  if (p.D > (1 << 21) || p.w_ld > (int64_t(1) << 21) || p.V > (1 << 30) || p.N > (1 << 30)) return -4;
+  return 0;
+}
+
+#define DET_TRY(call)             \
+  do {                            \
+    const int rc_ = (call);       \
+    if (rc_ != 0) return rc_;     \
+  } while (0)
+
+template <int DT>
+int pack(hipStream_t st, const PackArgs& a) {
+  const int blocks = a.rows < 4096 ? a.rows : 4096;
+  hipLaunchKernelGGL((pack_kernel<DT>), dim3(blocks), dim3(256), 0, st, a);
+  return static_cast<int>(hipGetLastError());
+}
+int pack_any(hipStream_t st, int dt, const PackArgs& a) {
+  return dt == kF32 ? pack<kF32>(st, a) : pack<kBF16>(st, a);  // 16-bit types are copied as bits
+}
+
+int pack_hidden(hipStream_t st, const DetVocabHead& p, const Plan& q, char* ws) {
+  PackArgs a = {};
+  a.src = p.x;
+  a.src_ld = p.x_ld;
+  a.list = p.rows + 4;
+  a.count = p.rows;
+  a.absmax = p.rows + 1;
+  a.dst = reinterpret_cast<u16*>(ws + q.off_h);
+  a.plane = int64_t(p.N) * q.ldh;
+  a.rows = p.N;
+  a.cols = p.D;
+  a.ld = q.ldh;
+  return pack_any(st, p.dtype, a);
+}
+
+// the weight rows v0 .. v0 + nv as an operand
+int weight_operand(hipStream_t st, const DetVocabHead& p, const Plan& q, char* ws, int v0, int nv, Operand* w) {
+  const int64_t es = p.dtype == kF32 ? 4 : 2;
+  const char* src = static_cast<const char*>(p.w) + v0 * p.w_ld * es;
+  if (!q.pack_w) {
+    *w = Operand{reinterpret_cast<const u16*>(src), 0, p.w_ld};
+    return 0;
+  }
+  PackArgs a = {};
+  a.src = src;
+  a.src_ld = p.w_ld;
+  a.absmax = p.rows + 2;
+  a.dst = reinterpret_cast<u16*>(ws + q.off_w);
+  a.plane = int64_t(q.chunk) * q.ldh;
+  a.rows = nv;
+  a.cols = p.D;
+  a.ld = q.ldh;
+  *w = Operand{a.dst, a.plane, q.ldh};
+  return pack_any(st, p.dtype, a);
+}
+
+GemmArgs logits_args(const DetVocabHead& p, const Plan& q, char* ws, const Operand& w, int v0, int nv) {
+  GemmArgs a = {};
+  a.A = Operand{reinterpret_cast<const u16*>(ws + q.off_h), int64_t(p.N) * q.ldh, q.ldh};
+  a.B = w;
+  a.m_dyn = p.rows;
+  a.info = p.rows;
+  a.M = p.N;
+  a.N = nv;
+  a.K = q.ldh;
+  if (p.bias != nullptr) a.bias = static_cast<const char*>(p.bias) + int64_t(v0) * (p.bias_dt == kF32 ? 4 : 2);
+  a.bias_dt = p.bias_dt;
+  a.c = p.inv_t * kLog2e;
+  a.inv_v = 1.f / static_cast<float>(p.V);
+  return a;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t det_vocab_head_ws_bytes(const DetVocabHead* p, int backward) {
+  if (p == nullptr || check_head(*p) != 0) return -1;
+  return plan(*p, backward != 0).total;
+}
+
+int det_vocab_head_forward(void* stream, const DetVocabHead* pp) {
+  if (pp == nullptr) return -1;
+  const DetVocabHead& p = *pp;
+  DET_TRY(check_head(p));
+  const Plan q = plan(p, false);
+  if (p.ws == nullptr || p.ws_bytes < q.total) return -6;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  char* ws = static_cast<char*>(p.ws);
+  int* list = p.rows + 4;
+
+  RowArgs r = {p.target, p.index, p.teacher, reinterpret_cast<uint8_t*>(ws + q.off_flag), p.rows, list, p.ignore,
+               p.index_ld, p.teacher_ld, p.N, p.K, p.wide, p.teacher_dt};
+  if (p.index != nullptr) hipLaunchKernelGGL(list_flags_kernel, dim3(ceil_div(p.N, 4)), dim3(256), 0, st, r);
+  hipLaunchKernelGGL(rows_kernel, dim3(1), dim3(1024), 0, st, r);
+  if (p.dtype == kF32) {
+    hipLaunchKernelGGL(absmax_kernel, dim3(p.N < 1024 ? p.N : 1024), dim3(256), 0, st, static_cast<const float*>(p.x), p.x_ld, p.N,
+                       p.D, p.rows + 1);
+    hipLaunchKernelGGL(absmax_kernel, dim3(p.V < 2048 ? p.V : 2048), dim3(256), 0, st, static_cast<const float*>(p.w), p.w_ld, p.V,
+                       p.D, p.rows + 2);
+  }
+  DET_TRY(static_cast<int>(hipGetLastError()));
+  DET_TRY(pack_hidden(st, p, q, ws));
+  for (int c = 0; c < q.nchunks; ++c) {
+    const int v0 = c * q.chunk, nv = p.V - v0 < q.chunk ? p.V - v0 : q.chunk;
+    Operand w;
+    DET_TRY(weight_operand(st, p, q, ws, v0, nv, &w));
+    GemmArgs a = logits_args(p, q, ws, w, v0, nv);
+    a.part = reinterpret_cast<float2*>(ws + q.off_part);
+    a.part_z = p.smooth != 0.f ? reinterpret_cast<float*>(ws + q.off_partz) : nullptr;
+    a.tile0 = v0 / kTile;
+    a.ntiles = q.ntiles;
+    DET_TRY((gemm<false, false, kStats>(st, p.dtype, a)));
+  }
+  FinishArgs f = {};
+  f.x = p.x;
+  f.w = p.w;
+  f.bias = p.bias;
+  f.x_ld = p.x_ld;
+  f.w_ld = p.w_ld;
+  f.dt = p.dtype;
+  f.bias_dt = p.bias_dt;
+  f.D = p.D;
+  f.V = p.V;
+  f.K = p.K;
+  f.N = p.N;
+  f.ntiles = q.ntiles;
+  f.info = p.rows;
+  f.list = list;
+  f.part = reinterpret_cast<const float2*>(ws + q.off_part);
+  f.part_z = p.smooth != 0.f ? reinterpret_cast<const float*>(ws + q.off_partz) : nullptr;
+  f.target = p.target;
+  f.index = p.index;
+  f.teacher = p.teacher;
+  f.index_ld = p.index_ld;
+  f.teacher_ld = p.teacher_ld;
+  f.wide = p.wide;
+  f.teacher_dt = p.teacher_dt;
+  f.inv_t = p.inv_t;
+  f.smooth = p.smooth;
+  f.top = p.stats;
+  f.log_s = p.stats + p.N;
+  f.picked = p.stats + int64_t(2) * p.N;
+  f.share = f.picked + int64_t(p.N) * p.K;
+  f.each = p.reduction == 0 ? p.loss : nullptr;
+  f.rows = reinterpret_cast<double*>(ws + q.off_rows);
+  if (f.each != nullptr) hipLaunchKernelGGL(zero_kernel, dim3(ceil_div(p.N, 1024) < 1024 ? ceil_div(p.N, 1024) : 1024), dim3(256), 0, st, p.loss, int64_t(p.N));
+  const dim3 fg(p.N < 8192 ? p.N : 8192);
+  if (p.dtype == kF32) hipLaunchKernelGGL(finish_kernel<kF32>, fg, dim3(256), 0, st, f);
+  else if (p.dtype == kBF16) hipLaunchKernelGGL(finish_kernel<kBF16>, fg, dim3(256), 0, st, f);
+  else hipLaunchKernelGGL(finish_kernel<kF16>, fg, dim3(256), 0, st, f);
+  if (f.each == nullptr) hipLaunchKernelGGL(reduce_kernel, dim3(1), dim3(1024), 0, st, f.rows, p.rows, p.reduction == 1, p.loss);
+  return static_cast<int>(hipGetLastError());
+}
+
+int det_vocab_head_backward(void* stream, const DetVocabHead* pp) {
+  if (pp == nullptr) return -1;
+  const DetVocabHead& p = *pp;
+  DET_TRY(check_head(p));
+  const Plan q = plan(p, true);
+  if (p.ws == nullptr || p.ws_bytes < q.total || p.gout == nullptr) return -6;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  char* ws = static_cast<char*>(p.ws);
+  int* list = p.rows + 4;
+  const bool f16 = p.dtype != kBF16;
+  float* row_w = reinterpret_cast<float*>(ws + q.off_roww);
+  float* alpha = reinterpret_cast<float*>(ws + q.off_alpha);
+  const float* picked = p.stats + int64_t(2) * p.N;
+  const float smooth_v = p.smooth / static_cast<float>(p.V);
+
+  WeightArgs wa = {static_cast<const float*>(p.gout), p.rows, list, row_w, alpha, 1.f / p.inv_t,
+                   f16 ? static_cast<float>(1 << kGExp) : 1.f, p.reduction == 0, p.reduction == 1};
+  hipLaunchKernelGGL(weights_kernel, dim3(1), dim3(1024), 0, st, wa);
+  DET_TRY(static_cast<int>(hipGetLastError()));
+  DET_TRY(pack_hidden(st, p, q, ws));
+  const int64_t es = p.dtype == kF32 ? 4 : 2;
+  for (int c = 0; c < q.nchunks; ++c) {
+    const int v0 = c * q.chunk, nv = p.V - v0 < q.chunk ? p.V - v0 : q.chunk;
+    const int ldg = static_cast<int>(up(nv, 64));  // columns past nv are zero
+    Operand w;
+    DET_TRY(weight_operand(st, p, q, ws, v0, nv, &w));
+    GemmArgs a = logits_args(p, q, ws, w, v0, nv);
+    a.top = p.stats;
+    a.log_s = p.stats + p.N;
+    a.row_w = row_w;
+    a.smooth_v = smooth_v;
+    a.G = reinterpret_cast<u16*>(ws + q.off_g);
+    a.g_plane = int64_t(p.N) * ldg;
+    a.ldg = ldg;
+    DET_TRY((gemm<false, false, kGrad>(st, p.dtype, a)));
+    ScatterArgs s = {p.rows, list, p.target, p.index, p.index_ld, p.wide, p.K, v0, nv, f16, q.planes, ldg,
+                     picked, picked + int64_t(p.N) * p.K, p.stats, p.stats + p.N, row_w, smooth_v, a.c, a.G, a.g_plane};
+    const int sb = ceil_div(int64_t(p.N) * p.K, 256);
+    hipLaunchKernelGGL(scatter_kernel, dim3(sb < 8192 ? sb : 8192), dim3(256), 0, st, s);
+    const Operand G = {a.G, a.g_plane, ldg};
+    if (p.db != nullptr) {
+      float* cs = reinterpret_cast<float*>(ws + q.off_cs);
+      hipLaunchKernelGGL(colsum_kernel, dim3(ceil_div(ldg, 256), q.csplits), dim3(256), 0, st, a.G, a.g_plane, q.planes, f16, ldg,
+                         p.rows, cs);
+      hipLaunchKernelGGL(dbias_kernel, dim3(ceil_div(nv, 256)), dim3(256), 0, st, cs, q.csplits, ldg, nv, alpha, p.db, int64_t(v0),
+                         p.bias_dt);
+    }
+    DET_TRY(static_cast<int>(hipGetLastError()));
+    if (p.dx != nullptr) {
+      GemmArgs d = {};
+      d.A = G;
+      d.B = w;
+      d.m_dyn = p.rows;
+      d.info = p.rows;
+      d.M = p.N;
+      d.N = q.ldh < p.D ? q.ldh : p.D;
+      d.K = nv;
+      d.splits = q.splits;
+      d.k_per_split = q.k_per_split;
+      d.out32 = reinterpret_cast<float*>(ws + q.off_dx);
+      d.ldo = q.ldh;
+      d.split_stride = int64_t(p.N) * q.ldh;
+      d.add = c > 0;
+      DET_TRY((gemm<false, true, kPartial>(st, p.dtype, d)));
+    }
+    if (p.dw != nullptr) {
+      GemmArgs d = {};
+      d.A = G;
+      d.B = Operand{reinterpret_cast<const u16*>(ws + q.off_h), int64_t(p.N) * q.ldh, q.ldh};
+      d.k_dyn = p.rows;
+      d.info = p.rows;
+      d.M = nv;
+      d.N = p.D;
+      d.K = p.N;
+      d.out = static_cast<char*>(p.dw) + int64_t(v0) * p.D * es;
+      d.ldo = p.D;
+      d.out_dt = p.dtype;
+      d.alpha = alpha;
+      DET_TRY((gemm<true, true, kOut>(st, p.dtype, d)));
+    }
+  }
+  if (p.dx != nullptr)
+    hipLaunchKernelGGL(dx_kernel, dim3(p.N), dim3(256), 0, st, reinterpret_cast<const float*>(ws + q.off_dx), q.splits,
+                       int64_t(p.N) * q.ldh, int64_t(q.ldh), p.rows, list, alpha, q.planes, p.dx, p.dtype, p.D);
+  return static_cast<int>(hipGetLastError());
+}
+
+}  // extern "C"
+
+// Mirrored by vocab_loss._LogitParams.
+struct DetVocabLogits {
+  const void *z, *index, *teacher;
+  void* dz;
+  const void* gout;
+  float* loss;
+  float* stats;         // [2, N] maxima and log2 of sums, [N, K] shares
+  int* info;            // [1]
+  void* ws;
+  int64_t ws_bytes, z_ld, index_ld, teacher_ld, dz_ld;
+  int N, V, K, dtype, wide, teacher_dt, reduction;
+  float inv_t;
+};
+
+namespace {
+
+LogitArgs logit_args(const DetVocabLogits& p) {
+  LogitArgs a = {};
+  a.z = p.z;
+  a.z_ld = p.z_ld;
+  a.dt = p.dtype;
+  a.N = p.N;
+  a.V = p.V;
+  a.K = p.K;
+  // few rows: a row is cut into segments until about eight blocks a CU run, none under 2048 long
+  int64_t segs = p.N < 2048 ? 2048 / p.N : 1;
+  const int64_t most = p.V / 2048 > 0 ? p.V / 2048 : 1;
+  if (segs > most) segs = most;
+  a.seg_len = static_cast<int>(up(ceil_div(p.V, segs), 8));
+  a.segs = ceil_div(p.V, a.seg_len);
+  a.index = p.index;
+  a.teacher = p.teacher;
+  a.index_ld = p.index_ld;
+  a.teacher_ld = p.teacher_ld;
+  a.wide = p.wide;
+  a.teacher_dt = p.teacher_dt;
+  a.inv_t = p.inv_t;
+  a.each = p.reduction == 0;
+  a.mean = p.reduction == 1;
+  a.top = p.stats;
+  a.log_s = p.stats + p.N;
+  a.share = p.stats + int64_t(2) * p.N;
+  a.info = p.info;
+  a.g = static_cast<const float*>(p.gout);
+  a.dz = p.dz;
+  a.dz_ld = p.dz_ld;
+  return a;
+}
+
+int check_logits(const DetVocabLogits& p) {
+  if (p.N < 1 || p.V < 1 || p.K < 1) return -1;
+  if (p.dtype < 0 || p.dtype > 2 || p.reduction < 0 || p.reduction > 2) return -2;
+  if (p.V > (1 << 30) || p.N > (1 << 20)) return -4;
+  return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t det_vocab_logits_ws_bytes(const DetVocabLogits* p) {
+  if (p == nullptr || check_logits(*p) != 0) return -1;
+  return up(int64_t(8) * p->N * logit_args(*p).segs, 256) + up(int64_t(8) * p->N, 256);
+}
+
+int det_vocab_logits_forward(void* stream, const DetVocabLogits* pp) {
+  if (pp == nullptr) return -1;
+  const DetVocabLogits& p = *pp;
+  DET_TRY(check_logits(p));
+  if (p.ws == nullptr || p.ws_bytes < det_vocab_logits_ws_bytes(pp)) return -6;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  LogitArgs a = logit_args(p);
+  char* ws = static_cast<char*>(p.ws);
+  a.part = reinterpret_cast<float2*>(ws);
+  a.rows = reinterpret_cast<double*>(ws + up(int64_t(8) * p.N * a.segs, 256));
+  a.loss_each = a.each ? p.loss : nullptr;
+  const dim3 grid(static_cast<unsigned>(p.N) * a.segs);
+  if (p.dtype == kF32) hipLaunchKernelGGL(logit_stats_kernel<kF32>, grid, dim3(256), 0, st, a);
+  else if (p.dtype == kBF16) hipLaunchKernelGGL(logit_stats_kernel<kBF16>, grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL(logit_stats_kernel<kF16>, grid, dim3(256), 0, st, a);
+  hipLaunchKernelGGL(logit_finish_kernel, dim3(ceil_div(p.N, 4)), dim3(256), 0, st, a);
+  hipLaunchKernelGGL(logit_reduce_kernel, dim3(1), dim3(1024), 0, st, a.rows, a.log_s, p.N, a.mean, p.info, a.each ? nullptr : p.loss);
+  return static_cast<int>(hipGetLastError());
+}
+
+int det_vocab_logits_backward(void* stream, const DetVocabLogits* pp) {
+  if (pp == nullptr) return -1;
+  const DetVocabLogits& p = *pp;
+  DET_TRY(check_logits(p));
+  if (p.gout == nullptr || p.dz == nullptr) return -6;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  LogitArgs a = logit_args(p);
+  const dim3 grid(static_cast<unsigned>(p.N) * a.segs);
+  if (p.dtype == kF32) hipLaunchKernelGGL(logit_grad_kernel<kF32>, grid, dim3(256), 0, st, a);
+  else if (p.dtype == kBF16) hipLaunchKernelGGL(logit_grad_kernel<kBF16>, grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL(logit_grad_kernel<kF16>, grid, dim3(256), 0, st, a);
+  return static_cast<int>(hipGetLastError());
+}
+
+}  // extern "C"

@@ -1,0 +1,342 @@
+"""Losses over a vocabulary, on the ``det_vocab.hip`` kernels.
+
+    linear_cross_entropy(x, W, target[, b])            CE(x W^T + b, target)
+    linear_topk_distill(x, W, teacher, index[, b])     T^2 KL(teacher's top logits || softmax((x W^T + b) / T))
+    topk_distill(logits, teacher, index)               the same for logits that are there already
+
+The ``linear_`` forms are a language model's output layer and its loss in one: the [rows, V] logits are
+never kept.  The forward reduces each tile of them to a maximum and a sum of exponentials; the backward
+walks the vocabulary in chunks of a bounded workspace, recomputes a chunk's logits, turns them into
+their gradient and multiplies that into the gradients of ``x`` and ``W``.  Rows that are ignored cost
+nothing.  Losses are fp32; sums, softmax statistics and gradients are accumulated in fp32; a chunk's
+logit gradient is held in the operands' type (fp32: two fp16 planes, 22 bits).
+
+GPU tensors (bf16, fp16, fp32) always run on the kernels; what those do not cover is refused.  CPU
+tensors run the plain composite below.  Both are differentiable once.
+"""
+import ctypes
+import math
+from typing import Any, Optional, Tuple
+
+import torch
+import torch.nn.functional as F
+
+from determined_1_amd.ops import _lib
+from determined_1_amd.ops.arena import landing_buffer
+from determined_1_amd.ops.functional import dtype_code
+from determined_1_amd.ops.transformer import _autocast, _null, _ptr, _stream
+
+_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+_FLOATS = (torch.float32, torch.bfloat16, torch.float16)
+
+
+class _HeadParams(ctypes.Structure):
+    """Mirror of ``DetVocabHead`` (det_vocab.hip)."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "w", "bias", "target", "index", "teacher", "dx", "dw", "db", "gout",
+                                                "loss", "stats", "rows", "ws")]
+                + [(n, ctypes.c_int64) for n in ("ws_bytes", "x_ld", "w_ld", "index_ld", "teacher_ld", "ignore")]
+                + [(n, ctypes.c_int32) for n in ("N", "D", "V", "K", "dtype", "bias_dt", "wide", "teacher_dt", "reduction")]
+                + [("inv_t", ctypes.c_float), ("smooth", ctypes.c_float)])
+
+
+class _LogitParams(ctypes.Structure):
+    """Mirror of ``DetVocabLogits`` (det_vocab.hip)."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("z", "index", "teacher", "dz", "gout", "loss", "stats", "info", "ws")]
+                + [(n, ctypes.c_int64) for n in ("ws_bytes", "z_ld", "index_ld", "teacher_ld", "dz_ld")]
+                + [(n, ctypes.c_int32) for n in ("N", "V", "K", "dtype", "wide", "teacher_dt", "reduction")]
+                + [("inv_t", ctypes.c_float)])
+
+
+def _rows_of(t: torch.Tensor) -> torch.Tensor:
+    """[..., C] as [rows, C] with a unit last stride (a view where the layout allows it)."""
+    t = t.reshape(-1, t.shape[-1])
+    return t if t.stride(1) == 1 or t.shape[1] == 1 and t.stride(0) >= 1 else t.contiguous()
+
+
+def _workspace(nbytes: int, like: torch.Tensor, what: str) -> torch.Tensor:
+    if nbytes < 0:
+        raise ValueError(f"{what}: sizes out of the kernels' range")
+    return torch.empty(nbytes, dtype=torch.uint8, device=like.device)
+
+
+def _head_params(x, weight, bias, target, teacher, index, opts) -> _HeadParams:
+    ignore, smooth, heat, reduction = opts
+    p = _HeadParams()
+    p.x, p.w, p.bias = x.data_ptr(), weight.data_ptr(), _ptr(bias)
+    p.x_ld, p.w_ld = x.stride(0), weight.stride(0)
+    p.N, p.D, p.V = x.shape[0], x.shape[1], weight.shape[0]
+    p.dtype, p.bias_dt = dtype_code(x.dtype), 0 if bias is None else dtype_code(bias.dtype)
+    p.ignore, p.smooth, p.inv_t, p.reduction = ignore, smooth, 1.0 / heat, _REDUCTIONS[reduction]
+    if target is not None:
+        p.target, p.K, p.wide = target.data_ptr(), 1, int(target.dtype == torch.int64)
+    else:
+        p.index, p.teacher, p.K = index.data_ptr(), teacher.data_ptr(), index.shape[1]
+        p.index_ld, p.teacher_ld = index.stride(0), teacher.stride(0)
+        p.wide, p.teacher_dt = int(index.dtype == torch.int64), dtype_code(teacher.dtype)
+    return p
+
+
+class _Head(torch.autograd.Function):
+    """x [N, D], weight [V, D]: unit last strides; target [N], or index and teacher [N, K]."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, target, teacher, index, opts):  # type: ignore[override]
+        dev = x.device
+        n, k = x.shape[0], 1 if index is None else index.shape[1]
+        loss = torch.empty(n if opts[3] == "none" else (), dtype=torch.float32, device=dev)
+        stats = torch.empty(n * (2 + 2 * k), dtype=torch.float32, device=dev)
+        rows = torch.empty(4 + n, dtype=torch.int32, device=dev)
+        p = _head_params(x, weight, bias, target, teacher, index, opts)
+        p.loss, p.rows, p.stats = loss.data_ptr(), rows.data_ptr(), stats.data_ptr()
+        lib = _lib.get_lib()
+        with torch.cuda.device(dev):
+            ws = _workspace(lib.det_vocab_head_ws_bytes(ctypes.byref(p), 0), x, "vocab_loss")
+            p.ws, p.ws_bytes = ws.data_ptr(), ws.numel()
+            _lib.check(lib.det_vocab_head_forward(_stream(x), ctypes.byref(p)), "det_vocab_head_forward")
+        ctx.save_for_backward(x, weight, bias, target, teacher, index, stats, rows)
+        ctx.opts = opts
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gout):  # type: ignore[override]
+        x, weight, bias, target, teacher, index, stats, rows = ctx.saved_tensors
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        gout = gout.float().contiguous()
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
+        dw = db = None
+        if need_w:
+            dw = landing_buffer(weight)
+            if dw is None or dw.dtype != weight.dtype or not dw.is_contiguous() or dw.shape != weight.shape:
+                dw = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device)
+        if need_b:
+            db = torch.empty(bias.shape, dtype=bias.dtype, device=bias.device)
+        p = _head_params(x, weight, bias, target, teacher, index, ctx.opts)
+        p.dx, p.dw, p.db, p.gout = _ptr(dx), _ptr(dw), _ptr(db), gout.data_ptr()
+        p.rows, p.stats = rows.data_ptr(), stats.data_ptr()
+        lib = _lib.get_lib()
+        with torch.cuda.device(x.device):
+            ws = _workspace(lib.det_vocab_head_ws_bytes(ctypes.byref(p), 1), x, "vocab_loss")
+            p.ws, p.ws_bytes = ws.data_ptr(), ws.numel()
+            _lib.check(lib.det_vocab_head_backward(_stream(x), ctypes.byref(p)), "det_vocab_head_backward")
+        return dx, dw, db, None, None, None, None
+
+
+class _Logits(torch.autograd.Function):
+    """logits [N, V], teacher and index [N, K]: unit last strides."""
+
+    @staticmethod
+    def _params(z, teacher, index, heat, reduction) -> _LogitParams:
+        p = _LogitParams()
+        p.z, p.index, p.teacher = z.data_ptr(), index.data_ptr(), teacher.data_ptr()
+        p.z_ld, p.index_ld, p.teacher_ld = z.stride(0), index.stride(0), teacher.stride(0)
+        p.N, p.V, p.K = z.shape[0], z.shape[1], index.shape[1]
+        p.dtype, p.wide, p.teacher_dt = dtype_code(z.dtype), int(index.dtype == torch.int64), dtype_code(teacher.dtype)
+        p.reduction, p.inv_t = _REDUCTIONS[reduction], 1.0 / heat
+        return p
+
+    @staticmethod
+    def forward(ctx, z, teacher, index, heat, reduction):  # type: ignore[override]
+        dev = z.device
+        n, k = z.shape[0], index.shape[1]
+        loss = torch.empty(n if reduction == "none" else (), dtype=torch.float32, device=dev)
+        stats = torch.empty(n * (2 + k) + 1, dtype=torch.float32, device=dev)  # the last one: how many rows have a list
+        p = _Logits._params(z, teacher, index, heat, reduction)
+        p.loss, p.stats, p.info = loss.data_ptr(), stats.data_ptr(), stats.data_ptr() + 4 * n * (2 + k)
+        lib = _lib.get_lib()
+        with torch.cuda.device(dev):
+            ws = _workspace(lib.det_vocab_logits_ws_bytes(ctypes.byref(p)), z, "topk_distill")
+            p.ws, p.ws_bytes = ws.data_ptr(), ws.numel()
+            _lib.check(lib.det_vocab_logits_forward(_stream(z), ctypes.byref(p)), "det_vocab_logits_forward")
+        ctx.save_for_backward(z, teacher, index, stats)
+        ctx.heat, ctx.reduction = heat, reduction
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gout):  # type: ignore[override]
+        z, teacher, index, stats = ctx.saved_tensors
+        n, k = z.shape[0], index.shape[1]
+        gout = gout.float().contiguous()
+        dz = torch.empty(z.shape, dtype=z.dtype, device=z.device)
+        p = _Logits._params(z, teacher, index, ctx.heat, ctx.reduction)
+        p.stats, p.info = stats.data_ptr(), stats.data_ptr() + 4 * n * (2 + k)
+        p.gout, p.dz, p.dz_ld = gout.data_ptr(), dz.data_ptr(), dz.stride(0)
+        with torch.cuda.device(z.device):
+            _lib.check(_lib.get_lib().det_vocab_logits_backward(_stream(z), ctypes.byref(p)), "det_vocab_logits_backward")
+        return dz, None, None, None, None
+
+
+# ------------------------------------------------------------------------------------------------
+# plain composite (CPU tensors)
+# ------------------------------------------------------------------------------------------------
+def _wide(t: torch.Tensor) -> torch.Tensor:
+    return t if t.dtype == torch.float64 else t.float()
+
+
+def _reduce(rows: torch.Tensor, kept: torch.Tensor, reduction: str) -> torch.Tensor:
+    rows = torch.where(kept, rows, torch.zeros_like(rows))
+    if reduction == "none":
+        return rows
+    return rows.sum() / kept.sum().clamp(min=1) if reduction == "mean" else rows.sum()
+
+
+def _pick(logp: torch.Tensor, index: torch.Tensor, there: torch.Tensor) -> torch.Tensor:
+    """logp at each index; NaN for one outside the vocabulary, 0 where there is no entry."""
+    v = logp.shape[-1]
+    got = logp.gather(1, index.long().clamp(0, v - 1))
+    outside = torch.zeros_like(got).masked_fill_(there & ((index < 0) | (index >= v)), math.nan)
+    got = got * (1.0 + outside)  # the gradient is NaN too
+    return torch.where(there, got, torch.zeros_like(got))
+
+
+def _plain_ce(z: torch.Tensor, target: torch.Tensor, ignore: int, smooth: float, reduction: str) -> torch.Tensor:
+    kept = target != ignore
+    z = torch.where(kept[:, None], z, torch.zeros_like(z))
+    logp = F.log_softmax(z, dim=1)
+    rows = -(1.0 - smooth) * _pick(logp, target[:, None], kept[:, None])[:, 0]
+    if smooth:
+        rows = rows - smooth * logp.mean(dim=1)
+    return _reduce(rows, kept, reduction)
+
+
+def _plain_distill(z: torch.Tensor, teacher: torch.Tensor, index: torch.Tensor, heat: float, reduction: str) -> torch.Tensor:
+    t = _wide(teacher).to(z.dtype) / heat
+    there = (index >= 0) & (t != -math.inf)
+    kept = there.any(dim=1)
+    z = torch.where(kept[:, None], z, torch.zeros_like(z))
+    logp = F.log_softmax(z / heat, dim=1)
+    logq = F.log_softmax(torch.where(there, t, torch.full_like(t, -math.inf)).masked_fill(~kept[:, None], 0.0), dim=1)
+    q = torch.where(there, logq.exp(), torch.zeros_like(logq))
+    there = there & (q != 0)
+    rows = torch.where(there, q * (logq.masked_fill(~there, 0.0) - _pick(logp, index, there)), torch.zeros_like(q)).sum(dim=1)
+    bad = torch.zeros_like(rows).masked_fill_((index >= z.shape[1]).any(dim=1), math.nan)
+    rows = rows * (1.0 + bad)
+    return _reduce(rows * heat * heat, kept, reduction)
+
+
+# ------------------------------------------------------------------------------------------------
+# public API
+# ------------------------------------------------------------------------------------------------
+def _check(ok: bool, what: str, message: str, error: Any = ValueError) -> None:
+    if not ok:
+        raise error(f"{what}: {message}")
+
+
+def _check_common(what: str, reduction: str, *ts: Optional[torch.Tensor]) -> None:
+    _check(reduction in _REDUCTIONS, what, f"reduction {reduction!r} is none of {sorted(_REDUCTIONS)}")
+    given = [t for t in ts if t is not None]
+    _check(all(t.device == given[0].device for t in given), what, "tensors on different devices")
+    _check(given[0].device.type in ("cpu", "cuda"), what, f"no kernels for {given[0].device}")
+
+
+def _check_float(what: str, x: torch.Tensor, name: str) -> None:
+    _check(x.dtype in _FLOATS or (x.dtype == torch.float64 and x.device.type == "cpu"), what,
+           f"{name} is {x.dtype}: bfloat16, float16 or float32 expected", TypeError)
+
+
+def _check_head(what: str, x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor]) -> None:
+    _check(x.dim() >= 1 and weight.dim() == 2 and x.shape[-1] == weight.shape[1] and weight.numel() > 0, what,
+           f"x [..., D] and weight [V, D] expected, got {tuple(x.shape)} and {tuple(weight.shape)}")
+    _check_float(what, x, "x")
+    _check(weight.dtype == x.dtype, what, f"x is {x.dtype} and weight {weight.dtype}", TypeError)
+    if bias is not None:
+        _check(bias.shape == (weight.shape[0],), what, f"bias of {weight.shape[0]} words expected, got {tuple(bias.shape)}")
+        _check(bias.dtype in (x.dtype, torch.float32), what, f"x is {x.dtype} and bias {bias.dtype}", TypeError)
+
+
+def _check_lists(what: str, lead: Tuple[int, ...], teacher: torch.Tensor, index: torch.Tensor, heat: float) -> None:
+    _check(index.dim() == len(lead) + 1 and tuple(index.shape[:-1]) == lead and index.shape[-1] > 0 and teacher.shape == index.shape,
+           what, f"teacher_logits and teacher_index {lead + ('K',)} expected, got {tuple(teacher.shape)} and {tuple(index.shape)}")
+    _check(index.dtype in (torch.int32, torch.int64), what, f"teacher_index is {index.dtype}: int32 or int64 expected", TypeError)
+    _check_float(what, teacher, "teacher_logits")
+    _check(2.0 ** -20 <= heat <= 2.0 ** 20, what, f"temperature {heat} is not within [2^-20, 2^20]")
+
+
+def _empty(reduction: str, lead: Tuple[int, ...], *ts: torch.Tensor) -> torch.Tensor:
+    """The loss of no rows: 0, with gradients of zeros."""
+    zero = sum((t * 0).sum().float() for t in ts if t is not None)
+    return zero if reduction != "none" else zero.expand(lead)
+
+
+def _linear(x, weight, bias, target, teacher, index, opts, lead) -> torch.Tensor:
+    (x, weight, bias), ac = _autocast(x, weight, bias)
+    if x.numel() == 0:
+        return _empty(opts[3], lead, x, weight, bias)
+    x2 = _rows_of(x)
+    if target is not None:
+        target = target.reshape(-1).contiguous()
+    else:
+        teacher, index = _rows_of(teacher.detach()), _rows_of(index)
+    if x.device.type == "cpu":
+        z = F.linear(_wide(x2), _wide(weight), None if bias is None else _wide(bias).to(_wide(x2).dtype))
+        loss = (_plain_ce(z, target, opts[0], opts[1], opts[3]) if target is not None
+                else _plain_distill(z, teacher, index, opts[2], opts[3]))
+    else:
+        if weight.stride(1) != 1:
+            weight = weight.contiguous()
+        if bias is not None:
+            bias = bias.contiguous()
+        with torch.autocast("cuda", enabled=False) if ac else _null():
+            loss = _Head.apply(x2, weight, bias, target, teacher, index, opts)
+    return loss.reshape(lead) if opts[3] == "none" else loss
+
+
+def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
+                         ignore_index: int = -100, label_smoothing: float = 0.0, reduction: str = "mean") -> torch.Tensor:
+    """``F.cross_entropy(F.linear(x, weight, bias), target, ...)`` without the logits.
+
+    x [..., D], weight [V, D], bias [V] (x's type or fp32), target [...] int32 or int64.  Rows whose target is
+    ``ignore_index`` have loss 0, no gradient, and take no work; a mean over none of them is 0.  A target
+    outside the vocabulary gives its row (and a mean or sum) a NaN loss and NaN gradients: nothing is read
+    out of bounds, and no host check waits for the GPU.  With ``reduction="none"`` under ``torch.no_grad()``
+    it scores tokens: the loss [...] is each target's negative log-probability."""
+    what = "linear_cross_entropy"
+    _check_common(what, reduction, x, weight, target, bias)
+    if not (torch.is_autocast_enabled("cuda") and x.is_cuda):
+        _check_head(what, x, weight, bias)
+    _check(tuple(target.shape) == tuple(x.shape[:-1]), what, f"target {tuple(x.shape[:-1])} expected, got {tuple(target.shape)}")
+    _check(target.dtype in (torch.int32, torch.int64), what, f"target is {target.dtype}: int32 or int64 expected", TypeError)
+    _check(0.0 <= label_smoothing <= 1.0, what, f"label_smoothing {label_smoothing} is not within [0, 1]")
+    return _linear(x, weight, bias, target, None, None, (int(ignore_index), float(label_smoothing), 1.0, reduction),
+                   tuple(x.shape[:-1]))
+
+
+def linear_topk_distill(x: torch.Tensor, weight: torch.Tensor, teacher_logits: torch.Tensor, teacher_index: torch.Tensor,
+                        bias: Optional[torch.Tensor] = None, *, temperature: float = 1.0, reduction: str = "mean") -> torch.Tensor:
+    """``topk_distill(F.linear(x, weight, bias), teacher_logits, teacher_index, ...)`` without the logits.
+
+    x [..., D], weight [V, D], bias [V]; the lists [..., K] as in ``topk_distill``."""
+    what = "linear_topk_distill"
+    _check_common(what, reduction, x, weight, teacher_logits, teacher_index, bias)
+    if not (torch.is_autocast_enabled("cuda") and x.is_cuda):
+        _check_head(what, x, weight, bias)
+    _check_lists(what, tuple(x.shape[:-1]), teacher_logits, teacher_index, float(temperature))
+    return _linear(x, weight, bias, None, teacher_logits, teacher_index, (-100, 0.0, float(temperature), reduction),
+                   tuple(x.shape[:-1]))
+
+
+def topk_distill(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_index: torch.Tensor, *, temperature: float = 1.0,
+                 reduction: str = "mean") -> torch.Tensor:
+    """Distillation from a teacher's top logits: ``T^2 sum_k q_k (log q_k - log p[index_k])`` a row, with
+    ``p = softmax(logits / T)`` over the vocabulary and ``q = softmax(teacher_logits / T)`` over the list.
+
+    logits [..., V]; teacher_logits and teacher_index [..., K] (int32 or int64; ``torch.topk``'s values and
+    indices), no gradient for them.  Entries with a negative index or a logit of -inf are absent, so lists
+    may be of any length up to K; a row without an entry has loss 0 and no gradient and does not count in a
+    mean; a mean over none is 0.  A word that is listed twice has the sum of its shares.  An index past the
+    vocabulary gives its row a NaN loss and NaN gradients."""
+    what = "topk_distill"
+    _check_common(what, reduction, logits, teacher_logits, teacher_index)
+    _check(logits.dim() >= 1 and logits.shape[-1] > 0, what, f"logits [..., V] expected, got {tuple(logits.shape)}")
+    _check_float(what, logits, "logits")
+    lead = tuple(logits.shape[:-1])
+    _check_lists(what, lead, teacher_logits, teacher_index, float(temperature))
+    if logits.numel() == 0:
+        return _empty(reduction, lead, logits)
+    z, teacher, index = _rows_of(logits), _rows_of(teacher_logits.detach()), _rows_of(teacher_index)
+    if logits.device.type == "cpu":
+        loss = _plain_distill(_wide(z), teacher, index, float(temperature), reduction)
+    else:
+        loss = _Logits.apply(z, teacher, index, float(temperature), reduction)
+    return loss.reshape(lead) if reduction == "none" else loss

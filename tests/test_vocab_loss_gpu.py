@@ -1,0 +1,512 @@
+"""Losses over a vocabulary (ops/vocab_loss.py, ops/csrc/det_vocab.hip) against their definitions in 64 bits.
+
+Tolerances, elementwise, from the roundings that the kernels make (u: half a step of a type, 2^-8 bf16,
+2^-11 fp16, 2^-24 fp32):
+  * a logit is a sum of D products in fp32: D 2^-24 sum |x w| at most, for split fp32 operands 2^-21
+    sum |x w| more (the dropped lo lo and the two planes' own roundings); an exponent y in units of log 2 is
+    rounded to 2^-24 |y|; call the sum of these E (absolute, so it is relative in p);
+  * a sum of V exponentials: (V / 64 + 64) 2^-24 relative (64 lanes at least, each adds V / 64 of them), the
+    exponential itself 2^-22;
+  * a share is 2^(t - log2 sum 2^t) of t = teacher / T in units of log 2: t and the logarithm are each rounded to
+    2^-24 |t| (relative in the share, times log 2), and the exponential and the sum to 2^-22 each:
+    2^-22 (4 + |teacher / T|) covers both directions;
+  * G = p - share - eps / V is rounded to the operands' type once (fp32: two planes, 2^-22; fp16 also
+    2^-38 absolutely), then summed in fp32 over V (dx) or N (dw, db) terms;
+  * a result is rounded to its type once.
+"""
+import math
+
+import pytest
+import torch
+
+from determined_1_amd.ops import vocab_loss
+from determined_1_amd.ops.vocab_loss import linear_cross_entropy, linear_topk_distill, topk_distill
+
+pytestmark = pytest.mark.gpu
+U = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
+TINY = {torch.bfloat16: 2.0 ** -126, torch.float16: 2.0 ** -24, torch.float32: 2.0 ** -126}
+NAMES = ("dx", "dweight", "dbias")
+
+
+def _definition(z, target, teacher, index, ignore, smooth, heat, reduction, gout):
+    """(loss, G, A): the loss, its derivative by z, and the magnitudes that G is a difference of."""
+    n, v = z.shape
+    q = torch.zeros_like(z)
+    if target is not None:
+        kept = target != ignore
+        q.scatter_(1, target.clamp(0, v - 1)[:, None], 1.0 - smooth)
+        q += smooth / v
+        entropy = torch.zeros(n, dtype=z.dtype, device=z.device)
+    else:
+        t = teacher.double() / heat
+        there = (index >= 0) & (t != -math.inf)
+        kept = there.any(1)
+        t = torch.where(there, t, torch.full_like(t, -math.inf))
+        t[~kept] = 0
+        share = torch.softmax(t, 1) * there
+        q.scatter_add_(1, index.long().clamp(min=0), share)
+        entropy = torch.xlogy(share, share).sum(1)
+    logp = torch.log_softmax(z / heat, 1)
+    rows = (entropy - torch.where(q > 0, q * logp, torch.zeros_like(q)).sum(1)) * heat * heat
+    rows = torch.where(kept, rows, torch.zeros_like(rows))
+    each = kept.double() / (kept.sum().clamp(min=1) if reduction == "mean" else 1)
+    up = (each * gout.double() * heat)[:, None]
+    loss = rows if reduction == "none" else (rows * each).sum()
+    zero = torch.zeros_like(z)  # an ignored row's p may be anything
+    return loss, torch.where(kept[:, None], up * (logp.exp() - q), zero), torch.where(kept[:, None], up.abs() * (logp.exp() + q), zero)
+
+
+def _near(got, ref, bound, name):
+    bound = bound + 1e-300
+    off = (got.double() - ref).abs()
+    assert got.shape == ref.shape, name
+    assert not got.isnan().any(), name
+    worst = (off / bound).max().item() if off.numel() else 0.0
+    assert worst <= 1.0, f"{name}: {worst:.2f} times its bound, off by {off.max().item():.3g}"
+
+
+def _sum_error(v):
+    return (v / 64 + 64) * 2.0 ** -24 + 2.0 ** -22
+
+
+def _share_error(teacher, heat):
+    t = (teacher.double().abs() / heat)
+    return 2.0 ** -22 * (4 + torch.where(torch.isfinite(t), t, torch.zeros_like(t)).amax(1))
+
+
+def _run_head(x, w, b, target=None, teacher=None, index=None, ignore=-100, smooth=0.0, heat=1.0, reduction="mean", gout=None):
+    leaves = [t.detach().requires_grad_(True) for t in (x, w, b) if t is not None]
+    lb = leaves[2] if b is not None else None
+    if target is not None:
+        loss = linear_cross_entropy(leaves[0], leaves[1], target, lb, ignore_index=ignore, label_smoothing=smooth, reduction=reduction)
+    else:
+        loss = linear_topk_distill(leaves[0], leaves[1], teacher, index, lb, temperature=heat, reduction=reduction)
+    gout = torch.ones_like(loss) if gout is None else gout
+    return loss.detach(), torch.autograd.grad(loss, leaves, gout), gout
+
+
+def _check_head(x, w, b, **kw):
+    dt = x.dtype
+    loss, grads, gout = _run_head(x, w, b, **kw)
+    args = dict(target=None, teacher=None, index=None, ignore=-100, smooth=0.0, heat=1.0, reduction="mean")
+    args.update({k: v for k, v in kw.items() if k != "gout"})
+    n, d, v = x.shape[0], x.shape[1], w.shape[0]
+    args["target"] = None if args["target"] is None else args["target"].long()
+    x64, w64 = x.double(), w.double()
+    z = x64 @ w64.t()
+    size = x64.abs() @ w64.abs().t()
+    if b is not None:
+        z = z + b.double()
+        size = size + b.double().abs()
+    ref, G, A = _definition(z, gout=gout, **args)
+    heat = args["heat"]
+    product = d * 2.0 ** -24 + (2.0 ** -21 if dt == torch.float32 else 0.0)
+    E = (2 * product * size.amax(1) + 3 * 2.0 ** -24 * (z / heat).abs().amax(1) * 1.5) / heat + _sum_error(v)  # [n]
+    E = torch.where(torch.isfinite(E), E, torch.zeros_like(E))
+    if args["teacher"] is not None:
+        E = E + _share_error(args["teacher"], heat)
+    row_bound = heat * heat * (2 * E + 2.0 ** -22 * (1 + (z / heat).abs().amax(1)))
+    row_bound = torch.where(torch.isfinite(row_bound), row_bound, torch.zeros_like(row_bound))
+    bound = row_bound + 2.0 ** -22 * ref.abs() if args["reduction"] == "none" else (
+        row_bound.mean() if args["reduction"] == "mean" else row_bound.sum()) + 2.0 ** -22 * ref.abs()
+    _near(loss, ref, bound, "loss")
+    u_g = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -22}[dt]
+    step = 0.0 if dt == torch.bfloat16 else 2.0 ** -38 * (gout.abs().max().item() * heat)
+    err = A * (u_g + E)[:, None] + step if A.numel() else A
+    err = err * (A.sum(1, keepdim=True) > 0)
+    split = 2.0 ** -21 if dt == torch.float32 else 0.0  # the two planes of w or x, and the lo lo
+    bounds = (err @ w64.abs() + (v * 2.0 ** -24 + split) * (A @ w64.abs()), err.t() @ x64.abs() + (n * 2.0 ** -24 + split) * (A.t() @ x64.abs()),
+              err.sum(0) + n * 2.0 ** -24 * A.sum(0))
+    refs = (G @ w64, G.t() @ x64, G.sum(0))
+    for name, got, r, e in zip(NAMES, grads, refs, bounds):
+        # e is first order; a result's own rounding comes on top, or half its smallest step
+        _near(got, r, 1.01 * e + U[got.dtype] * r.abs() * 1.01 + TINY[got.dtype], name)
+    return loss, grads
+
+
+def _tensors(gpu, n, d, v, dt, bias=True, seed=0):
+    g = torch.Generator(device=gpu).manual_seed(seed * 7919 + n * 31 + d * 7 + v)
+
+    def randn(*s, std=1.0):
+        return torch.randn(*s, generator=g, device=gpu).mul_(std)
+
+    return randn(n, d).to(dt), randn(v, d, std=1.5 / d ** 0.5).to(dt), randn(v, std=0.3).to(dt) if bias else None, g
+
+
+def _lists(gpu, g, n, v, k, dt=torch.float32):
+    first = torch.randint(0, v, (n, 1), generator=g, device=gpu)
+    step = torch.randint(1, v // k + 1, (n, 1), generator=g, device=gpu)
+    return torch.randn(n, k, generator=g, device=gpu).mul_(3).to(dt), (first + step * torch.arange(k, device=gpu)) % v
+
+
+SIZES = [(1, 64, 1000), (1, 1, 1), (3, 8, 5), (2, 200, 257), (64, 72, 256), (65, 100, 511), (255, 64, 2049), (257, 33, 300), (300, 850, 1003),
+         (1000, 128, 777), (513, 1111, 258), (40, 768, 30522)]
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("n,d,v", SIZES)
+def test_cross_entropy(gpu, n, d, v, dt):
+    x, w, b, g = _tensors(gpu, n, d, v, dt)
+    t = torch.randint(0, v, (n,), generator=g, device=gpu)
+    _check_head(x, w, b, target=t, gout=torch.tensor(16.0, device=gpu))
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("keep", [0.15, 0.7])
+def test_cross_entropy_masked_and_smoothed(gpu, dt, reduction, keep):
+    n, d, v = 700, 136, 1500
+    x, w, b, g = _tensors(gpu, n, d, v, dt)
+    t = torch.randint(0, v, (n,), generator=g, device=gpu).int()
+    t[torch.rand(n, generator=g, device=gpu) > keep] = 7  # a word of the vocabulary, ignored
+    gout = torch.randn(n, generator=g, device=gpu) if reduction == "none" else torch.tensor(-3.0, device=gpu)
+    _, grads = _check_head(x, w, b, target=t, ignore=7, smooth=0.1, reduction=reduction, gout=gout)
+    assert torch.equal(grads[0][t == 7], torch.zeros_like(grads[0][t == 7]))
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("n,d,v,k", [(1, 64, 1000, 1), (5, 24, 40, 40), (300, 128, 2050, 20), (130, 850, 999, 64), (70, 96, 5000, 130)])
+def test_distill_head(gpu, n, d, v, k, dt):
+    x, w, b, g = _tensors(gpu, n, d, v, dt)
+    teacher, index = _lists(gpu, g, n, v, k, dt)
+    gone = torch.rand(n, k, generator=g, device=gpu) < 0.3
+    index = torch.where(gone, torch.full_like(index, -1), index)
+    teacher[torch.rand(n, k, generator=g, device=gpu) < 0.1] = -math.inf
+    if n > 2:
+        index[1] = -1
+        teacher[2] = -math.inf
+    for heat, reduction in ((1.0, "mean"), (2.5, "none")):
+        gout = torch.rand(n, generator=g, device=gpu) if reduction == "none" else None
+        _check_head(x, w, b, teacher=teacher, index=index, heat=heat, reduction=reduction, gout=gout)
+
+
+def _check_logits(z, teacher, index, heat=1.0, reduction="mean", gout=None):
+    leaf = z.detach().requires_grad_(True)
+    loss = topk_distill(leaf, teacher, index, temperature=heat, reduction=reduction)
+    gout = torch.ones_like(loss) if gout is None else gout
+    (dz,) = torch.autograd.grad(loss, leaf, gout)
+    loss = loss.detach()
+    v = z.shape[1]
+    z64 = z.double()
+    ref, G, A = _definition(z64, None, teacher, index.long(), -100, 0.0, heat, reduction, gout)
+    top = torch.where(torch.isfinite(z64), z64.abs(), torch.zeros_like(z64)).amax(1) / heat
+    E = 3 * 2.0 ** -24 * 1.5 * top + _sum_error(v)
+    rows = heat * heat * (2 * E + 2.0 ** -22 * (1 + top) + _share_error(teacher, heat))
+    bound = rows + 2.0 ** -22 * ref.abs() if reduction == "none" else (rows.mean() if reduction == "mean" else rows.sum()) + 2.0 ** -22 * ref.abs()
+    _near(loss, ref, bound, "loss")
+    _near(dz, G, A * (E + _share_error(teacher, heat))[:, None] * 1.01 + 1.01 * U[z.dtype] * G.abs() + TINY[z.dtype], "dlogits")
+    return dz
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("n,v,k", [(1, 1, 1), (1, 5, 5), (3, 1000, 16), (8, 32000, 16), (1, 128000, 64), (700, 333, 100), (2100, 1021, 7), (33, 50021, 300)])
+def test_distill_logits(gpu, n, v, k, dt):
+    g = torch.Generator(device=gpu).manual_seed(n + v)
+    z = torch.randn(n, v, generator=g, device=gpu).mul_(2).to(dt)
+    teacher, index = _lists(gpu, g, n, v, k, dt)
+    index = torch.where(torch.rand(n, k, generator=g, device=gpu) < 0.3, torch.full_like(index, -1), index)
+    for heat, reduction in ((1.0, "mean"), (3.0, "none"), (2.0, "sum")):
+        gout = torch.rand(n, generator=g, device=gpu) if reduction == "none" else torch.tensor(2.0, device=gpu)
+        _check_logits(z, teacher, index, heat, reduction, gout)
+
+
+def test_distill_logits_of_masked_words_rows_and_doubles(gpu):
+    g = torch.Generator(device=gpu).manual_seed(5)
+    z = torch.randn(9, 4099, generator=g, device=gpu)
+    teacher, index = _lists(gpu, g, 9, 4099, 6)
+    index[0] = 4  # one word six times
+    index[1, 3:] = index[1, :3]
+    index[2] = -1
+    teacher[3] = -math.inf
+    z[:, 4000:] = -math.inf  # a padded vocabulary
+    index = torch.where(index >= 4000, index - 4000 + 5, index)
+    z[4, 100:200] = torch.finfo(torch.float32).min
+    z[2] = math.nan  # rows without a list may hold anything
+    z[3] = math.inf
+    dz = _check_logits(z, teacher, index.int(), 2.0)
+    assert torch.equal(dz[2:4], torch.zeros_like(dz[2:4])) and torch.equal(dz[:, 4000:], torch.zeros_like(dz[:, 4000:]))
+    # in a head, a word six times and one of no weight
+    x, w, b, g = _tensors(gpu, 9, 40, 4099, torch.float32)
+    _check_head(x, w, b, teacher=teacher, index=index.int(), heat=2.0)
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+def test_masked_words_and_ignored_rows_of_a_head(gpu, dt):
+    x, w, b, g = _tensors(gpu, 300, 64, 700, dt)
+    b[600:] = -math.inf  # words that cannot be chosen: a whole tile of them, and a part of one
+    b[256:512] = -math.inf
+    t = torch.randint(0, 250, (300,), generator=g, device=gpu)
+    t[::3] = -100
+    x[::3] = math.nan
+    loss, grads, _ = _run_head(x, w, b, target=t)
+    x0 = torch.where(x.isnan(), torch.zeros_like(x), x)
+    ref, ref_grads, _ = _run_head(x0, w, b, target=t)
+    assert torch.isfinite(loss) and torch.equal(loss, ref)
+    assert all(torch.equal(a, c) for a, c in zip(grads, ref_grads))
+    keep = torch.ones(700, dtype=torch.bool, device=gpu)
+    keep[600:] = keep[256:512] = False
+    short, short_grads = _check_head(x0, w[keep].contiguous(), b[keep].contiguous(), target=t)
+    assert abs(short.item() - loss.item()) <= 2.0 ** -16 * short.item()
+    assert torch.equal(grads[1][~keep], torch.zeros_like(grads[1][~keep]))
+
+
+def test_nothing_kept(gpu):
+    x, w, b, g = _tensors(gpu, 70, 64, 300, torch.bfloat16)
+    loss, grads, _ = _run_head(x, w, b, target=torch.full((70,), -100, device=gpu))
+    assert loss.item() == 0.0 and all(torch.equal(a, torch.zeros_like(a)) for a in grads)
+    teacher, index = _lists(gpu, g, 70, 300, 4)
+    loss, grads, _ = _run_head(x, w, b, teacher=teacher, index=index * 0 - 1, reduction="none")
+    assert torch.equal(loss, torch.zeros_like(loss)) and all(torch.equal(a, torch.zeros_like(a)) for a in grads)
+    z = torch.randn(70, 300, device=gpu, requires_grad=True)
+    topk_distill(z, teacher, index * 0 - 1).backward()
+    assert torch.equal(z.grad, torch.zeros_like(z))
+
+
+def test_words_outside_the_vocabulary_are_nan(gpu):
+    x, w, b, g = _tensors(gpu, 70, 64, 300, torch.bfloat16)
+    t = torch.randint(0, 300, (70,), generator=g, device=gpu)
+    t[3], t[5], t[6] = 300, -1, 2 ** 40
+    loss, grads, _ = _run_head(x, w, None, target=t, reduction="none")
+    bad = torch.zeros(70, dtype=torch.bool, device=gpu)
+    bad[3] = bad[5] = bad[6] = True
+    assert torch.equal(loss.isnan(), bad) and torch.equal(grads[0].isnan().any(1), bad) and grads[1].isnan().all()
+    teacher, index = _lists(gpu, g, 70, 300, 4)
+    index[3, 2], index[5, 0], index[6, 1] = 300, 2 ** 40, 2 ** 31 - 1
+    loss, grads, _ = _run_head(x, w, None, teacher=teacher, index=index, reduction="none")
+    assert torch.equal(loss.isnan(), bad) and torch.equal(grads[0].isnan().any(1), bad)
+    z = torch.randn(70, 300, device=gpu, requires_grad=True)
+    topk_distill(z, teacher, index, reduction="none").sum().backward()
+    assert torch.equal(z.grad.isnan().all(1), bad) and not z.grad[~bad].isnan().any()
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+def test_strides_and_offsets(gpu, dt):
+    n, d, v = 90, 128, 600
+    x, w, b, g = _tensors(gpu, n, d, v, dt)
+    t = torch.randint(0, v, (n,), generator=g, device=gpu)
+    loss, grads = _check_head(x, w, b, target=t)
+
+    def same(x2, w2, t2, b2):
+        assert torch.equal(x2, x) and torch.equal(w2, w)
+        l2, g2, _ = _run_head(x2, w2, b2, target=t2)
+        torch.testing.assert_close(l2, loss, rtol=2.0 ** -20, atol=0)
+        for a, c in zip(g2, grads):
+            torch.testing.assert_close(a, c, rtol=4 * U[dt] + 2.0 ** -18, atol=4 * U[dt] * c.abs().max().item())
+
+    same(x.t().contiguous().t(), w.t().contiguous().t(), t, b)          # columns first
+    wide = torch.zeros(v, d + 5, dtype=dt, device=gpu)
+    wide[:, 3:3 + d] = w                                               # odd rows, odd start
+    tall = torch.zeros(2 * n, d + 1, dtype=dt, device=gpu)
+    tall[::2, 1:] = x
+    same(tall[::2, 1:], wide[:, 3:3 + d], torch.stack([t, t], 1)[:, 0], torch.stack([b, b], 1)[:, 1])
+    same(x.expand(1, n, d)[0], w, t, b)
+    row = x[:1].expand(40, d)                                          # a broadcast row
+    lead, _, _ = _run_head(row, w, b, target=t[:40], reduction="none")
+    one, _, _ = _run_head(x[:1].repeat(40, 1), w, b, target=t[:40], reduction="none")
+    assert torch.equal(lead, one)
+    z = torch.randn(2, n, 2 * v + 1, generator=g, device=gpu).to(dt)
+    teacher, index = _lists(gpu, g, n, v, 8)
+    _check_logits(z[1, :, 1:v + 1], teacher.t().contiguous().t(), index.t().contiguous().t())
+    _check_logits(z[0].t().contiguous().t()[:, ::2][:, :v], teacher, index)
+
+
+def test_leading_shapes_and_partial_gradients(gpu):
+    x, w, b, g = _tensors(gpu, 24, 64, 300, torch.bfloat16)
+    t = torch.randint(0, 300, (24,), generator=g, device=gpu)
+    loss, grads, gout = _run_head(x, w, b, target=t, reduction="none")
+    xs = x.view(2, 3, 4, 64).detach().requires_grad_(True)
+    got = linear_cross_entropy(xs, w, t.view(2, 3, 4), b, reduction="none")
+    assert got.shape == (2, 3, 4) and torch.equal(got.view(-1), loss) and not w.requires_grad
+    (dx,) = torch.autograd.grad(got, xs, torch.ones_like(got))
+    assert torch.equal(dx.view(24, 64), grads[0])
+    wl, bl = w.detach().requires_grad_(True), b.detach().requires_grad_(True)
+    (dw,) = torch.autograd.grad(linear_cross_entropy(x, wl, t, b, reduction="none").sum(), wl)
+    (db,) = torch.autograd.grad(linear_cross_entropy(x, w, t, bl, reduction="none").sum(), bl)
+    assert torch.equal(dw, grads[1]) and torch.equal(db, grads[2])
+    # a bias in fp32 beside half operands
+    bf = b.float().requires_grad_(True)
+    (db,) = torch.autograd.grad(linear_cross_entropy(x, w, t, bf, reduction="sum"), bf)
+    assert db.dtype == torch.float32
+    torch.testing.assert_close(db, grads[2].float(), rtol=2.0 ** -7, atol=2.0 ** -8)
+    with torch.no_grad():
+        assert torch.equal(linear_cross_entropy(x[7], w, t[7], b, reduction="none"), linear_cross_entropy(x[7:8], w, t[7:8], b, reduction="none")[0])
+
+
+def test_gradients_against_differences(gpu):
+    n, d, v = 50, 96, 400
+    x, w, b, g = _tensors(gpu, n, d, v, torch.float32)
+    t = torch.randint(0, v, (n,), generator=g, device=gpu)
+    t[::4] = -100
+    teacher, index = _lists(gpu, g, n, v, 10)
+    for kw in (dict(target=t, smooth=0.1), dict(teacher=teacher, index=index, heat=2.0)):
+        loss, grads, _ = _run_head(x, w, b, **kw)
+        for i in range(3):
+            step = torch.randn(grads[i].shape, generator=g, device=gpu)
+            h = 2.0 ** -7 / step.norm().item()  # |h step| = 2^-7
+            ends = []
+            for s in (h, -h):
+                args = [x, w, b]
+                args[i] = args[i] + s * step
+                ends.append(_run_head(*args, **kw)[0].item())
+            slope = (ends[0] - ends[1]) / (2 * h)
+            # the losses' own error over 2 h, and the third derivative's term (|z'''| <= |x|^3 h^2 step^3 / 6 scale)
+            tol = (2.0 ** -19 * abs(loss.item())) / h + 0.01 * (grads[i].abs() * step.abs()).sum().item()
+            assert abs(slope - (grads[i] * step).sum().item()) <= tol
+
+
+def test_same_bits_again_and_on_another_stream(gpu):
+    x, w, b, g = _tensors(gpu, 500, 256, 3000, torch.bfloat16)
+    t = torch.randint(0, 3000, (500,), generator=g, device=gpu)
+    first = _run_head(x, w, b, target=t)
+    teacher, index = _lists(gpu, g, 500, 3000, 12)
+    z = torch.randn(500, 3000, generator=g, device=gpu)
+
+    def both():
+        leaf = z.detach().requires_grad_(True)
+        loss = topk_distill(leaf, teacher, index, temperature=2.0)
+        return loss.detach(), torch.autograd.grad(loss, leaf)[0]
+
+    first_d = both()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(gpu) for _ in range(2)]
+    got = []
+    for s in streams:  # two calls at one time
+        with torch.cuda.stream(s):
+            got.append((_run_head(x, w, b, target=t), both()))
+    torch.cuda.synchronize()
+    for (loss, grads, _), d in got:
+        assert torch.equal(loss, first[0]) and all(torch.equal(a, c) for a, c in zip(grads, first[1]))
+        assert all(torch.equal(a, c) for a, c in zip(d, first_d))
+
+
+def test_captured_step_replays(gpu):
+    x, w, b, g = _tensors(gpu, 200, 64, 1000, torch.bfloat16)
+    t = torch.randint(0, 1000, (200,), generator=g, device=gpu)
+    teacher, index = _lists(gpu, g, 200, 1000, 5)
+
+    def step(xl, wl, bl):
+        loss = linear_cross_entropy(xl, wl, t, bl, label_smoothing=0.1) + linear_topk_distill(xl, wl, teacher, index, bl, temperature=2.0)
+        return (loss,) + torch.autograd.grad(loss, (xl, wl, bl))
+
+    def fresh():
+        return [a.detach().clone().requires_grad_(True) for a in (x, w, b)]
+
+    graphs = []
+    for _ in range(2):  # two graphs with memory pools of their own
+        static = fresh()
+        s = torch.cuda.Stream(gpu)
+        s.wait_stream(torch.cuda.current_stream(gpu))
+        with torch.cuda.stream(s):
+            step(*static)
+        torch.cuda.current_stream(gpu).wait_stream(s)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step(*static)
+        graphs.append((graph, static, out))
+    for i in range(4):  # new inputs, more and fewer kept rows, eager work between the replays
+        x.copy_(torch.randn(200, 64, generator=g, device=gpu))
+        t.copy_(torch.randint(0, 1000, (200,), generator=g, device=gpu))
+        t[: 60 * i] = -100
+        index[i] = -1
+        ref = step(*fresh())
+        torch.cuda.synchronize()
+        for graph, static, out in graphs:
+            with torch.no_grad():
+                static[0].copy_(x)
+            graph.replay()
+        torch.cuda.synchronize()
+        for _, _, out in graphs:
+            assert all(torch.equal(a, c) for a, c in zip(out, ref))
+
+
+def test_a_students_training_steps(gpu):
+    """A teacher's top logits, a student with a tied head trained on targets and lists: the gradients of two steps, against
+    64 bits on the same parameters."""
+    g = torch.Generator(device=gpu).manual_seed(3)
+    v, d, n, k, heat = 1200, 96, 160, 16, 2.0
+    teacher_w = torch.randn(v, 64, generator=g, device=gpu)
+    emb = torch.nn.Parameter(torch.randn(v, d, generator=g, device=gpu).mul_(0.1))
+    body = torch.nn.Linear(d, d, device=gpu)
+    opt = torch.optim.SGD([emb, *body.parameters()], lr=0.5)
+    for step in range(2):
+        ids = torch.randint(0, v, (n,), generator=g, device=gpu)
+        target = torch.randint(0, v, (n,), generator=g, device=gpu)
+        target[::5] = -100
+        top = (torch.randn(n, 64, generator=g, device=gpu) @ teacher_w.t()).topk(k, dim=1)
+        opt.zero_grad()
+        h = torch.tanh(body(emb[ids]))
+        loss = 0.5 * linear_cross_entropy(h, emb, target) + 0.5 * linear_topk_distill(h, emb, top.values, top.indices, temperature=heat)
+        loss.backward()
+        e64 = emb.detach().double().requires_grad_(True)
+        h64 = torch.tanh(torch.nn.functional.linear(e64[ids], body.weight.detach().double(), body.bias.detach().double()))
+        z = h64 @ e64.t()
+        q = torch.zeros_like(z).scatter_(1, top.indices, torch.softmax(top.values.double() / heat, 1))
+        ref = 0.5 * torch.nn.functional.cross_entropy(z, target) + 0.5 * heat * heat * torch.nn.functional.kl_div(
+            torch.log_softmax(z / heat, 1), q, reduction="batchmean")
+        ref.backward()
+        # relative to the largest entry: products of 96 and 160 terms, fp32 roundings of a tanh, its backward and two products
+        assert abs(loss.item() - ref.item()) <= 2.0 ** -17 * abs(ref.item())
+        assert (emb.grad.double() - e64.grad).abs().max().item() <= 2.0 ** -14 * e64.grad.abs().max().item()
+        opt.step()
+
+
+def test_refusals_on_the_gpu(gpu):
+    x = torch.zeros(4, 8, device=gpu)
+    t = torch.zeros(4, dtype=torch.long, device=gpu)
+    with pytest.raises(TypeError):
+        linear_cross_entropy(x.double(), x.double(), t)
+    with pytest.raises(ValueError):
+        linear_cross_entropy(x, x, t.cpu())
+    with pytest.raises(ValueError):
+        topk_distill(x, x[:, :2], t[:, None].expand(4, 2).cpu())
+    leaf = x.clone().requires_grad_(True)
+    (grad,) = torch.autograd.grad(linear_cross_entropy(leaf, x, t), leaf, create_graph=True)
+    with pytest.raises(RuntimeError):
+        grad.sum().backward()
+
+
+def test_autocast(gpu):
+    x, w, b, g = _tensors(gpu, 100, 64, 500, torch.float32)
+    t = torch.randint(0, 500, (100,), generator=g, device=gpu)
+    wl = w.requires_grad_(True)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        loss = linear_cross_entropy(x, wl, t, b)
+    loss.backward()
+    ref, grads, _ = _run_head(x.bfloat16(), w.bfloat16(), b.bfloat16(), target=t)
+    assert torch.equal(loss.detach(), ref) and wl.grad.dtype == torch.float32 and torch.equal(wl.grad, grads[1].float())
+
+
+def test_the_kernels_refuse_what_they_do_not_cover(gpu):
+    """The C entries' own checks (before any launch)."""
+    import ctypes
+
+    lib = vocab_loss._lib.get_lib()
+    p = vocab_loss._HeadParams()
+    assert lib.det_vocab_head_ws_bytes(ctypes.byref(p), 0) == -1 and lib.det_vocab_head_forward(None, None) != 0
+    assert lib.det_vocab_head_forward(None, ctypes.byref(p)) != 0 and lib.det_vocab_head_backward(None, ctypes.byref(p)) != 0
+    q = vocab_loss._LogitParams()
+    assert lib.det_vocab_logits_ws_bytes(ctypes.byref(q)) == -1 and lib.det_vocab_logits_forward(None, ctypes.byref(q)) != 0
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32])
+def test_every_logit_at_the_lowest_value_is_a_uniform_row(gpu, dt):
+    low = torch.finfo(dt).min
+    z = torch.full((2, 5000), low, dtype=dt, device=gpu)
+    z[1, 7] = 1.0
+    teacher, index = torch.zeros(2, 1, device=gpu), torch.tensor([[11], [7]], device=gpu)
+    leaf = z.requires_grad_(True)
+    loss = topk_distill(leaf, teacher, index, reduction="none")
+    loss.sum().backward()
+    assert abs(loss[0].item() - math.log(5000)) < 2.0 ** -18 * 10 and loss[1].item() == 0.0
+    # log2 5000 = 12.3 is held to 2^-21, which is 2^-21 log 2 relative in p, and the exponential to 2^-22: 2^-20 together
+    torch.testing.assert_close(leaf.grad[0, :11].double(), torch.full((11,), 1 / 5000, dtype=torch.float64, device=gpu),
+                               rtol=2.0 ** -20 + U[dt], atol=TINY[dt])
+    assert leaf.grad[1].abs().max().item() == 0.0
+    if dt != torch.float16:  # (a head's logit of fp16's lowest value is an ordinary one)
+        x, w = torch.zeros(1, 64, dtype=dt, device=gpu), torch.zeros(5000, 64, dtype=dt, device=gpu)
+        b = torch.full((5000,), low, dtype=dt, device=gpu).requires_grad_(True)
+        loss = linear_cross_entropy(x, w, torch.tensor([11], device=gpu), b)
+        loss.backward()
+        assert abs(loss.item() - math.log(5000)) < 2.0 ** -18 * 10
+        torch.testing.assert_close(b.grad[:11].float(), torch.full((11,), 1 / 5000, device=gpu), rtol=2.0 ** -7, atol=0)
