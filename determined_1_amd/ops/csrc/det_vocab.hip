@@ -283,6 +283,16 @@ __device__ __forceinline__ void wait_vmcnt() {  // all but the wave's last N loa
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
+// a barrier that leaves fetches in flight and that nothing is scheduled across
+__device__ __forceinline__ void phase_barrier() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+__device__ __forceinline__ void wait_lgkm0() { __builtin_amdgcn_s_waitcnt(0xC07F); }
+
 __device__ __forceinline__ int xcd_remap(int bid, int nwg) {  // consecutive tiles on one XCD
   const int q = nwg >> 3, r = nwg & 7, x = bid & 7;
   return (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (bid >> 3);
@@ -382,9 +392,11 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(GemmArgs g) {
       __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(dst + s * 8192), 16, ok ? off : kOOB, 0, 0, 0);
     }
   };
-  auto stage = [&](int t) {
+  auto stage_a = [&](int t) {
     stage1(g.A, ACOL, m0, 0, t);
     stage1(g.A, ACOL, m0, 1, t);
+  };
+  auto stage_b = [&](int t) {
     stage1(g.B, BCOL, n0, 2, t);
     stage1(g.B, BCOL, n0, 3, t);
   };
@@ -415,6 +427,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(GemmArgs g) {
                         : *reinterpret_cast<const s16x8*>(base + s * 8192 + swz64((wc & 1) * 64 + j * 16 + fr, fch));
   };
   auto mfma = [&](int i0, int j0) {
+    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int s = 0; s < (PL == 1 ? 2 : 3); ++s)
 #pragma unroll
@@ -422,22 +435,53 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(GemmArgs g) {
 #pragma unroll
         for (int j = j0; j < j0 + 2; ++j)  // one plane: k halves 0, 1; two: hi hi, hi lo, lo hi
           acc[i][j] = mfma16<F16>(af[i][PL == 1 ? s : s >> 1], bf[j][PL == 1 ? s : s & 1], acc[i][j]);
+    __builtin_amdgcn_s_setprio(0);
   };
 
-  if (nk > 0) stage(0);
-  for (int t = 0; t < nk; ++t) {
-    wait_vmcnt<0>();  // this wave's pieces of stage t (a barrier alone does not wait for them)
-    __syncthreads();  // ... and every other wave's; stage t - 1 is read
-    if (t + 1 < nk) stage(t + 1);
-    read_a(t, 0);
-    read_a(t, 4);
-    read_b(t, 0);
-    read_b(t, 2);
-    mfma(0, 0);
-    mfma(0, 2);
-    mfma(4, 2);
-    mfma(4, 0);
+  // Four phases a stage, a quadrant of the wave's tile each: reads and fetches, barrier, matrix
+  // instructions, barrier.  The lower four waves run one barrier late, so on every SIMD one wave
+  // multiplies while the other reads and fetches.  A(t + 1) is fetched in the first phase of stage t, B(t + 2)
+  // in the last (B(t) is in registers since the second), where everything older has to have landed.
+  if (nk > 0) {
+    stage_a(0);
+    stage_b(0);
+    if (nk > 1) {
+      stage_b(1);
+      wait_vmcnt<4>();
+    } else {
+      wait_vmcnt<0>();
+    }
   }
+  phase_barrier();
+  if (wr == 1) phase_barrier();
+  for (int t = 0; t < nk; ++t) {
+    read_a(t, 0);
+    read_b(t, 0);
+    if (t + 1 < nk) stage_a(t + 1);
+    phase_barrier();
+    wait_lgkm0();
+    mfma(0, 0);
+    phase_barrier();
+    read_a(t, 4);
+    read_b(t, 2);
+    phase_barrier();
+    wait_lgkm0();
+    mfma(0, 2);
+    phase_barrier();
+    phase_barrier();
+    mfma(4, 2);
+    phase_barrier();
+    if (t + 2 < nk) {
+      stage_b(t + 2);
+      wait_vmcnt<4>();
+    } else {
+      wait_vmcnt<0>();
+    }
+    phase_barrier();
+    mfma(4, 0);
+    phase_barrier();
+  }
+  if (wr == 0) phase_barrier();
   __syncthreads();
 
   // acc[i][j][r]: row wr * 128 + i * 16 + fch * 4 + r, column wc * 64 + j * 16 + fr
