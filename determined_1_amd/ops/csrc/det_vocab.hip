@@ -125,7 +125,8 @@ struct RowArgs {
   const void* teacher;  // [N, K] logits (-inf: no entry)
   uint8_t* flag;        // [N], distillation
   int* info;
-  int* list;
+  int* list;   // [N] the kept rows, in order
+  int* pos;    // [N] a row's place in the list, or -1
   int64_t ignore, index_ld, teacher_ld;
   int N, K, wide, teacher_dt;
 };
@@ -154,7 +155,9 @@ __global__ void __launch_bounds__(1024) rows_kernel(RowArgs a) {
     __syncthreads();
     int before = base_n;
     for (int i = 0; i < w; ++i) before += wave_n[i];
-    if (keep) a.list[before + __popcll(votes & ((uint64_t(1) << lane) - 1))] = n;
+    const int at = before + __popcll(votes & ((uint64_t(1) << lane) - 1));
+    if (keep) a.list[at] = n;
+    if (n < a.N) a.pos[n] = keep ? at : -1;
     __syncthreads();
     if (tid == 0)
       for (int i = 0; i < 16; ++i) base_n += wave_n[i];
@@ -244,7 +247,7 @@ struct GemmArgs {
   const int* m_dyn;  // rows of A that count (null: M)
   const int* k_dyn;  // length of the sum (null: K)
   int M, N, K;
-  int splits, k_per_split;  // kPartial: blocks of one tile, each over k_per_split (a multiple of 64) of K
+  int chunk;                // kPartial: the longest K of the pass, which the splits are made for
   const int* info;          // scales of fp32 operands
   // kStats, kGrad: z = acc / scales + bias, c = log2(e) / T
   const void* bias;
@@ -261,20 +264,29 @@ struct GemmArgs {
   u16* G;              // [M][ldg]
   int64_t g_plane;
   int ldg;
-  // kPartial: out[split][M][ldo] fp32, added to what is there if `add`
+  // kPartial: out[split][M][ldo] fp32 (ldo % 4 == 0), added to what is there if `add`
   float* out32;
-  int64_t ldo, split_stride;
+  int64_t ldo;
   int add;
-  // kOut: out[m][n] of type out_dt, times *alpha and the scale of B
+  // kOut: out[m][n] of the operands' type (fp32 if split), times *alpha and the scale of B
   void* out;
-  int out_dt;
   const float* alpha;
 };
 
+// G w with few tiles: the sum over a chunk's words is cut until a block runs on every CU (one fills a
+// CU), no piece under 512 words.  Returns the length of a piece, a multiple of 64.
+__host__ __device__ inline int split_length(int tiles, int chunk) {
+  int splits = tiles < 256 ? 256 / tiles : 1;
+  const int most = chunk / 512 > 1 ? chunk / 512 : 1;
+  if (splits > most) splits = most;
+  return ((chunk + splits - 1) / splits + 63) / 64 * 64;
+}
+
 constexpr int kTile = 256, kThreads = 512;
 constexpr int kHalf = 16384, kStage = 4 * kHalf;
-constexpr int kLdc = kTile + 16;
-constexpr int kGemmSmem = (2 * kStage > kTile * kLdc * 2) ? 2 * kStage : kTile * kLdc * 2;
+constexpr int kLdc = kTile + 16, kLdc32 = kTile + 4;
+constexpr int kGemmSmem = kTile * kLdc * 2;
+static_assert(kGemmSmem >= 2 * kStage && kGemmSmem >= 128 * kLdc32 * 4, "the epilogues reuse the stages");
 constexpr unsigned kOOB = 0x80000000u;     // past kRange: the load returns zeros
 constexpr unsigned kRange = 0x7FFFFFF0u;
 
@@ -320,6 +332,25 @@ __device__ __forceinline__ f32x4 mfma16(s16x8 a, s16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
+// a wave's part of the tile, rounded to 16 bits, as rows of kLdc; REST leaves what the rounding took in acc
+template <bool F16, bool REST>
+__device__ __forceinline__ void tile_to_lds(f32x4 (&acc)[8][4], unsigned char* smem, int row0, int col0) {
+  typedef __attribute__((ext_vector_type(4))) u16 us4;
+  u16* ct = reinterpret_cast<u16*>(smem);
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      us4 o;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        o[r] = F16 ? f2h(acc[i][j][r]) : f2bf(acc[i][j][r]);
+        if (REST) acc[i][j][r] -= h2f(o[r]);
+      }
+      *reinterpret_cast<us4*>(ct + (row0 + i * 16) * kLdc + col0 + j * 16) = o;
+    }
+}
+
 template <bool F16, int PL, bool ACOL, bool BCOL, int EPI>
 __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(GemmArgs g) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -332,13 +363,20 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(GemmArgs g) {
   const int K = g.k_dyn != nullptr ? *g.k_dyn : g.K;
   const int ntm = (M + kTile - 1) / kTile, ntn = (g.N + kTile - 1) / kTile;
   const int total = ntm * ntn;
-  int split = 0, bid = blockIdx.x;
-  if (EPI == kPartial) {
-    split = bid % g.splits;
-    bid /= g.splits;
+  int split = 0, bid = blockIdx.x, kbeg = 0, kend = K;
+  if constexpr (EPI == kPartial) {
+    if (total == 0) return;
+    const int len = split_length(total, g.chunk), splits = (g.chunk + len - 1) / len;
+    if (bid >= total * splits) return;
+    bid = xcd_remap(bid, total * splits);
+    split = bid / total;  // the tiles of one piece, which share its words, stay together
+    bid -= split * total;
+    kbeg = split * len;
+    kend = kbeg + len < K ? kbeg + len : K;
+  } else {
+    if (bid >= total) return;  // the grid is sized for every row
+    bid = xcd_remap(bid, total);
   }
-  if (bid >= total) return;  // the grid is sized for every row
-  bid = xcd_remap(bid, total);
   // tiles go down eight row tiles before they go on to the next column tile: what runs at one time
   // on an XCD then shares both operands
   const int per = 8 * ntn, band = bid / per, left = ntm - band * 8;
@@ -346,9 +384,6 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(GemmArgs g) {
   const int in = bid - band * per;
   const int mt = band * 8 + in % high, nt = in / high;
   const int m0 = mt * kTile, n0 = nt * kTile;
-  const int kbeg = EPI == kPartial ? split * g.k_per_split : 0;
-  int kend = EPI == kPartial ? kbeg + g.k_per_split : K;
-  if (kend > K) kend = K;
   const int nk = kend > kbeg ? (kend - kbeg + KT - 1) / KT : 0;
 
   // this lane's 16-byte pieces of the four half tiles: "row" operands 16 rows a wave, 4 lanes a row;
@@ -434,7 +469,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(GemmArgs g) {
       for (int i = i0; i < i0 + 4; ++i)
 #pragma unroll
         for (int j = j0; j < j0 + 2; ++j)  // one plane: k halves 0, 1; two: hi hi, hi lo, lo hi
-          acc[i][j] = mfma16<F16>(af[i][PL == 1 ? s : s >> 1], bf[j][PL == 1 ? s : s & 1], acc[i][j]);
+          acc[i][j] = mfma16<F16>(bf[j][PL == 1 ? s : s & 1], af[i][PL == 1 ? s : s >> 1], acc[i][j]);
     __builtin_amdgcn_s_setprio(0);
   };
 
@@ -484,46 +519,57 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(GemmArgs g) {
   if (wr == 0) phase_barrier();
   __syncthreads();
 
-  // acc[i][j][r]: row wr * 128 + i * 16 + fch * 4 + r, column wc * 64 + j * 16 + fr
+  // The tile is transposed in the accumulators (B is the instruction's first operand), so that a lane's
+  // four consecutive values are of one row: acc[i][j][r] is row wr * 128 + i * 16 + fr, column
+  // wc * 64 + j * 16 + fch * 4 + r.  A row's reduction is 16 values in registers and two lane steps.
+  const int row0 = wr * 128 + fr, col0 = wc * 64 + fch * 4;
   if constexpr (EPI == kStats || EPI == kGrad) {
     const float zs = PL == 1 ? 1.f : pow2(-scale_exp(static_cast<uint32_t>(g.info[1]))) * pow2(-scale_exp(static_cast<uint32_t>(g.info[2])));
     const float c = g.c;
-    float bias[4];
-    bool cok[4];
+    f32x4 bias[4];  // -inf past the last word
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int col = n0 + wc * 64 + j * 16 + fr;
-      cok[j] = col < g.N;
-      bias[j] = g.bias != nullptr && cok[j] ? load_any(g.bias, col, g.bias_dt) : 0.f;
-    }
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int col = n0 + col0 + j * 16 + r;
+        bias[j][r] = col >= g.N ? kNegInf : g.bias != nullptr ? load_any(g.bias, col, g.bias_dt) : 0.f;
+      }
     if constexpr (EPI == kStats) {
       float* red = reinterpret_cast<float*>(smem);  // [3][4 column waves][256 rows]
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int i = 0; i < 8; ++i) {
+        float m = kNegInf, s = 0.f, sz = 0.f;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float z[4], m = kNegInf, s = 0.f, sz = 0.f;
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            z[j] = acc[i][j][r] * zs + bias[j];
-            if (cok[j]) {
-              m = fmaxf(m, z[j]);
-              sz = fmaf(z[j], g.inv_v, sz);
-            }
+          for (int r = 0; r < 4; ++r) {
+            acc[i][j][r] = acc[i][j][r] * zs + bias[j][r];
+            m = fmaxf(m, acc[i][j][r]);
           }
-          const float ref = m == kNegInf ? 0.f : m;
+        if (g.part_z != nullptr) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) s += cok[j] ? exp2_((z[j] - ref) * c) : 0.f;
-          join_lanes(m, s, 16, c);
-          if (g.part_z != nullptr)
-            for (int o = 1; o < 16; o <<= 1) sz += __shfl_xor(sz, o, 64);
-          if (fr == 0) {
-            const int row = wr * 128 + i * 16 + fch * 4 + r;
-            red[wc * 256 + row] = m;
-            red[1024 + wc * 256 + row] = s;
-            red[2048 + wc * 256 + row] = sz;
-          }
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sz += n0 + col0 + j * 16 + r < g.N ? acc[i][j][r] * g.inv_v : 0.f;
+          sz += __shfl_xor(sz, 16, 64);
+          sz += __shfl_xor(sz, 32, 64);
         }
+        m = fmaxf(m, __shfl_xor(m, 16, 64));
+        m = fmaxf(m, __shfl_xor(m, 32, 64));
+        const float ref = m == kNegInf ? 0.f : m;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s += exp2_((acc[i][j][r] - ref) * c);
+        s += __shfl_xor(s, 16, 64);
+        s += __shfl_xor(s, 32, 64);
+        if (fch == 0) {
+          const int at = wc * 256 + row0 + i * 16;
+          red[at] = m;
+          red[1024 + at] = s;
+          red[2048 + at] = sz;
+        }
+      }
       __syncthreads();
       if (tid < 256 && m0 + tid < M) {
         float m = red[tid], s = red[1024 + tid], sz = red[2048 + tid];
@@ -537,73 +583,93 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(GemmArgs g) {
         if (g.part_z != nullptr) g.part_z[at] = sz;
       }
     } else {
-      u16* ct = reinterpret_cast<u16*>(smem);
       // G once into the accumulators: both planes have to come from the same bits of it
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int i = 0; i < 8; ++i) {
+        const int row = m0 + row0 + i * 16;
+        const bool ok = row < M;
+        const float top = ok ? g.top[row] : 0.f, l = ok ? g.log_s[row] : 0.f, w = ok ? g.row_w[row] : 0.f;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int row = m0 + wr * 128 + i * 16 + fch * 4 + r;
-          const bool ok = row < M;
-          const float top = ok ? g.top[row] : 0.f, l = ok ? g.log_s[row] : 0.f, w = ok ? g.row_w[row] : 0.f;
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float p = exp2_(fmaf(acc[i][j][r] * zs + bias[j] - top, c, -l));
-            acc[i][j][r] = cok[j] && ok ? w * (p - g.smooth_v) : 0.f;
+          for (int r = 0; r < 4; ++r) {
+            const float p = exp2_(fmaf(acc[i][j][r] * zs + bias[j][r] - top, c, -l));
+            acc[i][j][r] = ok ? w * (p - g.smooth_v) : 0.f;
           }
-        }
+      }
 #pragma unroll
       for (int pl = 0; pl < PL; ++pl) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const u16 o = F16 ? f2h(acc[i][j][r]) : f2bf(acc[i][j][r]);
-              acc[i][j][r] -= F16 ? h2f(o) : 0.f;  // what is left, for the second plane
-              ct[(wr * 128 + i * 16 + fch * 4 + r) * kLdc + wc * 64 + j * 16 + fr] = o;
-            }
+        tile_to_lds<F16, PL == 2>(acc, smem, row0, col0);
         __syncthreads();
+        u16* G = g.G + pl * g.g_plane;
         for (int q = tid; q < kTile * (kTile / 8); q += kThreads) {
           const int row = q >> 5, cc = (q & 31) * 8;
           if (m0 + row < M && n0 + cc < g.ldg)
-            *reinterpret_cast<us8*>(g.G + pl * g.g_plane + static_cast<int64_t>(m0 + row) * g.ldg + n0 + cc) =
-                *reinterpret_cast<const us8*>(ct + row * kLdc + cc);
+            *reinterpret_cast<us8*>(G + static_cast<int64_t>(m0 + row) * g.ldg + n0 + cc) =
+                *reinterpret_cast<const us8*>(reinterpret_cast<const u16*>(smem) + row * kLdc + cc);
         }
         __syncthreads();
       }
     }
   } else if constexpr (EPI == kPartial) {
-    float* out = g.out32 + split * g.split_stride;
+    float* out = g.out32 + split * (M * g.ldo);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < 8; ++i) {
+      const int row = m0 + row0 + i * 16;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int row = m0 + wr * 128 + i * 16 + fch * 4 + r;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int col = n0 + wc * 64 + j * 16 + fr;
-          if (row < M && col < g.N) {
-            float* o = out + row * g.ldo + col;
-            *o = g.add ? *o + acc[i][j][r] : acc[i][j][r];
-          }
+      for (int j = 0; j < 4; ++j) {
+        const int col = n0 + col0 + j * 16;
+        if (row < M && col < g.ldo) {
+          f32x4* o = reinterpret_cast<f32x4*>(out + row * g.ldo + col);
+          f32x4 v = acc[i][j];
+          if (g.add) v += *o;
+          *o = v;
         }
       }
+    }
   } else {
     float alpha = *g.alpha;
     if (PL == 2) alpha *= pow2(-scale_exp(static_cast<uint32_t>(g.info[1])));
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int row = m0 + wr * 128 + i * 16 + fch * 4 + r;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int col = n0 + wc * 64 + j * 16 + fr;
-          if (row < M && col < g.N) store_any(g.out, row * g.ldo + col, g.out_dt, acc[i][j][r] * alpha);
+      for (int j = 0; j < 4; ++j) acc[i][j] *= alpha;
+    if constexpr (PL == 1) {
+      const bool wide = (g.ldo & 7) == 0 && (reinterpret_cast<uintptr_t>(g.out) & 15) == 0;
+      tile_to_lds<F16, false>(acc, smem, row0, col0);
+      __syncthreads();
+      const u16* ct = reinterpret_cast<const u16*>(smem);
+      u16* out = static_cast<u16*>(g.out);
+      if (wide) {
+        for (int q = tid; q < kTile * (kTile / 8); q += kThreads) {
+          const int row = q >> 5, cc = (q & 31) * 8;
+          if (m0 + row < M && n0 + cc < g.N)
+            *reinterpret_cast<us8*>(out + (m0 + row) * g.ldo + n0 + cc) = *reinterpret_cast<const us8*>(ct + row * kLdc + cc);
+        }
+      } else {
+        for (int q = tid; q < kTile * kTile; q += kThreads) {
+          const int row = q >> 8, cc = q & 255;
+          if (m0 + row < M && n0 + cc < g.N) out[(m0 + row) * g.ldo + n0 + cc] = ct[row * kLdc + cc];
         }
       }
+    } else {
+      float* ct = reinterpret_cast<float*>(smem);  // half the rows at a time
+      float* out = static_cast<float*>(g.out);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        if (wr == half)
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) *reinterpret_cast<f32x4*>(ct + (fr + i * 16) * kLdc32 + col0 + j * 16) = acc[i][j];
+        __syncthreads();
+        for (int q = tid; q < 128 * kTile; q += kThreads) {
+          const int row = q >> 8, cc = q & 255;
+          if (m0 + half * 128 + row < M && n0 + cc < g.N) out[(m0 + half * 128 + row) * g.ldo + n0 + cc] = ct[row * kLdc32 + cc];
+        }
+        __syncthreads();
+      }
+    }
   }
 #endif
 }
@@ -870,24 +936,41 @@ __global__ void __launch_bounds__(256) dbias_kernel(const float* part, int split
   store_any(db, at + v, dt, t * *alpha);
 }
 
-// dh: the sum of a kept row's partials, zeros for the others.  pos: binary search in the ordered list
-__global__ void __launch_bounds__(256) dx_kernel(const float* part, int splits, int64_t split_stride, int64_t ldo, const int* info,
-                                                 const int* list, const float* alpha, int planes, void* dx, int dt, int D) {
-  const int n = blockIdx.x;
-  int lo = 0, hi = info[0];
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (list[mid] < n) lo = mid + 1;
-    else hi = mid;
+// dh: the sum of a kept row's partials, zeros for the others
+__global__ void __launch_bounds__(256) dx_kernel(const float* part, int chunk, int64_t ldo, const int* info, const int* pos,
+                                                 const float* alpha, int planes, void* dx, int dt, int D) {
+  const int n = blockIdx.x, count = info[0], at = pos[n];
+  const int tiles = ((count + kTile - 1) / kTile) * ((D + kTile - 1) / kTile);
+  int splits = 0;
+  if (at >= 0) {
+    const int len = split_length(tiles, chunk);
+    splits = (chunk + len - 1) / len;
   }
-  const bool kept = lo < info[0] && list[lo] == n;
   float a = *alpha;
   if (planes == 2) a *= pow2(-scale_exp(static_cast<uint32_t>(info[2])));
-  for (int d = threadIdx.x; d < D; d += 256) {
-    float t = 0.f;
-    if (kept)
-      for (int s = 0; s < splits; ++s) t += part[s * split_stride + lo * ldo + d];
-    store_any(dx, static_cast<int64_t>(n) * D + d, dt, t * a);
+  const int64_t stride = count * ldo, out = static_cast<int64_t>(n) * D;
+  const bool wide = (D & 3) == 0 && (reinterpret_cast<uintptr_t>(dx) & 15) == 0;
+  for (int d = (blockIdx.y * 256 + threadIdx.x) * 4; d < D; d += gridDim.y * 1024) {
+    f32x4 t = f32x4{0.f, 0.f, 0.f, 0.f};
+    const float* p = part + at * ldo + d;
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s) t += *reinterpret_cast<const f32x4*>(p + s * stride);
+    t *= a;
+    if (wide) {
+      if (dt == kF32) {
+        *reinterpret_cast<f32x4*>(static_cast<float*>(dx) + out + d) = t;
+      } else {
+        typedef __attribute__((ext_vector_type(4))) u16 us4;
+        us4 o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = dt == kBF16 ? f2bf(t[e]) : f2h(t[e]);
+        *reinterpret_cast<us4*>(static_cast<u16*>(dx) + out + d) = o;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (d + e < D) store_any(dx, out + d + e, dt, t[e]);
+    }
   }
 }
 
@@ -1071,7 +1154,8 @@ int launch_gemm(hipStream_t st, const GemmArgs& a) {
   const void* fn = reinterpret_cast<const void*>(&gemm_kernel<F16, PL, ACOL, BCOL, EPI>);
   const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, kGemmSmem);
   if (e != hipSuccess) return static_cast<int>(e);
-  const int64_t tiles = static_cast<int64_t>(ceil_div(a.M, kTile)) * ceil_div(a.N, kTile) * (EPI == kPartial ? a.splits : 1);
+  int64_t tiles = static_cast<int64_t>(ceil_div(a.M, kTile)) * ceil_div(a.N, kTile);
+  if (EPI == kPartial && tiles < 256) tiles = 256;  // pieces of the sum, by how many rows are kept
   if (tiles >= (int64_t(1) << 31)) return -4;
   hipLaunchKernelGGL((gemm_kernel<F16, PL, ACOL, BCOL, EPI>), dim3(static_cast<unsigned>(tiles)), dim3(kThreads), kGemmSmem, st, a);
   return static_cast<int>(hipGetLastError());
@@ -1092,7 +1176,7 @@ struct DetVocabHead {
   const void* gout;               // backward: fp32 [1] or [N]
   float* loss;                    // forward: [1] or [N]
   float *stats;                   // [2, N] maxima and log2 of sums, [N, K] picked logits, [N, K] shares: forward writes, backward reads
-  int* rows;                      // [4 + N]: info, then the list of kept rows
+  int* rows;                      // [4 + 2 N]: info, the list of kept rows, each row's place in it: forward writes, backward reads
   void* ws;
   int64_t ws_bytes, x_ld, w_ld, index_ld, teacher_ld, ignore;
   int N, D, V, K, dtype, bias_dt, wide, teacher_dt, reduction;  // reduction 0 each row, 1 mean, 2 sum
@@ -1103,7 +1187,7 @@ namespace {
 
 // What both directions lay out in the workspace.
 struct Plan {
-  int planes, ldh, chunk, nchunks, ntiles, splits, k_per_split, csplits;
+  int planes, ldh, chunk, nchunks, ntiles, csplits;
   bool pack_w;
   int64_t off_h, off_w, off_flag, off_part, off_partz, off_rows, off_roww, off_alpha, off_g, off_dx, off_cs, total;
 };
@@ -1144,17 +1228,14 @@ Plan plan(const DetVocabHead& p, bool backward) {
     q.off_partz = p.smooth != 0.f ? take(int64_t(4) * p.N * q.ntiles) : 0;
     q.off_rows = take(int64_t(8) * p.N);
   } else {
-    // few tiles: the sum over the chunk is split until about two blocks a CU run, none under 512 long
-    const int64_t tiles = int64_t(ceil_div(p.N, kTile)) * ceil_div(p.D, kTile);
-    int64_t splits = tiles < 512 ? 512 / tiles : 1;
-    const int64_t most = q.chunk / 512 > 0 ? q.chunk / 512 : 1;
-    if (splits > most) splits = most;
-    q.k_per_split = static_cast<int>(up(ceil_div(q.chunk, splits), 64));
-    q.splits = ceil_div(q.chunk, q.k_per_split);
     q.off_roww = take(int64_t(4) * p.N);
     q.off_alpha = take(4);
     q.off_g = take(int64_t(2) * q.planes * p.N * q.chunk);
-    q.off_dx = p.dx != nullptr ? take(int64_t(4) * q.splits * p.N * q.ldh) : 0;
+    // at most 256 tiles' worth of partials, or a row's for every piece
+    int64_t dx = int64_t(q.chunk / 512 > 1 ? q.chunk / 512 : 1) * p.N * q.ldh;
+    if (dx > int64_t(256) * kTile * kTile) dx = int64_t(256) * kTile * kTile;
+    if (dx < int64_t(p.N) * q.ldh) dx = int64_t(p.N) * q.ldh;
+    q.off_dx = p.dx != nullptr ? take(4 * dx) : 0;
     q.csplits = p.N > 2048 ? 32 : ceil_div(p.N, 64);
     q.off_cs = p.db != nullptr ? take(int64_t(4) * q.csplits * q.chunk) : 0;
   }
@@ -1258,7 +1339,7 @@ int det_vocab_head_forward(void* stream, const DetVocabHead* pp) {
   char* ws = static_cast<char*>(p.ws);
   int* list = p.rows + 4;
 
-  RowArgs r = {p.target, p.index, p.teacher, reinterpret_cast<uint8_t*>(ws + q.off_flag), p.rows, list, p.ignore,
+  RowArgs r = {p.target, p.index, p.teacher, reinterpret_cast<uint8_t*>(ws + q.off_flag), p.rows, list, list + p.N, p.ignore,
                p.index_ld, p.teacher_ld, p.N, p.K, p.wide, p.teacher_dt};
   if (p.index != nullptr) hipLaunchKernelGGL(list_flags_kernel, dim3(ceil_div(p.N, 4)), dim3(256), 0, st, r);
   hipLaunchKernelGGL(rows_kernel, dim3(1), dim3(1024), 0, st, r);
@@ -1377,13 +1458,11 @@ int det_vocab_head_backward(void* stream, const DetVocabHead* pp) {
       d.m_dyn = p.rows;
       d.info = p.rows;
       d.M = p.N;
-      d.N = q.ldh < p.D ? q.ldh : p.D;
+      d.N = p.D;
       d.K = nv;
-      d.splits = q.splits;
-      d.k_per_split = q.k_per_split;
+      d.chunk = q.chunk;
       d.out32 = reinterpret_cast<float*>(ws + q.off_dx);
       d.ldo = q.ldh;
-      d.split_stride = int64_t(p.N) * q.ldh;
       d.add = c > 0;
       DET_TRY((gemm<false, true, kPartial>(st, p.dtype, d)));
     }
@@ -1398,14 +1477,14 @@ int det_vocab_head_backward(void* stream, const DetVocabHead* pp) {
       d.K = p.N;
       d.out = static_cast<char*>(p.dw) + int64_t(v0) * p.D * es;
       d.ldo = p.D;
-      d.out_dt = p.dtype;
       d.alpha = alpha;
       DET_TRY((gemm<true, true, kOut>(st, p.dtype, d)));
     }
   }
   if (p.dx != nullptr)
-    hipLaunchKernelGGL(dx_kernel, dim3(p.N), dim3(256), 0, st, reinterpret_cast<const float*>(ws + q.off_dx), q.splits,
-                       int64_t(p.N) * q.ldh, int64_t(q.ldh), p.rows, list, alpha, q.planes, p.dx, p.dtype, p.D);
+    hipLaunchKernelGGL(dx_kernel, dim3(p.N, ceil_div(p.D, 1024) < 64 ? ceil_div(p.D, 1024) : 64), dim3(256), 0, st,
+                       reinterpret_cast<const float*>(ws + q.off_dx), q.chunk, int64_t(q.ldh), p.rows, list + p.N, alpha, q.planes,
+                       p.dx, p.dtype, p.D);
   return static_cast<int>(hipGetLastError());
 }
 

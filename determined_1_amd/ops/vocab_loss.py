@@ -85,7 +85,7 @@ class _Head(torch.autograd.Function):
         n, k = x.shape[0], 1 if index is None else index.shape[1]
         loss = torch.empty(n if opts[3] == "none" else (), dtype=torch.float32, device=dev)
         stats = torch.empty(n * (2 + 2 * k), dtype=torch.float32, device=dev)
-        rows = torch.empty(4 + n, dtype=torch.int32, device=dev)
+        rows = torch.empty(4 + 2 * n, dtype=torch.int32, device=dev)
         p = _head_params(x, weight, bias, target, teacher, index, opts)
         p.loss, p.rows, p.stats = loss.data_ptr(), rows.data_ptr(), stats.data_ptr()
         lib = _lib.get_lib()
