@@ -127,8 +127,10 @@ struct RowArgs {
   int* info;
   int* list;   // [N] the kept rows, in order
   int* pos;    // [N] a row's place in the list, or -1
+  int* words;  // [kept] cross entropy: the target, or -1 outside the vocabulary
+  float* each; // [N] losses to clear for rows that do not count, or null
   int64_t ignore, index_ld, teacher_ld;
-  int N, K, wide, teacher_dt;
+  int N, K, V, wide, teacher_dt;
 };
 
 __global__ void __launch_bounds__(256) list_flags_kernel(RowArgs a) {
@@ -149,7 +151,16 @@ __global__ void __launch_bounds__(1024) rows_kernel(RowArgs a) {
   __syncthreads();
   for (int n0 = 0; n0 < a.N; n0 += 1024) {
     const int n = n0 + tid;
-    const bool keep = n < a.N && (a.target != nullptr ? load_index(a.target, n, a.wide) != a.ignore : a.flag[n] != 0);
+    bool keep = false;
+    int64_t word = 0;
+    if (n < a.N) {
+      if (a.target != nullptr) {
+        word = load_index(a.target, n, a.wide);
+        keep = word != a.ignore;
+      } else {
+        keep = a.flag[n] != 0;
+      }
+    }
     const uint64_t votes = __ballot(keep);
     if (lane == 0) wave_n[w] = __popcll(votes);
     __syncthreads();
@@ -157,7 +168,9 @@ __global__ void __launch_bounds__(1024) rows_kernel(RowArgs a) {
     for (int i = 0; i < w; ++i) before += wave_n[i];
     const int at = before + __popcll(votes & ((uint64_t(1) << lane) - 1));
     if (keep) a.list[at] = n;
+    if (keep && a.target != nullptr) a.words[at] = word >= 0 && word < a.V ? static_cast<int>(word) : -1;
     if (n < a.N) a.pos[n] = keep ? at : -1;
+    if (n < a.N && a.each != nullptr && !keep) a.each[n] = 0.f;
     __syncthreads();
     if (tid == 0)
       for (int i = 0; i < 16; ++i) base_n += wave_n[i];
@@ -170,19 +183,48 @@ __global__ void __launch_bounds__(1024) rows_kernel(RowArgs a) {
   }
 }
 
-// the largest finite magnitude of a [rows, cols] fp32 matrix into *out (bits; a maximum has no order)
-__global__ void __launch_bounds__(256) absmax_kernel(const float* x, int64_t ld, int rows, int cols, int* out) {
+// The largest finite magnitudes of the hidden states and the weights (fp32), as bits: blocks below
+// x_blocks go over x.  One atomic a block (eight thousand, one a wave, took 65 us of a 75 us launch); a
+// maximum does not depend on their order.
+struct Matrix {
+  const float* p;
+  int64_t ld;
+  int rows, cols;
+};
+
+__global__ void __launch_bounds__(256) absmax_kernel(Matrix x, Matrix w, int x_blocks, int* info) {
+  __shared__ uint32_t red[4];
+  const bool isx = blockIdx.x < static_cast<unsigned>(x_blocks);
+  const Matrix a = isx ? x : w;
+  const int64_t block = isx ? blockIdx.x : blockIdx.x - x_blocks, blocks = isx ? x_blocks : gridDim.x - x_blocks;
   uint32_t m = 0;
-  for (int r = blockIdx.x; r < rows; r += gridDim.x)
-    for (int c = threadIdx.x; c < cols; c += 256) {
-      const uint32_t b = __float_as_uint(x[r * ld + c]) & 0x7FFFFFFFu;
-      if (b < 0x7F800000u && b > m) m = b;
+  auto take = [&](float f) {
+    const uint32_t b = __float_as_uint(f) & 0x7FFFFFFFu;
+    if (b < 0x7F800000u && b > m) m = b;
+  };
+  const int64_t all = static_cast<int64_t>(a.rows) * a.cols;
+  if (a.ld == a.cols && (reinterpret_cast<uintptr_t>(a.p) & 15) == 0) {
+#pragma unroll 4
+    for (int64_t i = block * 256 + threadIdx.x; i < all / 4; i += blocks * 256) {
+      const f32x4 v = reinterpret_cast<const f32x4*>(a.p)[i];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) take(v[e]);
     }
+    if (block == 0 && threadIdx.x < (all & 3)) take(a.p[all - 1 - threadIdx.x]);
+  } else {
+    for (int64_t r = block * 4 + (threadIdx.x >> 6); r < a.rows; r += blocks * 4)
+      for (int c = threadIdx.x & 63; c < a.cols; c += 64) take(a.p[r * a.ld + c]);
+  }
   for (int o = 1; o < 64; o <<= 1) {
     const uint32_t v = __shfl_xor(m, o, 64);
     m = v > m ? v : m;
   }
-  if ((threadIdx.x & 63) == 0) atomicMax(reinterpret_cast<unsigned int*>(out), m);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 4; ++i) m = red[i] > m ? red[i] : m;
+    atomicMax(reinterpret_cast<unsigned int*>(info + (isx ? 1 : 2)), m);
+  }
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -200,30 +242,44 @@ struct PackArgs {
   int rows, cols, ld;  // ld % 8 == 0
 };
 
+// eight elements from any address (16-byte loads need no alignment here), zeros past the row's end
+template <class T>
+__device__ __forceinline__ void load8(const T* p, int there, T (&v)[8]) {
+  if (there >= 8) {
+    __builtin_memcpy(v, p, sizeof(v));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = e < there ? p[e] : T(0);
+  }
+}
+
 template <int DT>
 __global__ void __launch_bounds__(256) pack_kernel(PackArgs a) {
+  typedef typename Elem<DT>::type T;
   const int rows = a.count != nullptr ? *a.count : a.rows;
   const int chunks = a.ld >> 3;
   const float s = DT == kF32 ? pow2(scale_exp(static_cast<uint32_t>(*a.absmax))) : 1.f;
-  for (int r = blockIdx.x; r < rows; r += gridDim.x) {
+  // a thread per eight columns, whatever the width
+  const int64_t all = static_cast<int64_t>(rows) * chunks, step = gridDim.x * 256ll;
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < all; i += step) {
+    const int r = static_cast<int>(i / chunks), c = static_cast<int>(i - static_cast<int64_t>(r) * chunks) * 8;
     const int64_t from = static_cast<int64_t>(a.list != nullptr ? a.list[r] : r) * a.src_ld;
-    for (int c = threadIdx.x; c < chunks; c += 256) {
-      us8 hi, lo;
+    T v[8];
+    load8(static_cast<const T*>(a.src) + from + c, a.cols - c, v);
+    us8 hi, lo;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int col = c * 8 + e;
-        if constexpr (DT == kF32) {
-          const float x = col < a.cols ? static_cast<const float*>(a.src)[from + col] * s : 0.f;
-          hi[e] = f2h(x);
-          lo[e] = f2h(x - h2f(hi[e]));
-        } else {
-          hi[e] = col < a.cols ? static_cast<const u16*>(a.src)[from + col] : u16(0);
-        }
+    for (int e = 0; e < 8; ++e) {
+      if constexpr (DT == kF32) {
+        const float x = v[e] * s;
+        hi[e] = f2h(x);
+        lo[e] = f2h(x - h2f(hi[e]));
+      } else {
+        hi[e] = v[e];
       }
-      u16* d = a.dst + static_cast<int64_t>(r) * a.ld + c * 8;
-      *reinterpret_cast<us8*>(d) = hi;
-      if constexpr (DT == kF32) *reinterpret_cast<us8*>(d + a.plane) = lo;
     }
+    u16* d = a.dst + static_cast<int64_t>(r) * a.ld + c;
+    *reinterpret_cast<us8*>(d) = hi;
+    if constexpr (DT == kF32) *reinterpret_cast<us8*>(d + a.plane) = lo;
   }
 }
 
@@ -235,6 +291,18 @@ __global__ void __launch_bounds__(256) pack_kernel(PackArgs a) {
 // plane, or k 0-31 of the two planes of a split fp32 operand (three products a stage then).
 // Everything outside an operand's extents is fetched out of the buffer's range, which gives zeros.
 // ------------------------------------------------------------------------------------------------
+// A gradient's scale: G is held in [-1, 1] 2^k, row weights divided by the largest one's magnitude.
+struct Alpha {
+  const float* p;   // the loss's derivative, or the largest one of a row's
+  const int* info;
+  float scale;      // T / 2^k
+  int mean;
+  __device__ __forceinline__ float operator()() const {
+    const int count = info[0];
+    return *p * scale / (mean && count > 0 ? static_cast<float>(count) : 1.f);
+  }
+};
+
 struct Operand {
   const u16* p;
   int64_t plane, ld;
@@ -259,8 +327,16 @@ struct GemmArgs {
   int tile0, ntiles;
   // kGrad: p = 2^(c (z - top) - log2 sum)
   const float *top, *log_s;  // [M]
-  const float* row_w;        // [M]
+  const float* row_w;        // [M] (null: g_scale for each)
+  float g_scale;
   float smooth_v;      // eps / V
+  float* colsum;       // [tiles of M][ldg] G's column sums, or null
+  // kStats, kGrad for one target a row: the words (null for lists), the word of column 0, the target's
+  // logit (kStats writes it), its share
+  const int* words;
+  int v0;
+  float* picked;
+  float share;
   u16* G;              // [M][ldg]
   int64_t g_plane;
   int ldg;
@@ -270,7 +346,7 @@ struct GemmArgs {
   int add;
   // kOut: out[m][n] of the operands' type (fp32 if split), times *alpha and the scale of B
   void* out;
-  const float* alpha;
+  Alpha alpha;
 };
 
 // G w with few tiles: the sum over a chunk's words is cut until a block runs on every CU (one fills a
@@ -330,6 +406,12 @@ __device__ __forceinline__ f32x4 mfma16(s16x8 a, s16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   else
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// the value N lanes on in a row of 16
+template <int N>
+__device__ __forceinline__ float lane_ror(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x120 + N, 0xF, 0xF, true));
 }
 
 // a wave's part of the tile, rounded to 16 bits, as rows of kLdc; REST leaves what the rounding took in acc
@@ -539,6 +621,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(GemmArgs g) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         float m = kNegInf, s = 0.f, sz = 0.f;
+        const int row = m0 + row0 + i * 16;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -546,6 +629,17 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(GemmArgs g) {
             acc[i][j][r] = acc[i][j][r] * zs + bias[j][r];
             m = fmaxf(m, acc[i][j][r]);
           }
+        if (g.words != nullptr && row < M) {
+          const int at = g.words[row] - g.v0 - n0 - col0;  // j * 16 + r if the target is one of this lane's
+          if (static_cast<unsigned>(at) < 64u && (at & 15) < 4) {
+            float z = 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) z = at == j * 16 + r ? acc[i][j][r] : z;
+            g.picked[row] = z;
+          }
+        }
         if (g.part_z != nullptr) {
 #pragma unroll
           for (int j = 0; j < 4; ++j)
@@ -588,7 +682,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(GemmArgs g) {
       for (int i = 0; i < 8; ++i) {
         const int row = m0 + row0 + i * 16;
         const bool ok = row < M;
-        const float top = ok ? g.top[row] : 0.f, l = ok ? g.log_s[row] : 0.f, w = ok ? g.row_w[row] : 0.f;
+        const float top = ok ? g.top[row] : 0.f, l = ok ? g.log_s[row] : 0.f, w = ok && g.row_w != nullptr ? g.row_w[row] : g.g_scale;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -596,6 +690,35 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(GemmArgs g) {
             const float p = exp2_(fmaf(acc[i][j][r] * zs + bias[j][r] - top, c, -l));
             acc[i][j][r] = ok ? w * (p - g.smooth_v) : 0.f;
           }
+        if (g.words != nullptr && ok) {
+          const int at = g.words[row] - g.v0 - n0 - col0;
+          if (static_cast<unsigned>(at) < 64u && (at & 15) < 4) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) acc[i][j][r] -= at == j * 16 + r ? w * g.share : 0.f;
+          }
+        }
+      }
+      if (g.colsum != nullptr) {  // before G is rounded
+        float* red = reinterpret_cast<float*>(smem);  // [2 row waves][256 columns]
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          f32x4 t = acc[0][j];
+#pragma unroll
+          for (int i = 1; i < 8; ++i) t += acc[i][j];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            t[r] += lane_ror<8>(t[r]);
+            t[r] += lane_ror<4>(t[r]);
+            t[r] += lane_ror<2>(t[r]);
+            t[r] += lane_ror<1>(t[r]);
+          }
+          if (fr == 0) *reinterpret_cast<f32x4*>(red + wr * 256 + col0 + j * 16) = t;
+        }
+        __syncthreads();
+        if (tid < 256 && n0 + tid < g.ldg) g.colsum[static_cast<int64_t>(mt) * g.ldg + n0 + tid] = red[tid] + red[256 + tid];
+        __syncthreads();
       }
 #pragma unroll
       for (int pl = 0; pl < PL; ++pl) {
@@ -628,7 +751,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(GemmArgs g) {
       }
     }
   } else {
-    float alpha = *g.alpha;
+    float alpha = g.alpha();
     if (PL == 2) alpha *= pow2(-scale_exp(static_cast<uint32_t>(g.info[1])));
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -684,24 +807,39 @@ struct FinishArgs {
   const int *info, *list;
   const float2* part;
   const float* part_z;
-  const void *target, *index, *teacher;
+  const int* words;    // one target a row
+  const void *index, *teacher;
   int64_t index_ld, teacher_ld;
   int wide, teacher_dt;
   float inv_t, smooth;
   float *top, *log_s;  // [kept]
-  float* picked;       // [kept][K] logits of the picked words
+  float* picked;       // [kept][K] logits of the picked words (a target's: from the product)
   float* share;        // [kept][K]
   double* rows;        // losses [kept], for a mean or a sum (a row's may be past fp32 where their mean is not)
   float* each;         // losses [N], or null
 };
 
+// x . w for up to four weight rows at a time (null: none), by one wave
 template <int DT>
-__device__ __forceinline__ float dot_wave(const void* x, const void* w, int D, int lane) {
+__device__ __forceinline__ void dots_wave(const typename Elem<DT>::type* x, const typename Elem<DT>::type* const (&w)[4], int D, int lane,
+                                          float (&out)[4]) {
   typedef typename Elem<DT>::type T;
-  const T *a = static_cast<const T*>(x), *b = static_cast<const T*>(w);
-  float s = 0.f;
-  for (int d = lane; d < D; d += 64) s = fmaf(to_f<DT>(a[d]), to_f<DT>(b[d]), s);
-  return sum_lanes(s);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) out[q] = 0.f;
+  for (int d = lane * 8; d < D; d += 512) {
+    T a[8], b[4][8];
+    load8(x + d, D - d, a);
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (w[q] != nullptr) load8(w[q] + d, D - d, b[q]);
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (w[q] != nullptr)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) out[q] = fmaf(to_f<DT>(a[e]), to_f<DT>(b[q][e]), out[q]);
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q) out[q] = sum_lanes(out[q]);
 }
 
 // an entry of a teacher's list: absent if its word is negative or its logit -inf
@@ -717,88 +855,103 @@ __device__ __forceinline__ float diverge(float q, float t, float tt, float tl, f
   return q * (((t - tt) * inv_t - tl * kLn2) - ((z - top) * inv_t - log_s * kLn2));
 }
 
+// one target a row: a wave each
+__global__ void __launch_bounds__(256) finish_target_kernel(FinishArgs a) {
+  const int lane = threadIdx.x & 63, count = a.info[0];
+  for (int row = blockIdx.x * 4 + (threadIdx.x >> 6); row < count; row += gridDim.x * 4) {
+    float m = kNegInf, s = 0.f, sz = 0.f;
+    const int64_t at = static_cast<int64_t>(row) * a.ntiles;
+    for (int t = lane; t < a.ntiles; t += 64) {
+      const float2 v = a.part[at + t];
+      join(m, s, v.x, v.y, kLog2e);
+      if (a.part_z != nullptr) sz += a.part_z[at + t];
+    }
+    join_lanes(m, s, 64, kLog2e);
+    if (a.part_z != nullptr) sz = sum_lanes(sz);
+    if (lane == 0) {
+      const float log_s = log2f(s);
+      // a word outside the vocabulary: the row's loss and gradients are NaN
+      const float z = a.words[row] >= 0 ? a.picked[row] : __builtin_nanf("");
+      // with eps = 1 the target does not count, not even one of logit -inf
+      float loss = log_s * kLn2;
+      if (a.smooth != 1.f || z != z) loss += (1.f - a.smooth) * (m - z);
+      if (a.smooth != 0.f) loss += a.smooth * (m - sz);
+      a.top[row] = m;
+      a.log_s[row] = loss != loss ? loss : log_s;
+      if (a.each != nullptr) a.each[a.list[row]] = loss;
+      else a.rows[row] = loss;
+    }
+  }
+}
+
+// a list a row: a block each
 template <int DT>
-__global__ void __launch_bounds__(256) finish_kernel(FinishArgs a) {
-  __shared__ float red[4][4];
+__global__ void __launch_bounds__(256) finish_list_kernel(FinishArgs a) {
+  __shared__ float red[4][3];
   typedef typename Elem<DT>::type T;
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
   const int count = a.info[0];
   const float c = a.inv_t * kLog2e;
   for (int row = blockIdx.x; row < count; row += gridDim.x) {
     const int n = a.list[row];
-    float m = kNegInf, s = 0.f, sz = 0.f;
+    float m = kNegInf, s = 0.f;
     for (int t = tid; t < a.ntiles; t += 256) {
       const float2 v = a.part[static_cast<int64_t>(row) * a.ntiles + t];
       join(m, s, v.x, v.y, c);
-      if (a.part_z != nullptr) sz += a.part_z[static_cast<int64_t>(row) * a.ntiles + t];
     }
     join_lanes(m, s, 64, c);
-    sz = sum_lanes(sz);
     __syncthreads();
     if (lane == 0) {
       red[wv][0] = m;
       red[wv][1] = s;
-      red[wv][2] = sz;
     }
     __syncthreads();
     m = red[0][0];
     s = red[0][1];
-    sz = red[0][2];
-    for (int w = 1; w < 4; ++w) {
-      join(m, s, red[w][0], red[w][1], c);
-      sz += red[w][2];
-    }
+    for (int w = 1; w < 4; ++w) join(m, s, red[w][0], red[w][1], c);
     const float log_s = log2f(s);
     const T* x = static_cast<const T*>(a.x) + n * a.x_ld;
-    auto logit = [&](int64_t word) {
-      const float z = dot_wave<DT>(x, static_cast<const T*>(a.w) + word * a.w_ld, a.D, lane);
-      return a.bias != nullptr ? z + load_any(a.bias, word, a.bias_dt) : z;
-    };
+    const int64_t i0 = n * a.index_ld, t0 = n * a.teacher_ld, k0 = static_cast<int64_t>(row) * a.K;
+    float tt = kNegInf, ts = 0.f;
+    for (int k = lane; k < a.K; k += 64) {  // every wave goes over the whole list
+      int64_t word;
+      float t;
+      if (list_entry(a.index, i0 + k, a.wide, a.teacher, t0 + k, a.teacher_dt, word, t)) join(tt, ts, t, 1.f, c);
+    }
+    join_lanes(tt, ts, 64, c);
+    const float tl = log2f(ts);
     float loss = 0.f;  // this wave's part
-    // a word outside the vocabulary: the row's loss and gradients are NaN
-    if (a.target != nullptr) {
-      if (wv == 0) {
-        const int64_t word = load_index(a.target, n, a.wide);
-        float z = __builtin_nanf("");
-        if (word >= 0 && word < a.V) z = logit(word);
-        if (lane == 0) {
-          a.picked[row] = z;
-          a.share[row] = 1.f - a.smooth;
-        }
-        // T = 1; with eps = 1 the target does not count, not even one of logit -inf
-        loss = log_s * kLn2;
-        if (a.smooth != 1.f || z != z) loss += (1.f - a.smooth) * (m - z);
-        if (a.smooth != 0.f) loss += a.smooth * (m - sz);
+    for (int k = wv * 4; k < a.K; k += 16) {
+      const T* w[4];
+      int64_t word[4];
+      float t[4], z[4];
+      bool there[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        there[q] = k + q < a.K && list_entry(a.index, i0 + k + q, a.wide, a.teacher, t0 + k + q, a.teacher_dt, word[q], t[q]);
+        w[q] = there[q] && word[q] < a.V ? static_cast<const T*>(a.w) + word[q] * a.w_ld : nullptr;
       }
-    } else {
-      float tt = kNegInf, ts = 0.f;
-      const int64_t i0 = n * a.index_ld, t0 = n * a.teacher_ld;
-      for (int k = lane; k < a.K; k += 64) {  // every wave goes over the whole list
-        int64_t word;
-        float t;
-        if (list_entry(a.index, i0 + k, a.wide, a.teacher, t0 + k, a.teacher_dt, word, t)) join(tt, ts, t, 1.f, c);
-      }
-      join_lanes(tt, ts, 64, c);
-      const float tl = log2f(ts);
-      for (int k = wv; k < a.K; k += 4) {
-        int64_t word;
-        float t, z = 0.f, q = 0.f;
-        if (list_entry(a.index, i0 + k, a.wide, a.teacher, t0 + k, a.teacher_dt, word, t)) {
-          q = exp2_(fmaf(t - tt, c, -tl));
-          if (word >= a.V) loss = __builtin_nanf("");
-          else z = logit(word);
-          loss += diverge(q, t, tt, tl, z, m, log_s, a.inv_t);
+      dots_wave<DT>(x, w, a.D, lane, z);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        float share = 0.f;
+        if (there[q]) {
+          share = exp2_(fmaf(t[q] - tt, c, -tl));
+          // a word outside the vocabulary: the row's loss and gradients are NaN
+          if (word[q] >= a.V) loss = __builtin_nanf("");
+          else if (a.bias != nullptr) z[q] += load_any(a.bias, word[q], a.bias_dt);
+          loss += diverge(share, t[q], tt, tl, z[q], m, log_s, a.inv_t);
         }
-        if (lane == 0) {
-          a.picked[static_cast<int64_t>(row) * a.K + k] = z;
-          a.share[static_cast<int64_t>(row) * a.K + k] = q;
+        if (lane == 0 && k + q < a.K) {
+          a.picked[k0 + k + q] = z[q];
+          a.share[k0 + k + q] = share;
         }
       }
     }
-    if (lane == 0) red[wv][3] = loss;
+    if (lane == 0) red[wv][2] = loss;
     __syncthreads();
     if (tid == 0) {
-      const float t = (red[0][3] + red[1][3]) + (red[2][3] + red[3][3]);
+      const float t = (red[0][2] + red[1][2]) + (red[2][2] + red[3][2]);
       a.top[row] = m;
       a.log_s[row] = t != t ? t : log_s;
       const double all = static_cast<double>(t) / (static_cast<double>(a.inv_t) * a.inv_t);
@@ -824,21 +977,15 @@ __global__ void __launch_bounds__(1024) reduce_kernel(const double* rows, const 
   }
 }
 
-__global__ void __launch_bounds__(256) zero_kernel(float* p, int64_t n) {
-  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) p[i] = 0.f;
-}
-
 // ------------------------------------------------------------------------------------------------
-// Backward: what each row weighs.  row_w[c] = g_n / max |g| (1 for one g) times 2^kGExp for fp16 G,
-// *alpha = max |g| T / (2^kGExp) (/ rows for a mean): G itself stays within [-1, 1] 2^kGExp.
+// Backward of losses by row: row_w[c] = g_n / max |g| times 2^kGExp for fp16 G, *top = max |g|.  (A mean
+// and a sum have one weight for all, and need none of this.)
 // ------------------------------------------------------------------------------------------------
 struct WeightArgs {
-  const float* g;  // [1], or [N] (each)
+  const float* g;  // [N]
   const int *info, *list;
-  float* row_w;
-  float* alpha;
-  float heat, g_scale;
-  int each, mean;
+  float *row_w, *top;
+  float g_scale;
 };
 
 __global__ void __launch_bounds__(1024) weights_kernel(WeightArgs a) {
@@ -846,35 +993,30 @@ __global__ void __launch_bounds__(1024) weights_kernel(WeightArgs a) {
   const int count = a.info[0];
   float top = 0.f;
   bool nan = false;
-  if (a.each) {
-    for (int c = threadIdx.x; c < count; c += 1024) {
-      const float g = fabsf(a.g[a.list[c]]);
-      nan |= g != g;
-      top = fmaxf(top, g);
-    }
-    if (nan) top = __builtin_huge_valf();
-    top = max_lanes(top);
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
-    __syncthreads();
-    top = part[0];
-    for (int w = 1; w < 16; ++w) top = fmaxf(top, part[w]);
-  } else {
-    top = a.g[0];
+  for (int c = threadIdx.x; c < count; c += 1024) {
+    const float g = fabsf(a.g[a.list[c]]);
+    nan |= g != g;
+    top = fmaxf(top, g);
   }
-  for (int c = threadIdx.x; c < count; c += 1024)
-    a.row_w[c] = (a.each ? (top == 0.f ? 0.f : a.g[a.list[c]] / top) : 1.f) * a.g_scale;
-  if (threadIdx.x == 0) *a.alpha = top * a.heat / a.g_scale / (a.mean && count > 0 ? static_cast<float>(count) : 1.f);
+  if (nan) top = __builtin_huge_valf();
+  top = max_lanes(top);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
+  __syncthreads();
+  top = part[0];
+  for (int w = 1; w < 16; ++w) top = fmaxf(top, part[w]);
+  for (int c = threadIdx.x; c < count; c += 1024) a.row_w[c] = top == 0.f ? 0.f : a.g[a.list[c]] / top * a.g_scale;
+  if (threadIdx.x == 0) *a.top = top;
 }
 
-// the picked words' entries of a chunk's G, from the fp32 logits of the forward pass (a word twice in
-// a list: its entries add up, and each of them writes the same value)
+// the listed words' entries of a chunk's G, from the fp32 logits of the forward pass (a word twice in
+// a list: its shares add up, and each of its entries writes the same value)
 struct ScatterArgs {
   const int *info, *list;
-  const void *target, *index;
+  const void* index;
   int64_t index_ld;
   int wide, K, v0, nv, f16, planes, ldg;
   const float *picked, *share, *top, *log_s, *row_w;
-  float smooth_v, c;
+  float g_scale, c;
   u16* G;
   int64_t g_plane;
 };
@@ -883,27 +1025,23 @@ __global__ void __launch_bounds__(256) scatter_kernel(ScatterArgs a) {
   const int count = a.info[0];
   const int64_t all = static_cast<int64_t>(count) * a.K;
   for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < all; i += gridDim.x * 256ll) {
-    const int c = static_cast<int>(i / a.K), k = static_cast<int>(i - static_cast<int64_t>(c) * a.K);
-    const int n = a.list[c];
-    const int64_t word = a.target != nullptr ? load_index(a.target, n, a.wide) : load_index(a.index, n * a.index_ld + k, a.wide);
-    if (word < a.v0 || word >= a.v0 + a.nv) continue;
-    const float* share = a.share + static_cast<int64_t>(c) * a.K;
-    float s = share[k];
-    if (a.target == nullptr) {
-      s = 0.f;
-      for (int j = 0; j < a.K; ++j)
-        if (load_index(a.index, n * a.index_ld + j, a.wide) == word) s += share[j];
-      if (share[k] == 0.f) continue;  // G has p already, or another entry writes it
-    }
-    const float v = a.row_w[c] * ((exp2_(fmaf(a.picked[i] - a.top[c], a.c, -a.log_s[c])) - a.smooth_v) - s);
-    u16* o = a.G + static_cast<int64_t>(c) * a.ldg + (word - a.v0);
+    const int row = static_cast<int>(i / a.K), k = static_cast<int>(i - static_cast<int64_t>(row) * a.K);
+    const int64_t i0 = a.list[row] * a.index_ld, word = load_index(a.index, i0 + k, a.wide);
+    const float* share = a.share + static_cast<int64_t>(row) * a.K;
+    if (word < a.v0 || word >= a.v0 + a.nv || share[k] == 0.f) continue;  // no share: another entry's, or p alone
+    float s = 0.f;
+    for (int j = 0; j < a.K; ++j)
+      if (load_index(a.index, i0 + j, a.wide) == word) s += share[j];
+    const float w = a.row_w != nullptr ? a.row_w[row] : a.g_scale;
+    const float v = w * (exp2_(fmaf(a.picked[i] - a.top[row], a.c, -a.log_s[row])) - s);
+    u16* o = a.G + static_cast<int64_t>(row) * a.ldg + (word - a.v0);
     const u16 hi = a.f16 ? f2h(v) : f2bf(v);
     *o = hi;
     if (a.planes == 2) o[a.g_plane] = f2h(v - h2f(hi));
   }
 }
 
-// column sums of a chunk's G (rows split over blockIdx.y), then the bias gradient
+// column sums of a chunk's G after the scatter (rows split over blockIdx.y)
 __global__ void __launch_bounds__(256) colsum_kernel(const u16* G, int64_t g_plane, int planes, int f16, int ldg, const int* info,
                                                      float* part) {
   __shared__ float red[8][256 + 8];
@@ -927,18 +1065,21 @@ __global__ void __launch_bounds__(256) colsum_kernel(const u16* G, int64_t g_pla
   if (blockIdx.x * 256 + tid < ldg) part[static_cast<int64_t>(blockIdx.y) * ldg + blockIdx.x * 256 + tid] = t;
 }
 
-__global__ void __launch_bounds__(256) dbias_kernel(const float* part, int splits, int ldg, int nv, const float* alpha, void* db,
-                                                    int64_t at, int dt) {
+// the bias gradient from column sums (of `splits` parts, or with 0 one for every tile of kept rows)
+__global__ void __launch_bounds__(256) dbias_kernel(const float* part, int splits, int ldg, int nv, Alpha alpha, void* db, int64_t at,
+                                                    int dt) {
   const int v = blockIdx.x * 256 + threadIdx.x;
   if (v >= nv) return;
+  if (splits == 0) splits = (alpha.info[0] + kTile - 1) / kTile;
   float t = 0.f;
+#pragma unroll 8
   for (int s = 0; s < splits; ++s) t += part[static_cast<int64_t>(s) * ldg + v];
-  store_any(db, at + v, dt, t * *alpha);
+  store_any(db, at + v, dt, t * alpha());
 }
 
 // dh: the sum of a kept row's partials, zeros for the others
 __global__ void __launch_bounds__(256) dx_kernel(const float* part, int chunk, int64_t ldo, const int* info, const int* pos,
-                                                 const float* alpha, int planes, void* dx, int dt, int D) {
+                                                 Alpha alpha, int planes, void* dx, int dt, int D) {
   const int n = blockIdx.x, count = info[0], at = pos[n];
   const int tiles = ((count + kTile - 1) / kTile) * ((D + kTile - 1) / kTile);
   int splits = 0;
@@ -946,7 +1087,7 @@ __global__ void __launch_bounds__(256) dx_kernel(const float* part, int chunk, i
     const int len = split_length(tiles, chunk);
     splits = (chunk + len - 1) / len;
   }
-  float a = *alpha;
+  float a = alpha();
   if (planes == 2) a *= pow2(-scale_exp(static_cast<uint32_t>(info[2])));
   const int64_t stride = count * ldo, out = static_cast<int64_t>(n) * D;
   const bool wide = (D & 3) == 0 && (reinterpret_cast<uintptr_t>(dx) & 15) == 0;
@@ -1176,9 +1317,10 @@ struct DetVocabHead {
   const void* gout;               // backward: fp32 [1] or [N]
   float* loss;                    // forward: [1] or [N]
   float *stats;                   // [2, N] maxima and log2 of sums, [N, K] picked logits, [N, K] shares: forward writes, backward reads
-  int* rows;                      // [4 + 2 N]: info, the list of kept rows, each row's place in it: forward writes, backward reads
+  int* rows;                      // [4 + 3 N]: info, the list of kept rows, each row's place in it, targets: forward writes, backward reads
+  void* operands;                 // the packed operands: forward writes, backward reads
   void* ws;
-  int64_t ws_bytes, x_ld, w_ld, index_ld, teacher_ld, ignore;
+  int64_t ws_bytes, operand_bytes, x_ld, w_ld, index_ld, teacher_ld, ignore;
   int N, D, V, K, dtype, bias_dt, wide, teacher_dt, reduction;  // reduction 0 each row, 1 mean, 2 sum
   float inv_t, smooth;
 };
@@ -1188,8 +1330,9 @@ namespace {
 // What both directions lay out in the workspace.
 struct Plan {
   int planes, ldh, chunk, nchunks, ntiles, csplits;
-  bool pack_w;
-  int64_t off_h, off_w, off_flag, off_part, off_partz, off_rows, off_roww, off_alpha, off_g, off_dx, off_cs, total;
+  bool pack_w, keep_w;
+  int64_t kept;  // bytes of the operands that the backward pass finds again: the rows, and the weights if they are packed whole
+  int64_t off_w, off_flag, off_part, off_partz, off_rows, off_roww, off_alpha, off_g, off_dx, off_cs, total;
 };
 
 constexpr int64_t kChunkBytes = int64_t(256) << 20;  // G of one chunk, and the packed weights of one
@@ -1199,12 +1342,15 @@ Plan plan(const DetVocabHead& p, bool backward) {
   q.planes = p.dtype == kF32 ? 2 : 1;
   q.ldh = static_cast<int>(up(p.D, 8));
   q.pack_w = p.dtype == kF32 || p.D % 8 != 0 || p.w_ld % 8 != 0 || (reinterpret_cast<uintptr_t>(p.w) & 15) != 0;
+  const int64_t w_bytes = int64_t(2) * q.planes * p.V * q.ldh, h_bytes = up(int64_t(2) * q.planes * p.N * q.ldh, 256);
+  q.keep_w = q.pack_w && w_bytes <= kChunkBytes;
+  q.kept = h_bytes + (q.keep_w ? w_bytes : 0);
   int64_t chunk = up(p.V, kTile);
   if (backward) {
     const int64_t fit = kChunkBytes / (int64_t(2) * q.planes * p.N) / kTile * kTile;
     if (chunk > fit) chunk = fit;
   }
-  if (q.pack_w) {
+  if (q.pack_w && !q.keep_w) {
     const int64_t fit = kChunkBytes / (int64_t(2) * q.planes * q.ldh) / kTile * kTile;
     if (chunk > fit) chunk = fit;
   }
@@ -1220,8 +1366,7 @@ Plan plan(const DetVocabHead& p, bool backward) {
     at += up(bytes, 256);
     return o;
   };
-  q.off_h = take(int64_t(2) * q.planes * p.N * q.ldh);
-  q.off_w = q.pack_w ? take(int64_t(2) * q.planes * q.chunk * q.ldh) : 0;
+  q.off_w = q.pack_w && !q.keep_w ? take(int64_t(2) * q.planes * q.chunk * q.ldh) : 0;
   if (!backward) {
     q.off_flag = take(p.N);
     q.off_part = take(int64_t(8) * p.N * q.ntiles);
@@ -1236,7 +1381,8 @@ Plan plan(const DetVocabHead& p, bool backward) {
     if (dx > int64_t(256) * kTile * kTile) dx = int64_t(256) * kTile * kTile;
     if (dx < int64_t(p.N) * q.ldh) dx = int64_t(p.N) * q.ldh;
     q.off_dx = p.dx != nullptr ? take(4 * dx) : 0;
-    q.csplits = p.N > 2048 ? 32 : ceil_div(p.N, 64);
+    // column sums: from the product's tiles for one target a row, from G for lists (which change it)
+    q.csplits = p.index == nullptr ? ceil_div(p.N, kTile) : p.N > 2048 ? 32 : ceil_div(p.N, 64);
     q.off_cs = p.db != nullptr ? take(int64_t(4) * q.csplits * q.chunk) : 0;
   }
   q.total = at;
@@ -1260,7 +1406,8 @@ int check_head(const DetVocabHead& p) {
 
 template <int DT>
 int pack(hipStream_t st, const PackArgs& a) {
-  const int blocks = a.rows < 4096 ? a.rows : 4096;
+  const int64_t need = (static_cast<int64_t>(a.rows) * (a.ld / 8) + 255) / 256;
+  const int blocks = static_cast<int>(need < 8192 ? need : 8192);
   hipLaunchKernelGGL((pack_kernel<DT>), dim3(blocks), dim3(256), 0, st, a);
   return static_cast<int>(hipGetLastError());
 }
@@ -1268,14 +1415,16 @@ int pack_any(hipStream_t st, int dt, const PackArgs& a) {
   return dt == kF32 ? pack<kF32>(st, a) : pack<kBF16>(st, a);  // 16-bit types are copied as bits
 }
 
-int pack_hidden(hipStream_t st, const DetVocabHead& p, const Plan& q, char* ws) {
+u16* hidden_planes(const DetVocabHead& p) { return static_cast<u16*>(p.operands); }
+
+int pack_hidden(hipStream_t st, const DetVocabHead& p, const Plan& q) {
   PackArgs a = {};
   a.src = p.x;
   a.src_ld = p.x_ld;
   a.list = p.rows + 4;
   a.count = p.rows;
   a.absmax = p.rows + 1;
-  a.dst = reinterpret_cast<u16*>(ws + q.off_h);
+  a.dst = hidden_planes(p);
   a.plane = int64_t(p.N) * q.ldh;
   a.rows = p.N;
   a.cols = p.D;
@@ -1283,8 +1432,8 @@ int pack_hidden(hipStream_t st, const DetVocabHead& p, const Plan& q, char* ws) 
   return pack_any(st, p.dtype, a);
 }
 
-// the weight rows v0 .. v0 + nv as an operand
-int weight_operand(hipStream_t st, const DetVocabHead& p, const Plan& q, char* ws, int v0, int nv, Operand* w) {
+// the weight rows v0 .. v0 + nv as an operand; packs them (all: once, in the forward pass)
+int weight_operand(hipStream_t st, const DetVocabHead& p, const Plan& q, char* ws, int v0, int nv, bool first, Operand* w) {
   const int64_t es = p.dtype == kF32 ? 4 : 2;
   const char* src = static_cast<const char*>(p.w) + v0 * p.w_ld * es;
   if (!q.pack_w) {
@@ -1292,21 +1441,21 @@ int weight_operand(hipStream_t st, const DetVocabHead& p, const Plan& q, char* w
     return 0;
   }
   PackArgs a = {};
-  a.src = src;
+  a.src = q.keep_w ? p.w : src;
   a.src_ld = p.w_ld;
   a.absmax = p.rows + 2;
-  a.dst = reinterpret_cast<u16*>(ws + q.off_w);
-  a.plane = int64_t(q.chunk) * q.ldh;
-  a.rows = nv;
+  a.dst = reinterpret_cast<u16*>(q.keep_w ? static_cast<char*>(p.operands) + up(int64_t(2) * q.planes * p.N * q.ldh, 256) : ws + q.off_w);
+  a.plane = int64_t(q.keep_w ? p.V : q.chunk) * q.ldh;
+  a.rows = q.keep_w ? p.V : nv;
   a.cols = p.D;
   a.ld = q.ldh;
-  *w = Operand{a.dst, a.plane, q.ldh};
-  return pack_any(st, p.dtype, a);
+  *w = Operand{a.dst + (q.keep_w ? int64_t(v0) * q.ldh : 0), a.plane, q.ldh};
+  return q.keep_w && !first ? 0 : pack_any(st, p.dtype, a);
 }
 
-GemmArgs logits_args(const DetVocabHead& p, const Plan& q, char* ws, const Operand& w, int v0, int nv) {
+GemmArgs logits_args(const DetVocabHead& p, const Plan& q, const Operand& w, int v0, int nv) {
   GemmArgs a = {};
-  a.A = Operand{reinterpret_cast<const u16*>(ws + q.off_h), int64_t(p.N) * q.ldh, q.ldh};
+  a.A = Operand{hidden_planes(p), int64_t(p.N) * q.ldh, q.ldh};
   a.B = w;
   a.m_dyn = p.rows;
   a.info = p.rows;
@@ -1317,12 +1466,21 @@ GemmArgs logits_args(const DetVocabHead& p, const Plan& q, char* ws, const Opera
   a.bias_dt = p.bias_dt;
   a.c = p.inv_t * kLog2e;
   a.inv_v = 1.f / static_cast<float>(p.V);
+  if (p.target != nullptr) a.words = p.rows + 4 + int64_t(2) * p.N;
+  a.v0 = v0;
+  a.picked = p.stats + int64_t(2) * p.N;
+  a.share = 1.f - p.smooth;
   return a;
 }
 
 }  // namespace
 
 extern "C" {
+
+int64_t det_vocab_head_operand_bytes(const DetVocabHead* p) {
+  if (p == nullptr || check_head(*p) != 0) return -1;
+  return plan(*p, false).kept;
+}
 
 int64_t det_vocab_head_ws_bytes(const DetVocabHead* p, int backward) {
   if (p == nullptr || check_head(*p) != 0) return -1;
@@ -1334,28 +1492,27 @@ int det_vocab_head_forward(void* stream, const DetVocabHead* pp) {
   const DetVocabHead& p = *pp;
   DET_TRY(check_head(p));
   const Plan q = plan(p, false);
-  if (p.ws == nullptr || p.ws_bytes < q.total) return -6;
+  if (p.ws == nullptr || p.ws_bytes < q.total || p.operands == nullptr || p.operand_bytes < q.kept) return -6;
   hipStream_t st = static_cast<hipStream_t>(stream);
   char* ws = static_cast<char*>(p.ws);
   int* list = p.rows + 4;
 
-  RowArgs r = {p.target, p.index, p.teacher, reinterpret_cast<uint8_t*>(ws + q.off_flag), p.rows, list, list + p.N, p.ignore,
-               p.index_ld, p.teacher_ld, p.N, p.K, p.wide, p.teacher_dt};
+  RowArgs r = {p.target, p.index, p.teacher, reinterpret_cast<uint8_t*>(ws + q.off_flag), p.rows, list, list + p.N, list + int64_t(2) * p.N,
+               p.reduction == 0 ? p.loss : nullptr, p.ignore, p.index_ld, p.teacher_ld, p.N, p.K, p.V, p.wide, p.teacher_dt};
   if (p.index != nullptr) hipLaunchKernelGGL(list_flags_kernel, dim3(ceil_div(p.N, 4)), dim3(256), 0, st, r);
   hipLaunchKernelGGL(rows_kernel, dim3(1), dim3(1024), 0, st, r);
   if (p.dtype == kF32) {
-    hipLaunchKernelGGL(absmax_kernel, dim3(p.N < 1024 ? p.N : 1024), dim3(256), 0, st, static_cast<const float*>(p.x), p.x_ld, p.N,
-                       p.D, p.rows + 1);
-    hipLaunchKernelGGL(absmax_kernel, dim3(p.V < 2048 ? p.V : 2048), dim3(256), 0, st, static_cast<const float*>(p.w), p.w_ld, p.V,
-                       p.D, p.rows + 2);
+    const int xb = p.N < 512 ? ceil_div(p.N, 4) : 128, wb = p.V < 2048 ? ceil_div(p.V, 4) : 512;
+    hipLaunchKernelGGL(absmax_kernel, dim3(xb + wb), dim3(256), 0, st, Matrix{static_cast<const float*>(p.x), p.x_ld, p.N, p.D},
+                       Matrix{static_cast<const float*>(p.w), p.w_ld, p.V, p.D}, xb, p.rows);
   }
   DET_TRY(static_cast<int>(hipGetLastError()));
-  DET_TRY(pack_hidden(st, p, q, ws));
+  DET_TRY(pack_hidden(st, p, q));
   for (int c = 0; c < q.nchunks; ++c) {
     const int v0 = c * q.chunk, nv = p.V - v0 < q.chunk ? p.V - v0 : q.chunk;
     Operand w;
-    DET_TRY(weight_operand(st, p, q, ws, v0, nv, &w));
-    GemmArgs a = logits_args(p, q, ws, w, v0, nv);
+    DET_TRY(weight_operand(st, p, q, ws, v0, nv, c == 0, &w));
+    GemmArgs a = logits_args(p, q, w, v0, nv);
     a.part = reinterpret_cast<float2*>(ws + q.off_part);
     a.part_z = p.smooth != 0.f ? reinterpret_cast<float*>(ws + q.off_partz) : nullptr;
     a.tile0 = v0 / kTile;
@@ -1379,7 +1536,7 @@ int det_vocab_head_forward(void* stream, const DetVocabHead* pp) {
   f.list = list;
   f.part = reinterpret_cast<const float2*>(ws + q.off_part);
   f.part_z = p.smooth != 0.f ? reinterpret_cast<const float*>(ws + q.off_partz) : nullptr;
-  f.target = p.target;
+  f.words = list + int64_t(2) * p.N;
   f.index = p.index;
   f.teacher = p.teacher;
   f.index_ld = p.index_ld;
@@ -1394,11 +1551,15 @@ int det_vocab_head_forward(void* stream, const DetVocabHead* pp) {
   f.share = f.picked + int64_t(p.N) * p.K;
   f.each = p.reduction == 0 ? p.loss : nullptr;
   f.rows = reinterpret_cast<double*>(ws + q.off_rows);
-  if (f.each != nullptr) hipLaunchKernelGGL(zero_kernel, dim3(ceil_div(p.N, 1024) < 1024 ? ceil_div(p.N, 1024) : 1024), dim3(256), 0, st, p.loss, int64_t(p.N));
-  const dim3 fg(p.N < 8192 ? p.N : 8192);
-  if (p.dtype == kF32) hipLaunchKernelGGL(finish_kernel<kF32>, fg, dim3(256), 0, st, f);
-  else if (p.dtype == kBF16) hipLaunchKernelGGL(finish_kernel<kBF16>, fg, dim3(256), 0, st, f);
-  else hipLaunchKernelGGL(finish_kernel<kF16>, fg, dim3(256), 0, st, f);
+  if (p.target != nullptr) {
+    const int blocks = ceil_div(p.N, 4);
+    hipLaunchKernelGGL(finish_target_kernel, dim3(blocks < 4096 ? blocks : 4096), dim3(256), 0, st, f);
+  } else {
+    const dim3 fg(p.N < 8192 ? p.N : 8192);
+    if (p.dtype == kF32) hipLaunchKernelGGL(finish_list_kernel<kF32>, fg, dim3(256), 0, st, f);
+    else if (p.dtype == kBF16) hipLaunchKernelGGL(finish_list_kernel<kBF16>, fg, dim3(256), 0, st, f);
+    else hipLaunchKernelGGL(finish_list_kernel<kF16>, fg, dim3(256), 0, st, f);
+  }
   if (f.each == nullptr) hipLaunchKernelGGL(reduce_kernel, dim3(1), dim3(1024), 0, st, f.rows, p.rows, p.reduction == 1, p.loss);
   return static_cast<int>(hipGetLastError());
 }
@@ -1408,48 +1569,53 @@ int det_vocab_head_backward(void* stream, const DetVocabHead* pp) {
   const DetVocabHead& p = *pp;
   DET_TRY(check_head(p));
   const Plan q = plan(p, true);
-  if (p.ws == nullptr || p.ws_bytes < q.total || p.gout == nullptr) return -6;
+  if (p.ws == nullptr || p.ws_bytes < q.total || p.operands == nullptr || p.operand_bytes < q.kept || p.gout == nullptr) return -6;
   hipStream_t st = static_cast<hipStream_t>(stream);
   char* ws = static_cast<char*>(p.ws);
   int* list = p.rows + 4;
   const bool f16 = p.dtype != kBF16;
-  float* row_w = reinterpret_cast<float*>(ws + q.off_roww);
-  float* alpha = reinterpret_cast<float*>(ws + q.off_alpha);
   const float* picked = p.stats + int64_t(2) * p.N;
-  const float smooth_v = p.smooth / static_cast<float>(p.V);
-
-  WeightArgs wa = {static_cast<const float*>(p.gout), p.rows, list, row_w, alpha, 1.f / p.inv_t,
-                   f16 ? static_cast<float>(1 << kGExp) : 1.f, p.reduction == 0, p.reduction == 1};
-  hipLaunchKernelGGL(weights_kernel, dim3(1), dim3(1024), 0, st, wa);
-  DET_TRY(static_cast<int>(hipGetLastError()));
-  DET_TRY(pack_hidden(st, p, q, ws));
+  const float g_scale = f16 ? static_cast<float>(1 << kGExp) : 1.f;
+  Alpha alpha = {static_cast<const float*>(p.gout), p.rows, 1.f / (p.inv_t * g_scale), p.reduction == 1};
+  float* row_w = nullptr;
+  if (p.reduction == 0) {
+    row_w = reinterpret_cast<float*>(ws + q.off_roww);
+    float* top = reinterpret_cast<float*>(ws + q.off_alpha);
+    hipLaunchKernelGGL(weights_kernel, dim3(1), dim3(1024), 0, st, WeightArgs{alpha.p, p.rows, list, row_w, top, g_scale});
+    DET_TRY(static_cast<int>(hipGetLastError()));
+    alpha.p = top;
+  }
   const int64_t es = p.dtype == kF32 ? 4 : 2;
   for (int c = 0; c < q.nchunks; ++c) {
     const int v0 = c * q.chunk, nv = p.V - v0 < q.chunk ? p.V - v0 : q.chunk;
     const int ldg = static_cast<int>(up(nv, 64));  // columns past nv are zero
     Operand w;
-    DET_TRY(weight_operand(st, p, q, ws, v0, nv, &w));
-    GemmArgs a = logits_args(p, q, ws, w, v0, nv);
+    DET_TRY(weight_operand(st, p, q, ws, v0, nv, false, &w));
+    GemmArgs a = logits_args(p, q, w, v0, nv);
+    float* cs = p.db != nullptr ? reinterpret_cast<float*>(ws + q.off_cs) : nullptr;
     a.top = p.stats;
     a.log_s = p.stats + p.N;
     a.row_w = row_w;
-    a.smooth_v = smooth_v;
+    a.g_scale = g_scale;
+    a.smooth_v = p.smooth / static_cast<float>(p.V);
+    a.colsum = p.target != nullptr ? cs : nullptr;
     a.G = reinterpret_cast<u16*>(ws + q.off_g);
     a.g_plane = int64_t(p.N) * ldg;
     a.ldg = ldg;
     DET_TRY((gemm<false, false, kGrad>(st, p.dtype, a)));
-    ScatterArgs s = {p.rows, list, p.target, p.index, p.index_ld, p.wide, p.K, v0, nv, f16, q.planes, ldg,
-                     picked, picked + int64_t(p.N) * p.K, p.stats, p.stats + p.N, row_w, smooth_v, a.c, a.G, a.g_plane};
-    const int sb = ceil_div(int64_t(p.N) * p.K, 256);
-    hipLaunchKernelGGL(scatter_kernel, dim3(sb < 8192 ? sb : 8192), dim3(256), 0, st, s);
-    const Operand G = {a.G, a.g_plane, ldg};
-    if (p.db != nullptr) {
-      float* cs = reinterpret_cast<float*>(ws + q.off_cs);
-      hipLaunchKernelGGL(colsum_kernel, dim3(ceil_div(ldg, 256), q.csplits), dim3(256), 0, st, a.G, a.g_plane, q.planes, f16, ldg,
-                         p.rows, cs);
-      hipLaunchKernelGGL(dbias_kernel, dim3(ceil_div(nv, 256)), dim3(256), 0, st, cs, q.csplits, ldg, nv, alpha, p.db, int64_t(v0),
-                         p.bias_dt);
+    if (p.index != nullptr) {
+      ScatterArgs s = {p.rows, list, p.index, p.index_ld, p.wide, p.K, v0, nv, f16, q.planes, ldg, picked,
+                       picked + int64_t(p.N) * p.K, a.top, a.log_s, row_w, g_scale, a.c, a.G, a.g_plane};
+      const int64_t sb = (int64_t(p.N) * p.K + 255) / 256;
+      hipLaunchKernelGGL(scatter_kernel, dim3(sb < 8192 ? static_cast<unsigned>(sb) : 8192u), dim3(256), 0, st, s);
+      if (cs != nullptr)
+        hipLaunchKernelGGL(colsum_kernel, dim3(ceil_div(ldg, 256), q.csplits), dim3(256), 0, st, a.G, a.g_plane, q.planes, f16, ldg,
+                           p.rows, cs);
     }
+    const Operand G = {a.G, a.g_plane, ldg};
+    if (cs != nullptr)
+      hipLaunchKernelGGL(dbias_kernel, dim3(ceil_div(nv, 256)), dim3(256), 0, st, cs, p.target != nullptr ? 0 : q.csplits, ldg, nv, alpha,
+                         p.db, int64_t(v0), p.bias_dt);
     DET_TRY(static_cast<int>(hipGetLastError()));
     if (p.dx != nullptr) {
       GemmArgs d = {};
@@ -1469,7 +1635,7 @@ int det_vocab_head_backward(void* stream, const DetVocabHead* pp) {
     if (p.dw != nullptr) {
       GemmArgs d = {};
       d.A = G;
-      d.B = Operand{reinterpret_cast<const u16*>(ws + q.off_h), int64_t(p.N) * q.ldh, q.ldh};
+      d.B = Operand{hidden_planes(p), int64_t(p.N) * q.ldh, q.ldh};
       d.k_dyn = p.rows;
       d.info = p.rows;
       d.M = nv;

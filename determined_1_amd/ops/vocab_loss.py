@@ -33,8 +33,8 @@ _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 class _HeadParams(ctypes.Structure):
     """Mirror of ``DetVocabHead`` (det_vocab.hip)."""
     _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "w", "bias", "target", "index", "teacher", "dx", "dw", "db", "gout",
-                                                "loss", "stats", "rows", "ws")]
-                + [(n, ctypes.c_int64) for n in ("ws_bytes", "x_ld", "w_ld", "index_ld", "teacher_ld", "ignore")]
+                                                "loss", "stats", "rows", "operands", "ws")]
+                + [(n, ctypes.c_int64) for n in ("ws_bytes", "operand_bytes", "x_ld", "w_ld", "index_ld", "teacher_ld", "ignore")]
                 + [(n, ctypes.c_int32) for n in ("N", "D", "V", "K", "dtype", "bias_dt", "wide", "teacher_dt", "reduction")]
                 + [("inv_t", ctypes.c_float), ("smooth", ctypes.c_float)])
 
@@ -85,22 +85,23 @@ class _Head(torch.autograd.Function):
         n, k = x.shape[0], 1 if index is None else index.shape[1]
         loss = torch.empty(n if opts[3] == "none" else (), dtype=torch.float32, device=dev)
         stats = torch.empty(n * (2 + 2 * k), dtype=torch.float32, device=dev)
-        rows = torch.empty(4 + 2 * n, dtype=torch.int32, device=dev)
+        rows = torch.empty(4 + 3 * n, dtype=torch.int32, device=dev)
         p = _head_params(x, weight, bias, target, teacher, index, opts)
         p.loss, p.rows, p.stats = loss.data_ptr(), rows.data_ptr(), stats.data_ptr()
         lib = _lib.get_lib()
         with torch.cuda.device(dev):
             ws = _workspace(lib.det_vocab_head_ws_bytes(ctypes.byref(p), 0), x, "vocab_loss")
-            p.ws, p.ws_bytes = ws.data_ptr(), ws.numel()
+            operands = _workspace(lib.det_vocab_head_operand_bytes(ctypes.byref(p)), x, "vocab_loss")
+            p.ws, p.ws_bytes, p.operands, p.operand_bytes = ws.data_ptr(), ws.numel(), operands.data_ptr(), operands.numel()
             _lib.check(lib.det_vocab_head_forward(_stream(x), ctypes.byref(p)), "det_vocab_head_forward")
-        ctx.save_for_backward(x, weight, bias, target, teacher, index, stats, rows)
+        ctx.save_for_backward(x, weight, bias, target, teacher, index, stats, rows, operands)
         ctx.opts = opts
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gout):  # type: ignore[override]
-        x, weight, bias, target, teacher, index, stats, rows = ctx.saved_tensors
+        x, weight, bias, target, teacher, index, stats, rows, operands = ctx.saved_tensors
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         gout = gout.float().contiguous()
         dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
@@ -113,7 +114,7 @@ class _Head(torch.autograd.Function):
             db = torch.empty(bias.shape, dtype=bias.dtype, device=bias.device)
         p = _head_params(x, weight, bias, target, teacher, index, ctx.opts)
         p.dx, p.dw, p.db, p.gout = _ptr(dx), _ptr(dw), _ptr(db), gout.data_ptr()
-        p.rows, p.stats = rows.data_ptr(), stats.data_ptr()
+        p.rows, p.stats, p.operands, p.operand_bytes = rows.data_ptr(), stats.data_ptr(), operands.data_ptr(), operands.numel()
         lib = _lib.get_lib()
         with torch.cuda.device(x.device):
             ws = _workspace(lib.det_vocab_head_ws_bytes(ctypes.byref(p), 1), x, "vocab_loss")
