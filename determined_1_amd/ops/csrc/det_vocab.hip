@@ -414,22 +414,24 @@ __device__ __forceinline__ float lane_ror(float v) {
   return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x120 + N, 0xF, 0xF, true));
 }
 
-// a wave's part of the tile, rounded to 16 bits, as rows of kLdc; REST leaves what the rounding took in acc
-template <bool F16, bool REST>
-__device__ __forceinline__ void tile_to_lds(f32x4 (&acc)[8][4], unsigned char* smem, int row0, int col0) {
+// a wave's part of the tile, rounded to 16 bits, as rows of kLdc; two planes: what the rounding took 128 rows on
+template <bool F16, int PL>
+__device__ __forceinline__ void tile_to_lds(const f32x4 (&acc)[8][4], unsigned char* smem, int row0, int col0) {
   typedef __attribute__((ext_vector_type(4))) u16 us4;
   u16* ct = reinterpret_cast<u16*>(smem);
 #pragma unroll
   for (int i = 0; i < 8; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      us4 o;
+      us4 hi, lo;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        o[r] = F16 ? f2h(acc[i][j][r]) : f2bf(acc[i][j][r]);
-        if (REST) acc[i][j][r] -= h2f(o[r]);
+        hi[r] = F16 ? f2h(acc[i][j][r]) : f2bf(acc[i][j][r]);
+        lo[r] = PL == 2 ? f2h(acc[i][j][r] - h2f(hi[r])) : u16(0);
       }
-      *reinterpret_cast<us4*>(ct + (row0 + i * 16) * kLdc + col0 + j * 16) = o;
+      u16* o = ct + (row0 + i * 16) * kLdc + col0 + j * 16;
+      *reinterpret_cast<us4*>(o) = hi;
+      if (PL == 2) *reinterpret_cast<us4*>(o + 128 * kLdc) = lo;
     }
 }
 
@@ -720,18 +722,19 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(GemmArgs g) {
         if (tid < 256 && n0 + tid < g.ldg) g.colsum[static_cast<int64_t>(mt) * g.ldg + n0 + tid] = red[tid] + red[256 + tid];
         __syncthreads();
       }
-#pragma unroll
-      for (int pl = 0; pl < PL; ++pl) {
-        tile_to_lds<F16, PL == 2>(acc, smem, row0, col0);
+      // one plane: the whole tile through LDS; two: both planes of half the rows at a time
+#pragma unroll 1
+      for (int half = 0; half < PL; ++half) {
+        const int rows = kTile / PL;
+        if (PL == 1 || wr == half) tile_to_lds<F16, PL>(acc, smem, PL == 1 ? row0 : fr, col0);
         __syncthreads();
-        u16* G = g.G + pl * g.g_plane;
         for (int q = tid; q < kTile * (kTile / 8); q += kThreads) {
-          const int row = q >> 5, cc = (q & 31) * 8;
+          const int at = q >> 5, cc = (q & 31) * 8, pl = at / rows, row = half * rows + at % rows;
           if (m0 + row < M && n0 + cc < g.ldg)
-            *reinterpret_cast<us8*>(G + static_cast<int64_t>(m0 + row) * g.ldg + n0 + cc) =
-                *reinterpret_cast<const us8*>(reinterpret_cast<const u16*>(smem) + row * kLdc + cc);
+            *reinterpret_cast<us8*>(g.G + pl * g.g_plane + static_cast<int64_t>(m0 + row) * g.ldg + n0 + cc) =
+                *reinterpret_cast<const us8*>(reinterpret_cast<const u16*>(smem) + at * kLdc + cc);
         }
-        __syncthreads();
+        if (half + 1 < PL) __syncthreads();
       }
     }
   } else if constexpr (EPI == kPartial) {
@@ -759,7 +762,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(GemmArgs g) {
       for (int j = 0; j < 4; ++j) acc[i][j] *= alpha;
     if constexpr (PL == 1) {
       const bool wide = (g.ldo & 7) == 0 && (reinterpret_cast<uintptr_t>(g.out) & 15) == 0;
-      tile_to_lds<F16, false>(acc, smem, row0, col0);
+      tile_to_lds<F16, 1>(acc, smem, row0, col0);
       __syncthreads();
       const u16* ct = reinterpret_cast<const u16*>(smem);
       u16* out = static_cast<u16*>(g.out);
