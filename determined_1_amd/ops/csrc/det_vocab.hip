@@ -286,9 +286,8 @@ __global__ void __launch_bounds__(256) pack_kernel(PackArgs a) {
 // ------------------------------------------------------------------------------------------------
 // The products.  C tile 256 x 256, 8 waves as 2 (rows) x 4 (columns) of 128 x 64, v_mfma 16x16x32.
 // An operand lies with its k contiguous ("row": element (i, k) at i * ld + k) or strided ("col":
-// (i, k) at k * ld + i, read back from LDS transposed).  LDS holds two stages of four 16 KiB half
-// tiles (A rows 0-127, 128-255, B 0-127, 128-255), each two 8 KiB images: k 0-31 and 32-63 of one
-// plane, or k 0-31 of the two planes of a split fp32 operand (three products a stage then).
+// (i, k) at k * ld + i, read back from LDS transposed).  LDS holds 8 KiB images of 128 rows (or columns)
+// by 32 k, in stages of both operands' 256 and, for a split fp32 operand, both planes.
 // Everything outside an operand's extents is fetched out of the buffer's range, which gives zeros.
 // ------------------------------------------------------------------------------------------------
 // A gradient's scale: G is held in [-1, 1] 2^k, row weights divided by the largest one's magnitude.
@@ -371,6 +370,21 @@ __device__ __forceinline__ void wait_vmcnt() {  // all but the wave's last N loa
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
+// 16 bytes a lane from base + off (zeros past kRange) to the wave's 1 KiB at `dst` in LDS.  In assembly,
+// because after the builtin the compiler waits for every fetch in flight before a transposed read of LDS;
+// it has no register output, and wait_vmcnt is the wait for it.  base and dst are the wave's own.
+__device__ __forceinline__ void fetch16(const u16* base, unsigned off, unsigned char* dst) {
+  const uint64_t b = reinterpret_cast<uint64_t>(base);
+  typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
+  const u32x4 r = {static_cast<unsigned>(b), static_cast<unsigned>(b >> 32) & 0xFFFFu, kRange, 0x00020000u};
+  const unsigned at = reinterpret_cast<uintptr_t>((lds_void*)dst);
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 4\n\t"  // m0 needs one state, a scalar register that a vector instruction wrote five
+      "buffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at), "v"(off), "s"(r)
+      : "memory", "m0");
+}
+
 // a barrier that leaves fetches in flight and that nothing is scheduled across
 __device__ __forceinline__ void phase_barrier() {
   __builtin_amdgcn_sched_barrier(0);
@@ -385,18 +399,19 @@ __device__ __forceinline__ int xcd_remap(int bid, int nwg) {  // consecutive til
   const int q = nwg >> 3, r = nwg & 7, x = bid & 7;
   return (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + (bid >> 3);
 }
-// "row" images: 64-byte rows, chunk ch of row r at ch ^ f(r)
-__device__ __forceinline__ int swz64(int row, int ch) { return row * 64 + ((ch ^ ((-(row >> 2)) & 3)) << 4); }
-// "col" images: [32 k][64 columns], 128-byte rows
-__device__ __forceinline__ int swz128_ch(int row, int ch) { return ch ^ ((((row >> 1) & 1) << 1) | (((row >> 3) & 1) << 2)); }
+// Where 16-byte chunk ch of an image's row lies: at ch ^ swz(row), so that the fragment reads have no bank
+// conflicts.  "Row" operands of two planes: 64-byte rows; of one: 128-byte rows; "col": [32 k][64 columns].
+__device__ __forceinline__ int swz64_row(int row) { return (-(row >> 2)) & 3; }
+__device__ __forceinline__ int swz128_row(int row) { return (row >> 1) & 7; }
+__device__ __forceinline__ int swz128_col(int row) { return (((row >> 1) & 1) << 1) | (((row >> 3) & 1) << 2); }
 
 // columns c0..c0+15 x 32 k of a [32][64] image: lane (g = lane >> 4, i = lane & 15) gets k 8g..8g+7 of column c0 + i
 __device__ __forceinline__ s16x8 tr_frag(const unsigned char* sub, int c0, int lane) {
   const int g = lane >> 4, q = (lane >> 2) & 3, p = lane & 3;
   const int col = c0 + 4 * p;
   const int r0 = 8 * g + q, r1 = r0 + 4;
-  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(sub + r0 * 128 + (swz128_ch(r0, col >> 3) << 4) + ((col & 4) << 1)));
-  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(sub + r1 * 128 + (swz128_ch(r1, col >> 3) << 4) + ((col & 4) << 1)));
+  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(sub + r0 * 128 + (((col >> 3) ^ swz128_col(r0)) << 4) + ((col & 4) << 1)));
+  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(sub + r1 * 128 + (((col >> 3) ^ swz128_col(r1)) << 4) + ((col & 4) << 1)));
   return s16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 }
 
@@ -470,54 +485,63 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(GemmArgs g) {
   const int m0 = mt * kTile, n0 = nt * kTile;
   const int nk = kend > kbeg ? (kend - kbeg + KT - 1) / KT : 0;
 
-  // this lane's 16-byte pieces of the four half tiles: "row" operands 16 rows a wave, 4 lanes a row;
-  // "col" operands 8 k rows of a 64-column image a wave, 8 lanes a row; chunks swizzled at the source
-  const int rrow = lane >> 2, rch = (lane & 3) ^ ((-(rrow >> 2)) & 3);
-  const int crow = (wid & 3) * 8 + (lane >> 3), csub = wid >> 2, cch = swz128_ch(crow, lane & 7);
-  unsigned voff[4];
-  bool vok[4];
+  // This lane's 16-byte pieces of the four half tiles (0, 1: A; 2, 3: B), two 1 KiB pieces a wave and half
+  // tile.  "Row" operands of one plane: 8 rows of 64 k a piece, whole 128-byte lines; of two planes: 16 rows
+  // of 32 k of either.  "Col" operands: 8 k rows of 64 columns of either image.  Chunks are swizzled at the
+  // source.
+  unsigned voff[4][2];
+  bool vok[4][2];
+  int rk[2];  // k of a "row" piece's chunk, within the stage
+  const int crow = (wid & 3) * 8 + (lane >> 3);
 #pragma unroll
-  for (int h = 0; h < 4; ++h) {
-    const bool isa = h < 2, col = isa ? ACOL : BCOL;
-    const int64_t ld = isa ? g.A.ld : g.B.ld;
-    const int origin = isa ? m0 : n0, extent = isa ? M : g.N;
-    if (!col) {
-      const int r = (h & 1) * 128 + wid * 16 + rrow;
-      vok[h] = origin + r < extent;
-      voff[h] = static_cast<unsigned>(r * ld * 2 + rch * 16);
-    } else {
-      const int c = (h & 1) * 128 + csub * 64 + cch * 8;
-      vok[h] = origin + c < extent;
-      voff[h] = static_cast<unsigned>(crow * ld * 2 + c * 2);
+  for (int s = 0; s < 2; ++s) {
+    const int rrow = PL == 1 ? wid * 16 + s * 8 + (lane >> 3) : wid * 16 + (lane >> 2);
+    rk[s] = (PL == 1 ? (lane & 7) ^ swz128_row(rrow) : (lane & 3) ^ swz64_row(rrow)) * 8;
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      const bool isa = h < 2, col = isa ? ACOL : BCOL;
+      const int64_t ld = isa ? g.A.ld : g.B.ld;
+      const int origin = isa ? m0 : n0, extent = isa ? M : g.N;
+      if (!col) {
+        const int r = (h & 1) * 128 + rrow;
+        vok[h][s] = origin + r < extent;
+        voff[h][s] = static_cast<unsigned>(r * ld * 2 + rk[s] * 2);
+      } else {
+        const int c = (h & 1) * 128 + (wid >> 2) * 64 + ((lane & 7) ^ swz128_col(crow)) * 8;
+        vok[h][s] = origin + c < extent;
+        voff[h][s] = static_cast<unsigned>(crow * ld * 2 + c * 2);
+      }
     }
   }
-  auto stage1 = [&](const Operand& op, bool col, int origin, int h, int t) {
-    unsigned char* dst = smem + (t & 1) * kStage + h * kHalf + wid * 1024;
+  // this wave's pieces of half tile h of stage t
+  auto fetch_half = [&](int h, int t) {
+    const bool isa = h < 2, col = isa ? ACOL : BCOL;
+    const Operand& op = isa ? g.A : g.B;
+    unsigned char* half = smem + (t & 1) * kStage + h * kHalf;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       const u16* base = op.p + (PL == 2 ? s * op.plane : 0);
-      const int k0 = kbeg + t * KT + (PL == 1 ? s * 32 : 0);
+      int k0 = kbeg + t * KT;
       bool ok;
-      unsigned off = voff[h];
+      unsigned off = voff[h][s];
       if (!col) {
-        base += origin * op.ld;
-        ok = vok[h] && k0 + rch * 8 < kend;
-        off += static_cast<unsigned>(k0) * 2u;
+        base += (isa ? m0 : n0) * op.ld + k0;
+        ok = vok[h][s] && k0 + rk[s] < kend;
       } else {
-        base += k0 * op.ld + origin;
-        ok = vok[h] && k0 + crow < kend;
+        if (PL == 1) k0 += s * 32;
+        base += k0 * op.ld + (isa ? m0 : n0);
+        ok = vok[h][s] && k0 + crow < kend;
       }
-      const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<u16*>(base), 0, kRange, 0x00020000);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(dst + s * 8192), 16, ok ? off : kOOB, 0, 0, 0);
+      fetch16(base, ok ? off : kOOB, half + (!col && PL == 1 ? wid * 2048 + s * 1024 : s * 8192 + wid * 1024));
     }
   };
-  auto stage_a = [&](int t) {
-    stage1(g.A, ACOL, m0, 0, t);
-    stage1(g.A, ACOL, m0, 1, t);
-  };
-  auto stage_b = [&](int t) {
-    stage1(g.B, BCOL, n0, 2, t);
-    stage1(g.B, BCOL, n0, 3, t);
+  const int fr = lane & 15, fch = lane >> 4;
+  // rows (or columns) r0 .. r0 + 15 of a half tile, part s: its k 32 s .. 32 s + 31, or its plane s
+  auto frag = [&](bool col, const unsigned char* half, int r0, int s) -> s16x8 {
+    if (col) return tr_frag(half + s * 8192 + (r0 >> 6) * 4096, r0 & 63, lane);
+    const int r = r0 + fr;
+    if (PL == 1) return *reinterpret_cast<const s16x8*>(half + r * 128 + (((s * 4 + fch) ^ swz128_row(r)) << 4));
+    return *reinterpret_cast<const s16x8*>(half + s * 8192 + r * 64 + ((fch ^ swz64_row(r)) << 4));
   };
 
   f32x4 acc[8][4];
@@ -525,48 +549,55 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(GemmArgs g) {
   for (int i = 0; i < 8; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // Two stages (64 k, or 32 k of both planes), four phases a stage, a quadrant of the wave's tile each:
+  // fragment reads or fetches, a barrier, 16 or 24 matrix instructions (k halves 0 and 1; hi hi, hi lo, lo
+  // hi), a barrier.  The lower four waves run one barrier late, so on every SIMD one wave multiplies while
+  // the other reads and fetches.  All of a stage's fragments are in registers after its second phase, and
+  // the stage after next is fetched into its place in the fourth, two phases on, where everything older has
+  // to have landed.  With transposed reads or two planes A waits for the first phase of the next stage
+  // (8192 x 4096 x 128000 bf16: G w 7.06 against 7.22 ms, G^T h 7.37 against 7.93; word LM's split logits
+  // 0.135 against 0.155), without it loses (logits 6.4 against 6.8).  Also measured for the logits: a ring
+  // of five stages of 32 k 3 to 6 % slower, four waves of 128 x 128 with reads between the matrix
+  // instructions 7 %, fetches of half lines 2 %, raised wave priority around the matrix instructions 1 %.
+  constexpr bool kAhead = PL == 1 && !ACOL && !BCOL;
   s16x8 af[8][2], bf[4][2];
-  const int fr = lane & 15, fch = lane >> 4;
+  auto fetch_a = [&](int t) {
+    fetch_half(0, t);
+    fetch_half(1, t);
+  };
+  auto fetch_b = [&](int t) {
+    fetch_half(2, t);
+    fetch_half(3, t);
+  };
   auto read_a = [&](int t, int i0) {
     const unsigned char* base = smem + (t & 1) * kStage + wr * kHalf;
 #pragma unroll
     for (int i = i0; i < i0 + 4; ++i)
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
-        af[i][s] = ACOL ? tr_frag(base + s * 8192 + (i >> 2) * 4096, (i * 16) & 63, lane)
-                        : *reinterpret_cast<const s16x8*>(base + s * 8192 + swz64(i * 16 + fr, fch));
+      for (int s = 0; s < 2; ++s) af[i][s] = frag(ACOL, base, i * 16, s);
   };
   auto read_b = [&](int t, int j0) {
     const unsigned char* base = smem + (t & 1) * kStage + (2 + (wc >> 1)) * kHalf;
 #pragma unroll
     for (int j = j0; j < j0 + 2; ++j)
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
-        bf[j][s] = BCOL ? tr_frag(base + s * 8192 + (wc & 1) * 4096, j * 16, lane)
-                        : *reinterpret_cast<const s16x8*>(base + s * 8192 + swz64((wc & 1) * 64 + j * 16 + fr, fch));
+      for (int s = 0; s < 2; ++s) bf[j][s] = frag(BCOL, base, (wc & 1) * 64 + j * 16, s);
   };
   auto mfma = [&](int i0, int j0) {
-    __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int s = 0; s < (PL == 1 ? 2 : 3); ++s)
 #pragma unroll
       for (int i = i0; i < i0 + 4; ++i)
 #pragma unroll
-        for (int j = j0; j < j0 + 2; ++j)  // one plane: k halves 0, 1; two: hi hi, hi lo, lo hi
-          acc[i][j] = mfma16<F16>(bf[j][PL == 1 ? s : s & 1], af[i][PL == 1 ? s : s >> 1], acc[i][j]);
-    __builtin_amdgcn_s_setprio(0);
+        for (int j = j0; j < j0 + 2; ++j) acc[i][j] = mfma16<F16>(bf[j][PL == 1 ? s : s & 1], af[i][PL == 1 ? s : s >> 1], acc[i][j]);
   };
-
-  // Four phases a stage, a quadrant of the wave's tile each: reads and fetches, barrier, matrix
-  // instructions, barrier.  The lower four waves run one barrier late, so on every SIMD one wave
-  // multiplies while the other reads and fetches.  A(t + 1) is fetched in the first phase of stage t, B(t + 2)
-  // in the last (B(t) is in registers since the second), where everything older has to have landed.
   if (nk > 0) {
-    stage_a(0);
-    stage_b(0);
+    fetch_a(0);
+    fetch_b(0);
     if (nk > 1) {
-      stage_b(1);
-      wait_vmcnt<4>();
+      if (kAhead) fetch_a(1);
+      fetch_b(1);
+      wait_vmcnt<kAhead ? 8 : 4>();
     } else {
       wait_vmcnt<0>();
     }
@@ -576,7 +607,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(GemmArgs g) {
   for (int t = 0; t < nk; ++t) {
     read_a(t, 0);
     read_b(t, 0);
-    if (t + 1 < nk) stage_a(t + 1);
+    if (!kAhead && t + 1 < nk) fetch_a(t + 1);
     phase_barrier();
     wait_lgkm0();
     mfma(0, 0);
@@ -591,8 +622,9 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(GemmArgs g) {
     mfma(4, 2);
     phase_barrier();
     if (t + 2 < nk) {
-      stage_b(t + 2);
-      wait_vmcnt<4>();
+      if (kAhead) fetch_a(t + 2);
+      fetch_b(t + 2);
+      wait_vmcnt<kAhead ? 8 : 4>();
     } else {
       wait_vmcnt<0>();
     }
