@@ -360,8 +360,9 @@ __host__ __device__ inline int split_length(int tiles, int chunk) {
 constexpr int kTile = 256, kThreads = 512;
 constexpr int kHalf = 16384, kStage = 4 * kHalf;
 constexpr int kLdc = kTile + 16, kLdc32 = kTile + 4;
-constexpr int kGemmSmem = kTile * kLdc * 2;
-static_assert(kGemmSmem >= 2 * kStage && kGemmSmem >= 128 * kLdc32 * 4, "the epilogues reuse the stages");
+constexpr int kSideOff = kTile * kLdc * 2;  // the rows' and words' numbers for the epilogue, behind the tile
+constexpr int kGemmSmem = kSideOff + kTile * 20;
+static_assert(kSideOff >= 2 * kStage && kSideOff >= 128 * kLdc32 * 4, "the epilogues reuse the stages");
 constexpr unsigned kOOB = 0x80000000u;     // past kRange: the load returns zeros
 constexpr unsigned kRange = 0x7FFFFFF0u;
 
@@ -544,6 +545,29 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(GemmArgs g) {
     return *reinterpret_cast<const s16x8*>(half + s * 8192 + r * 64 + ((fch ^ swz64_row(r)) << 4));
   };
 
+  // what the epilogue needs of each row (maximum, log of the sum, weight, target relative to the tile) and
+  // word (bias; -inf past the last) goes to LDS ahead of the products: there it would be loads in a row
+  f32x4* side_row = reinterpret_cast<f32x4*>(smem + kSideOff);
+  float* side_col = reinterpret_cast<float*>(smem + kSideOff + kTile * 16);
+  if constexpr (EPI == kStats || EPI == kGrad) {
+    if (tid < kTile) {
+      const int row = m0 + tid;
+      f32x4 v = {0.f, 0.f, 0.f, __int_as_float(-1)};
+      if (row < M) {
+        if (EPI == kGrad) {
+          v[0] = g.top[row];
+          v[1] = g.log_s[row];
+          v[2] = g.row_w != nullptr ? g.row_w[row] : g.g_scale;
+        }
+        if (g.words != nullptr) v[3] = __int_as_float(g.words[row] - g.v0 - n0);
+      }
+      side_row[tid] = v;
+    } else {
+      const int col = n0 + tid - kTile;
+      side_col[tid - kTile] = col >= g.N ? kNegInf : g.bias != nullptr ? load_any(g.bias, col, g.bias_dt) : 0.f;
+    }
+  }
+
   f32x4 acc[8][4];
 #pragma unroll
   for (int i = 0; i < 8; ++i)
@@ -642,20 +666,14 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(GemmArgs g) {
   if constexpr (EPI == kStats || EPI == kGrad) {
     const float zs = PL == 1 ? 1.f : pow2(-scale_exp(static_cast<uint32_t>(g.info[1]))) * pow2(-scale_exp(static_cast<uint32_t>(g.info[2])));
     const float c = g.c;
-    f32x4 bias[4];  // -inf past the last word
+    f32x4 bias[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int col = n0 + col0 + j * 16 + r;
-        bias[j][r] = col >= g.N ? kNegInf : g.bias != nullptr ? load_any(g.bias, col, g.bias_dt) : 0.f;
-      }
+    for (int j = 0; j < 4; ++j) bias[j] = *reinterpret_cast<const f32x4*>(side_col + col0 + j * 16);
     if constexpr (EPI == kStats) {
       float* red = reinterpret_cast<float*>(smem);  // [3][4 column waves][256 rows]
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         float m = kNegInf, s = 0.f, sz = 0.f;
-        const int row = m0 + row0 + i * 16;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -663,15 +681,15 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(GemmArgs g) {
             acc[i][j][r] = acc[i][j][r] * zs + bias[j][r];
             m = fmaxf(m, acc[i][j][r]);
           }
-        if (g.words != nullptr && row < M) {
-          const int at = g.words[row] - g.v0 - n0 - col0;  // j * 16 + r if the target is one of this lane's
+        if (g.words != nullptr) {
+          const int at = __float_as_int(side_row[row0 + i * 16][3]) - col0;  // j * 16 + r if the target is one of this lane's
           if (static_cast<unsigned>(at) < 64u && (at & 15) < 4) {
             float z = 0.f;
 #pragma unroll
             for (int j = 0; j < 4; ++j)
 #pragma unroll
               for (int r = 0; r < 4; ++r) z = at == j * 16 + r ? acc[i][j][r] : z;
-            g.picked[row] = z;
+            g.picked[m0 + row0 + i * 16] = z;
           }
         }
         if (g.part_z != nullptr) {
@@ -714,9 +732,9 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(GemmArgs g) {
       // G once into the accumulators: both planes have to come from the same bits of it
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int row = m0 + row0 + i * 16;
-        const bool ok = row < M;
-        const float top = ok ? g.top[row] : 0.f, l = ok ? g.log_s[row] : 0.f, w = ok && g.row_w != nullptr ? g.row_w[row] : g.g_scale;
+        const bool ok = m0 + row0 + i * 16 < M;
+        const f32x4 of = side_row[row0 + i * 16];
+        const float top = of[0], l = of[1], w = of[2];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -724,8 +742,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(GemmArgs g) {
             const float p = exp2_(fmaf(acc[i][j][r] * zs + bias[j][r] - top, c, -l));
             acc[i][j][r] = ok ? w * (p - g.smooth_v) : 0.f;
           }
-        if (g.words != nullptr && ok) {
-          const int at = g.words[row] - g.v0 - n0 - col0;
+        if (g.words != nullptr) {
+          const int at = __float_as_int(of[3]) - col0;
           if (static_cast<unsigned>(at) < 64u && (at & 15) < 4) {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
@@ -1192,6 +1210,17 @@ __device__ __forceinline__ void walk(const typename Elem<DT>::type* p, int lo, i
   }
   const int rest = start + whole * W;
   if (tid < hi - rest) f(rest + tid, to_f<DT>(p[rest + tid]));
+}
+
+// whether a row's list has an entry, found by one wave
+__device__ __forceinline__ bool has_list(const LogitArgs& a, int n, int lane) {
+  bool any = false;
+  for (int k = lane; k < a.K; k += 64) {
+    int64_t word;
+    float t;
+    any |= list_entry(a.index, n * a.index_ld + k, a.wide, a.teacher, n * a.teacher_ld + k, a.teacher_dt, word, t);
+  }
+  return __ballot(any) != 0;
 }
 
 template <int DT>
