@@ -1192,27 +1192,32 @@ struct LogitArgs {
   int64_t dz_ld;
 };
 
-// elements of a segment in 16-byte pieces: f(column, value) for the ragged ends, and for whole pieces
-template <int DT, class F>
-__device__ __forceinline__ void walk(const typename Elem<DT>::type* p, int lo, int hi, int tid, int nthr, F&& f) {
+// One pass over a segment, four 16-byte pieces a thread in flight: f(column, its W values) for the whole
+// pieces from the first 16-byte boundary on, f1(column, value) for what is before and behind them.
+template <int DT, class F, class F1>
+__device__ __forceinline__ void walk(const typename Elem<DT>::type* p, int lo, int hi, int tid, F&& f, F1&& f1) {
   typedef typename Elem<DT>::type T;
   constexpr int W = 16 / sizeof(T);
   typedef __attribute__((ext_vector_type(W))) T V;
   const int mis = static_cast<int>((reinterpret_cast<uintptr_t>(p + lo) & 15) / sizeof(T));
   int start = lo + (mis ? W - mis : 0);
   if (start > hi) start = hi;
-  const int whole = (hi - start) / W;
-  if (tid < start - lo) f(lo + tid, to_f<DT>(p[lo + tid]));
-  for (int i = tid; i < whole; i += nthr) {
-    const V v = *reinterpret_cast<const V*>(p + start + i * W);
+  const int whole = (hi - start) / W, rest = start + whole * W;
+  if (tid < start - lo) f1(lo + tid, p[lo + tid]);
+  if (tid < hi - rest) f1(rest + tid, p[rest + tid]);
+  const V* q = reinterpret_cast<const V*>(p + start);
+  int i = tid;
+  for (; i + 3 * 256 < whole; i += 4 * 256) {
+    V v[4];
 #pragma unroll
-    for (int e = 0; e < W; ++e) f(start + i * W + e, to_f<DT>(v[e]));
+    for (int u = 0; u < 4; ++u) v[u] = q[i + u * 256];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) f(start + (i + u * 256) * W, v[u]);
   }
-  const int rest = start + whole * W;
-  if (tid < hi - rest) f(rest + tid, to_f<DT>(p[rest + tid]));
+  for (; i < whole; i += 256) f(start + i * W, q[i]);
 }
 
-// whether a row's list has an entry, found by one wave
+// whether a row's list has an entry (every wave of a block finds the same)
 __device__ __forceinline__ bool has_list(const LogitArgs& a, int n, int lane) {
   bool any = false;
   for (int k = lane; k < a.K; k += 64) {
@@ -1223,40 +1228,10 @@ __device__ __forceinline__ bool has_list(const LogitArgs& a, int n, int lane) {
   return __ballot(any) != 0;
 }
 
-template <int DT>
-__global__ void __launch_bounds__(256) logit_stats_kernel(LogitArgs a) {
-  __shared__ float red[2][4];
-  typedef typename Elem<DT>::type T;
-  const int n = blockIdx.x / a.segs, seg = blockIdx.x - n * a.segs, tid = threadIdx.x;
-  const T* z = static_cast<const T*>(a.z) + n * a.z_ld;
-  const int lo = seg * a.seg_len;
-  int hi = lo + a.seg_len;
-  if (hi > a.V) hi = a.V;
+// a row's loss and shares from its maximum and sum, by one wave; returns the loss (all lanes)
+__device__ __forceinline__ double finish_row(const LogitArgs& a, int n, float m, float s, int lane, bool& kept) {
   const float c = a.inv_t * kLog2e;
-  float m = kNegInf, s = 0.f;
-  if (lo < hi) walk<DT>(z, lo, hi, tid, 256, [&](int, float v) { join(m, s, v, 1.f, c); });
-  join_lanes(m, s, 64, c);
-  if ((tid & 63) == 0) {
-    red[0][tid >> 6] = m;
-    red[1][tid >> 6] = s;
-  }
-  __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < 4; ++w) join(m, s, red[0][w], red[1][w], c);
-    a.part[static_cast<int64_t>(n) * a.segs + seg] = make_float2(m, s);
-  }
-}
-
-__global__ void __launch_bounds__(256) logit_finish_kernel(LogitArgs a) {
-  const int n = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (n >= a.N) return;
-  const float c = a.inv_t * kLog2e;
-  float m = kNegInf, s = 0.f, tt = kNegInf, ts = 0.f;
-  for (int t = lane; t < a.segs; t += 64) {
-    const float2 v = a.part[static_cast<int64_t>(n) * a.segs + t];
-    join(m, s, v.x, v.y, c);
-  }
-  join_lanes(m, s, 64, c);
+  float tt = kNegInf, ts = 0.f;
   const float log_s = log2f(s);
   const int64_t i0 = n * a.index_ld, t0 = n * a.teacher_ld;
   int64_t word;
@@ -1264,13 +1239,14 @@ __global__ void __launch_bounds__(256) logit_finish_kernel(LogitArgs a) {
   for (int k = lane; k < a.K; k += 64)
     if (list_entry(a.index, i0 + k, a.wide, a.teacher, t0 + k, a.teacher_dt, word, t)) join(tt, ts, t, 1.f, c);
   join_lanes(tt, ts, 64, c);
-  const bool kept = !(ts == 0.f);  // no entry: (-inf, 0); a NaN among them: NaN
+  kept = !(ts == 0.f);  // no entry: (-inf, 0); a NaN among them: NaN
   const float tl = log2f(ts);
   float loss = 0.f;
   for (int k = lane; k < a.K; k += 64) {
     float q = 0.f, z = 0.f;
     if (list_entry(a.index, i0 + k, a.wide, a.teacher, t0 + k, a.teacher_dt, word, t)) {
       q = exp2_(fmaf(t - tt, c, -tl));
+      // a word outside the vocabulary: the row's loss and gradients are NaN
       if (word >= a.V) loss = __builtin_nanf("");
       else z = load_any(a.z, n * a.z_ld + word, a.dt);
       loss += diverge(q, t, tt, tl, z, m, log_s, a.inv_t);
@@ -1278,49 +1254,137 @@ __global__ void __launch_bounds__(256) logit_finish_kernel(LogitArgs a) {
     a.share[static_cast<int64_t>(n) * a.K + k] = q;
   }
   loss = sum_lanes(loss);
+  const double all = kept ? static_cast<double>(loss) / (static_cast<double>(a.inv_t) * a.inv_t) : 0.0;
   if (lane == 0) {
-    const double all = kept ? static_cast<double>(loss) / (static_cast<double>(a.inv_t) * a.inv_t) : 0.0;
     if (a.loss_each != nullptr) a.loss_each[n] = static_cast<float>(all);
     else a.rows[n] = all;
     a.top[n] = m;
     a.log_s[n] = kept ? (loss != loss ? loss : log_s) : __builtin_huge_valf();
   }
+  return all;
 }
 
-// the kept rows, and the sum or mean of their losses
-__global__ void __launch_bounds__(1024) logit_reduce_kernel(const double* rows, const float* log_s, int N, int mean, int* info, float* out) {
+// Maximum and sum of a segment; with one segment a row its loss too.  Bound by the read: 4096 x 128000
+// bf16 runs at 5 TB/s.  A piece's maximum first, so that an element costs one exponential.
+template <int DT>
+__global__ void __launch_bounds__(256) logit_stats_kernel(LogitArgs a) {
+  __shared__ float red[2][4];
+  typedef typename Elem<DT>::type T;
+  constexpr int W = 16 / sizeof(T);
+  typedef __attribute__((ext_vector_type(W))) T V;
+  const int n = blockIdx.x / a.segs, seg = blockIdx.x - n * a.segs, tid = threadIdx.x, lane = tid & 63;
+  const T* z = static_cast<const T*>(a.z) + n * a.z_ld;
+  const int lo = seg * a.seg_len;
+  int hi = lo + a.seg_len;
+  if (hi > a.V) hi = a.V;
+  const float c = a.inv_t * kLog2e;
+  float m = kNegInf, s = 0.f;
+  if (lo < hi && has_list(a, n, lane))
+    walk<DT>(
+        z, lo, hi, tid,
+        [&](int, V v) {
+          float x[W], top = m;
+#pragma unroll
+          for (int e = 0; e < W; ++e) {
+            x[e] = to_f<DT>(v[e]);
+            top = fmaxf(top, x[e]);
+          }
+          const float ref = top == kNegInf ? 0.f : top;
+          s *= exp2_((m - ref) * c);
+#pragma unroll
+          for (int e = 0; e < W; ++e) s += exp2_((x[e] - ref) * c);
+          m = top;
+        },
+        [&](int, T v) { join(m, s, to_f<DT>(v), 1.f, c); });
+  join_lanes(m, s, 64, c);
+  if (lane == 0) {
+    red[0][tid >> 6] = m;
+    red[1][tid >> 6] = s;
+  }
+  __syncthreads();
+  if (tid < 64) {
+    m = red[0][0];
+    s = red[1][0];
+    for (int w = 1; w < 4; ++w) join(m, s, red[0][w], red[1][w], c);
+    bool kept;
+    if (a.segs == 1) finish_row(a, n, m, s, lane, kept);
+    else if (tid == 0) a.part[static_cast<int64_t>(n) * a.segs + seg] = make_float2(m, s);
+  }
+}
+
+__device__ __forceinline__ void join_segments(const LogitArgs& a, int n, int lane, float& m, float& s) {
+  const float c = a.inv_t * kLog2e;
+  m = kNegInf;
+  s = 0.f;
+  for (int t = lane; t < a.segs; t += 64) {
+    const float2 v = a.part[static_cast<int64_t>(n) * a.segs + t];
+    join(m, s, v.x, v.y, c);
+  }
+  join_lanes(m, s, 64, c);
+}
+
+__global__ void __launch_bounds__(256) logit_finish_kernel(LogitArgs a) {
+  const int n = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (n >= a.N) return;
+  float m, s;
+  bool kept;
+  join_segments(a, n, lane, m, s);
+  finish_row(a, n, m, s, lane, kept);
+}
+
+// the kept rows, and the sum or mean of their losses; with `finish` the rows' segments are joined first
+__global__ void __launch_bounds__(1024) logit_reduce_kernel(LogitArgs a, int finish, float* out) {
   __shared__ double part[16];
   __shared__ int cnt[16];
-  double s = 0.0;
-  int c = 0;
-  for (int i = threadIdx.x; i < N; i += 1024) {
-    if (out != nullptr) s += rows[i];
-    c += log_s[i] != __builtin_huge_valf();
+  const int wv = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  double sum = 0.0;
+  int count = 0;
+  if (finish) {
+    for (int n = wv; n < a.N; n += 16) {
+      float m, s;
+      bool kept;
+      join_segments(a, n, lane, m, s);
+      const double loss = finish_row(a, n, m, s, lane, kept);
+      sum += loss;
+      count += kept;
+    }
+  } else {
+    for (int i = threadIdx.x; i < a.N; i += 1024) {
+      sum += a.rows[i];
+      count += a.log_s[i] != __builtin_huge_valf();
+    }
+    for (int o = 1; o < 64; o <<= 1) {
+      sum += __shfl_xor(sum, o, 64);
+      count += __shfl_xor(count, o, 64);
+    }
   }
-  for (int o = 1; o < 64; o <<= 1) {
-    s += __shfl_xor(s, o, 64);
-    c += __shfl_xor(c, o, 64);
-  }
-  if ((threadIdx.x & 63) == 0) {
-    part[threadIdx.x >> 6] = s;
-    cnt[threadIdx.x >> 6] = c;
+  if (lane == 0) {
+    part[wv] = sum;
+    cnt[wv] = count;
   }
   __syncthreads();
   if (threadIdx.x == 0) {
-    s = 0.0;
-    c = 0;
+    sum = 0.0;
+    count = 0;
     for (int w = 0; w < 16; ++w) {
-      s += part[w];
-      c += cnt[w];
+      sum += part[w];
+      count += cnt[w];
     }
-    info[0] = c;
-    if (out != nullptr) *out = static_cast<float>(mean && c > 0 ? s / c : s);
+    a.info[0] = count;
+    *out = static_cast<float>(a.mean && count > 0 ? sum / count : sum);
   }
 }
 
+// The gradient: one read, one write, then the listed words of the segment once more, from the fp32
+// arithmetic (a word's entries add up their shares and write the same value).
 template <int DT>
 __global__ void __launch_bounds__(256) logit_grad_kernel(LogitArgs a) {
+  constexpr int kList = 512;
+  __shared__ int list_word[kList];
+  __shared__ float list_share[kList];
   typedef typename Elem<DT>::type T;
+  constexpr int W = 16 / sizeof(T);
+  typedef __attribute__((ext_vector_type(W))) T V;
   const int n = blockIdx.x / a.segs, seg = blockIdx.x - n * a.segs, tid = threadIdx.x;
   const T* z = static_cast<const T*>(a.z) + n * a.z_ld;
   T* dz = static_cast<T*>(a.dz) + n * a.dz_ld;
@@ -1329,22 +1393,47 @@ __global__ void __launch_bounds__(256) logit_grad_kernel(LogitArgs a) {
   if (hi > a.V) hi = a.V;
   if (lo >= hi) return;
   const float top = a.top[n], log_s = a.log_s[n], c = a.inv_t * kLog2e;
-  if (log_s == __builtin_huge_valf()) {  // a row without a list
-    for (int v = lo + tid; v < hi; v += 256) dz[v] = from_f<DT>(0.f);
+  if (log_s == __builtin_huge_valf()) {  // a row without a list: zeros, and no read
+    const V none = {};
+    for (int v = lo + tid * W; v < hi; v += 256 * W) {
+      if (v + W <= hi) __builtin_memcpy(dz + v, &none, sizeof(V));
+      else
+        for (int e = v; e < hi; ++e) dz[e] = from_f<DT>(0.f);
+    }
     return;
   }
   const int count = a.info[0];
   const float g = a.g[a.each ? n : 0] / a.inv_t / (a.mean && count > 0 ? static_cast<float>(count) : 1.f);
-  walk<DT>(z, lo, hi, tid, 256, [&](int v, float x) { dz[v] = from_f<DT>(g * exp2_(fmaf(x - top, c, -log_s))); });
+  walk<DT>(
+      z, lo, hi, tid,
+      [&](int v, V x) {
+        V o;
+#pragma unroll
+        for (int e = 0; e < W; ++e) o[e] = from_f<DT>(g * exp2_(fmaf(to_f<DT>(x[e]) - top, c, -log_s)));
+        __builtin_memcpy(dz + v, &o, sizeof(V));  // 16 bytes, of any alignment
+      },
+      [&](int v, T x) { dz[v] = from_f<DT>(g * exp2_(fmaf(to_f<DT>(x) - top, c, -log_s))); });
   wait_vmcnt<0>();
-  __syncthreads();  // every p is written; the picked words are written over
-  for (int k = tid; k < a.K; k += 256) {
-    const int64_t word = load_index(a.index, n * a.index_ld + k, a.wide);
-    if (word < lo || word >= hi) continue;
+  __syncthreads();  // every p is written
+  const int64_t i0 = n * a.index_ld;
+  for (int k0 = 0; k0 < a.K; k0 += 256) {
+    const int k = k0 + tid;
+    const int64_t word = k < a.K ? load_index(a.index, i0 + k, a.wide) : -1;
+    const bool mine = word >= lo && word < hi;
     float s = 0.f;
-    for (int j = 0; j < a.K; ++j)
-      if (load_index(a.index, n * a.index_ld + j, a.wide) == word) s += a.share[static_cast<int64_t>(n) * a.K + j];
-    dz[word] = from_f<DT>(g * (exp2_(fmaf(to_f<DT>(z[word]) - top, c, -log_s)) - s));
+    for (int j0 = 0; j0 < a.K; j0 += kList) {
+      const int there = a.K - j0 < kList ? a.K - j0 : kList;
+      __syncthreads();
+      for (int j = tid; j < there; j += 256) {
+        const int64_t w = load_index(a.index, i0 + j0 + j, a.wide);
+        list_word[j] = w >= lo && w < hi ? static_cast<int>(w) : -1;
+        list_share[j] = a.share[static_cast<int64_t>(n) * a.K + j0 + j];
+      }
+      __syncthreads();
+      if (mine)
+        for (int j = 0; j < there; ++j) s += list_word[j] == static_cast<int>(word) ? list_share[j] : 0.f;
+    }
+    if (mine) dz[word] = from_f<DT>(g * (exp2_(fmaf(to_f<DT>(z[word]) - top, c, -log_s)) - s));
   }
 }
 
@@ -1800,8 +1889,10 @@ int det_vocab_logits_forward(void* stream, const DetVocabLogits* pp) {
   if (p.dtype == kF32) hipLaunchKernelGGL(logit_stats_kernel<kF32>, grid, dim3(256), 0, st, a);
   else if (p.dtype == kBF16) hipLaunchKernelGGL(logit_stats_kernel<kBF16>, grid, dim3(256), 0, st, a);
   else hipLaunchKernelGGL(logit_stats_kernel<kF16>, grid, dim3(256), 0, st, a);
-  hipLaunchKernelGGL(logit_finish_kernel, dim3(ceil_div(p.N, 4)), dim3(256), 0, st, a);
-  hipLaunchKernelGGL(logit_reduce_kernel, dim3(1), dim3(1024), 0, st, a.rows, a.log_s, p.N, a.mean, p.info, a.each ? nullptr : p.loss);
+  // a loss for each row needs no sum; a few rows are finished by the block that sums them
+  const bool few = p.N <= 32 && !a.each;
+  if (a.segs > 1 && !few) hipLaunchKernelGGL(logit_finish_kernel, dim3(ceil_div(p.N, 4)), dim3(256), 0, st, a);
+  if (!a.each) hipLaunchKernelGGL(logit_reduce_kernel, dim3(1), dim3(1024), 0, st, a, a.segs > 1 && few ? 1 : 0, p.loss);
   return static_cast<int>(hipGetLastError());
 }
 
