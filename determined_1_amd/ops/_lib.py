@@ -254,11 +254,10 @@ _SIGNATURES = {
                        c_int, ctypes.c_int64, c_void_p, c_int], c_int),
     # det_vocab.hip: losses over a vocabulary.  stream, const DetVocabHead* / DetVocabLogits* (vocab_loss._HeadParams,
     # _LogitParams)
-    "det_vocab_head_operand_bytes": ([c_void_p], c_i64),
-    "det_vocab_head_ws_bytes": ([c_void_p, c_int], c_i64),
+    "det_vocab_head_bytes": ([c_void_p, c_int], c_i64),
     "det_vocab_head_forward": ([c_void_p, c_void_p], c_int),
     "det_vocab_head_backward": ([c_void_p, c_void_p], c_int),
-    "det_vocab_logits_ws_bytes": ([c_void_p], c_i64),
+    "det_vocab_logits_bytes": ([c_void_p], c_i64),
     "det_vocab_logits_forward": ([c_void_p, c_void_p], c_int),
     "det_vocab_logits_backward": ([c_void_p, c_void_p], c_int),
 }

@@ -1469,11 +1469,9 @@ struct DetVocabHead {
   void *dx, *dw, *db;             // backward: null where not wanted
   const void* gout;               // backward: fp32 [1] or [N]
   float* loss;                    // forward: [1] or [N]
-  float *stats;                   // [2, N] maxima and log2 of sums, [N, K] picked logits, [N, K] shares: forward writes, backward reads
-  int* rows;                      // [4 + 3 N]: info, the list of kept rows, each row's place in it, targets: forward writes, backward reads
-  void* operands;                 // the packed operands: forward writes, backward reads
+  void* kept;                     // what the forward pass leaves for the backward pass (Head, below)
   void* ws;
-  int64_t ws_bytes, operand_bytes, x_ld, w_ld, index_ld, teacher_ld, ignore;
+  int64_t ws_bytes, kept_bytes, x_ld, w_ld, index_ld, teacher_ld, ignore;
   int N, D, V, K, dtype, bias_dt, wide, teacher_dt, reduction;  // reduction 0 each row, 1 mean, 2 sum
   float inv_t, smooth;
 };
@@ -1484,7 +1482,7 @@ namespace {
 struct Plan {
   int planes, ldh, chunk, nchunks, ntiles, csplits;
   bool pack_w, keep_w;
-  int64_t kept;  // bytes of the operands that the backward pass finds again: the rows, and the weights if they are packed whole
+  int64_t off_rows_info, off_h, off_kw, kept;  // in `kept`
   int64_t off_w, off_flag, off_part, off_partz, off_rows, off_roww, off_alpha, off_g, off_dx, off_cs, total;
 };
 
@@ -1497,7 +1495,10 @@ Plan plan(const DetVocabHead& p, bool backward) {
   q.pack_w = p.dtype == kF32 || p.D % 8 != 0 || p.w_ld % 8 != 0 || (reinterpret_cast<uintptr_t>(p.w) & 15) != 0;
   const int64_t w_bytes = int64_t(2) * q.planes * p.V * q.ldh, h_bytes = up(int64_t(2) * q.planes * p.N * q.ldh, 256);
   q.keep_w = q.pack_w && w_bytes <= kChunkBytes;
-  q.kept = h_bytes + (q.keep_w ? w_bytes : 0);
+  q.off_rows_info = up(int64_t(8) * p.N * (1 + p.K), 256);
+  q.off_h = q.off_rows_info + up(int64_t(4) * (4 + 3 * int64_t(p.N)), 256);
+  q.off_kw = q.off_h + h_bytes;
+  q.kept = q.off_kw + (q.keep_w ? w_bytes : 0);
   int64_t chunk = up(p.V, kTile);
   if (backward) {
     const int64_t fit = kChunkBytes / (int64_t(2) * q.planes * p.N) / kTile * kTile;
@@ -1568,16 +1569,29 @@ int pack_any(hipStream_t st, int dt, const PackArgs& a) {
   return dt == kF32 ? pack<kF32>(st, a) : pack<kBF16>(st, a);  // 16-bit types are copied as bits
 }
 
-u16* hidden_planes(const DetVocabHead& p) { return static_cast<u16*>(p.operands); }
+// The call with its kept parts in place.
+struct Head : DetVocabHead {
+  float* stats;  // [2, N] maxima and log2 of sums, [N, K] picked logits, [N, K] shares
+  int* rows;     // [4 + 3 N]: info, the list of kept rows, each row's place in it, targets
+  u16* hidden;   // the packed hidden states
+  u16* weights;  // the packed weights, if they are packed whole
+  Head(const DetVocabHead& p, const Plan& q) : DetVocabHead(p) {
+    char* at = static_cast<char*>(p.kept);
+    stats = reinterpret_cast<float*>(at);
+    rows = reinterpret_cast<int*>(at + q.off_rows_info);
+    hidden = reinterpret_cast<u16*>(at + q.off_h);
+    weights = reinterpret_cast<u16*>(at + q.off_kw);
+  }
+};
 
-int pack_hidden(hipStream_t st, const DetVocabHead& p, const Plan& q) {
+int pack_hidden(hipStream_t st, const Head& p, const Plan& q) {
   PackArgs a = {};
   a.src = p.x;
   a.src_ld = p.x_ld;
   a.list = p.rows + 4;
   a.count = p.rows;
   a.absmax = p.rows + 1;
-  a.dst = hidden_planes(p);
+  a.dst = p.hidden;
   a.plane = int64_t(p.N) * q.ldh;
   a.rows = p.N;
   a.cols = p.D;
@@ -1586,7 +1600,7 @@ int pack_hidden(hipStream_t st, const DetVocabHead& p, const Plan& q) {
 }
 
 // the weight rows v0 .. v0 + nv as an operand; packs them (all: once, in the forward pass)
-int weight_operand(hipStream_t st, const DetVocabHead& p, const Plan& q, char* ws, int v0, int nv, bool first, Operand* w) {
+int weight_operand(hipStream_t st, const Head& p, const Plan& q, char* ws, int v0, int nv, bool first, Operand* w) {
   const int64_t es = p.dtype == kF32 ? 4 : 2;
   const char* src = static_cast<const char*>(p.w) + v0 * p.w_ld * es;
   if (!q.pack_w) {
@@ -1597,7 +1611,7 @@ int weight_operand(hipStream_t st, const DetVocabHead& p, const Plan& q, char* w
   a.src = q.keep_w ? p.w : src;
   a.src_ld = p.w_ld;
   a.absmax = p.rows + 2;
-  a.dst = reinterpret_cast<u16*>(q.keep_w ? static_cast<char*>(p.operands) + up(int64_t(2) * q.planes * p.N * q.ldh, 256) : ws + q.off_w);
+  a.dst = q.keep_w ? p.weights : reinterpret_cast<u16*>(ws + q.off_w);
   a.plane = int64_t(q.keep_w ? p.V : q.chunk) * q.ldh;
   a.rows = q.keep_w ? p.V : nv;
   a.cols = p.D;
@@ -1606,9 +1620,9 @@ int weight_operand(hipStream_t st, const DetVocabHead& p, const Plan& q, char* w
   return q.keep_w && !first ? 0 : pack_any(st, p.dtype, a);
 }
 
-GemmArgs logits_args(const DetVocabHead& p, const Plan& q, const Operand& w, int v0, int nv) {
+GemmArgs logits_args(const Head& p, const Plan& q, const Operand& w, int v0, int nv) {
   GemmArgs a = {};
-  a.A = Operand{hidden_planes(p), int64_t(p.N) * q.ldh, q.ldh};
+  a.A = Operand{p.hidden, int64_t(p.N) * q.ldh, q.ldh};
   a.B = w;
   a.m_dyn = p.rows;
   a.info = p.rows;
@@ -1630,22 +1644,19 @@ GemmArgs logits_args(const DetVocabHead& p, const Plan& q, const Operand& w, int
 
 extern "C" {
 
-int64_t det_vocab_head_operand_bytes(const DetVocabHead* p) {
+// bytes of `kept` (what 0), of the forward pass's workspace (1), of the backward pass's (2)
+int64_t det_vocab_head_bytes(const DetVocabHead* p, int what) {
   if (p == nullptr || check_head(*p) != 0) return -1;
-  return plan(*p, false).kept;
-}
-
-int64_t det_vocab_head_ws_bytes(const DetVocabHead* p, int backward) {
-  if (p == nullptr || check_head(*p) != 0) return -1;
-  return plan(*p, backward != 0).total;
+  const Plan q = plan(*p, what == 2);
+  return what == 0 ? q.kept : q.total;
 }
 
 int det_vocab_head_forward(void* stream, const DetVocabHead* pp) {
   if (pp == nullptr) return -1;
-  const DetVocabHead& p = *pp;
-  DET_TRY(check_head(p));
-  const Plan q = plan(p, false);
-  if (p.ws == nullptr || p.ws_bytes < q.total || p.operands == nullptr || p.operand_bytes < q.kept) return -6;
+  DET_TRY(check_head(*pp));
+  const Plan q = plan(*pp, false);
+  if (pp->ws == nullptr || pp->ws_bytes < q.total || pp->kept == nullptr || pp->kept_bytes < q.kept) return -6;
+  const Head p(*pp, q);
   hipStream_t st = static_cast<hipStream_t>(stream);
   char* ws = static_cast<char*>(p.ws);
   int* list = p.rows + 4;
@@ -1719,10 +1730,10 @@ int det_vocab_head_forward(void* stream, const DetVocabHead* pp) {
 
 int det_vocab_head_backward(void* stream, const DetVocabHead* pp) {
   if (pp == nullptr) return -1;
-  const DetVocabHead& p = *pp;
-  DET_TRY(check_head(p));
-  const Plan q = plan(p, true);
-  if (p.ws == nullptr || p.ws_bytes < q.total || p.operands == nullptr || p.operand_bytes < q.kept || p.gout == nullptr) return -6;
+  DET_TRY(check_head(*pp));
+  const Plan q = plan(*pp, true);
+  if (pp->ws == nullptr || pp->ws_bytes < q.total || pp->kept == nullptr || pp->kept_bytes < q.kept || pp->gout == nullptr) return -6;
+  const Head p(*pp, q);
   hipStream_t st = static_cast<hipStream_t>(stream);
   char* ws = static_cast<char*>(p.ws);
   int* list = p.rows + 4;
@@ -1788,7 +1799,7 @@ int det_vocab_head_backward(void* stream, const DetVocabHead* pp) {
     if (p.dw != nullptr) {
       GemmArgs d = {};
       d.A = G;
-      d.B = Operand{hidden_planes(p), int64_t(p.N) * q.ldh, q.ldh};
+      d.B = Operand{p.hidden, int64_t(p.N) * q.ldh, q.ldh};
       d.k_dyn = p.rows;
       d.info = p.rows;
       d.M = nv;
@@ -1815,15 +1826,17 @@ struct DetVocabLogits {
   void* dz;
   const void* gout;
   float* loss;
-  float* stats;         // [2, N] maxima and log2 of sums, [N, K] shares
-  int* info;            // [1]
-  void* ws;
-  int64_t ws_bytes, z_ld, index_ld, teacher_ld, dz_ld;
+  // [2, N] maxima and log2 of sums, [N, K] shares, how many rows have a list: forward writes, backward reads;
+  // then the forward pass's workspace
+  float* kept;
+  int64_t kept_bytes, z_ld, index_ld, teacher_ld, dz_ld;
   int N, V, K, dtype, wide, teacher_dt, reduction;
   float inv_t;
 };
 
 namespace {
+
+int64_t logit_kept(const DetVocabLogits& p) { return up(int64_t(4) * p.N * (2 + p.K) + 4, 256); }
 
 LogitArgs logit_args(const DetVocabLogits& p) {
   LogitArgs a = {};
@@ -1848,10 +1861,14 @@ LogitArgs logit_args(const DetVocabLogits& p) {
   a.inv_t = p.inv_t;
   a.each = p.reduction == 0;
   a.mean = p.reduction == 1;
-  a.top = p.stats;
-  a.log_s = p.stats + p.N;
-  a.share = p.stats + int64_t(2) * p.N;
-  a.info = p.info;
+  a.top = p.kept;
+  a.log_s = p.kept + p.N;
+  a.share = p.kept + int64_t(2) * p.N;
+  a.info = reinterpret_cast<int*>(a.share + int64_t(p.N) * p.K);
+  char* ws = reinterpret_cast<char*>(p.kept) + logit_kept(p);
+  a.part = reinterpret_cast<float2*>(ws);
+  a.rows = reinterpret_cast<double*>(ws + up(int64_t(8) * p.N * a.segs, 256));
+  a.loss_each = a.each ? p.loss : nullptr;
   a.g = static_cast<const float*>(p.gout);
   a.dz = p.dz;
   a.dz_ld = p.dz_ld;
@@ -1869,22 +1886,18 @@ int check_logits(const DetVocabLogits& p) {
 
 extern "C" {
 
-int64_t det_vocab_logits_ws_bytes(const DetVocabLogits* p) {
+int64_t det_vocab_logits_bytes(const DetVocabLogits* p) {
   if (p == nullptr || check_logits(*p) != 0) return -1;
-  return up(int64_t(8) * p->N * logit_args(*p).segs, 256) + up(int64_t(8) * p->N, 256);
+  return logit_kept(*p) + up(int64_t(8) * p->N * logit_args(*p).segs, 256) + up(int64_t(8) * p->N, 256);
 }
 
 int det_vocab_logits_forward(void* stream, const DetVocabLogits* pp) {
   if (pp == nullptr) return -1;
   const DetVocabLogits& p = *pp;
   DET_TRY(check_logits(p));
-  if (p.ws == nullptr || p.ws_bytes < det_vocab_logits_ws_bytes(pp)) return -6;
+  if (p.kept == nullptr || p.kept_bytes < det_vocab_logits_bytes(pp)) return -6;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  LogitArgs a = logit_args(p);
-  char* ws = static_cast<char*>(p.ws);
-  a.part = reinterpret_cast<float2*>(ws);
-  a.rows = reinterpret_cast<double*>(ws + up(int64_t(8) * p.N * a.segs, 256));
-  a.loss_each = a.each ? p.loss : nullptr;
+  const LogitArgs a = logit_args(p);
   const dim3 grid(static_cast<unsigned>(p.N) * a.segs);
   if (p.dtype == kF32) hipLaunchKernelGGL(logit_stats_kernel<kF32>, grid, dim3(256), 0, st, a);
   else if (p.dtype == kBF16) hipLaunchKernelGGL(logit_stats_kernel<kBF16>, grid, dim3(256), 0, st, a);
@@ -1900,7 +1913,7 @@ int det_vocab_logits_backward(void* stream, const DetVocabLogits* pp) {
   if (pp == nullptr) return -1;
   const DetVocabLogits& p = *pp;
   DET_TRY(check_logits(p));
-  if (p.gout == nullptr || p.dz == nullptr) return -6;
+  if (p.gout == nullptr || p.dz == nullptr || p.kept == nullptr || p.kept_bytes < det_vocab_logits_bytes(pp)) return -6;
   hipStream_t st = static_cast<hipStream_t>(stream);
   LogitArgs a = logit_args(p);
   const dim3 grid(static_cast<unsigned>(p.N) * a.segs);

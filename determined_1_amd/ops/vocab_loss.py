@@ -33,16 +33,16 @@ _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 class _HeadParams(ctypes.Structure):
     """Mirror of ``DetVocabHead`` (det_vocab.hip)."""
     _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "w", "bias", "target", "index", "teacher", "dx", "dw", "db", "gout",
-                                                "loss", "stats", "rows", "operands", "ws")]
-                + [(n, ctypes.c_int64) for n in ("ws_bytes", "operand_bytes", "x_ld", "w_ld", "index_ld", "teacher_ld", "ignore")]
+                                                "loss", "kept", "ws")]
+                + [(n, ctypes.c_int64) for n in ("ws_bytes", "kept_bytes", "x_ld", "w_ld", "index_ld", "teacher_ld", "ignore")]
                 + [(n, ctypes.c_int32) for n in ("N", "D", "V", "K", "dtype", "bias_dt", "wide", "teacher_dt", "reduction")]
                 + [("inv_t", ctypes.c_float), ("smooth", ctypes.c_float)])
 
 
 class _LogitParams(ctypes.Structure):
     """Mirror of ``DetVocabLogits`` (det_vocab.hip)."""
-    _fields_ = ([(n, ctypes.c_void_p) for n in ("z", "index", "teacher", "dz", "gout", "loss", "stats", "info", "ws")]
-                + [(n, ctypes.c_int64) for n in ("ws_bytes", "z_ld", "index_ld", "teacher_ld", "dz_ld")]
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("z", "index", "teacher", "dz", "gout", "loss", "kept")]
+                + [(n, ctypes.c_int64) for n in ("kept_bytes", "z_ld", "index_ld", "teacher_ld", "dz_ld")]
                 + [(n, ctypes.c_int32) for n in ("N", "V", "K", "dtype", "wide", "teacher_dt", "reduction")]
                 + [("inv_t", ctypes.c_float)])
 
@@ -53,27 +53,15 @@ def _rows_of(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(1) == 1 or t.shape[1] == 1 and t.stride(0) >= 1 else t.contiguous()
 
 
-def _workspace(nbytes: int, like: torch.Tensor, what: str) -> torch.Tensor:
+def _buffer(nbytes: int, like: torch.Tensor, what: str) -> torch.Tensor:
     if nbytes < 0:
         raise ValueError(f"{what}: sizes out of the kernels' range")
     return torch.empty(nbytes, dtype=torch.uint8, device=like.device)
 
 
-def _head_params(x, weight, bias, target, teacher, index, opts) -> _HeadParams:
-    ignore, smooth, heat, reduction = opts
-    p = _HeadParams()
-    p.x, p.w, p.bias = x.data_ptr(), weight.data_ptr(), _ptr(bias)
-    p.x_ld, p.w_ld = x.stride(0), weight.stride(0)
-    p.N, p.D, p.V = x.shape[0], x.shape[1], weight.shape[0]
-    p.dtype, p.bias_dt = dtype_code(x.dtype), 0 if bias is None else dtype_code(bias.dtype)
-    p.ignore, p.smooth, p.inv_t, p.reduction = ignore, smooth, 1.0 / heat, _REDUCTIONS[reduction]
-    if target is not None:
-        p.target, p.K, p.wide = target.data_ptr(), 1, int(target.dtype == torch.int64)
-    else:
-        p.index, p.teacher, p.K = index.data_ptr(), teacher.data_ptr(), index.shape[1]
-        p.index_ld, p.teacher_ld = index.stride(0), teacher.stride(0)
-        p.wide, p.teacher_dt = int(index.dtype == torch.int64), dtype_code(teacher.dtype)
-    return p
+def _on(t: torch.Tensor):
+    """The tensor's device as the current one (a kernel is launched on the current device)."""
+    return _null() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 class _Head(torch.autograd.Function):
@@ -81,28 +69,44 @@ class _Head(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, target, teacher, index, opts):  # type: ignore[override]
-        dev = x.device
-        n, k = x.shape[0], 1 if index is None else index.shape[1]
-        loss = torch.empty(n if opts[3] == "none" else (), dtype=torch.float32, device=dev)
-        stats = torch.empty(n * (2 + 2 * k), dtype=torch.float32, device=dev)
-        rows = torch.empty(4 + 3 * n, dtype=torch.int32, device=dev)
-        p = _head_params(x, weight, bias, target, teacher, index, opts)
-        p.loss, p.rows, p.stats = loss.data_ptr(), rows.data_ptr(), stats.data_ptr()
-        lib = _lib.get_lib()
-        with torch.cuda.device(dev):
-            ws = _workspace(lib.det_vocab_head_ws_bytes(ctypes.byref(p), 0), x, "vocab_loss")
-            operands = _workspace(lib.det_vocab_head_operand_bytes(ctypes.byref(p)), x, "vocab_loss")
-            p.ws, p.ws_bytes, p.operands, p.operand_bytes = ws.data_ptr(), ws.numel(), operands.data_ptr(), operands.numel()
-            _lib.check(lib.det_vocab_head_forward(_stream(x), ctypes.byref(p)), "det_vocab_head_forward")
-        ctx.save_for_backward(x, weight, bias, target, teacher, index, stats, rows, operands)
-        ctx.opts = opts
+        ignore, smooth, heat, reduction = opts
+        p = _HeadParams()
+        p.N, p.D = x.shape
+        p.V = weight.shape[0]
+        p.x, p.w, p.x_ld, p.w_ld = x.data_ptr(), weight.data_ptr(), x.stride(0), weight.stride(0)
+        p.dtype = dtype_code(x.dtype)
+        if bias is not None:
+            p.bias, p.bias_dt = bias.data_ptr(), dtype_code(bias.dtype)
+        p.ignore, p.smooth, p.inv_t, p.reduction = ignore, smooth, 1.0 / heat, _REDUCTIONS[reduction]
+        if target is not None:
+            p.target, p.K, p.wide = target.data_ptr(), 1, target.dtype == torch.int64
+        else:
+            p.index, p.teacher, p.K = index.data_ptr(), teacher.data_ptr(), index.shape[1]
+            p.index_ld, p.teacher_ld = index.stride(0), teacher.stride(0)
+            p.wide, p.teacher_dt = index.dtype == torch.int64, dtype_code(teacher.dtype)
+        ref, lib = ctypes.byref(p), _lib.get_lib()
+        loss = torch.empty(p.N if reduction == "none" else (), dtype=torch.float32, device=x.device)
+        kept = _buffer(lib.det_vocab_head_bytes(ref, 0), x, "vocab_loss")
+        ws = _buffer(lib.det_vocab_head_bytes(ref, 1), x, "vocab_loss")
+        p.loss, p.kept, p.ws = loss.data_ptr(), kept.data_ptr(), ws.data_ptr()
+        p.kept_bytes, p.ws_bytes = kept.numel(), ws.numel()
+        with _on(x):
+            _lib.check(lib.det_vocab_head_forward(_stream(x), ref), "det_vocab_head_forward")
+        ctx.save_for_backward(x, weight, bias, target, teacher, index, kept)
+        ctx.params = p
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gout):  # type: ignore[override]
-        x, weight, bias, target, teacher, index, stats, rows, operands = ctx.saved_tensors
+        x, weight, bias, target, teacher, index, kept = ctx.saved_tensors
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        p = _HeadParams.from_buffer_copy(ctx.params)
+        # the pointers anew: saved-tensor hooks may have moved what was saved
+        p.x, p.w, p.x_ld, p.w_ld, p.kept = x.data_ptr(), weight.data_ptr(), x.stride(0), weight.stride(0), kept.data_ptr()
+        p.bias, p.target = _ptr(bias), _ptr(target)
+        if index is not None:
+            p.index, p.teacher, p.index_ld, p.teacher_ld = index.data_ptr(), teacher.data_ptr(), index.stride(0), teacher.stride(0)
         gout = gout.float().contiguous()
         dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
         dw = db = None
@@ -112,14 +116,12 @@ class _Head(torch.autograd.Function):
                 dw = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device)
         if need_b:
             db = torch.empty(bias.shape, dtype=bias.dtype, device=bias.device)
-        p = _head_params(x, weight, bias, target, teacher, index, ctx.opts)
         p.dx, p.dw, p.db, p.gout = _ptr(dx), _ptr(dw), _ptr(db), gout.data_ptr()
-        p.rows, p.stats, p.operands, p.operand_bytes = rows.data_ptr(), stats.data_ptr(), operands.data_ptr(), operands.numel()
-        lib = _lib.get_lib()
-        with torch.cuda.device(x.device):
-            ws = _workspace(lib.det_vocab_head_ws_bytes(ctypes.byref(p), 1), x, "vocab_loss")
-            p.ws, p.ws_bytes = ws.data_ptr(), ws.numel()
-            _lib.check(lib.det_vocab_head_backward(_stream(x), ctypes.byref(p)), "det_vocab_head_backward")
+        ref, lib = ctypes.byref(p), _lib.get_lib()
+        ws = _buffer(lib.det_vocab_head_bytes(ref, 2), x, "vocab_loss")
+        p.ws, p.ws_bytes = ws.data_ptr(), ws.numel()
+        with _on(x):
+            _lib.check(lib.det_vocab_head_backward(_stream(x), ref), "det_vocab_head_backward")
         return dx, dw, db, None, None, None, None
 
 
@@ -127,43 +129,35 @@ class _Logits(torch.autograd.Function):
     """logits [N, V], teacher and index [N, K]: unit last strides."""
 
     @staticmethod
-    def _params(z, teacher, index, heat, reduction) -> _LogitParams:
-        p = _LogitParams()
-        p.z, p.index, p.teacher = z.data_ptr(), index.data_ptr(), teacher.data_ptr()
-        p.z_ld, p.index_ld, p.teacher_ld = z.stride(0), index.stride(0), teacher.stride(0)
-        p.N, p.V, p.K = z.shape[0], z.shape[1], index.shape[1]
-        p.dtype, p.wide, p.teacher_dt = dtype_code(z.dtype), int(index.dtype == torch.int64), dtype_code(teacher.dtype)
-        p.reduction, p.inv_t = _REDUCTIONS[reduction], 1.0 / heat
-        return p
-
-    @staticmethod
     def forward(ctx, z, teacher, index, heat, reduction):  # type: ignore[override]
-        dev = z.device
-        n, k = z.shape[0], index.shape[1]
-        loss = torch.empty(n if reduction == "none" else (), dtype=torch.float32, device=dev)
-        stats = torch.empty(n * (2 + k) + 1, dtype=torch.float32, device=dev)  # the last one: how many rows have a list
-        p = _Logits._params(z, teacher, index, heat, reduction)
-        p.loss, p.stats, p.info = loss.data_ptr(), stats.data_ptr(), stats.data_ptr() + 4 * n * (2 + k)
-        lib = _lib.get_lib()
-        with torch.cuda.device(dev):
-            ws = _workspace(lib.det_vocab_logits_ws_bytes(ctypes.byref(p)), z, "topk_distill")
-            p.ws, p.ws_bytes = ws.data_ptr(), ws.numel()
-            _lib.check(lib.det_vocab_logits_forward(_stream(z), ctypes.byref(p)), "det_vocab_logits_forward")
-        ctx.save_for_backward(z, teacher, index, stats)
-        ctx.heat, ctx.reduction = heat, reduction
+        p = _LogitParams()
+        p.N, p.V = z.shape
+        p.z, p.index, p.teacher, p.K = z.data_ptr(), index.data_ptr(), teacher.data_ptr(), index.shape[1]
+        p.z_ld, p.index_ld, p.teacher_ld = z.stride(0), index.stride(0), teacher.stride(0)
+        p.dtype, p.wide, p.teacher_dt = dtype_code(z.dtype), index.dtype == torch.int64, dtype_code(teacher.dtype)
+        p.reduction, p.inv_t = _REDUCTIONS[reduction], 1.0 / heat
+        ref, lib = ctypes.byref(p), _lib.get_lib()
+        loss = torch.empty(p.N if reduction == "none" else (), dtype=torch.float32, device=z.device)
+        kept = _buffer(lib.det_vocab_logits_bytes(ref), z, "topk_distill")
+        p.loss, p.kept, p.kept_bytes = loss.data_ptr(), kept.data_ptr(), kept.numel()
+        with _on(z):
+            _lib.check(lib.det_vocab_logits_forward(_stream(z), ref), "det_vocab_logits_forward")
+        ctx.save_for_backward(z, teacher, index, kept)
+        ctx.params = p
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gout):  # type: ignore[override]
-        z, teacher, index, stats = ctx.saved_tensors
-        n, k = z.shape[0], index.shape[1]
+        z, teacher, index, kept = ctx.saved_tensors
+        p = _LogitParams.from_buffer_copy(ctx.params)
+        # the pointers anew: saved-tensor hooks may have moved what was saved
+        p.z, p.index, p.teacher, p.kept = z.data_ptr(), index.data_ptr(), teacher.data_ptr(), kept.data_ptr()
+        p.z_ld, p.index_ld, p.teacher_ld = z.stride(0), index.stride(0), teacher.stride(0)
         gout = gout.float().contiguous()
         dz = torch.empty(z.shape, dtype=z.dtype, device=z.device)
-        p = _Logits._params(z, teacher, index, ctx.heat, ctx.reduction)
-        p.stats, p.info = stats.data_ptr(), stats.data_ptr() + 4 * n * (2 + k)
         p.gout, p.dz, p.dz_ld = gout.data_ptr(), dz.data_ptr(), dz.stride(0)
-        with torch.cuda.device(z.device):
+        with _on(z):
             _lib.check(_lib.get_lib().det_vocab_logits_backward(_stream(z), ctypes.byref(p)), "det_vocab_logits_backward")
         return dz, None, None, None, None
 

@@ -483,10 +483,10 @@ def test_the_kernels_refuse_what_they_do_not_cover(gpu):
 
     lib = vocab_loss._lib.get_lib()
     p = vocab_loss._HeadParams()
-    assert lib.det_vocab_head_ws_bytes(ctypes.byref(p), 0) == -1 and lib.det_vocab_head_forward(None, None) != 0
+    assert lib.det_vocab_head_bytes(ctypes.byref(p), 0) == -1 and lib.det_vocab_head_forward(None, None) != 0
     assert lib.det_vocab_head_forward(None, ctypes.byref(p)) != 0 and lib.det_vocab_head_backward(None, ctypes.byref(p)) != 0
     q = vocab_loss._LogitParams()
-    assert lib.det_vocab_logits_ws_bytes(ctypes.byref(q)) == -1 and lib.det_vocab_logits_forward(None, ctypes.byref(q)) != 0
+    assert lib.det_vocab_logits_bytes(ctypes.byref(q)) == -1 and lib.det_vocab_logits_forward(None, ctypes.byref(q)) != 0
 
 
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32])
@@ -510,3 +510,31 @@ def test_every_logit_at_the_lowest_value_is_a_uniform_row(gpu, dt):
         loss.backward()
         assert abs(loss.item() - math.log(5000)) < 2.0 ** -18 * 10
         torch.testing.assert_close(b.grad[:11].float(), torch.full((11,), 1 / 5000, device=gpu), rtol=2.0 ** -7, atol=0)
+
+
+def test_saved_tensors_may_move(gpu):
+    x, w, b, g = _tensors(gpu, 90, 64, 700, torch.float32)
+    t = torch.randint(0, 700, (90,), generator=g, device=gpu)
+    teacher, index = _lists(gpu, g, 90, 700, 6)
+
+    def all_three():
+        leaves = [a.detach().requires_grad_(True) for a in (x, w, b)]
+        z = torch.nn.functional.linear(*leaves)
+        loss = (linear_cross_entropy(leaves[0], leaves[1], t, leaves[2]) + topk_distill(z, teacher, index)
+                + linear_topk_distill(leaves[0], leaves[1], teacher, index, leaves[2]))
+        return loss, leaves
+
+    loss, leaves = all_three()
+    ref = torch.autograd.grad(loss, leaves)
+    held = []
+
+    def pack(a):
+        held.append(a.cpu())
+        return len(held) - 1
+
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda h: held[h].to(gpu)):
+        loss, leaves = all_three()
+    junk = torch.full((1 << 22,), float("nan"), device=gpu)  # (takes the place of what was freed)
+    got = torch.autograd.grad(loss, leaves)
+    del junk
+    assert all(torch.equal(a, c) for a, c in zip(got, ref))
