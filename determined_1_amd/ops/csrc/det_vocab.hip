@@ -872,25 +872,27 @@ struct FinishArgs {
   float* each;         // losses [N], or null
 };
 
-// x . w for up to four weight rows at a time (null: none), by one wave
+// x . w for four weight rows at a time, by one wave; nothing stands between the loads of a step
 template <int DT>
 __device__ __forceinline__ void dots_wave(const typename Elem<DT>::type* x, const typename Elem<DT>::type* const (&w)[4], int D, int lane,
                                           float (&out)[4]) {
   typedef typename Elem<DT>::type T;
 #pragma unroll
   for (int q = 0; q < 4; ++q) out[q] = 0.f;
-  for (int d = lane * 8; d < D; d += 512) {
+  auto step = [&](int d, int there) {
     T a[8], b[4][8];
-    load8(x + d, D - d, a);
+    load8(x + d, there, a);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) load8(w[q] + d, there, b[q]);
 #pragma unroll
     for (int q = 0; q < 4; ++q)
-      if (w[q] != nullptr) load8(w[q] + d, D - d, b[q]);
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-      if (w[q] != nullptr)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) out[q] = fmaf(to_f<DT>(a[e]), to_f<DT>(b[q][e]), out[q]);
-  }
+      for (int e = 0; e < 8; ++e) out[q] = fmaf(to_f<DT>(a[e]), to_f<DT>(b[q][e]), out[q]);
+  };
+  const int whole = D & ~511;
+#pragma unroll 2
+  for (int d = 0; d < whole; d += 512) step(d + lane * 8, 8);
+  if (whole + lane * 8 < D) step(whole + lane * 8, D - whole - lane * 8);
 #pragma unroll
   for (int q = 0; q < 4; ++q) out[q] = sum_lanes(out[q]);
 }
@@ -982,7 +984,7 @@ __global__ void __launch_bounds__(256) finish_list_kernel(FinishArgs a) {
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         there[q] = k + q < a.K && list_entry(a.index, i0 + k + q, a.wide, a.teacher, t0 + k + q, a.teacher_dt, word[q], t[q]);
-        w[q] = there[q] && word[q] < a.V ? static_cast<const T*>(a.w) + word[q] * a.w_ld : nullptr;
+        w[q] = static_cast<const T*>(a.w) + (there[q] && word[q] < a.V ? word[q] : 0) * a.w_ld;  // (absent: any row, not used)
       }
       dots_wave<DT>(x, w, a.D, lane, z);
 #pragma unroll
@@ -991,8 +993,12 @@ __global__ void __launch_bounds__(256) finish_list_kernel(FinishArgs a) {
         if (there[q]) {
           share = exp2_(fmaf(t[q] - tt, c, -tl));
           // a word outside the vocabulary: the row's loss and gradients are NaN
-          if (word[q] >= a.V) loss = __builtin_nanf("");
-          else if (a.bias != nullptr) z[q] += load_any(a.bias, word[q], a.bias_dt);
+          if (word[q] >= a.V) {
+            loss = __builtin_nanf("");
+            z[q] = 0.f;
+          } else if (a.bias != nullptr) {
+            z[q] += load_any(a.bias, word[q], a.bias_dt);
+          }
           loss += diverge(share, t[q], tt, tl, z[q], m, log_s, a.inv_t);
         }
         if (lane == 0 && k + q < a.K) {
