@@ -315,15 +315,16 @@ struct GemmArgs {
   const int* k_dyn;  // length of the sum (null: K)
   int M, N, K;
   int chunk;                // kPartial: the longest K of the pass, which the splits are made for
+  int cut;                  // whether the last round's tiles may be cut in two
   const int* info;          // scales of fp32 operands
   // kStats, kGrad: z = acc / scales + bias, c = log2(e) / T
   const void* bias;
   int bias_dt;
   float c;
-  float2* part;   // kStats [M][tiles of N]: maximum and sum
+  float2* part;   // kStats [M][parts], 128 columns each: maximum and sum
   float* part_z;  // sum of z / V, or null
   float inv_v;
-  int tile0, ntiles;
+  int parts;
   // kGrad: p = 2^(c (z - top) - log2 sum)
   const float *top, *log_s;  // [M]
   const float* row_w;        // [M] (null: g_scale for each)
@@ -431,14 +432,14 @@ __device__ __forceinline__ float lane_ror(float v) {
 }
 
 // a wave's part of the tile, rounded to 16 bits, as rows of kLdc; two planes: what the rounding took 128 rows on
-template <bool F16, int PL>
-__device__ __forceinline__ void tile_to_lds(const f32x4 (&acc)[8][4], unsigned char* smem, int row0, int col0) {
+template <bool F16, int PL, int FN>
+__device__ __forceinline__ void tile_to_lds(const f32x4 (&acc)[8][FN], unsigned char* smem, int row0, int col0) {
   typedef __attribute__((ext_vector_type(4))) u16 us4;
   u16* ct = reinterpret_cast<u16*>(smem);
 #pragma unroll
   for (int i = 0; i < 8; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < FN; ++j) {
       us4 hi, lo;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -451,39 +452,72 @@ __device__ __forceinline__ void tile_to_lds(const f32x4 (&acc)[8][4], unsigned c
     }
 }
 
-template <bool F16, int PL, bool ACOL, bool BCOL, int EPI>
-__global__ void __launch_bounds__(kThreads, 1) gemm_kernel(GemmArgs g) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  constexpr int KT = PL == 1 ? 64 : 32;  // k per stage
-  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wr = wid >> 2, wc = wid & 3;
+// Where a block works: 256 rows from m0, 256 columns (or, of a tile cut in two, 128) from n0, k from kbeg to kend.
+struct Place {
+  int M, m0, n0, kbeg, kend, split;
+  bool half;
+};
+
+// The blocks of a product: one a tile.  Fewer tiles than CUs: a sum (kPartial) is cut into pieces;
+// otherwise, where the last round of 256 has at most half its CUs busy, its tiles are cut into two halves
+// of 128 columns (a half takes about two thirds of a tile's time).  Counts depend on how many rows are
+// kept, so a grid is sized for all of them and the blocks behind the last one return.
+__device__ __forceinline__ int gemm_blocks(const GemmArgs& g, int epi) {
   const int M = g.m_dyn != nullptr ? *g.m_dyn : g.M;
+  const int tiles = ((M + kTile - 1) / kTile) * ((g.N + kTile - 1) / kTile);
+  if (epi == kPartial && tiles < 256) {
+    const int len = split_length(tiles > 0 ? tiles : 1, g.chunk);
+    return tiles * ((g.chunk + len - 1) / len);
+  }
+  const int last = tiles & 255;
+  return tiles + (g.cut && last <= 128 ? last : 0);
+}
+
+__device__ __forceinline__ Place gemm_place(const GemmArgs& g, int epi, int bid, int blocks) {
+  Place at;
+  at.M = g.m_dyn != nullptr ? *g.m_dyn : g.M;
   const int K = g.k_dyn != nullptr ? *g.k_dyn : g.K;
-  const int ntm = (M + kTile - 1) / kTile, ntn = (g.N + kTile - 1) / kTile;
-  const int total = ntm * ntn;
-  int split = 0, bid = blockIdx.x, kbeg = 0, kend = K;
-  if constexpr (EPI == kPartial) {
-    if (total == 0) return;
-    const int len = split_length(total, g.chunk), splits = (g.chunk + len - 1) / len;
-    if (bid >= total * splits) return;
-    bid = xcd_remap(bid, total * splits);
-    split = bid / total;  // the tiles of one piece, which share its words, stay together
-    bid -= split * total;
-    kbeg = split * len;
-    kend = kbeg + len < K ? kbeg + len : K;
+  const int ntm = (at.M + kTile - 1) / kTile, ntn = (g.N + kTile - 1) / kTile, tiles = ntm * ntn;
+  at.split = at.kbeg = 0;
+  at.kend = K;
+  at.half = false;
+  int tile, side = 0;
+  if (epi == kPartial && tiles < 256) {
+    const int len = split_length(tiles, g.chunk);
+    tile = xcd_remap(bid, blocks);
+    at.split = tile / tiles;  // the tiles of one piece, which share its words, stay together
+    tile -= at.split * tiles;
+    at.kbeg = at.split * len;
+    at.kend = at.kbeg + len < K ? at.kbeg + len : K;
   } else {
-    if (bid >= total) return;  // the grid is sized for every row
-    bid = xcd_remap(bid, total);
+    const int whole = 2 * tiles - blocks;  // (blocks - tiles of them are cut)
+    if (bid < whole) {
+      tile = xcd_remap(bid, whole);
+    } else {
+      const int h = xcd_remap(bid - whole, blocks - whole);
+      tile = whole + (h >> 1);
+      side = h & 1;
+      at.half = true;
+    }
   }
   // tiles go down eight row tiles before they go on to the next column tile: what runs at one time
   // on an XCD then shares both operands
-  const int per = 8 * ntn, band = bid / per, left = ntm - band * 8;
-  const int high = left < 8 ? left : 8;
-  const int in = bid - band * per;
-  const int mt = band * 8 + in % high, nt = in / high;
-  const int m0 = mt * kTile, n0 = nt * kTile;
+  const int per = 8 * ntn, band = tile / per, left = ntm - band * 8;
+  const int high = left < 8 ? left : 8, in = tile - band * per;
+  at.m0 = (band * 8 + in % high) * kTile;
+  at.n0 = in / high * kTile + side * 128;
+  return at;
+}
+
+// One block's tile; FN: fragments of 16 columns a wave, 4, or 2 of a tile cut in two.
+template <bool F16, int PL, bool ACOL, bool BCOL, int EPI, int FN>
+__device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Place& at, unsigned char* smem) {
+  constexpr int KT = PL == 1 ? 64 : 32;  // k per stage
+  constexpr int BN = FN * 64, JH = FN / 2;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wr = wid >> 2, wc = wid & 3;
+  const int M = at.M, m0 = at.m0, n0 = at.n0, kbeg = at.kbeg, kend = at.kend;
   const int nk = kend > kbeg ? (kend - kbeg + KT - 1) / KT : 0;
 
   // This lane's 16-byte pieces of the four half tiles (0, 1: A; 2, 3: B), two 1 KiB pieces a wave and half
@@ -562,17 +596,17 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(GemmArgs g) {
         if (g.words != nullptr) v[3] = __int_as_float(g.words[row] - g.v0 - n0);
       }
       side_row[tid] = v;
-    } else {
+    } else if (tid < kTile + BN) {
       const int col = n0 + tid - kTile;
       side_col[tid - kTile] = col >= g.N ? kNegInf : g.bias != nullptr ? load_any(g.bias, col, g.bias_dt) : 0.f;
     }
   }
 
-  f32x4 acc[8][4];
+  f32x4 acc[8][FN];
 #pragma unroll
   for (int i = 0; i < 8; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   // Two stages (64 k, or 32 k of both planes), four phases a stage, a quadrant of the wave's tile each:
   // fragment reads or fetches, a barrier, 16 or 24 matrix instructions (k halves 0 and 1; hi hi, hi lo, lo
   // hi), a barrier.  The lower four waves run one barrier late, so on every SIMD one wave multiplies while
@@ -584,14 +618,15 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(GemmArgs g) {
   // of five stages of 32 k 3 to 6 % slower, four waves of 128 x 128 with reads between the matrix
   // instructions 7 %, fetches of half lines 2 %, raised wave priority around the matrix instructions 1 %.
   constexpr bool kAhead = PL == 1 && !ACOL && !BCOL;
-  s16x8 af[8][2], bf[4][2];
+  constexpr int kLeft = (kAhead ? 4 : 0) + FN;  // fetches of the stage after next
+  s16x8 af[8][2], bf[FN][2];
   auto fetch_a = [&](int t) {
     fetch_half(0, t);
     fetch_half(1, t);
   };
   auto fetch_b = [&](int t) {
     fetch_half(2, t);
-    fetch_half(3, t);
+    if (FN == 4) fetch_half(3, t);
   };
   auto read_a = [&](int t, int i0) {
     const unsigned char* base = smem + (t & 1) * kStage + wr * kHalf;
@@ -601,11 +636,12 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(GemmArgs g) {
       for (int s = 0; s < 2; ++s) af[i][s] = frag(ACOL, base, i * 16, s);
   };
   auto read_b = [&](int t, int j0) {
-    const unsigned char* base = smem + (t & 1) * kStage + (2 + (wc >> 1)) * kHalf;
+    const int c0 = wc * (FN * 16);  // within the tile
+    const unsigned char* base = smem + (t & 1) * kStage + (2 + (c0 >> 7)) * kHalf;
 #pragma unroll
-    for (int j = j0; j < j0 + 2; ++j)
+    for (int j = j0; j < j0 + JH; ++j)
 #pragma unroll
-      for (int s = 0; s < 2; ++s) bf[j][s] = frag(BCOL, base, (wc & 1) * 64 + j * 16, s);
+      for (int s = 0; s < 2; ++s) bf[j][s] = frag(BCOL, base, (c0 & 127) + j * 16, s);
   };
   auto mfma = [&](int i0, int j0) {
 #pragma unroll
@@ -613,7 +649,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(GemmArgs g) {
 #pragma unroll
       for (int i = i0; i < i0 + 4; ++i)
 #pragma unroll
-        for (int j = j0; j < j0 + 2; ++j) acc[i][j] = mfma16<F16>(bf[j][PL == 1 ? s : s & 1], af[i][PL == 1 ? s : s >> 1], acc[i][j]);
+        for (int j = j0; j < j0 + JH; ++j) acc[i][j] = mfma16<F16>(bf[j][PL == 1 ? s : s & 1], af[i][PL == 1 ? s : s >> 1], acc[i][j]);
   };
   if (nk > 0) {
     fetch_a(0);
@@ -621,7 +657,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(GemmArgs g) {
     if (nk > 1) {
       if (kAhead) fetch_a(1);
       fetch_b(1);
-      wait_vmcnt<kAhead ? 8 : 4>();
+      wait_vmcnt<kLeft>();
     } else {
       wait_vmcnt<0>();
     }
@@ -637,18 +673,18 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(GemmArgs g) {
     mfma(0, 0);
     phase_barrier();
     read_a(t, 4);
-    read_b(t, 2);
+    read_b(t, JH);
     phase_barrier();
     wait_lgkm0();
-    mfma(0, 2);
+    mfma(0, JH);
     phase_barrier();
     phase_barrier();
-    mfma(4, 2);
+    mfma(4, JH);
     phase_barrier();
     if (t + 2 < nk) {
       if (kAhead) fetch_a(t + 2);
       fetch_b(t + 2);
-      wait_vmcnt<kAhead ? 8 : 4>();
+      wait_vmcnt<kLeft>();
     } else {
       wait_vmcnt<0>();
     }
@@ -661,40 +697,40 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(GemmArgs g) {
 
   // The tile is transposed in the accumulators (B is the instruction's first operand), so that a lane's
   // four consecutive values are of one row: acc[i][j][r] is row wr * 128 + i * 16 + fr, column
-  // wc * 64 + j * 16 + fch * 4 + r.  A row's reduction is 16 values in registers and two lane steps.
-  const int row0 = wr * 128 + fr, col0 = wc * 64 + fch * 4;
+  // wc * 16 FN + j * 16 + fch * 4 + r.  A row's reduction is 4 FN values in registers and two lane steps.
+  const int row0 = wr * 128 + fr, col0 = wc * (FN * 16) + fch * 4;
   if constexpr (EPI == kStats || EPI == kGrad) {
     const float zs = PL == 1 ? 1.f : pow2(-scale_exp(static_cast<uint32_t>(g.info[1]))) * pow2(-scale_exp(static_cast<uint32_t>(g.info[2])));
     const float c = g.c;
     f32x4 bias[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) bias[j] = *reinterpret_cast<const f32x4*>(side_col + col0 + j * 16);
+    for (int j = 0; j < FN; ++j) bias[j] = *reinterpret_cast<const f32x4*>(side_col + col0 + j * 16);
     if constexpr (EPI == kStats) {
       float* red = reinterpret_cast<float*>(smem);  // [3][4 column waves][256 rows]
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         float m = kNegInf, s = 0.f, sz = 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < FN; ++j)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             acc[i][j][r] = acc[i][j][r] * zs + bias[j][r];
             m = fmaxf(m, acc[i][j][r]);
           }
         if (g.words != nullptr) {
-          const int at = __float_as_int(side_row[row0 + i * 16][3]) - col0;  // j * 16 + r if the target is one of this lane's
-          if (static_cast<unsigned>(at) < 64u && (at & 15) < 4) {
+          const int word = __float_as_int(side_row[row0 + i * 16][3]) - col0;  // j * 16 + r if the target is one of this lane's
+          if (static_cast<unsigned>(word) < FN * 16u && (word & 15) < 4) {
             float z = 0.f;
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < FN; ++j)
 #pragma unroll
-              for (int r = 0; r < 4; ++r) z = at == j * 16 + r ? acc[i][j][r] : z;
+              for (int r = 0; r < 4; ++r) z = word == j * 16 + r ? acc[i][j][r] : z;
             g.picked[m0 + row0 + i * 16] = z;
           }
         }
         if (g.part_z != nullptr) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
+          for (int j = 0; j < FN; ++j)
 #pragma unroll
             for (int r = 0; r < 4; ++r) sz += n0 + col0 + j * 16 + r < g.N ? acc[i][j][r] * g.inv_v : 0.f;
           sz += __shfl_xor(sz, 16, 64);
@@ -704,16 +740,16 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(GemmArgs g) {
         m = fmaxf(m, __shfl_xor(m, 32, 64));
         const float ref = m == kNegInf ? 0.f : m;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < FN; ++j)
 #pragma unroll
           for (int r = 0; r < 4; ++r) s += exp2_((acc[i][j][r] - ref) * c);
         s += __shfl_xor(s, 16, 64);
         s += __shfl_xor(s, 32, 64);
         if (fch == 0) {
-          const int at = wc * 256 + row0 + i * 16;
-          red[at] = m;
-          red[1024 + at] = s;
-          red[2048 + at] = sz;
+          const int to = wc * 256 + row0 + i * 16;
+          red[to] = m;
+          red[1024 + to] = s;
+          red[2048 + to] = sz;
         }
       }
       __syncthreads();
@@ -724,9 +760,14 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(GemmArgs g) {
           join(m, s, red[w * 256 + tid], red[1024 + w * 256 + tid], c);
           sz += red[2048 + w * 256 + tid];
         }
-        const int64_t at = static_cast<int64_t>(m0 + tid) * g.ntiles + g.tile0 + nt;
-        g.part[at] = make_float2(m, s);
-        if (g.part_z != nullptr) g.part_z[at] = sz;
+        // a place for every 128 columns; a whole tile fills two
+        const int64_t to = static_cast<int64_t>(m0 + tid) * g.parts + (g.v0 + n0) / 128;
+        g.part[to] = make_float2(m, s);
+        if (FN == 4) g.part[to + 1] = make_float2(kNegInf, 0.f);
+        if (g.part_z != nullptr) {
+          g.part_z[to] = sz;
+          if (FN == 4) g.part_z[to + 1] = 0.f;
+        }
       }
     } else {
       // G once into the accumulators: both planes have to come from the same bits of it
@@ -736,26 +777,26 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(GemmArgs g) {
         const f32x4 of = side_row[row0 + i * 16];
         const float top = of[0], l = of[1], w = of[2];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < FN; ++j)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const float p = exp2_(fmaf(acc[i][j][r] * zs + bias[j][r] - top, c, -l));
             acc[i][j][r] = ok ? w * (p - g.smooth_v) : 0.f;
           }
         if (g.words != nullptr) {
-          const int at = __float_as_int(of[3]) - col0;
-          if (static_cast<unsigned>(at) < 64u && (at & 15) < 4) {
+          const int word = __float_as_int(of[3]) - col0;
+          if (static_cast<unsigned>(word) < FN * 16u && (word & 15) < 4) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < FN; ++j)
 #pragma unroll
-              for (int r = 0; r < 4; ++r) acc[i][j][r] -= at == j * 16 + r ? w * g.share : 0.f;
+              for (int r = 0; r < 4; ++r) acc[i][j][r] -= word == j * 16 + r ? w * g.share : 0.f;
           }
         }
       }
       if (g.colsum != nullptr) {  // before G is rounded
         float* red = reinterpret_cast<float*>(smem);  // [2 row waves][256 columns]
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < FN; ++j) {
           f32x4 t = acc[0][j];
 #pragma unroll
           for (int i = 1; i < 8; ++i) t += acc[i][j];
@@ -769,7 +810,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(GemmArgs g) {
           if (fr == 0) *reinterpret_cast<f32x4*>(red + wr * 256 + col0 + j * 16) = t;
         }
         __syncthreads();
-        if (tid < 256 && n0 + tid < g.ldg) g.colsum[static_cast<int64_t>(mt) * g.ldg + n0 + tid] = red[tid] + red[256 + tid];
+        if (tid < BN && n0 + tid < g.ldg) g.colsum[static_cast<int64_t>(m0 / kTile) * g.ldg + n0 + tid] = red[tid] + red[256 + tid];
         __syncthreads();
       }
       // one plane: the whole tile through LDS; two: both planes of half the rows at a time
@@ -778,22 +819,22 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(GemmArgs g) {
         const int rows = kTile / PL;
         if (PL == 1 || wr == half) tile_to_lds<F16, PL>(acc, smem, PL == 1 ? row0 : fr, col0);
         __syncthreads();
-        for (int q = tid; q < kTile * (kTile / 8); q += kThreads) {
-          const int at = q >> 5, cc = (q & 31) * 8, pl = at / rows, row = half * rows + at % rows;
+        for (int q = tid; q < kTile * (BN / 8); q += kThreads) {
+          const int line = q / (BN / 8), cc = (q % (BN / 8)) * 8, pl = line / rows, row = half * rows + line % rows;
           if (m0 + row < M && n0 + cc < g.ldg)
             *reinterpret_cast<us8*>(g.G + pl * g.g_plane + static_cast<int64_t>(m0 + row) * g.ldg + n0 + cc) =
-                *reinterpret_cast<const us8*>(reinterpret_cast<const u16*>(smem) + at * kLdc + cc);
+                *reinterpret_cast<const us8*>(reinterpret_cast<const u16*>(smem) + line * kLdc + cc);
         }
         if (half + 1 < PL) __syncthreads();
       }
     }
   } else if constexpr (EPI == kPartial) {
-    float* out = g.out32 + split * (M * g.ldo);
+    float* out = g.out32 + at.split * (M * g.ldo);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int row = m0 + row0 + i * 16;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < FN; ++j) {
         const int col = n0 + col0 + j * 16;
         if (row < M && col < g.ldo) {
           f32x4* o = reinterpret_cast<f32x4*>(out + row * g.ldo + col);
@@ -809,7 +850,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(GemmArgs g) {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] *= alpha;
+      for (int j = 0; j < FN; ++j) acc[i][j] *= alpha;
     if constexpr (PL == 1) {
       const bool wide = (g.ldo & 7) == 0 && (reinterpret_cast<uintptr_t>(g.out) & 15) == 0;
       tile_to_lds<F16, 1>(acc, smem, row0, col0);
@@ -817,14 +858,14 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(GemmArgs g) {
       const u16* ct = reinterpret_cast<const u16*>(smem);
       u16* out = static_cast<u16*>(g.out);
       if (wide) {
-        for (int q = tid; q < kTile * (kTile / 8); q += kThreads) {
-          const int row = q >> 5, cc = (q & 31) * 8;
+        for (int q = tid; q < kTile * (BN / 8); q += kThreads) {
+          const int row = q / (BN / 8), cc = (q % (BN / 8)) * 8;
           if (m0 + row < M && n0 + cc < g.N)
             *reinterpret_cast<us8*>(out + (m0 + row) * g.ldo + n0 + cc) = *reinterpret_cast<const us8*>(ct + row * kLdc + cc);
         }
       } else {
-        for (int q = tid; q < kTile * kTile; q += kThreads) {
-          const int row = q >> 8, cc = q & 255;
+        for (int q = tid; q < kTile * BN; q += kThreads) {
+          const int row = q / BN, cc = q % BN;
           if (m0 + row < M && n0 + cc < g.N) out[(m0 + row) * g.ldo + n0 + cc] = ct[row * kLdc + cc];
         }
       }
@@ -837,18 +878,34 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(GemmArgs g) {
 #pragma unroll
           for (int i = 0; i < 8; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) *reinterpret_cast<f32x4*>(ct + (fr + i * 16) * kLdc32 + col0 + j * 16) = acc[i][j];
+            for (int j = 0; j < FN; ++j) *reinterpret_cast<f32x4*>(ct + (fr + i * 16) * kLdc32 + col0 + j * 16) = acc[i][j];
         __syncthreads();
-        for (int q = tid; q < 128 * kTile; q += kThreads) {
-          const int row = q >> 8, cc = q & 255;
+        for (int q = tid; q < 128 * BN; q += kThreads) {
+          const int row = q / BN, cc = q % BN;
           if (m0 + half * 128 + row < M && n0 + cc < g.N) out[(m0 + half * 128 + row) * g.ldo + n0 + cc] = ct[row * kLdc32 + cc];
         }
         __syncthreads();
       }
     }
   }
+}
+
+template <bool F16, int PL, bool ACOL, bool BCOL, int EPI>
+__device__ __forceinline__ void gemm_block(const GemmArgs& g, int bid, int blocks, unsigned char* smem) {
+  const Place at = gemm_place(g, EPI, bid, blocks);
+  if (at.half) gemm_tile<F16, PL, ACOL, BCOL, EPI, 2>(g, at, smem);
+  else gemm_tile<F16, PL, ACOL, BCOL, EPI, 4>(g, at, smem);
+}
+
+template <bool F16, int PL, bool ACOL, bool BCOL, int EPI>
+__global__ void __launch_bounds__(kThreads, 1) gemm_kernel(GemmArgs g) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  const int blocks = gemm_blocks(g, EPI);
+  if (static_cast<int>(blockIdx.x) < blocks) gemm_block<F16, PL, ACOL, BCOL, EPI>(g, blockIdx.x, blocks, smem);
 #endif
 }
+
 
 // ------------------------------------------------------------------------------------------------
 // Joining a row's tiles, its K picked logits, its loss.  One wave a row (cross entropy) or four (lists).
@@ -856,7 +913,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(GemmArgs g) {
 struct FinishArgs {
   const void *x, *w, *bias;
   int64_t x_ld, w_ld;
-  int dt, bias_dt, D, V, K, ntiles, N;
+  int dt, bias_dt, D, V, K, parts, N;
   const int *info, *list;
   const float2* part;
   const float* part_z;
@@ -915,8 +972,8 @@ __global__ void __launch_bounds__(256) finish_target_kernel(FinishArgs a) {
   const int lane = threadIdx.x & 63, count = a.info[0];
   for (int row = blockIdx.x * 4 + (threadIdx.x >> 6); row < count; row += gridDim.x * 4) {
     float m = kNegInf, s = 0.f, sz = 0.f;
-    const int64_t at = static_cast<int64_t>(row) * a.ntiles;
-    for (int t = lane; t < a.ntiles; t += 64) {
+    const int64_t at = static_cast<int64_t>(row) * a.parts;
+    for (int t = lane; t < a.parts; t += 64) {
       const float2 v = a.part[at + t];
       join(m, s, v.x, v.y, kLog2e);
       if (a.part_z != nullptr) sz += a.part_z[at + t];
@@ -950,8 +1007,8 @@ __global__ void __launch_bounds__(256) finish_list_kernel(FinishArgs a) {
   for (int row = blockIdx.x; row < count; row += gridDim.x) {
     const int n = a.list[row];
     float m = kNegInf, s = 0.f;
-    for (int t = tid; t < a.ntiles; t += 256) {
-      const float2 v = a.part[static_cast<int64_t>(row) * a.ntiles + t];
+    for (int t = tid; t < a.parts; t += 256) {
+      const float2 v = a.part[static_cast<int64_t>(row) * a.parts + t];
       join(m, s, v.x, v.y, c);
     }
     join_lanes(m, s, 64, c);
@@ -1455,7 +1512,8 @@ int launch_gemm(hipStream_t st, const GemmArgs& a) {
   const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, kGemmSmem);
   if (e != hipSuccess) return static_cast<int>(e);
   int64_t tiles = static_cast<int64_t>(ceil_div(a.M, kTile)) * ceil_div(a.N, kTile);
-  if (EPI == kPartial && tiles < 256) tiles = 256;  // pieces of the sum, by how many rows are kept
+  tiles += 128;                                     // cut ones of the last round
+  if (EPI == kPartial && tiles < 256) tiles = 256;  // pieces of the sum
   if (tiles >= (int64_t(1) << 31)) return -4;
   hipLaunchKernelGGL((gemm_kernel<F16, PL, ACOL, BCOL, EPI>), dim3(static_cast<unsigned>(tiles)), dim3(kThreads), kGemmSmem, st, a);
   return static_cast<int>(hipGetLastError());
@@ -1486,7 +1544,7 @@ namespace {
 
 // What both directions lay out in the workspace.
 struct Plan {
-  int planes, ldh, chunk, nchunks, ntiles, csplits;
+  int planes, ldh, chunk, nchunks, parts, csplits;
   bool pack_w, keep_w;
   int64_t off_rows_info, off_h, off_kw, kept;  // in `kept`
   int64_t off_w, off_flag, off_part, off_partz, off_rows, off_roww, off_alpha, off_g, off_dx, off_cs, total;
@@ -1519,7 +1577,7 @@ Plan plan(const DetVocabHead& p, bool backward) {
   q.nchunks = ceil_div(p.V, chunk);
   q.chunk = static_cast<int>(up(ceil_div(p.V, q.nchunks), kTile));  // even chunks
   q.nchunks = ceil_div(p.V, q.chunk);
-  q.ntiles = ceil_div(p.V, kTile);
+  q.parts = 2 * ceil_div(p.V, kTile);
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t o = at;
@@ -1529,8 +1587,8 @@ Plan plan(const DetVocabHead& p, bool backward) {
   q.off_w = q.pack_w && !q.keep_w ? take(int64_t(2) * q.planes * q.chunk * q.ldh) : 0;
   if (!backward) {
     q.off_flag = take(p.N);
-    q.off_part = take(int64_t(8) * p.N * q.ntiles);
-    q.off_partz = p.smooth != 0.f ? take(int64_t(4) * p.N * q.ntiles) : 0;
+    q.off_part = take(int64_t(8) * p.N * q.parts);
+    q.off_partz = p.smooth != 0.f ? take(int64_t(4) * p.N * q.parts) : 0;
     q.off_rows = take(int64_t(8) * p.N);
   } else {
     q.off_roww = take(int64_t(4) * p.N);
@@ -1637,6 +1695,7 @@ GemmArgs logits_args(const Head& p, const Plan& q, const Operand& w, int v0, int
   a.K = q.ldh;
   if (p.bias != nullptr) a.bias = static_cast<const char*>(p.bias) + int64_t(v0) * (p.bias_dt == kF32 ? 4 : 2);
   a.bias_dt = p.bias_dt;
+  a.cut = 1;
   a.c = p.inv_t * kLog2e;
   a.inv_v = 1.f / static_cast<float>(p.V);
   if (p.target != nullptr) a.words = p.rows + 4 + int64_t(2) * p.N;
@@ -1685,8 +1744,7 @@ int det_vocab_head_forward(void* stream, const DetVocabHead* pp) {
     GemmArgs a = logits_args(p, q, w, v0, nv);
     a.part = reinterpret_cast<float2*>(ws + q.off_part);
     a.part_z = p.smooth != 0.f ? reinterpret_cast<float*>(ws + q.off_partz) : nullptr;
-    a.tile0 = v0 / kTile;
-    a.ntiles = q.ntiles;
+    a.parts = q.parts;
     DET_TRY((gemm<false, false, kStats>(st, p.dtype, a)));
   }
   FinishArgs f = {};
@@ -1701,7 +1759,7 @@ int det_vocab_head_forward(void* stream, const DetVocabHead* pp) {
   f.V = p.V;
   f.K = p.K;
   f.N = p.N;
-  f.ntiles = q.ntiles;
+  f.parts = q.parts;
   f.info = p.rows;
   f.list = list;
   f.part = reinterpret_cast<const float2*>(ws + q.off_part);
@@ -1797,6 +1855,7 @@ int det_vocab_head_backward(void* stream, const DetVocabHead* pp) {
       d.N = p.D;
       d.K = nv;
       d.chunk = q.chunk;
+      d.cut = 1;
       d.out32 = reinterpret_cast<float*>(ws + q.off_dx);
       d.ldo = q.ldh;
       d.add = c > 0;
@@ -1811,6 +1870,7 @@ int det_vocab_head_backward(void* stream, const DetVocabHead* pp) {
       d.M = nv;
       d.N = p.D;
       d.K = p.N;
+      d.cut = 1;
       d.out = static_cast<char*>(p.dw) + int64_t(v0) * p.D * es;
       d.ldo = p.D;
       d.alpha = alpha;
