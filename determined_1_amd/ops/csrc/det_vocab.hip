@@ -143,41 +143,58 @@ __global__ void __launch_bounds__(256) list_flags_kernel(RowArgs a) {
   if (lane == 0) a.flag[n] = votes != 0;
 }
 
+// one block; eight neighbouring rows a thread, whose targets are read together
 __global__ void __launch_bounds__(1024) rows_kernel(RowArgs a) {
   __shared__ int wave_n[16];
-  __shared__ int base_n;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  if (tid == 0) base_n = 0;
-  __syncthreads();
-  for (int n0 = 0; n0 < a.N; n0 += 1024) {
-    const int n = n0 + tid;
-    bool keep = false;
-    int64_t word = 0;
-    if (n < a.N) {
-      if (a.target != nullptr) {
-        word = load_index(a.target, n, a.wide);
-        keep = word != a.ignore;
-      } else {
-        keep = a.flag[n] != 0;
+  int done = 0;  // kept rows of earlier rounds
+  for (int n0 = 0; n0 < a.N; n0 += 8192) {
+    const int first = n0 + tid * 8;
+    int64_t word[8];
+    unsigned keep = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      word[e] = 0;
+      if (first + e < a.N) {
+        if (a.target != nullptr) {
+          word[e] = load_index(a.target, first + e, a.wide);
+          keep |= (word[e] != a.ignore ? 1u : 0u) << e;
+        } else {
+          keep |= (a.flag[first + e] != 0 ? 1u : 0u) << e;
+        }
       }
     }
-    const uint64_t votes = __ballot(keep);
-    if (lane == 0) wave_n[w] = __popcll(votes);
+    const int mine = __popc(keep);
+    int upto = mine;  // with the lanes below
+    for (int o = 1; o < 64; o <<= 1) {
+      const int v = __shfl_up(upto, o, 64);
+      if (lane >= o) upto += v;
+    }
+    if (lane == 63) wave_n[w] = upto;
     __syncthreads();
-    int before = base_n;
-    for (int i = 0; i < w; ++i) before += wave_n[i];
-    const int at = before + __popcll(votes & ((uint64_t(1) << lane) - 1));
-    if (keep) a.list[at] = n;
-    if (keep && a.target != nullptr) a.words[at] = word >= 0 && word < a.V ? static_cast<int>(word) : -1;
-    if (n < a.N) a.pos[n] = keep ? at : -1;
-    if (n < a.N && a.each != nullptr && !keep) a.each[n] = 0.f;
-    __syncthreads();
-    if (tid == 0)
-      for (int i = 0; i < 16; ++i) base_n += wave_n[i];
+    int at = done + upto - mine;
+    for (int i = 0; i < 16; ++i) {
+      if (i < w) at += wave_n[i];
+      done += wave_n[i];
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int n = first + e;
+      if (n >= a.N) continue;
+      const bool k = (keep >> e) & 1;
+      a.pos[n] = k ? at : -1;
+      if (k) {
+        a.list[at] = n;
+        if (a.target != nullptr) a.words[at] = word[e] >= 0 && word[e] < a.V ? static_cast<int>(word[e]) : -1;
+        ++at;
+      } else if (a.each != nullptr) {
+        a.each[n] = 0.f;
+      }
+    }
     __syncthreads();
   }
   if (tid == 0) {
-    a.info[0] = base_n;
+    a.info[0] = done;
     a.info[1] = 0;
     a.info[2] = 0;
   }
@@ -1550,7 +1567,7 @@ struct Plan {
   int64_t off_w, off_flag, off_part, off_partz, off_rows, off_roww, off_alpha, off_g, off_dx, off_cs, total;
 };
 
-constexpr int64_t kChunkBytes = int64_t(256) << 20;  // G of one chunk, and the packed weights of one
+constexpr int64_t kChunkBytes = int64_t(512) << 20;  // G of one chunk, and the packed weights of one
 
 Plan plan(const DetVocabHead& p, bool backward) {
   Plan q = {};
