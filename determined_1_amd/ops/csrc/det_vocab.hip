@@ -537,54 +537,70 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Place& at, un
   const int M = at.M, m0 = at.m0, n0 = at.n0, kbeg = at.kbeg, kend = at.kend;
   const int nk = kend > kbeg ? (kend - kbeg + KT - 1) / KT : 0;
 
-  // This lane's 16-byte pieces of the four half tiles (0, 1: A; 2, 3: B), two 1 KiB pieces a wave and half
-  // tile.  "Row" operands of one plane: 8 rows of 64 k a piece, whole 128-byte lines; of two planes: 16 rows
-  // of 32 k of either.  "Col" operands: 8 k rows of 64 columns of either image.  Chunks are swizzled at the
-  // source.
+  // This lane's part of the four half tiles (0, 1: A; 2, 3: B): a wave fetches two 1 KiB pieces of each, q 0
+  // of what a stage's first phase reads and q 1 of what only its second does (a "col" B: both for the first).
+  // "Row" operands of one plane: 8 rows of 64 k, whole 128-byte lines; of two planes: 16 rows of 32 k of
+  // either.  "Col" operands: 8 k rows of 64 columns.  Chunks are swizzled at the source.
+  constexpr bool kBSplit = !BCOL && FN == 4;  // B's pieces in order of need: columns 0-31, then 32-63 of a wave
   unsigned voff[4][2];
   bool vok[4][2];
-  int rk[2];  // k of a "row" piece's chunk, within the stage
+  int rk[4][2];  // k of a "row" piece's chunk, within the stage
   const int crow = (wid & 3) * 8 + (lane >> 3);
+  auto piece_row = [&](int h, int q) {  // the first row of a "row" piece
+    const int w = PL == 1 ? wid : wid >> 1, each = PL == 1 ? 8 : 16;
+    if (h < 2 || !kBSplit) return q * 64 + w * each;
+    return (w * each >> 5) * 64 + (w * each & 31) + q * 32;
+  };
 #pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    const int rrow = PL == 1 ? wid * 16 + s * 8 + (lane >> 3) : wid * 16 + (lane >> 2);
-    rk[s] = (PL == 1 ? (lane & 7) ^ swz128_row(rrow) : (lane & 3) ^ swz64_row(rrow)) * 8;
+  for (int h = 0; h < 4; ++h)
 #pragma unroll
-    for (int h = 0; h < 4; ++h) {
+    for (int q = 0; q < 2; ++q) {
       const bool isa = h < 2, col = isa ? ACOL : BCOL;
       const int64_t ld = isa ? g.A.ld : g.B.ld;
       const int origin = isa ? m0 : n0, extent = isa ? M : g.N;
       if (!col) {
-        const int r = (h & 1) * 128 + rrow;
-        vok[h][s] = origin + r < extent;
-        voff[h][s] = static_cast<unsigned>(r * ld * 2 + rk[s] * 2);
+        const int row = piece_row(h, q) + (PL == 1 ? lane >> 3 : lane >> 2), r = (h & 1) * 128 + row;
+        rk[h][q] = (PL == 1 ? (lane & 7) ^ swz128_row(row) : (lane & 3) ^ swz64_row(row)) * 8;
+        vok[h][q] = origin + r < extent;
+        voff[h][q] = static_cast<unsigned>(r * ld * 2 + rk[h][q] * 2);
       } else {
-        const int c = (h & 1) * 128 + (wid >> 2) * 64 + ((lane & 7) ^ swz128_col(crow)) * 8;
-        vok[h][s] = origin + c < extent;
-        voff[h][s] = static_cast<unsigned>(crow * ld * 2 + c * 2);
+        const int c = (h & 1) * 128 + q * 64 + ((lane & 7) ^ swz128_col(crow)) * 8;
+        rk[h][q] = 0;
+        vok[h][q] = origin + c < extent;
+        voff[h][q] = static_cast<unsigned>(crow * ld * 2 + c * 2);
       }
     }
-  }
-  // this wave's pieces of half tile h of stage t
-  auto fetch_half = [&](int h, int t) {
+  auto fetch = [&](int h, int q, int t) {
     const bool isa = h < 2, col = isa ? ACOL : BCOL;
     const Operand& op = isa ? g.A : g.B;
+    const int part = col ? wid >> 2 : wid & 1;  // which 32 k, or which plane ("row" of one plane: neither)
     unsigned char* half = smem + (t & 1) * kStage + h * kHalf;
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const u16* base = op.p + (PL == 2 ? s * op.plane : 0);
-      int k0 = kbeg + t * KT;
-      bool ok;
-      unsigned off = voff[h][s];
-      if (!col) {
-        base += (isa ? m0 : n0) * op.ld + k0;
-        ok = vok[h][s] && k0 + rk[s] < kend;
-      } else {
-        if (PL == 1) k0 += s * 32;
-        base += k0 * op.ld + (isa ? m0 : n0);
-        ok = vok[h][s] && k0 + crow < kend;
-      }
-      fetch16(base, ok ? off : kOOB, half + (!col && PL == 1 ? wid * 2048 + s * 1024 : s * 8192 + wid * 1024));
+    const u16* base = op.p + (PL == 2 ? part * op.plane : 0);
+    int k0 = kbeg + t * KT;
+    bool ok;
+    if (!col) {
+      base += (isa ? m0 : n0) * op.ld + k0;
+      ok = vok[h][q] && k0 + rk[h][q] < kend;
+      half += PL == 1 ? piece_row(h, q) * 128 : part * 8192 + piece_row(h, q) * 64;
+    } else {
+      if (PL == 1) k0 += part * 32;
+      base += k0 * op.ld + (isa ? m0 : n0);
+      ok = vok[h][q] && k0 + crow < kend;
+      half += part * 8192 + q * 4096 + (wid & 3) * 1024;
+    }
+    fetch16(base, ok ? voff[h][q] : kOOB, half);
+  };
+  // a stage's fetches in the order that they are issued in, two a group
+  auto group = [&](int which, int t) {
+    if (which == 0 || which == 3) {
+      fetch(0, which & 1, t);
+      fetch(1, which & 1, t);
+    } else if (kBSplit) {
+      fetch(2, which - 1, t);
+      fetch(3, which - 1, t);
+    } else if (FN == 4 || which == 1) {
+      fetch(1 + which, 0, t);
+      fetch(1 + which, 1, t);
     }
   };
   const int fr = lane & 15, fch = lane >> 4;
@@ -625,26 +641,15 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Place& at, un
 #pragma unroll
     for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   // Two stages (64 k, or 32 k of both planes), four phases a stage, a quadrant of the wave's tile each:
-  // fragment reads or fetches, a barrier, 16 or 24 matrix instructions (k halves 0 and 1; hi hi, hi lo, lo
-  // hi), a barrier.  The lower four waves run one barrier late, so on every SIMD one wave multiplies while
-  // the other reads and fetches.  All of a stage's fragments are in registers after its second phase, and
-  // the stage after next is fetched into its place in the fourth, two phases on, where everything older has
-  // to have landed.  With transposed reads or two planes A waits for the first phase of the next stage
-  // (8192 x 4096 x 128000 bf16: G w 7.06 against 7.22 ms, G^T h 7.37 against 7.93; word LM's split logits
-  // 0.135 against 0.155), without it loses (logits 6.4 against 6.8).  Also measured for the logits: a ring
-  // of five stages of 32 k 3 to 6 % slower, four waves of 128 x 128 with reads between the matrix
-  // instructions 7 %, fetches of half lines 2 %, raised wave priority around the matrix instructions 1 %.
-  constexpr bool kAhead = PL == 1 && !ACOL && !BCOL;
-  constexpr int kLeft = (kAhead ? 4 : 0) + FN;  // fetches of the stage after next
+  // fragment reads and two fetches, a barrier, 16 or 24 matrix instructions (k halves 0 and 1; hi hi, hi lo,
+  // lo hi), a barrier.  The lower four waves run one barrier late, so on every SIMD one wave multiplies while
+  // the other reads and fetches.  All of a stage's fragments are in registers after its second phase.  A
+  // place is fetched into again two phases after its last read: the stage after next's A for its first
+  // phase in the third, B in the fourth and the next first, A for the second phase in the next second, so
+  // that every phase issues as many (all eight in one phase held its barrier up); what a phase reads has
+  // landed a phase before, with kAfterB or kAfterA fetches still on their way.
+  constexpr int kAfterB = kBSplit ? 8 : 6, kAfterA = FN == 4 ? 6 : 4, kRest = kBSplit ? 4 : 2;
   s16x8 af[8][2], bf[FN][2];
-  auto fetch_a = [&](int t) {
-    fetch_half(0, t);
-    fetch_half(1, t);
-  };
-  auto fetch_b = [&](int t) {
-    fetch_half(2, t);
-    if (FN == 4) fetch_half(3, t);
-  };
   auto read_a = [&](int t, int i0) {
     const unsigned char* base = smem + (t & 1) * kStage + wr * kHalf;
 #pragma unroll
@@ -669,14 +674,16 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Place& at, un
         for (int j = j0; j < j0 + JH; ++j) acc[i][j] = mfma16<F16>(bf[j][PL == 1 ? s : s & 1], af[i][PL == 1 ? s : s >> 1], acc[i][j]);
   };
   if (nk > 0) {
-    fetch_a(0);
-    fetch_b(0);
+    group(0, 0);
+    group(1, 0);
+    group(2, 0);
+    group(3, 0);
     if (nk > 1) {
-      if (kAhead) fetch_a(1);
-      fetch_b(1);
-      wait_vmcnt<kLeft>();
+      group(0, 1);
+      group(1, 1);
+      wait_vmcnt<kAfterB>();
     } else {
-      wait_vmcnt<0>();
+      wait_vmcnt<kRest>();
     }
   }
   phase_barrier();
@@ -684,26 +691,32 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Place& at, un
   for (int t = 0; t < nk; ++t) {
     read_a(t, 0);
     read_b(t, 0);
-    if (!kAhead && t + 1 < nk) fetch_a(t + 1);
+    if (t + 1 < nk) {
+      group(2, t + 1);
+      wait_vmcnt<kAfterA>();
+    } else {
+      wait_vmcnt<0>();
+    }
     phase_barrier();
     wait_lgkm0();
     mfma(0, 0);
     phase_barrier();
     read_a(t, 4);
     read_b(t, JH);
+    if (t + 1 < nk) group(3, t + 1);
     phase_barrier();
     wait_lgkm0();
     mfma(0, JH);
     phase_barrier();
+    if (t + 2 < nk) group(0, t + 2);
     phase_barrier();
     mfma(4, JH);
     phase_barrier();
     if (t + 2 < nk) {
-      if (kAhead) fetch_a(t + 2);
-      fetch_b(t + 2);
-      wait_vmcnt<kLeft>();
+      group(1, t + 2);
+      wait_vmcnt<kAfterB>();
     } else {
-      wait_vmcnt<0>();
+      wait_vmcnt<kRest>();
     }
     phase_barrier();
     mfma(4, 0);
