@@ -16,7 +16,7 @@ tensors run the plain composite below.  Both are differentiable once.
 """
 import ctypes
 import math
-from typing import Any, Optional, Tuple
+from typing import Any, Optional
 
 import torch
 import torch.nn.functional as F
@@ -49,8 +49,13 @@ class _LogitParams(ctypes.Structure):
 
 def _rows_of(t: torch.Tensor) -> torch.Tensor:
     """[..., C] as [rows, C] with a unit last stride (a view where the layout allows it)."""
-    t = t.reshape(-1, t.shape[-1])
-    return t if t.stride(1) == 1 or t.shape[1] == 1 and t.stride(0) >= 1 else t.contiguous()
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    return t if t.stride(1) == 1 else t.contiguous()
+
+
+def _apart(teacher: torch.Tensor) -> torch.Tensor:
+    return teacher.detach() if teacher.requires_grad else teacher
 
 
 def _buffer(nbytes: int, like: torch.Tensor, what: str) -> torch.Tensor:
@@ -213,56 +218,68 @@ def _plain_distill(z: torch.Tensor, teacher: torch.Tensor, index: torch.Tensor, 
 # ------------------------------------------------------------------------------------------------
 # public API
 # ------------------------------------------------------------------------------------------------
-def _check(ok: bool, what: str, message: str, error: Any = ValueError) -> None:
-    if not ok:
-        raise error(f"{what}: {message}")
+def _refuse(what: str, message: str, error: Any = ValueError) -> None:
+    raise error(f"{what}: {message}")
 
 
-def _check_common(what: str, reduction: str, *ts: Optional[torch.Tensor]) -> None:
-    _check(reduction in _REDUCTIONS, what, f"reduction {reduction!r} is none of {sorted(_REDUCTIONS)}")
-    given = [t for t in ts if t is not None]
-    _check(all(t.device == given[0].device for t in given), what, "tensors on different devices")
-    _check(given[0].device.type in ("cpu", "cuda"), what, f"no kernels for {given[0].device}")
+def _check_common(what: str, reduction: str, first: torch.Tensor, *ts: Optional[torch.Tensor]) -> None:
+    if reduction not in _REDUCTIONS:
+        _refuse(what, f"reduction {reduction!r} is none of {sorted(_REDUCTIONS)}")
+    device = first.device
+    for t in ts:
+        if t is not None and t.device != device:
+            _refuse(what, f"tensors on {device} and {t.device}")
+    if device.type not in ("cpu", "cuda"):
+        _refuse(what, f"no kernels for {device}")
 
 
 def _check_float(what: str, x: torch.Tensor, name: str) -> None:
-    _check(x.dtype in _FLOATS or (x.dtype == torch.float64 and x.device.type == "cpu"), what,
-           f"{name} is {x.dtype}: bfloat16, float16 or float32 expected", TypeError)
+    if x.dtype not in _FLOATS and not (x.dtype == torch.float64 and x.device.type == "cpu"):
+        _refuse(what, f"{name} is {x.dtype}: bfloat16, float16 or float32 expected", TypeError)
 
 
 def _check_head(what: str, x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor]) -> None:
-    _check(x.dim() >= 1 and weight.dim() == 2 and x.shape[-1] == weight.shape[1] and weight.numel() > 0, what,
-           f"x [..., D] and weight [V, D] expected, got {tuple(x.shape)} and {tuple(weight.shape)}")
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or weight.numel() == 0:
+        _refuse(what, f"x [..., D] and weight [V, D] expected, got {tuple(x.shape)} and {tuple(weight.shape)}")
+    if bias is not None and bias.shape != weight.shape[:1]:
+        _refuse(what, f"bias of {weight.shape[0]} words expected, got {tuple(bias.shape)}")
+    if x.is_cuda and torch.is_autocast_enabled("cuda"):
+        return  # which casts them alike
     _check_float(what, x, "x")
-    _check(weight.dtype == x.dtype, what, f"x is {x.dtype} and weight {weight.dtype}", TypeError)
-    if bias is not None:
-        _check(bias.shape == (weight.shape[0],), what, f"bias of {weight.shape[0]} words expected, got {tuple(bias.shape)}")
-        _check(bias.dtype in (x.dtype, torch.float32), what, f"x is {x.dtype} and bias {bias.dtype}", TypeError)
+    if weight.dtype != x.dtype:
+        _refuse(what, f"x is {x.dtype} and weight {weight.dtype}", TypeError)
+    if bias is not None and bias.dtype not in (x.dtype, torch.float32):
+        _refuse(what, f"x is {x.dtype} and bias {bias.dtype}", TypeError)
 
 
-def _check_lists(what: str, lead: Tuple[int, ...], teacher: torch.Tensor, index: torch.Tensor, heat: float) -> None:
-    _check(index.dim() == len(lead) + 1 and tuple(index.shape[:-1]) == lead and index.shape[-1] > 0 and teacher.shape == index.shape,
-           what, f"teacher_logits and teacher_index {lead + ('K',)} expected, got {tuple(teacher.shape)} and {tuple(index.shape)}")
-    _check(index.dtype in (torch.int32, torch.int64), what, f"teacher_index is {index.dtype}: int32 or int64 expected", TypeError)
+def _check_lists(what: str, lead: torch.Size, teacher: torch.Tensor, index: torch.Tensor, heat: float) -> None:
+    if index.shape[:-1] != lead or index.dim() == 0 or index.shape[-1] == 0 or teacher.shape != index.shape:
+        _refuse(what, f"teacher_logits and teacher_index {tuple(lead) + ('K',)} expected, got {tuple(teacher.shape)} and "
+                      f"{tuple(index.shape)}")
+    if index.dtype not in (torch.int32, torch.int64):
+        _refuse(what, f"teacher_index is {index.dtype}: int32 or int64 expected", TypeError)
     _check_float(what, teacher, "teacher_logits")
-    _check(2.0 ** -20 <= heat <= 2.0 ** 20, what, f"temperature {heat} is not within [2^-20, 2^20]")
+    if not 2.0 ** -20 <= heat <= 2.0 ** 20:
+        _refuse(what, f"temperature {heat} is not within [2^-20, 2^20]")
 
 
-def _empty(reduction: str, lead: Tuple[int, ...], *ts: torch.Tensor) -> torch.Tensor:
+def _empty(reduction: str, lead: torch.Size, *ts: Optional[torch.Tensor]) -> torch.Tensor:
     """The loss of no rows: 0, with gradients of zeros."""
     zero = sum((t * 0).sum().float() for t in ts if t is not None)
     return zero if reduction != "none" else zero.expand(lead)
 
 
 def _linear(x, weight, bias, target, teacher, index, opts, lead) -> torch.Tensor:
-    (x, weight, bias), ac = _autocast(x, weight, bias)
+    ac = x.is_cuda and torch.is_autocast_enabled("cuda")
+    if ac:
+        (x, weight, bias), _ = _autocast(x, weight, bias)
     if x.numel() == 0:
         return _empty(opts[3], lead, x, weight, bias)
     x2 = _rows_of(x)
     if target is not None:
-        target = target.reshape(-1).contiguous()
+        target = target.reshape(-1).contiguous() if target.dim() != 1 or not target.is_contiguous() else target
     else:
-        teacher, index = _rows_of(teacher.detach()), _rows_of(index)
+        teacher, index = _rows_of(_apart(teacher)), _rows_of(index)
     if x.device.type == "cpu":
         z = F.linear(_wide(x2), _wide(weight), None if bias is None else _wide(bias).to(_wide(x2).dtype))
         loss = (_plain_ce(z, target, opts[0], opts[1], opts[3]) if target is not None
@@ -270,11 +287,11 @@ def _linear(x, weight, bias, target, teacher, index, opts, lead) -> torch.Tensor
     else:
         if weight.stride(1) != 1:
             weight = weight.contiguous()
-        if bias is not None:
+        if bias is not None and bias.stride(0) != 1:
             bias = bias.contiguous()
         with torch.autocast("cuda", enabled=False) if ac else _null():
             loss = _Head.apply(x2, weight, bias, target, teacher, index, opts)
-    return loss.reshape(lead) if opts[3] == "none" else loss
+    return loss if opts[3] != "none" or len(lead) == 1 else loss.reshape(lead)
 
 
 def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
@@ -288,13 +305,15 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     it scores tokens: the loss [...] is each target's negative log-probability."""
     what = "linear_cross_entropy"
     _check_common(what, reduction, x, weight, target, bias)
-    if not (torch.is_autocast_enabled("cuda") and x.is_cuda):
-        _check_head(what, x, weight, bias)
-    _check(tuple(target.shape) == tuple(x.shape[:-1]), what, f"target {tuple(x.shape[:-1])} expected, got {tuple(target.shape)}")
-    _check(target.dtype in (torch.int32, torch.int64), what, f"target is {target.dtype}: int32 or int64 expected", TypeError)
-    _check(0.0 <= label_smoothing <= 1.0, what, f"label_smoothing {label_smoothing} is not within [0, 1]")
-    return _linear(x, weight, bias, target, None, None, (int(ignore_index), float(label_smoothing), 1.0, reduction),
-                   tuple(x.shape[:-1]))
+    _check_head(what, x, weight, bias)
+    lead = x.shape[:-1]
+    if target.shape != lead:
+        _refuse(what, f"target {tuple(lead)} expected, got {tuple(target.shape)}")
+    if target.dtype not in (torch.int32, torch.int64):
+        _refuse(what, f"target is {target.dtype}: int32 or int64 expected", TypeError)
+    if not 0.0 <= label_smoothing <= 1.0:
+        _refuse(what, f"label_smoothing {label_smoothing} is not within [0, 1]")
+    return _linear(x, weight, bias, target, None, None, (int(ignore_index), float(label_smoothing), 1.0, reduction), lead)
 
 
 def linear_topk_distill(x: torch.Tensor, weight: torch.Tensor, teacher_logits: torch.Tensor, teacher_index: torch.Tensor,
@@ -304,11 +323,10 @@ def linear_topk_distill(x: torch.Tensor, weight: torch.Tensor, teacher_logits: t
     x [..., D], weight [V, D], bias [V]; the lists [..., K] as in ``topk_distill``."""
     what = "linear_topk_distill"
     _check_common(what, reduction, x, weight, teacher_logits, teacher_index, bias)
-    if not (torch.is_autocast_enabled("cuda") and x.is_cuda):
-        _check_head(what, x, weight, bias)
-    _check_lists(what, tuple(x.shape[:-1]), teacher_logits, teacher_index, float(temperature))
-    return _linear(x, weight, bias, None, teacher_logits, teacher_index, (-100, 0.0, float(temperature), reduction),
-                   tuple(x.shape[:-1]))
+    _check_head(what, x, weight, bias)
+    lead, heat = x.shape[:-1], float(temperature)
+    _check_lists(what, lead, teacher_logits, teacher_index, heat)
+    return _linear(x, weight, bias, None, teacher_logits, teacher_index, (-100, 0.0, heat, reduction), lead)
 
 
 def topk_distill(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_index: torch.Tensor, *, temperature: float = 1.0,
@@ -323,15 +341,16 @@ def topk_distill(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ind
     vocabulary gives its row a NaN loss and NaN gradients."""
     what = "topk_distill"
     _check_common(what, reduction, logits, teacher_logits, teacher_index)
-    _check(logits.dim() >= 1 and logits.shape[-1] > 0, what, f"logits [..., V] expected, got {tuple(logits.shape)}")
+    if logits.dim() < 1 or logits.shape[-1] == 0:
+        _refuse(what, f"logits [..., V] expected, got {tuple(logits.shape)}")
     _check_float(what, logits, "logits")
-    lead = tuple(logits.shape[:-1])
-    _check_lists(what, lead, teacher_logits, teacher_index, float(temperature))
+    lead, heat = logits.shape[:-1], float(temperature)
+    _check_lists(what, lead, teacher_logits, teacher_index, heat)
     if logits.numel() == 0:
         return _empty(reduction, lead, logits)
-    z, teacher, index = _rows_of(logits), _rows_of(teacher_logits.detach()), _rows_of(teacher_index)
+    z, teacher, index = _rows_of(logits), _rows_of(_apart(teacher_logits)), _rows_of(teacher_index)
     if logits.device.type == "cpu":
-        loss = _plain_distill(_wide(z), teacher, index, float(temperature), reduction)
+        loss = _plain_distill(_wide(z), teacher, index, heat, reduction)
     else:
-        loss = _Logits.apply(z, teacher, index, float(temperature), reduction)
-    return loss.reshape(lead) if reduction == "none" else loss
+        loss = _Logits.apply(z, teacher, index, heat, reduction)
+    return loss if reduction != "none" or len(lead) == 1 else loss.reshape(lead)
