@@ -1590,7 +1590,9 @@ Plan plan(const DetVocabHead& p, bool backward) {
   Plan q = {};
   q.planes = p.dtype == kF32 ? 2 : 1;
   q.ldh = static_cast<int>(up(p.D, 8));
-  q.pack_w = p.dtype == kF32 || p.D % 8 != 0 || p.w_ld % 8 != 0 || (reinterpret_cast<uintptr_t>(p.w) & 15) != 0;
+  // read as they are: 16-byte rows, and 256 of them within 32-bit offsets
+  q.pack_w = p.dtype == kF32 || p.D % 8 != 0 || p.w_ld % 8 != 0 || (reinterpret_cast<uintptr_t>(p.w) & 15) != 0 ||
+             p.w_ld > (int64_t(1) << 21);
   const int64_t w_bytes = int64_t(2) * q.planes * p.V * q.ldh, h_bytes = up(int64_t(2) * q.planes * p.N * q.ldh, 256);
   q.keep_w = q.pack_w && w_bytes <= kChunkBytes;
   q.off_rows_info = up(int64_t(8) * p.N * (1 + p.K), 256);
@@ -1646,7 +1648,7 @@ int check_head(const DetVocabHead& p) {
   if (p.dtype < 0 || p.dtype > 2 || p.reduction < 0 || p.reduction > 2) return -2;
   if ((p.target == nullptr) == (p.index == nullptr)) return -3;
   // offsets inside a tile are 32-bit: 256 rows of an operand, 64 rows of G
-  if (p.D > (1 << 21) || p.w_ld > (int64_t(1) << 21) || p.V > (1 << 30) || p.N > (1 << 30)) return -4;
+  if (p.D > (1 << 21) || p.V > (1 << 30) || p.N > (1 << 30)) return -4;
   return 0;
 }
 
@@ -1979,7 +1981,7 @@ LogitArgs logit_args(const DetVocabLogits& p) {
 int check_logits(const DetVocabLogits& p) {
   if (p.N < 1 || p.V < 1 || p.K < 1) return -1;
   if (p.dtype < 0 || p.dtype > 2 || p.reduction < 0 || p.reduction > 2) return -2;
-  if (p.V > (1 << 30) || p.N > (1 << 20)) return -4;
+  if (p.V > (1 << 30) || p.N > (1 << 30)) return -4;
   return 0;
 }
 

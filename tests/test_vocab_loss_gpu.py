@@ -19,8 +19,10 @@ import math
 import pytest
 import torch
 
+from determined_1_amd import pytorch
 from determined_1_amd.ops import vocab_loss
 from determined_1_amd.ops.vocab_loss import linear_cross_entropy, linear_topk_distill, topk_distill
+from tests.utils import Recorder, run
 
 pytestmark = pytest.mark.gpu
 U = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
@@ -538,3 +540,136 @@ def test_saved_tensors_may_move(gpu):
     got = torch.autograd.grad(loss, leaves)
     del junk
     assert all(torch.equal(a, c) for a, c in zip(got, ref))
+
+
+def test_offsets_past_32_bits(gpu):
+    """Logits and weights of more than 2^31 elements, and rows far apart."""
+    n, v, k = 17000, 128000, 4  # 2.2e9 logits
+    g = torch.Generator(device=gpu).manual_seed(1)
+    z = torch.empty(n, v, dtype=torch.bfloat16, device=gpu).normal_(generator=g)
+    teacher, index = _lists(gpu, g, n, v, k)
+    z.requires_grad_(True)
+    topk_distill(z, teacher, index, reduction="none").sum().backward()
+    rows = torch.tensor([0, 1, 16776, 16777, 16999], device=gpu)  # 16777 * 128000 is the first row past 2^31
+    got = z.grad[rows]
+    z.grad = None
+    _, G, A = _definition(z.detach()[rows].double(), None, teacher[rows], index[rows], -100, 0.0, 1.0, "none", torch.ones(5, device=gpu))
+    _near(got, G, A * 2.0 ** -14 + 1.01 * U[torch.bfloat16] * G.abs(), "dlogits")
+    del z, got
+    v, d = 530000, 4096  # 2.2e9 weights
+    w = torch.empty(v, d, dtype=torch.bfloat16, device=gpu).normal_(std=0.02, generator=g)
+    x = torch.randn(3, d, generator=g, device=gpu).bfloat16()
+    t = torch.tensor([0, 524288, v - 1], device=gpu)
+    _check_words(x, w, t)
+    # rows of the weight further apart than 2^21 elements
+    wide = torch.zeros(40, (1 << 21) + 8, dtype=torch.bfloat16, device=gpu)
+    wide[:, :64] = torch.randn(40, 64, generator=g, device=gpu)
+    _check_head(x[:, :64], wide[:, :64], None, target=torch.tensor([3, 39, 0], device=gpu))
+
+
+def _check_words(x, w, t):
+    """Cross entropy of a weight that is too large for a copy in 64 bits: the loss, dx, and the targets' rows of dweight."""
+    lx, lw = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+    loss = linear_cross_entropy(lx, lw, t, reduction="none")
+    dx, dw = torch.autograd.grad(loss, [lx, lw], torch.ones_like(loss))
+    z = torch.cat([x.double() @ part.double().t() for part in w.split(50000)], 1)
+    logp = torch.log_softmax(z, 1)
+    # logits of magnitude 6 from 4096 products: 4096 2^-24 sum |x w| < 2^-6 at worst, in the loss twice
+    assert (loss.detach().double() + logp.gather(1, t[:, None])[:, 0]).abs().max().item() <= 2.0 ** -5
+    G = logp.exp()
+    G[torch.arange(len(t)), t] -= 1
+    ref = sum(G[:, i:i + 50000] @ w[i:i + 50000].double() for i in range(0, w.shape[0], 50000))
+    # p to 2^-5, G to 2^-8 and dx to 2^-8, of sums of |G w| of about 0.02 for the target and for all others together
+    assert (dx.double() - ref).abs().max().item() <= 2.0 ** -5 * w.float().abs().amax().item()
+    refw = G[:, t].t() @ x.double()
+    assert (dw[t].double() - refw).abs().max().item() <= 2.0 ** -7 * refw.abs().max().item()
+
+
+@pytest.mark.parametrize("k,v", [(700, 1500), (4000, 4000)])
+def test_long_lists(gpu, k, v):
+    g = torch.Generator(device=gpu).manual_seed(k)
+    z = torch.randn(6, v, generator=g, device=gpu)
+    teacher = torch.randn(6, k, generator=g, device=gpu)
+    index = torch.stack([torch.randperm(v, generator=g, device=gpu)[:k] for _ in range(6)]).int()
+    index[1, k // 2:] = index[1, :k - k // 2]  # every word of it twice
+    _check_logits(z, teacher, index, 2.0)
+    x, w, b, _ = _tensors(gpu, 6, 48, v, torch.bfloat16)
+    _check_head(x, w, b, teacher=teacher, index=index, heat=2.0)
+
+
+def test_no_rows_and_a_teacher_that_learns(gpu):
+    x, w, b, g = _tensors(gpu, 5, 64, 300, torch.bfloat16)
+    leaf, wl = x[:0].requires_grad_(True), w.detach().requires_grad_(True)
+    loss = linear_cross_entropy(leaf, wl, torch.zeros(0, dtype=torch.long, device=gpu), b)
+    loss.backward()
+    assert loss.item() == 0.0 and loss.dtype == torch.float32 and leaf.grad.shape == (0, 64) and torch.equal(wl.grad, torch.zeros_like(w))
+    teacher, index = _lists(gpu, g, 5, 300, 4)
+    teacher.requires_grad_(True)
+    assert not topk_distill(torch.randn(5, 300, device=gpu), teacher, index).requires_grad
+    assert not linear_topk_distill(x, w, teacher, index, b).requires_grad
+
+
+class _HeadTrial(pytorch.PyTorchTrial):
+    """A student's output layer in a trial: targets and a teacher's lists, scored without its logits."""
+
+    def __init__(self, context):
+        self.context = context
+        torch.manual_seed(0)
+        self.net = torch.nn.Sequential(torch.nn.Linear(24, 64), torch.nn.Tanh(), torch.nn.Linear(64, 700))
+        self.model = context.wrap_model(self.net)
+        self.opt = context.wrap_optimizer(torch.optim.SGD(self.model.parameters(), lr=0.1, momentum=0.9))
+
+    def build_training_data_loader(self):
+        g = torch.Generator().manual_seed(1)
+        t = torch.randint(0, 700, (96, 12), generator=g)
+        t[torch.rand(96, 12, generator=g) < 0.3] = -100
+        index = torch.randint(0, 100, (96, 12, 5), generator=g) + 100 * torch.arange(5)
+        data = (torch.randn(96, 12, 24, generator=g), t, torch.randn(96, 12, 5, generator=g), index)
+        return pytorch.DataLoader(torch.utils.data.TensorDataset(*data), batch_size=self.context.get_per_slot_batch_size())
+
+    def build_validation_data_loader(self):
+        return self.build_training_data_loader()
+
+    def train_batch(self, batch, epoch_idx, batch_idx):
+        x, t, teacher, index = batch
+        head = self.net[2]
+        h = self.net[:2](x)
+        loss = linear_cross_entropy(h, head.weight, t, head.bias) + linear_topk_distill(h, head.weight, teacher, index, head.bias,
+                                                                                       temperature=2.0)
+        self.context.backward(loss)
+        self.context.step_optimizer(self.opt)
+        return {"loss": loss}
+
+    def evaluate_batch(self, batch):
+        x, t, teacher, index = batch
+        head = self.net[2]
+        return {"validation_loss": linear_cross_entropy(self.net[:2](x), head.weight, t, head.bias)}
+
+
+def test_trial_eager_and_replayed(gpu, monkeypatch):
+    """The same steps through the trial controller (arenas, gradients landing in place, the fused optimizer), eagerly and
+    replayed from a captured graph."""
+    got, landed = {}, []
+    orig = vocab_loss.landing_buffer
+
+    def spy(p):
+        b = orig(p)
+        landed.append(b is not None)
+        return b
+
+    monkeypatch.setattr(vocab_loss, "landing_buffer", spy)
+    for graph in ("0", "1"):
+        monkeypatch.setenv("DET_HIP_GRAPH", graph)
+        ctrl, resp = run(_HeadTrial, {"global_batch_size": 16}, Recorder().train(1, 18, 0).validate(1, 18), use_gpu=True,
+                         records_per_epoch=96)
+        torch.cuda.synchronize()
+        params = torch.cat([p.detach().float().reshape(-1) for p in ctrl.context.models[0].parameters()]).cpu()
+        got[graph] = params, resp[1]["metrics"]["validation_metrics"]["validation_loss"]
+        if graph == "0":
+            assert any(landed)
+        else:
+            assert ctrl._graph is not None and ctrl._graph.disabled_reason is None and ctrl._graph.stats()["replays"] >= 10
+    assert torch.isfinite(got["0"][0]).all()
+    # 18 steps of the same kernels; the body's library products may add in another order when captured
+    torch.testing.assert_close(got["1"][0], got["0"][0], rtol=1e-4, atol=1e-5)
+    assert abs(got["1"][1] - got["0"][1]) <= 1e-4 * abs(got["0"][1])
