@@ -190,6 +190,10 @@ def _pick(logp: torch.Tensor, index: torch.Tensor, there: torch.Tensor) -> torch
     return torch.where(there, got, torch.zeros_like(got))
 
 
+def _there(teacher: torch.Tensor, index: torch.Tensor) -> torch.Tensor:
+    return (index >= 0) & (teacher != -math.inf)
+
+
 def _plain_ce(z: torch.Tensor, target: torch.Tensor, ignore: int, smooth: float, reduction: str) -> torch.Tensor:
     kept = target != ignore
     z = torch.where(kept[:, None], z, torch.zeros_like(z))
@@ -202,7 +206,7 @@ def _plain_ce(z: torch.Tensor, target: torch.Tensor, ignore: int, smooth: float,
 
 def _plain_distill(z: torch.Tensor, teacher: torch.Tensor, index: torch.Tensor, heat: float, reduction: str) -> torch.Tensor:
     t = _wide(teacher).to(z.dtype) / heat
-    there = (index >= 0) & (t != -math.inf)
+    there = _there(t, index)
     kept = there.any(dim=1)
     z = torch.where(kept[:, None], z, torch.zeros_like(z))
     logp = F.log_softmax(z / heat, dim=1)
@@ -281,7 +285,9 @@ def _linear(x, weight, bias, target, teacher, index, opts, lead) -> torch.Tensor
     else:
         teacher, index = _rows_of(_apart(teacher)), _rows_of(index)
     if x.device.type == "cpu":
-        z = F.linear(_wide(x2), _wide(weight), None if bias is None else _wide(bias).to(_wide(x2).dtype))
+        kept = target != opts[0] if target is not None else _there(teacher, index).any(dim=1)
+        wide = _wide(x2).masked_fill(~kept[:, None], 0.0)  # what an ignored row holds does not matter
+        z = F.linear(wide, _wide(weight), None if bias is None else _wide(bias).to(wide.dtype))
         loss = (_plain_ce(z, target, opts[0], opts[1], opts[3]) if target is not None
                 else _plain_distill(z, teacher, index, opts[2], opts[3]))
     else:

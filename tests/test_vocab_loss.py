@@ -74,9 +74,11 @@ def test_rows_without_a_target():
     # an ignored row's values do not matter, whatever they are
     with torch.no_grad():
         x[3] = math.nan
-    t = torch.tensor([1, 2, 3, -100, 5, 6, 7])
-    loss = linear_cross_entropy(x, w, t)
-    assert math.isfinite(loss.item())
+    w.requires_grad_(True)
+    index[3] = -1
+    for loss in (linear_cross_entropy(x, w, torch.tensor([1, 2, 3, -100, 5, 6, 7])), linear_topk_distill(x, w, teacher, index)):
+        assert math.isfinite(loss.item())
+        assert all(torch.isfinite(g).all() for g in torch.autograd.grad(loss, [x, w]))
 
 
 def test_words_outside_the_vocabulary_are_nan():

@@ -561,6 +561,10 @@ def test_offsets_past_32_bits(gpu):
     x = torch.randn(3, d, generator=g, device=gpu).bfloat16()
     t = torch.tensor([0, 524288, v - 1], device=gpu)
     _check_words(x, w, t)
+    del w
+    w = torch.empty(280000, d, device=gpu).normal_(std=0.02, generator=g)  # two planes of it are packed chunk by chunk
+    _check_words(x.float(), w, torch.tensor([0, 131072, 279999], device=gpu))
+    del w
     # rows of the weight further apart than 2^21 elements
     wide = torch.zeros(40, (1 << 21) + 8, dtype=torch.bfloat16, device=gpu)
     wide[:, :64] = torch.randn(40, 64, generator=g, device=gpu)
@@ -583,6 +587,29 @@ def _check_words(x, w, t):
     assert (dx.double() - ref).abs().max().item() <= 2.0 ** -5 * w.float().abs().amax().item()
     refw = G[:, t].t() @ x.double()
     assert (dw[t].double() - refw).abs().max().item() <= 2.0 ** -7 * refw.abs().max().item()
+
+
+@pytest.mark.parametrize("n,dt", [(2000, torch.bfloat16), (1000, torch.float32)])
+def test_chunks_of_the_vocabulary(gpu, n, dt):
+    """More than one chunk of logit gradients (512 MiB), a target, a list and a masked word on either side of their border."""
+    v = 150000
+    x, w, b, g = _tensors(gpu, n, 40, v, dt)
+    t = torch.randint(0, v, (n,), generator=g, device=gpu)
+    t[::7] = -100
+    _check_head(x, w, b, target=t, smooth=0.1, reduction="sum")
+    teacher, index = _lists(gpu, g, n, v, 6)
+    index[:, 0], index[:, 1] = 75007, 75008
+    index[5] = -1
+    _check_head(x, w, b, teacher=teacher, index=index, heat=2.0)
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("n,d,v", [(5000, 64, 300), (3000, 300, 129), (1500, 130, 2000)])
+def test_many_rows_of_a_small_vocabulary(gpu, n, d, v, dt):
+    x, w, b, g = _tensors(gpu, n, d, v, dt)
+    t = torch.randint(0, v, (n,), generator=g, device=gpu)
+    t[torch.rand(n, generator=g, device=gpu) < 0.4] = -100
+    _check_head(x, w, b, target=t, gout=torch.tensor(64.0, device=gpu))
 
 
 @pytest.mark.parametrize("k,v", [(700, 1500), (4000, 4000)])
@@ -673,3 +700,19 @@ def test_trial_eager_and_replayed(gpu, monkeypatch):
     # 18 steps of the same kernels; the body's library products may add in another order when captured
     torch.testing.assert_close(got["1"][0], got["0"][0], rtol=1e-4, atol=1e-5)
     assert abs(got["1"][1] - got["0"][1]) <= 1e-4 * abs(got["0"][1])
+
+
+def test_backward_twice(gpu):
+    x, w, b, g = _tensors(gpu, 70, 100, 300, torch.float32)
+    t = torch.randint(0, 300, (70,), generator=g, device=gpu)
+    teacher, index = _lists(gpu, g, 70, 300, 4)
+    leaves = [a.requires_grad_(True) for a in (x, w, b)]
+    loss = linear_cross_entropy(x, w, t, b) + linear_topk_distill(x, w, teacher, index, b)
+    first = torch.autograd.grad(loss, leaves, retain_graph=True)
+    again = torch.autograd.grad(loss, leaves)
+    assert all(torch.equal(a, c) for a, c in zip(first, again))
+    loss = linear_cross_entropy(x, w, t, b)
+    with torch.no_grad():
+        x.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
