@@ -10,20 +10,27 @@
 // and have one derivative, G_nv = c_n (p_nv - eps / V - sum_k s_nk [a_nk = v]), from which
 //     dh_n = sum_v G_nv w_v        dw_v = sum_n G_nv h_n        db_v = sum_n G_nv.
 //
-// Forward: one product [rows x D] . [D x V] whose epilogue reduces each 256 x 256 tile of logits to a
-// maximum and a sum of exponentials per row; a joining pass per row adds the K picked logits (dot
-// products of their own).  Backward: the vocabulary is walked in chunks; per chunk the product runs
-// again, its epilogue writes G (16 bits) to a workspace, and two more products read it.  Four products
-// of 2 N V D operations in all, for the three that a program with the logits in memory needs.
+// Forward: one product [rows x D] . [D x V] whose epilogue reduces each tile of logits to a maximum and a
+// sum of exponentials per row (and hands out the target's logit); a joining pass per row, which for lists
+// adds the K listed logits, dot products of their own.  Backward: the vocabulary is walked in chunks; per
+// chunk the product runs again, its epilogue writes G to a workspace, and two more products read it.  Four
+// products of 2 N V D operations in all, for the three that a program with the logits in memory needs.
+// What bounds it, 8192 x 4096 x 128000 bf16 in 27.2 ms: the matrix units, 1.26 PFLOP/s over the four (logits
+// 6.3 ms, G 6.7, G w 6.7, G^T h 7.2); for few rows the reads of w (one row against 128000 x 4096: 5.3 TB/s).
 //
 // Rows without a target are dropped before the products (an ordered list of the kept ones, made on the
 // device; tiles past its end return), so a masked-language-model step with 15 % targets costs 15 %.
+//
+// G is held in the operands' 16 bits, which the matrix units take: each entry is off by half a step (bf16
+// 2^-8), at random, so a gradient of many terms is off by about as much as its own rounding once more (bf16
+// 2048 x 2048 x 32000: 0.0023 against 0.0017 of its size).  Everything else is fp32.
 //
 // fp32 operands become two fp16 planes each, x s = hi + lo with s a power of two that puts the tensor's
 // largest finite magnitude at 2^14..2^15, and a product is hi hi + hi lo + lo hi in fp32 accumulators:
 // each operand is held to 2^-23 of itself (2^-39 of the tensor's largest value at worst) and the
 // dropped lo lo is below 2^-22 of its product, the size of one fp32 rounding, at a third of the matrix
-// units' 16-bit rate instead of the sixteenth that their fp32 instructions have.
+// units' 16-bit rate instead of the sixteenth that their fp32 instructions have (2240 x 850 x 10000: off by
+// 5e-7 of the gradients' size, an fp32 product by 1.8e-6).
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -116,7 +123,8 @@ __device__ __forceinline__ int64_t load_index(const void* p, int64_t i, int wide
 constexpr int kGExp = 14;  // fp16 G is held times 2^14: |G| <= 1 stays below 65504, its smallest step is 2^-38
 
 // ------------------------------------------------------------------------------------------------
-// Rows: the ordered list of the rows that count.  info[0] = how many, info[1], info[2] = the largest
+// Rows: the ordered list of the rows that count, by one block (its order is what makes it one: 7 us for
+// 4608 rows, 14 for 8192).  info[0] = how many, info[1], info[2] = the largest
 // finite magnitudes (as bits) of the hidden states and the weights, cleared here for absmax_kernel.
 // ------------------------------------------------------------------------------------------------
 struct RowArgs {
@@ -252,7 +260,9 @@ __global__ void __launch_bounds__(256) absmax_kernel(Matrix x, Matrix w, int x_b
 
 // ------------------------------------------------------------------------------------------------
 // Operands of the products: 16-bit rows, 16-byte aligned, columns past the width zero.  Copies the
-// rows of `list` (or all), and splits fp32 into two fp16 planes.
+// rows of `list` (or all), and splits fp32 into two fp16 planes.  Bound by memory: 128000 x 4096 fp32 in
+// 0.85 ms, 4.9 TB/s.  The hidden states always (their kept rows move together), weights only if they are
+// fp32, of a width or a row distance that 16 bytes do not divide, or misaligned.
 // ------------------------------------------------------------------------------------------------
 struct PackArgs {
   const void* src;
@@ -311,6 +321,9 @@ __global__ void __launch_bounds__(256) pack_kernel(PackArgs a) {
 // An operand lies with its k contiguous ("row": element (i, k) at i * ld + k) or strided ("col":
 // (i, k) at k * ld + i, read back from LDS transposed).  LDS holds 8 KiB images of 128 rows (or columns)
 // by 32 k, in stages of both operands' 256 and, for a split fp32 operand, both planes.
+// Bound by what feeds the matrix units: a stage of 64 k is 2048 cycles of them and of fragment reads (192 KiB)
+// and fetches (64 KiB) through LDS nearly as many, which share its port; 0.93 us a stage with neither, 1.1 with
+// one of them, 1.3 with both, 1.45 with data that makes the clock drop.
 // Everything outside an operand's extents is fetched out of the buffer's range, which gives zeros.
 // ------------------------------------------------------------------------------------------------
 // A gradient's scale: G is held in [-1, 1] 2^k, row weights divided by the largest one's magnitude.
@@ -1008,7 +1021,7 @@ __device__ __forceinline__ float diverge(float q, float t, float tt, float tl, f
   return q * (((t - tt) * inv_t - tl * kLn2) - ((z - top) * inv_t - log_s * kLn2));
 }
 
-// one target a row: a wave each
+// one target a row: a wave each (8192 rows of 1000 parts in 13 us)
 __global__ void __launch_bounds__(256) finish_target_kernel(FinishArgs a) {
   const int lane = threadIdx.x & 63, count = a.info[0];
   for (int row = blockIdx.x * 4 + (threadIdx.x >> 6); row < count; row += gridDim.x * 4) {
@@ -1037,7 +1050,8 @@ __global__ void __launch_bounds__(256) finish_target_kernel(FinishArgs a) {
   }
 }
 
-// a list a row: a block each
+// a list a row: a block each, four waves with four words' rows at a time (2048 x 64 words of 2048 bf16, 537 MB
+// from the caches, in 76 us)
 template <int DT>
 __global__ void __launch_bounds__(256) finish_list_kernel(FinishArgs a) {
   __shared__ float red[4][3];
@@ -1235,7 +1249,8 @@ __global__ void __launch_bounds__(256) dbias_kernel(const float* part, int split
 }
 
 // The sum of a row's partials: of dh (pos: a row's place among the kept ones; zeros for the others), or of
-// dw (pos null; rows of words, pieces of the kept rows)
+// dw (pos null; rows of words, pieces of the kept rows).  Bound by memory (4608 rows, 28 pieces of 691 kept:
+// 59 MB in 13 us)
 __global__ void __launch_bounds__(256) sum_kernel(const float* part, int span, int64_t ldo, const int* info, const int* pos,
                                                   Alpha alpha, int planes, void* dx, int dt, int D) {
   const int n = blockIdx.x, at = pos != nullptr ? pos[n] : n, count = pos != nullptr ? info[0] : gridDim.x;

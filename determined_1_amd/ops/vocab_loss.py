@@ -12,7 +12,11 @@ nothing.  Losses are fp32; sums, softmax statistics and gradients are accumulate
 logit gradient is held in the operands' type (fp32: two fp16 planes, 22 bits).
 
 GPU tensors (bf16, fp16, fp32) always run on the kernels; what those do not cover is refused.  CPU
-tensors run the plain composite below.  Both are differentiable once.
+tensors run the plain composite below.  The kernels are differentiable once.
+
+Memory of a ``linear_`` call: between forward and backward the kept rows of ``x`` once more, 8 K bytes a
+row, and weights that had to be packed (fp32, or rows that 16 bytes do not divide) up to 4 GiB of them;
+in the backward 512 MiB for a chunk's logit gradient and fp32 sums of ``x``'s gradient.
 """
 import ctypes
 import math
