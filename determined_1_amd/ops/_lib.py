@@ -19,7 +19,7 @@ from typing import Optional
 _HERE = pathlib.Path(__file__).resolve().parent
 LIB_NAME = "libdetkernels.so"
 LIB_PATH = _HERE / LIB_NAME
-ABI_VERSION = 22
+ABI_VERSION = 23
 
 _lock = threading.Lock()
 _lib = None  # type: Optional[ctypes.CDLL]

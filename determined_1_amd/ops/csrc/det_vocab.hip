@@ -13,10 +13,12 @@
 // Forward: one product [rows x D] . [D x V] whose epilogue reduces each tile of logits to a maximum and a
 // sum of exponentials per row (and hands out the target's logit); a joining pass per row, which for lists
 // adds the K listed logits, dot products of their own.  Backward: the vocabulary is walked in chunks; per
-// chunk the product runs again, its epilogue writes G to a workspace, and two more products read it.  Four
-// products of 2 N V D operations in all, for the three that a program with the logits in memory needs.
-// What bounds it, 8192 x 4096 x 128000 bf16 in 27.2 ms: the matrix units, 1.26 PFLOP/s over the four (logits
-// 6.3 ms, G 6.7, G w 6.7, G^T h 7.2); for few rows the reads of w (one row against 128000 x 4096: 5.3 TB/s).
+// chunk G is written to a workspace, and two more products read it.  G comes from the tile's exponentials,
+// which the forward held in 16 bits as far as the caller's bound goes (2 GiB unless it says otherwise), and past
+// that from the product once more, in its epilogue.  What bounds it, 8192 x 4096 x 128000 bf16 in 22.2 ms: the
+// matrix units, 1.23 PFLOP/s over the three products (logits 6.8 ms, G w 6.9, G^T h 7.4; G from 2 GB of
+// exponentials 0.8, where the product again takes 6.7); for few rows the reads of w (one row against
+// 128000 x 4096: 5.3 TB/s).
 //
 // Rows without a target are dropped before the products (an ordered list of the kept ones, made on the
 // device; tiles past its end return), so a masked-language-model step with 15 % targets costs 15 %.
@@ -61,6 +63,13 @@ __device__ __forceinline__ float bf2f(u16 u) { return __uint_as_float(static_cas
 __device__ __forceinline__ u16 f2bf(float f) { return __builtin_bit_cast(u16, static_cast<__bf16>(f)); }
 __device__ __forceinline__ float h2f(u16 u) { return static_cast<float>(__builtin_bit_cast(_Float16, u)); }
 __device__ __forceinline__ u16 f2h(float f) { return __builtin_bit_cast(u16, static_cast<_Float16>(f)); }
+
+// The value as an fp32 register.  Without it the compiler may round a product to fp16 in one instruction for
+// the upper plane and from fp32 for the lower one: at a tie the planes then miss each other by a step.
+__device__ __forceinline__ float settled(float v) {
+  asm("" : "+v"(v));
+  return v;
+}
 
 template <int DT>
 __device__ __forceinline__ float to_f(typename Elem<DT>::type v) {
@@ -358,6 +367,10 @@ struct GemmArgs {
   int bias_dt;
   float c;
   float2* part;   // kStats [M][parts], 128 columns each: maximum and sum
+  // kStats: the first `held` words' exponentials below the tile's maximum (null: none), and the maxima
+  void* E;        // [M][held], 11-bit numbers or fp32
+  float* tops;    // [M][held / 128]
+  int held;       // (a multiple of 256)
   float* part_z;  // sum of z / V, or null
   float inv_v;
   int parts;
@@ -479,14 +492,23 @@ __device__ __forceinline__ void tile_to_lds(const f32x4 (&acc)[8][FN], unsigned 
       us4 hi, lo;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        hi[r] = F16 ? f2h(acc[i][j][r]) : f2bf(acc[i][j][r]);
-        lo[r] = PL == 2 ? f2h(acc[i][j][r] - h2f(hi[r])) : u16(0);
+        const float v = PL == 2 ? settled(acc[i][j][r]) : acc[i][j][r];
+        hi[r] = F16 ? f2h(v) : f2bf(v);
+        lo[r] = PL == 2 ? f2h(v - h2f(hi[r])) : u16(0);
       }
       u16* o = ct + (row0 + i * 16) * kLdc + col0 + j * 16;
       *reinterpret_cast<us4*>(o) = hi;
       if (PL == 2) *reinterpret_cast<us4*>(o + 128 * kLdc) = lo;
     }
 }
+
+// An exponential of at most 1 in 16 bits: five of exponent, down to 2^-31, and eleven behind the point, so it
+// is off by at most 2^-12 of itself; zeros stand for what is smaller.
+__device__ __forceinline__ u16 hold_bits(float e) {
+  const int q = static_cast<int>((__float_as_uint(e) + 0x800u) >> 12) - (96 << 11);
+  return static_cast<u16>(q < 0 ? 0 : q > 65535 ? 65535 : q);
+}
+__device__ __forceinline__ float held_value(unsigned q) { return q == 0 ? 0.f : __uint_as_float((q + (96u << 11)) << 12); }
 
 // Where a block works: 256 rows from m0, 256 columns (or, of a tile cut in two, 128) from n0, k from kbeg to kend.
 struct Place {
@@ -795,7 +817,10 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Place& at, un
 #pragma unroll
         for (int j = 0; j < FN; ++j)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) s += exp2_((acc[i][j][r] - ref) * c);
+          for (int r = 0; r < 4; ++r) {
+            acc[i][j][r] = exp2_((acc[i][j][r] - ref) * c);
+            s += acc[i][j][r];
+          }
         s += __shfl_xor(s, 16, 64);
         s += __shfl_xor(s, 32, 64);
         if (fch == 0) {
@@ -814,12 +839,68 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Place& at, un
           sz += red[2048 + w * 256 + tid];
         }
         // a place for every 128 columns; a whole tile fills two
-        const int64_t to = static_cast<int64_t>(m0 + tid) * g.parts + (g.v0 + n0) / 128;
+        const int at128 = (g.v0 + n0) / 128;
+        const int64_t to = static_cast<int64_t>(m0 + tid) * g.parts + at128;
         g.part[to] = make_float2(m, s);
         if (FN == 4 || at.lone) g.part[to + 1] = make_float2(kNegInf, 0.f);
         if (g.part_z != nullptr) {
           g.part_z[to] = sz;
           if (FN == 4 || at.lone) g.part_z[to + 1] = 0.f;
+        }
+        if (g.E != nullptr && g.v0 + n0 < g.held) {
+          float* tops = g.tops + static_cast<int64_t>(m0 + tid) * (g.held / 128) + at128;
+          tops[0] = m;
+          if (FN == 4 || at.lone) tops[1] = m;
+        }
+      }
+      if (g.E != nullptr && g.v0 + n0 < g.held) {
+        // e = 2^(c (z - the tile's maximum)), from those below the wave's
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float own = red[wc * 256 + row0 + i * 16];
+          const float m = fmaxf(fmaxf(red[row0 + i * 16], red[256 + row0 + i * 16]), fmaxf(red[512 + row0 + i * 16], red[768 + row0 + i * 16]));
+          const float f = own == kNegInf ? 0.f : exp2_((own - m) * c);
+#pragma unroll
+          for (int j = 0; j < FN; ++j) acc[i][j] *= f;
+        }
+        __syncthreads();
+        if constexpr (PL == 1) {
+          typedef __attribute__((ext_vector_type(4))) u16 us4;
+          u16* ct = reinterpret_cast<u16*>(smem);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) {
+              us4 v;
+#pragma unroll
+              for (int r = 0; r < 4; ++r) v[r] = hold_bits(acc[i][j][r]);
+              *reinterpret_cast<us4*>(ct + (row0 + i * 16) * kLdc + col0 + j * 16) = v;
+            }
+          __syncthreads();
+          u16* out = static_cast<u16*>(g.E) + g.v0 + n0;
+          for (int q = tid; q < kTile * (BN / 8); q += kThreads) {
+            const int row = q / (BN / 8), cc = (q % (BN / 8)) * 8;
+            if (m0 + row < M) *reinterpret_cast<us8*>(out + static_cast<int64_t>(m0 + row) * g.held + cc) = *reinterpret_cast<const us8*>(ct + row * kLdc + cc);
+          }
+        } else {
+          float* ct = reinterpret_cast<float*>(smem);  // half the rows at a time
+          float* out = static_cast<float*>(g.E) + g.v0 + n0;
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            if (wr == half)
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int j = 0; j < FN; ++j) *reinterpret_cast<f32x4*>(ct + (fr + i * 16) * kLdc32 + col0 + j * 16) = acc[i][j];
+            __syncthreads();
+            for (int q = tid; q < 128 * (BN / 4); q += kThreads) {
+              const int row = half * 128 + q / (BN / 4), cc = (q % (BN / 4)) * 4;
+              if (m0 + row < M)
+                *reinterpret_cast<f32x4*>(out + static_cast<int64_t>(m0 + row) * g.held + cc) =
+                    *reinterpret_cast<const f32x4*>(ct + (row - half * 128) * kLdc32 + cc);
+            }
+            __syncthreads();
+          }
         }
       }
     } else {
@@ -1181,6 +1262,81 @@ __global__ void __launch_bounds__(1024) weights_kernel(WeightArgs a) {
 
 // the listed words' entries of a chunk's G, from the fp32 logits of the forward pass (a word twice in
 // a list: its shares add up, and each of its entries writes the same value)
+// ------------------------------------------------------------------------------------------------
+// G of the words whose exponentials the forward pass left: w (e 2^(c (the tile's maximum - top) - log2 sum) -
+// eps / V), minus the target's share; as the product's epilogue writes it.  A block has 256 rows of 64
+// words, eight lanes a row.  Bound by memory (2048 x 32000, 2 bytes in and 2 out: 54 us, 4.9 TB/s).
+// ------------------------------------------------------------------------------------------------
+struct HeldArgs {
+  const void* E;
+  const float* tops;
+  int held;       // (a multiple of 256)
+  const int* info;
+  const float *top, *log_s, *row_w;
+  float g_scale, c, smooth_v, share;
+  const int* words;  // one target a row (null for lists)
+  int v0;
+  float* colsum;     // [tiles of rows][ldg] or null
+  u16* G;
+  int64_t g_plane;
+  int ldg;
+};
+
+template <int DT>
+__global__ void __launch_bounds__(256) held_kernel(HeldArgs a) {
+  constexpr bool kF = DT == kF32;
+  const int M = a.info[0], tid = threadIdx.x, across = a.ldg / 64, down = static_cast<int>(blockIdx.x) / across;
+  const int col0 = (static_cast<int>(blockIdx.x) - down * across) * 64, col = col0 + (tid & 7) * 8, m0 = down * kTile;
+  if (m0 >= M) return;
+  float sums[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int it = 0; it < 8; ++it) {
+    const int row = m0 + it * 32 + (tid >> 3);
+    if (row >= M) continue;
+    const int64_t at = static_cast<int64_t>(row) * a.held + col;
+    float g[8];
+    if constexpr (kF) {
+      const f32x4* e = reinterpret_cast<const f32x4*>(static_cast<const float*>(a.E) + at);
+      const f32x4 lo = __builtin_nontemporal_load(e), hi = __builtin_nontemporal_load(e + 1);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        g[k] = lo[k];
+        g[k + 4] = hi[k];
+      }
+    } else {
+      const us8 e = __builtin_nontemporal_load(reinterpret_cast<const us8*>(static_cast<const u16*>(a.E) + at));
+#pragma unroll
+      for (int k = 0; k < 8; ++k) g[k] = held_value(e[k]);
+    }
+    const float w = a.row_w != nullptr ? a.row_w[row] : a.g_scale;
+    const float tile = a.tops[static_cast<int64_t>(row) * (a.held / 128) + col / 128];
+    const float f = exp2_(fmaf(tile - a.top[row], a.c, -a.log_s[row]));
+    const int word = a.words != nullptr ? a.words[row] - a.v0 - col : -1;
+    us8 hi, lo;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      g[k] = settled(w * (fmaf(g[k], f, -a.smooth_v) - (word == k ? a.share : 0.f)));
+      sums[k] += g[k];
+      hi[k] = DT == kBF16 ? f2bf(g[k]) : f2h(g[k]);
+      lo[k] = kF ? f2h(g[k] - h2f(hi[k])) : u16(0);
+    }
+    u16* o = a.G + static_cast<int64_t>(row) * a.ldg + col;
+    *reinterpret_cast<us8*>(o) = hi;
+    if (kF) *reinterpret_cast<us8*>(o + a.g_plane) = lo;
+  }
+  if (a.colsum == nullptr) return;
+  __shared__ float red[32][64 + 4];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) red[tid >> 3][(tid & 7) * 8 + k] = sums[k];
+  __syncthreads();
+  if (tid < 64) {
+    float t = 0.f;
+#pragma unroll
+    for (int r = 0; r < 32; ++r) t += red[r][tid];
+    a.colsum[static_cast<int64_t>(down) * a.ldg + col0 + tid] = t;
+  }
+}
+
 struct ScatterArgs {
   const int *info, *list;
   const void* index;
@@ -1204,7 +1360,7 @@ __global__ void __launch_bounds__(256) scatter_kernel(ScatterArgs a) {
     for (int j = 0; j < a.K; ++j)
       if (load_index(a.index, i0 + j, a.wide) == word) s += share[j];
     const float w = a.row_w != nullptr ? a.row_w[row] : a.g_scale;
-    const float v = w * (exp2_(fmaf(a.picked[i] - a.top[row], a.c, -a.log_s[row])) - s);
+    const float v = settled(w * (exp2_(fmaf(a.picked[i] - a.top[row], a.c, -a.log_s[row])) - s));
     u16* o = a.G + static_cast<int64_t>(row) * a.ldg + (word - a.v0);
     const u16 hi = a.f16 ? f2h(v) : f2bf(v);
     *o = hi;
@@ -1598,6 +1754,7 @@ struct DetVocabHead {
   void* kept;                     // what the forward pass leaves for the backward pass (Head, below)
   void* ws;
   int64_t ws_bytes, kept_bytes, x_ld, w_ld, index_ld, teacher_ld, ignore;
+  int64_t hold_bytes;             // exponentials that the forward pass may hold for the backward pass (0: none follows)
   int N, D, V, K, dtype, bias_dt, wide, teacher_dt, reduction;  // reduction 0 each row, 1 mean, 2 sum
   float inv_t, smooth;
 };
@@ -1606,9 +1763,9 @@ namespace {
 
 // What both directions lay out in the workspace.
 struct Plan {
-  int planes, ldh, chunk, nchunks, parts, csplits;
+  int planes, ldh, chunk, nchunks, parts, csplits, held;
   bool pack_w, keep_w, split_w;
-  int64_t off_rows_info, off_h, off_kw, kept;  // in `kept`
+  int64_t off_rows_info, off_h, off_e, off_tops, off_kw, kept;  // in `kept`
   int64_t off_w, off_flag, off_part, off_partz, off_rows, off_roww, off_alpha, off_g, off_dx, off_dw, off_cs, total;
 };
 
@@ -1626,22 +1783,29 @@ Plan plan(const DetVocabHead& p, bool backward) {
   q.keep_w = q.pack_w && w_bytes <= kKeepBytes;
   q.off_rows_info = up(int64_t(8) * p.N * (1 + p.K), 256);
   q.off_h = q.off_rows_info + up(int64_t(4) * (4 + 3 * int64_t(p.N)), 256);
-  q.off_kw = q.off_h + h_bytes;
-  q.kept = q.off_kw + (q.keep_w ? w_bytes : 0);
-  int64_t chunk = up(p.V, kTile);
-  if (backward) {
-    const int64_t fit = kChunkBytes / (int64_t(2) * q.planes * p.N) / kTile * kTile;
-    if (chunk > fit) chunk = fit;
-  }
-  if (q.pack_w && !q.keep_w) {
-    const int64_t fit = kChunkBytes / (int64_t(2) * q.planes * q.ldh) / kTile * kTile;
-    if (chunk > fit) chunk = fit;
-  }
-  if (chunk > (1 << 20)) chunk = 1 << 20;  // 256 rows of G stay within 32-bit offsets
-  if (chunk < kTile) chunk = kTile;
-  q.nchunks = ceil_div(p.V, chunk);
-  q.chunk = static_cast<int>(up(ceil_div(p.V, q.nchunks), kTile));  // even chunks
+  auto chunks = [&](bool of_g) {
+    int64_t chunk = up(p.V, kTile);
+    if (of_g) {
+      const int64_t fit = kChunkBytes / (int64_t(2) * q.planes * p.N) / kTile * kTile;
+      if (chunk > fit) chunk = fit;
+    }
+    if (q.pack_w && !q.keep_w) {
+      const int64_t fit = kChunkBytes / (int64_t(2) * q.planes * q.ldh) / kTile * kTile;
+      if (chunk > fit) chunk = fit;
+    }
+    if (chunk > (1 << 20)) chunk = 1 << 20;  // 256 rows of G stay within 32-bit offsets
+    if (chunk < kTile) chunk = kTile;
+    return static_cast<int>(up(ceil_div(p.V, ceil_div(p.V, chunk)), kTile));  // even ones
+  };
+  q.chunk = chunks(backward);
   q.nchunks = ceil_div(p.V, q.chunk);
+  const int gc = chunks(true);
+  const int64_t held = p.hold_bytes / (int64_t(2) * q.planes * p.N) / gc * gc;  // whole chunks of G
+  q.held = static_cast<int>(held < up(p.V, gc) ? held : up(p.V, gc));
+  q.off_e = q.off_h + h_bytes;
+  q.off_tops = q.off_e + int64_t(2) * q.planes * p.N * q.held;
+  q.off_kw = q.off_tops + up(int64_t(4) * p.N * (q.held / 128), 256);
+  q.kept = q.off_kw + (q.keep_w ? w_bytes : 0);
   q.parts = 2 * ceil_div(p.V, kTile);
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
@@ -1681,6 +1845,7 @@ int check_head(const DetVocabHead& p) {
   if (p.N < 1 || p.D < 1 || p.V < 1 || p.K < 1) return -1;
   if (p.dtype < 0 || p.dtype > 2 || p.reduction < 0 || p.reduction > 2) return -2;
   if ((p.target == nullptr) == (p.index == nullptr)) return -3;
+  if (p.hold_bytes < 0) return -5;
   // offsets inside a tile are 32-bit: 256 rows of an operand, 64 rows of G
   if (p.D > (1 << 21) || p.V > (1 << 30) || p.N > (1 << 30)) return -4;
   return 0;
@@ -1708,12 +1873,16 @@ struct Head : DetVocabHead {
   float* stats;  // [2, N] maxima and log2 of sums, [N, K] picked logits, [N, K] shares
   int* rows;     // [4 + 3 N]: info, the list of kept rows, each row's place in it, targets
   u16* hidden;   // the packed hidden states
+  char* e;       // exponentials of the first q.held words' logits
+  float* tops;   // their tiles' maxima
   u16* weights;  // the packed weights, if they are packed whole
   Head(const DetVocabHead& p, const Plan& q) : DetVocabHead(p) {
     char* at = static_cast<char*>(p.kept);
     stats = reinterpret_cast<float*>(at);
     rows = reinterpret_cast<int*>(at + q.off_rows_info);
     hidden = reinterpret_cast<u16*>(at + q.off_h);
+    e = at + q.off_e;
+    tops = reinterpret_cast<float*>(at + q.off_tops);
     weights = reinterpret_cast<u16*>(at + q.off_kw);
   }
 };
@@ -1815,6 +1984,9 @@ int det_vocab_head_forward(void* stream, const DetVocabHead* pp) {
     a.part = reinterpret_cast<float2*>(ws + q.off_part);
     a.part_z = p.smooth != 0.f ? reinterpret_cast<float*>(ws + q.off_partz) : nullptr;
     a.parts = q.parts;
+    a.E = q.held > 0 ? p.e : nullptr;
+    a.tops = p.tops;
+    a.held = q.held;
     DET_TRY((gemm<false, false, kStats>(st, p.dtype, a)));
   }
   FinishArgs f = {};
@@ -1887,8 +2059,9 @@ int det_vocab_head_backward(void* stream, const DetVocabHead* pp) {
   for (int c = 0; c < q.nchunks; ++c) {
     const int v0 = c * q.chunk, nv = p.V - v0 < q.chunk ? p.V - v0 : q.chunk;
     const int ldg = static_cast<int>(up(nv, 64));  // columns past nv are zero
-    Operand w;
-    DET_TRY(weight_operand(st, p, q, ws, v0, nv, false, &w));
+    const bool held = v0 < q.held;
+    Operand w = {};
+    if (!held || p.dx != nullptr) DET_TRY(weight_operand(st, p, q, ws, v0, nv, false, &w));
     GemmArgs a = logits_args(p, q, w, v0, nv);
     float* cs = p.db != nullptr ? reinterpret_cast<float*>(ws + q.off_cs) : nullptr;
     a.top = p.stats;
@@ -1900,7 +2073,16 @@ int det_vocab_head_backward(void* stream, const DetVocabHead* pp) {
     a.G = reinterpret_cast<u16*>(ws + q.off_g);
     a.g_plane = int64_t(p.N) * ldg;
     a.ldg = ldg;
-    DET_TRY((gemm<false, false, kGrad>(st, p.dtype, a)));
+    if (held) {
+      const HeldArgs h = {p.e + int64_t(2) * q.planes * v0, p.tops + v0 / 128, q.held, p.rows, a.top, a.log_s, row_w, g_scale, a.c, a.smooth_v, a.share, a.words, v0,
+                          a.colsum, a.G, a.g_plane, ldg};
+      const dim3 hg(static_cast<unsigned>(ldg / 64) * ceil_div(p.N, kTile));
+      if (p.dtype == kF32) hipLaunchKernelGGL(held_kernel<kF32>, hg, dim3(256), 0, st, h);
+      else if (p.dtype == kBF16) hipLaunchKernelGGL(held_kernel<kBF16>, hg, dim3(256), 0, st, h);
+      else hipLaunchKernelGGL(held_kernel<kF16>, hg, dim3(256), 0, st, h);
+    } else {
+      DET_TRY((gemm<false, false, kGrad>(st, p.dtype, a)));
+    }
     if (p.index != nullptr) {
       ScatterArgs s = {p.rows, list, p.index, p.index_ld, p.wide, p.K, v0, nv, f16, q.planes, ldg, picked,
                        picked + int64_t(p.N) * p.K, a.top, a.log_s, row_w, g_scale, a.c, a.G, a.g_plane};

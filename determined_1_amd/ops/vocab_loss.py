@@ -4,19 +4,22 @@
     linear_topk_distill(x, W, teacher, index[, b])     T^2 KL(teacher's top logits || softmax((x W^T + b) / T))
     topk_distill(logits, teacher, index)               the same for logits that are there already
 
-The ``linear_`` forms are a language model's output layer and its loss in one: the [rows, V] logits are
-never kept.  The forward reduces each tile of them to a maximum and a sum of exponentials; the backward
-walks the vocabulary in chunks of a bounded workspace, recomputes a chunk's logits, turns them into
-their gradient and multiplies that into the gradients of ``x`` and ``W``.  Rows that are ignored cost
-nothing.  Losses are fp32; sums, softmax statistics and gradients are accumulated in fp32; a chunk's
-logit gradient is held in the operands' type (fp32: two fp16 planes, 22 bits).
+The ``linear_`` forms are a language model's output layer and its loss in one, walking the vocabulary in
+chunks: the [rows, V] logits are never in memory.  The forward reduces each tile of them to a maximum and
+a sum of exponentials; the backward turns a chunk at a time into the logits' gradient and multiplies that
+into the gradients of ``x`` and ``W``.  It makes a chunk from exponentials that the forward held, of as many
+chunks as ``hold_bytes`` has room for, and from the logits computed again past those.  Rows that are
+ignored cost nothing.  Losses are fp32; sums, softmax statistics and gradients are accumulated in fp32; a
+chunk's logit gradient is held in the operands' type (fp32: two fp16 planes, 22 bits), exponentials in 16
+bits with a step of 2^-11 (fp32: as they are).
 
 GPU tensors (bf16, fp16, fp32) always run on the kernels; what those do not cover is refused.  CPU
 tensors run the plain composite below.  The kernels are differentiable once.
 
-Memory of a ``linear_`` call: between forward and backward the kept rows of ``x`` once more, 8 K bytes a
-row, and weights that had to be packed (fp32, or rows that 16 bytes do not divide) up to 4 GiB of them;
-in the backward 512 MiB for a chunk's logit gradient and fp32 sums of ``x``'s gradient.
+Memory of a ``linear_`` call: between forward and backward at most ``hold_bytes`` (2 or, for fp32, 4 bytes a
+logit) and two percent more, the kept rows of ``x`` once more, 8 K bytes a row, and weights that had to be packed
+(fp32, or rows that 16 bytes do not divide) up to 4 GiB of them; in the backward 512 MiB for a chunk's logit
+gradient and fp32 sums of ``x``'s gradient.  Under ``torch.no_grad()`` none of these exponentials.
 """
 import ctypes
 import math
@@ -31,6 +34,7 @@ from determined_1_amd.ops.functional import dtype_code
 from determined_1_amd.ops.transformer import _autocast, _null, _ptr, _stream
 
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+HOLD_BYTES = 2 << 30  # under one percent of the card's memory
 _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 
 
@@ -38,7 +42,8 @@ class _HeadParams(ctypes.Structure):
     """Mirror of ``DetVocabHead`` (det_vocab.hip)."""
     _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "w", "bias", "target", "index", "teacher", "dx", "dw", "db", "gout",
                                                 "loss", "kept", "ws")]
-                + [(n, ctypes.c_int64) for n in ("ws_bytes", "kept_bytes", "x_ld", "w_ld", "index_ld", "teacher_ld", "ignore")]
+                + [(n, ctypes.c_int64) for n in ("ws_bytes", "kept_bytes", "x_ld", "w_ld", "index_ld", "teacher_ld", "ignore",
+                                                "hold_bytes")]
                 + [(n, ctypes.c_int32) for n in ("N", "D", "V", "K", "dtype", "bias_dt", "wide", "teacher_dt", "reduction")]
                 + [("inv_t", ctypes.c_float), ("smooth", ctypes.c_float)])
 
@@ -78,7 +83,7 @@ class _Head(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, target, teacher, index, opts):  # type: ignore[override]
-        ignore, smooth, heat, reduction = opts
+        ignore, smooth, heat, reduction, hold_bytes = opts
         p = _HeadParams()
         p.N, p.D = x.shape
         p.V = weight.shape[0]
@@ -86,7 +91,7 @@ class _Head(torch.autograd.Function):
         p.dtype = dtype_code(x.dtype)
         if bias is not None:
             p.bias, p.bias_dt = bias.data_ptr(), dtype_code(bias.dtype)
-        p.ignore, p.smooth, p.inv_t, p.reduction = ignore, smooth, 1.0 / heat, _REDUCTIONS[reduction]
+        p.ignore, p.smooth, p.inv_t, p.reduction, p.hold_bytes = ignore, smooth, 1.0 / heat, _REDUCTIONS[reduction], hold_bytes
         if target is not None:
             p.target, p.K, p.wide = target.data_ptr(), 1, target.dtype == torch.int64
         else:
@@ -271,6 +276,12 @@ def _check_lists(what: str, lead: torch.Size, teacher: torch.Tensor, index: torc
         _refuse(what, f"temperature {heat} is not within [2^-20, 2^20]")
 
 
+def _bytes(what: str, hold_bytes: int) -> int:
+    if not isinstance(hold_bytes, int) or not 0 <= hold_bytes < 2 ** 63:
+        _refuse(what, f"hold_bytes {hold_bytes!r} is not a number of bytes")
+    return hold_bytes
+
+
 def _empty(reduction: str, lead: torch.Size, *ts: Optional[torch.Tensor]) -> torch.Tensor:
     """The loss of no rows: 0, with gradients of zeros."""
     zero = sum((t * 0).sum().float() for t in ts if t is not None)
@@ -299,20 +310,24 @@ def _linear(x, weight, bias, target, teacher, index, opts, lead) -> torch.Tensor
             weight = weight.contiguous()
         if bias is not None and bias.stride(0) != 1:
             bias = bias.contiguous()
+        if not torch.is_grad_enabled() or not (x2.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
+            opts = (*opts[:4], 0)  # no backward pass to hold anything for
         with torch.autocast("cuda", enabled=False) if ac else _null():
             loss = _Head.apply(x2, weight, bias, target, teacher, index, opts)
     return loss if opts[3] != "none" or len(lead) == 1 else loss.reshape(lead)
 
 
 def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
-                         ignore_index: int = -100, label_smoothing: float = 0.0, reduction: str = "mean") -> torch.Tensor:
+                         ignore_index: int = -100, label_smoothing: float = 0.0, reduction: str = "mean",
+                         hold_bytes: int = HOLD_BYTES) -> torch.Tensor:
     """``F.cross_entropy(F.linear(x, weight, bias), target, ...)`` without the logits.
 
     x [..., D], weight [V, D], bias [V] (x's type or fp32), target [...] int32 or int64.  Rows whose target is
     ``ignore_index`` have loss 0, no gradient, and take no work; a mean over none of them is 0.  A target
     outside the vocabulary gives its row (and a mean or sum) a NaN loss and NaN gradients: nothing is read
     out of bounds, and no host check waits for the GPU.  With ``reduction="none"`` under ``torch.no_grad()``
-    it scores tokens: the loss [...] is each target's negative log-probability."""
+    it scores tokens: the loss [...] is each target's negative log-probability.  ``hold_bytes`` bounds what a
+    call holds of its logits' exponentials for its backward pass; 0 recomputes all of them there."""
     what = "linear_cross_entropy"
     _check_common(what, reduction, x, weight, target, bias)
     _check_head(what, x, weight, bias)
@@ -323,20 +338,24 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
         _refuse(what, f"target is {target.dtype}: int32 or int64 expected", TypeError)
     if not 0.0 <= label_smoothing <= 1.0:
         _refuse(what, f"label_smoothing {label_smoothing} is not within [0, 1]")
-    return _linear(x, weight, bias, target, None, None, (int(ignore_index), float(label_smoothing), 1.0, reduction), lead)
+    opts = (int(ignore_index), float(label_smoothing), 1.0, reduction, _bytes(what, hold_bytes))
+    return _linear(x, weight, bias, target, None, None, opts, lead)
 
 
 def linear_topk_distill(x: torch.Tensor, weight: torch.Tensor, teacher_logits: torch.Tensor, teacher_index: torch.Tensor,
-                        bias: Optional[torch.Tensor] = None, *, temperature: float = 1.0, reduction: str = "mean") -> torch.Tensor:
+                        bias: Optional[torch.Tensor] = None, *, temperature: float = 1.0, reduction: str = "mean",
+                        hold_bytes: int = HOLD_BYTES) -> torch.Tensor:
     """``topk_distill(F.linear(x, weight, bias), teacher_logits, teacher_index, ...)`` without the logits.
 
-    x [..., D], weight [V, D], bias [V]; the lists [..., K] as in ``topk_distill``."""
+    x [..., D], weight [V, D], bias [V]; the lists [..., K] as in ``topk_distill``; ``hold_bytes`` as in
+    ``linear_cross_entropy``."""
     what = "linear_topk_distill"
     _check_common(what, reduction, x, weight, teacher_logits, teacher_index, bias)
     _check_head(what, x, weight, bias)
     lead, heat = x.shape[:-1], float(temperature)
     _check_lists(what, lead, teacher_logits, teacher_index, heat)
-    return _linear(x, weight, bias, None, teacher_logits, teacher_index, (-100, 0.0, heat, reduction), lead)
+    opts = (-100, 0.0, heat, reduction, _bytes(what, hold_bytes))
+    return _linear(x, weight, bias, None, teacher_logits, teacher_index, opts, lead)
 
 
 def topk_distill(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_index: torch.Tensor, *, temperature: float = 1.0,

@@ -126,6 +126,8 @@ def test_losses_of_half_types_are_fp32():
 @pytest.mark.parametrize("error,change", [
     (ValueError, dict(reduction="average")),
     (ValueError, dict(label_smoothing=1.5)),
+    (ValueError, dict(hold_bytes=-1)),
+    (ValueError, dict(hold_bytes=0.5)),
     (ValueError, dict(target=torch.zeros(6, dtype=torch.long))),
     (ValueError, dict(target=torch.zeros(7, 1, dtype=torch.long))),
     (TypeError, dict(target=torch.zeros(7))),

@@ -10,6 +10,8 @@ Tolerances, elementwise, from the roundings that the kernels make (u: half a ste
   * a share is 2^(t - log2 sum 2^t) of t = teacher / T in units of log 2: t and the logarithm are each rounded to
     2^-24 |t| (relative in the share, times log 2), and the exponential and the sum to 2^-22 each:
     2^-22 (4 + |teacher / T|) covers both directions;
+  * the p of held words comes from exponentials that 16-bit operands hold to 2^-12 of themselves and 2^-31 of
+    their tile's largest (hold_bits);
   * G = p - share - eps / V is rounded to the operands' type once (fp32: two planes, 2^-22; fp16 also
     2^-38 absolutely), then summed in fp32 over V (dx) or N (dw, db) terms;
   * a result is rounded to its type once.
@@ -76,22 +78,24 @@ def _share_error(teacher, heat):
     return 2.0 ** -22 * (4 + torch.where(torch.isfinite(t), t, torch.zeros_like(t)).amax(1))
 
 
-def _run_head(x, w, b, target=None, teacher=None, index=None, ignore=-100, smooth=0.0, heat=1.0, reduction="mean", gout=None):
+def _run_head(x, w, b, target=None, teacher=None, index=None, ignore=-100, smooth=0.0, heat=1.0, reduction="mean", gout=None,
+              hold_bytes=vocab_loss.HOLD_BYTES):
     leaves = [t.detach().requires_grad_(True) for t in (x, w, b) if t is not None]
     lb = leaves[2] if b is not None else None
     if target is not None:
-        loss = linear_cross_entropy(leaves[0], leaves[1], target, lb, ignore_index=ignore, label_smoothing=smooth, reduction=reduction)
+        loss = linear_cross_entropy(leaves[0], leaves[1], target, lb, ignore_index=ignore, label_smoothing=smooth, reduction=reduction,
+                                    hold_bytes=hold_bytes)
     else:
-        loss = linear_topk_distill(leaves[0], leaves[1], teacher, index, lb, temperature=heat, reduction=reduction)
+        loss = linear_topk_distill(leaves[0], leaves[1], teacher, index, lb, temperature=heat, reduction=reduction, hold_bytes=hold_bytes)
     gout = torch.ones_like(loss) if gout is None else gout
     return loss.detach(), torch.autograd.grad(loss, leaves, gout), gout
 
 
-def _check_head(x, w, b, **kw):
+def _check_head(x, w, b, got=None, **kw):
     dt = x.dtype
-    loss, grads, gout = _run_head(x, w, b, **kw)
+    loss, grads, gout = got or _run_head(x, w, b, **kw)
     args = dict(target=None, teacher=None, index=None, ignore=-100, smooth=0.0, heat=1.0, reduction="mean")
-    args.update({k: v for k, v in kw.items() if k != "gout"})
+    args.update({k: v for k, v in kw.items() if k not in ("gout", "hold_bytes")})
     n, d, v = x.shape[0], x.shape[1], w.shape[0]
     args["target"] = None if args["target"] is None else args["target"].long()
     x64, w64 = x.double(), w.double()
@@ -114,7 +118,8 @@ def _check_head(x, w, b, **kw):
     _near(loss, ref, bound, "loss")
     u_g = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -22}[dt]
     step = 0.0 if dt == torch.bfloat16 else 2.0 ** -38 * (gout.abs().max().item() * heat)
-    err = A * (u_g + E)[:, None] + step if A.numel() else A
+    held = 0.0 if dt == torch.float32 else 2.0 ** -12
+    err = A * (u_g + held + E)[:, None] + 2.0 ** -19 * held * A.amax(1, keepdim=True) + step if A.numel() else A
     err = err * (A.sum(1, keepdim=True) > 0)
     split = 2.0 ** -21 if dt == torch.float32 else 0.0  # the two planes of w or x, and the lo lo
     bounds = (err @ w64.abs() + (v * 2.0 ** -24 + split) * (A @ w64.abs()), err.t() @ x64.abs() + (n * 2.0 ** -24 + split) * (A.t() @ x64.abs()),
@@ -589,18 +594,78 @@ def _check_words(x, w, t):
     assert (dw[t].double() - refw).abs().max().item() <= 2.0 ** -7 * refw.abs().max().item()
 
 
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("kind", ["target", "list"])
+@pytest.mark.parametrize("n,d,v", [(1, 8, 7), (300, 129, 1111), (513, 64, 641)])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32])
+def test_logits_that_are_not_held(gpu, n, d, v, dt, kind, reduction):
+    """The logits again in the backward pass, as those that ``hold_bytes`` has no room for."""
+    x, w, b, g = _tensors(gpu, n, d, v, dt)
+    gout = torch.randn(n, generator=g, device=gpu) if reduction == "none" else None
+    if kind == "target":
+        target = torch.randint(0, v, (n,), generator=g, device=gpu)
+        target[1::3] = -100
+        kw = dict(target=target, smooth=0.1)
+    else:
+        teacher, index = torch.randn(n, 5, generator=g, device=gpu), torch.stack([torch.randperm(v, device=gpu)[:5] for _ in range(n)])
+        kw = dict(teacher=teacher, index=index, heat=2.0)
+    _check_head(x, w, b, reduction=reduction, gout=gout, hold_bytes=0, **kw)
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32])
+def test_held_exponentials_of_far_apart_tiles(gpu, dt):
+    """Tiles whose maxima are hundreds apart, and tiles and words that are masked at the lowest value and at
+    -inf: as if the masked words were not there."""
+    n, d, v = 260, 16, 1400
+    x, w, b, g = _tensors(gpu, n, d, v, dt)
+    b = b.float()
+    b[:256] -= 300.0
+    b[1024:1100] += 200.0
+    there = torch.ones(v, dtype=torch.bool, device=gpu)
+    for lo, hi, value in ((256, 300, torch.finfo(torch.float32).min), (512, 768, -math.inf), (768, 1024, torch.finfo(torch.float32).min)):
+        b[lo:hi] = value
+        there[lo:hi] = False
+    target = torch.randint(1024, 1100, (n,), generator=g, device=gpu)
+    loss, (dx, dw, db), gout = _run_head(x, w, b, target=target)
+    assert not dw[~there].any() and not db[~there].any()
+    place = (there.cumsum(0) - 1)[target]
+    _check_head(x, w[there], b[there], got=(loss, (dx, dw[there], db[there]), gout), target=place)
+
+
+@pytest.mark.parametrize("hold_bytes", [0, 600 << 20, vocab_loss.HOLD_BYTES])  # no chunk, one, both
 @pytest.mark.parametrize("n,dt", [(2000, torch.bfloat16), (1000, torch.float32)])
-def test_chunks_of_the_vocabulary(gpu, n, dt):
+def test_chunks_of_the_vocabulary(gpu, n, dt, hold_bytes):
     """More than one chunk of logit gradients (512 MiB), a target, a list and a masked word on either side of their border."""
     v = 150000
     x, w, b, g = _tensors(gpu, n, 40, v, dt)
     t = torch.randint(0, v, (n,), generator=g, device=gpu)
     t[::7] = -100
-    _check_head(x, w, b, target=t, smooth=0.1, reduction="sum")
+    _check_head(x, w, b, target=t, smooth=0.1, reduction="sum", hold_bytes=hold_bytes)
     teacher, index = _lists(gpu, g, n, v, 6)
     index[:, 0], index[:, 1] = 75007, 75008
     index[5] = -1
-    _check_head(x, w, b, teacher=teacher, index=index, heat=2.0)
+    _check_head(x, w, b, teacher=teacher, index=index, heat=2.0, hold_bytes=hold_bytes)
+
+
+def test_what_a_call_holds(gpu):
+    """The bytes between forward and backward: of the exponentials at most ``hold_bytes``, none under no_grad."""
+    n, d, v = 1024, 64, 30000
+    x, w, b, g = _tensors(gpu, n, d, v, torch.bfloat16)
+    w.requires_grad_(True)
+    t = torch.randint(0, v, (n,), generator=g, device=gpu)
+    rest = 2 * n * d + 32 * n + (4 << 20)  # (the allocator's blocks of 2 MiB)
+    for hold_bytes in (0, 2 * n * 29000, 2 * n * 31000):  # the vocabulary is one chunk here
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        loss = linear_cross_entropy(x, w, t, b, hold_bytes=hold_bytes)
+        used = torch.cuda.memory_allocated() - before
+        assert used <= rest + (hold_bytes * 1.02 if hold_bytes >= 2 * n * v else 0), (hold_bytes, used)
+        with torch.no_grad():
+            before = torch.cuda.memory_allocated()
+            scored = linear_cross_entropy(x, w, t, b, hold_bytes=hold_bytes)
+            assert torch.cuda.memory_allocated() - before <= rest
+        assert torch.equal(loss, scored)
+        del loss, scored
 
 
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32])
