@@ -23,9 +23,11 @@
 // Rows without a target are dropped before the products (an ordered list of the kept ones, made on the
 // device; tiles past its end return), so a masked-language-model step with 15 % targets costs 15 %.
 //
-// G is held in the operands' 16 bits, which the matrix units take: each entry is off by half a step (bf16
-// 2^-8), at random, so a gradient of many terms is off by about as much as its own rounding once more (bf16
-// 2048 x 2048 x 32000: 0.0023 against 0.0017 of its size).  Everything else is fp32.
+// G is held in the operands' 16 bits, which the matrix units take: each entry is off by at most half a step
+// (bf16 2^-8), at random, so gradients of many rows are off by about as much as their own rounding once more
+// (bf16 2048 x 2048 x 32000: 0.0024 against 0.0017 of their size).  With few rows one entry of one row can
+// decide: there G is two 16-bit rows each, the second what the first one's rounding took, which only fills
+// what is left of a tile.  Everything else is fp32.
 //
 // fp32 operands become two fp16 planes each, x s = hi + lo with s a power of two that puts the tensor's
 // largest finite magnitude at 2^14..2^15, and a product is hi hi + hi lo + lo hi in fp32 accumulators:
@@ -282,6 +284,7 @@ struct PackArgs {
   u16* dst;
   int64_t plane;     // elements between the planes
   int rows, cols, ld;  // ld % 8 == 0
+  int twice;         // the rows once more behind the last one
 };
 
 // eight elements from any address (16-byte loads need no alignment here), zeros past the row's end
@@ -322,6 +325,7 @@ __global__ void __launch_bounds__(256) pack_kernel(PackArgs a) {
     u16* d = a.dst + static_cast<int64_t>(r) * a.ld + c;
     *reinterpret_cast<us8*>(d) = hi;
     if constexpr (DT == kF32) *reinterpret_cast<us8*>(d + a.plane) = lo;
+    else if (a.twice) *reinterpret_cast<us8*>(d + static_cast<int64_t>(rows) * a.ld) = hi;
   }
 }
 
@@ -358,6 +362,7 @@ struct GemmArgs {
   Operand A, B;
   const int* m_dyn;  // rows of A that count (null: M)
   const int* k_dyn;  // length of the sum (null: K)
+  int twice;         // rows of G are two: kGrad writes both, kPartial and kOut read twice as many as m_dyn or k_dyn says
   int M, N, K;
   int chunk;                // kPartial of words: the longest K of the pass, which the splits are made for
   int cut;                  // whether the last round's tiles may be cut in two
@@ -480,8 +485,9 @@ __device__ __forceinline__ float lane_ror(float v) {
   return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x120 + N, 0xF, 0xF, true));
 }
 
-// a wave's part of the tile, rounded to 16 bits, as rows of kLdc; two planes: what the rounding took 128 rows on
-template <bool F16, int PL, int FN>
+// A wave's part of the tile, rounded to 16 bits, as rows of kLdc; two planes: what the rounding took 128 rows on.
+// REST (one plane): what the rounding took, in place of the tile that is there.
+template <bool F16, int PL, int FN, bool REST = false>
 __device__ __forceinline__ void tile_to_lds(const f32x4 (&acc)[8][FN], unsigned char* smem, int row0, int col0) {
   typedef __attribute__((ext_vector_type(4))) u16 us4;
   u16* ct = reinterpret_cast<u16*>(smem);
@@ -489,14 +495,15 @@ __device__ __forceinline__ void tile_to_lds(const f32x4 (&acc)[8][FN], unsigned 
   for (int i = 0; i < 8; ++i)
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
+      u16* o = ct + (row0 + i * 16) * kLdc + col0 + j * 16;
       us4 hi, lo;
+      if (REST) lo = *reinterpret_cast<const us4*>(o);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float v = PL == 2 ? settled(acc[i][j][r]) : acc[i][j][r];
+        const float v = PL == 2 ? settled(acc[i][j][r]) : REST ? acc[i][j][r] - (F16 ? h2f(lo[r]) : bf2f(lo[r])) : acc[i][j][r];
         hi[r] = F16 ? f2h(v) : f2bf(v);
-        lo[r] = PL == 2 ? f2h(v - h2f(hi[r])) : u16(0);
+        if (PL == 2) lo[r] = f2h(v - h2f(hi[r]));
       }
-      u16* o = ct + (row0 + i * 16) * kLdc + col0 + j * 16;
       *reinterpret_cast<us4*>(o) = hi;
       if (PL == 2) *reinterpret_cast<us4*>(o + 128 * kLdc) = lo;
     }
@@ -520,11 +527,17 @@ struct Place {
 // otherwise, where the last round of 256 has at most half its CUs busy, its tiles are cut into two halves
 // of 128 columns (a half takes about two thirds of a tile's time).  Counts depend on how many rows are
 // kept, so a grid is sized for all of them and the blocks behind the last one return.
+__device__ __forceinline__ int rows_of(const GemmArgs& g, int epi) {
+  const int two = epi >= kPartial ? g.twice : 0;
+  return g.m_dyn != nullptr ? *g.m_dyn << two : g.M;
+}
+__device__ __forceinline__ int sum_of(const GemmArgs& g) { return g.k_dyn != nullptr ? *g.k_dyn << g.twice : g.K; }
+
 __device__ __forceinline__ int gemm_blocks(const GemmArgs& g, int epi) {
-  const int M = g.m_dyn != nullptr ? *g.m_dyn : g.M;
+  const int M = rows_of(g, epi);
   const int tiles = ((M + kTile - 1) / kTile) * ((g.N + kTile - 1) / kTile);
   if (epi == kPartial && tiles < 256) {
-    const int span = g.k_dyn != nullptr ? *g.k_dyn : g.chunk;
+    const int span = g.k_dyn != nullptr ? sum_of(g) : g.chunk;
     if (tiles == 0 || span == 0) return 0;
     const int len = split_length(tiles, span);
     return tiles * ((span + len - 1) / len);
@@ -535,8 +548,8 @@ __device__ __forceinline__ int gemm_blocks(const GemmArgs& g, int epi) {
 
 __device__ __forceinline__ Place gemm_place(const GemmArgs& g, int epi, int bid, int blocks) {
   Place at;
-  at.M = g.m_dyn != nullptr ? *g.m_dyn : g.M;
-  const int K = g.k_dyn != nullptr ? *g.k_dyn : g.K;
+  at.M = rows_of(g, epi);
+  const int K = sum_of(g);
   const int ntm = (at.M + kTile - 1) / kTile, ntn = (g.N + kTile - 1) / kTile, tiles = ntm * ntn;
   at.split = at.kbeg = 0;
   at.kend = K;
@@ -904,7 +917,6 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Place& at, un
         }
       }
     } else {
-      // G once into the accumulators: both planes have to come from the same bits of it
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const bool ok = m0 + row0 + i * 16 < M;
@@ -947,19 +959,26 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Place& at, un
         if (tid < BN && n0 + tid < g.ldg) g.colsum[static_cast<int64_t>(m0 / kTile) * g.ldg + n0 + tid] = red[tid] + red[256 + tid];
         __syncthreads();
       }
-      // one plane: the whole tile through LDS; two: both planes of half the rows at a time
-#pragma unroll 1
-      for (int half = 0; half < PL; ++half) {
-        const int rows = kTile / PL;
-        if (PL == 1 || wr == half) tile_to_lds<F16, PL>(acc, smem, PL == 1 ? row0 : fr, col0);
+      // one plane: the whole tile through LDS, and again if G's rows are two; two: both planes of half the
+      // rows at a time
+      const int rows = kTile / PL;
+      auto pass = [&](int half) {
+        const int to = PL == 1 ? half * M : half * rows;
         __syncthreads();
         for (int q = tid; q < kTile * (BN / 8); q += kThreads) {
-          const int line = q / (BN / 8), cc = (q % (BN / 8)) * 8, pl = line / rows, row = half * rows + line % rows;
-          if (m0 + row < M && n0 + cc < g.ldg)
-            *reinterpret_cast<us8*>(g.G + pl * g.g_plane + static_cast<int64_t>(m0 + row) * g.ldg + n0 + cc) =
+          const int line = q / (BN / 8), cc = (q % (BN / 8)) * 8, pl = line / rows, row = m0 + line % rows;
+          if (row + (PL == 1 ? 0 : to) < M && n0 + cc < g.ldg)
+            *reinterpret_cast<us8*>(g.G + pl * g.g_plane + static_cast<int64_t>(row + to) * g.ldg + n0 + cc) =
                 *reinterpret_cast<const us8*>(reinterpret_cast<const u16*>(smem) + line * kLdc + cc);
         }
-        if (half + 1 < PL) __syncthreads();
+      };
+      if (PL == 1 || wr == 0) tile_to_lds<F16, PL>(acc, smem, PL == 1 ? row0 : fr, col0);
+      pass(0);
+      if (PL == 2 || g.twice) {
+        __syncthreads();
+        if (PL == 1) tile_to_lds<F16, 1, FN, true>(acc, smem, row0, col0);
+        else if (wr == 1) tile_to_lds<F16, PL>(acc, smem, fr, col0);
+        pass(1);
       }
     }
   } else if constexpr (EPI == kPartial) {
@@ -1279,7 +1298,7 @@ struct HeldArgs {
   float* colsum;     // [tiles of rows][ldg] or null
   u16* G;
   int64_t g_plane;
-  int ldg;
+  int ldg, twice;
 };
 
 template <int DT>
@@ -1318,11 +1337,12 @@ __global__ void __launch_bounds__(256) held_kernel(HeldArgs a) {
       g[k] = settled(w * (fmaf(g[k], f, -a.smooth_v) - (word == k ? a.share : 0.f)));
       sums[k] += g[k];
       hi[k] = DT == kBF16 ? f2bf(g[k]) : f2h(g[k]);
-      lo[k] = kF ? f2h(g[k] - h2f(hi[k])) : u16(0);
+      lo[k] = DT == kBF16 ? f2bf(g[k] - bf2f(hi[k])) : f2h(g[k] - h2f(hi[k]));
     }
     u16* o = a.G + static_cast<int64_t>(row) * a.ldg + col;
     *reinterpret_cast<us8*>(o) = hi;
     if (kF) *reinterpret_cast<us8*>(o + a.g_plane) = lo;
+    else if (a.twice) *reinterpret_cast<us8*>(o + static_cast<int64_t>(M) * a.ldg) = lo;
   }
   if (a.colsum == nullptr) return;
   __shared__ float red[32][64 + 4];
@@ -1346,6 +1366,7 @@ struct ScatterArgs {
   float g_scale, c;
   u16* G;
   int64_t g_plane;
+  int twice;
 };
 
 __global__ void __launch_bounds__(256) scatter_kernel(ScatterArgs a) {
@@ -1365,16 +1386,17 @@ __global__ void __launch_bounds__(256) scatter_kernel(ScatterArgs a) {
     const u16 hi = a.f16 ? f2h(v) : f2bf(v);
     *o = hi;
     if (a.planes == 2) o[a.g_plane] = f2h(v - h2f(hi));
+    else if (a.twice) o[static_cast<int64_t>(count) * a.ldg] = a.f16 ? f2h(v - h2f(hi)) : f2bf(v - bf2f(hi));
   }
 }
 
 // column sums of a chunk's G after the scatter (rows split over blockIdx.y)
 __global__ void __launch_bounds__(256) colsum_kernel(const u16* G, int64_t g_plane, int planes, int f16, int ldg, const int* info,
-                                                     float* part) {
+                                                     int twice, float* part) {
   __shared__ float red[8][256 + 8];
   const int tid = threadIdx.x, cg = tid & 31, rg = tid >> 5;
   const int col = blockIdx.x * 256 + cg * 8;
-  const int count = info[0];
+  const int count = info[0] << twice;
   float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   if (col < ldg)
     for (int r = blockIdx.y * 8 + rg; r < count; r += gridDim.y * 8)
@@ -1407,9 +1429,9 @@ __global__ void __launch_bounds__(256) dbias_kernel(const float* part, int split
 // The sum of a row's partials: of dh (pos: a row's place among the kept ones; zeros for the others), or of
 // dw (pos null; rows of words, pieces of the kept rows).  Bound by memory (4608 rows, 28 pieces of 691 kept:
 // 59 MB in 13 us)
-__global__ void __launch_bounds__(256) sum_kernel(const float* part, int span, int64_t ldo, const int* info, const int* pos,
+__global__ void __launch_bounds__(256) sum_kernel(const float* part, int span, int64_t ldo, const int* info, const int* pos, int twice,
                                                   Alpha alpha, int planes, void* dx, int dt, int D) {
-  const int n = blockIdx.x, at = pos != nullptr ? pos[n] : n, count = pos != nullptr ? info[0] : gridDim.x;
+  const int n = blockIdx.x, at = pos != nullptr ? pos[n] : n, count = pos != nullptr ? info[0] << twice : gridDim.x;
   const int tiles = ((count + kTile - 1) / kTile) * ((D + kTile - 1) / kTile);
   int splits = 0;
   if (pos == nullptr) span = info[0];
@@ -1426,6 +1448,9 @@ __global__ void __launch_bounds__(256) sum_kernel(const float* part, int span, i
     const float* p = part + at * ldo + d;
 #pragma unroll 4
     for (int s = 0; s < splits; ++s) t += *reinterpret_cast<const f32x4*>(p + s * stride);
+    if (twice)
+#pragma unroll 4
+      for (int s = 0; s < splits; ++s) t += *reinterpret_cast<const f32x4*>(p + info[0] * ldo + s * stride);
     t *= a;
     if (wide) {
       if (dt == kF32) {
@@ -1763,23 +1788,28 @@ namespace {
 
 // What both directions lay out in the workspace.
 struct Plan {
-  int planes, ldh, chunk, nchunks, parts, csplits, held;
+  int planes, ldh, chunk, nchunks, parts, csplits, held, twice;
   bool pack_w, keep_w, split_w;
   int64_t off_rows_info, off_h, off_e, off_tops, off_kw, kept;  // in `kept`
   int64_t off_w, off_flag, off_part, off_partz, off_rows, off_roww, off_alpha, off_g, off_dx, off_dw, off_cs, total;
 };
 
 constexpr int64_t kChunkBytes = int64_t(512) << 20;  // G of one chunk, and the packed weights of one
+// Rows of G are two where both of all fit one tile of rows.  The mean square of 128 rounding errors is near its
+// expectation; of one it is up to 5 times that.  A step against 128000 x 4096 bf16: 16 rows 775 us, of one each
+// 757; 128 rows 1004 and 873.
+constexpr int kFewRows = 128;
 constexpr int64_t kKeepBytes = int64_t(4) << 30;      // packed weights that are held from forward to backward
 
 Plan plan(const DetVocabHead& p, bool backward) {
   Plan q = {};
   q.planes = p.dtype == kF32 ? 2 : 1;
   q.ldh = static_cast<int>(up(p.D, 8));
+  q.twice = p.dtype != kF32 && p.N <= kFewRows;
   // read as they are: 16-byte rows, and 256 of them within 32-bit offsets
   q.pack_w = p.dtype == kF32 || p.D % 8 != 0 || p.w_ld % 8 != 0 || (reinterpret_cast<uintptr_t>(p.w) & 15) != 0 ||
              p.w_ld > (int64_t(1) << 21);
-  const int64_t w_bytes = int64_t(2) * q.planes * p.V * q.ldh, h_bytes = up(int64_t(2) * q.planes * p.N * q.ldh, 256);
+  const int64_t w_bytes = int64_t(2) * q.planes * p.V * q.ldh, h_bytes = up((int64_t(2) * q.planes * p.N * q.ldh) << q.twice, 256);
   q.keep_w = q.pack_w && w_bytes <= kKeepBytes;
   q.off_rows_info = up(int64_t(8) * p.N * (1 + p.K), 256);
   q.off_h = q.off_rows_info + up(int64_t(4) * (4 + 3 * int64_t(p.N)), 256);
@@ -1822,14 +1852,14 @@ Plan plan(const DetVocabHead& p, bool backward) {
   } else {
     q.off_roww = take(int64_t(4) * p.N);
     q.off_alpha = take(4);
-    q.off_g = take(int64_t(2) * q.planes * p.N * q.chunk);
+    q.off_g = take((int64_t(2) * q.planes * p.N * q.chunk) << q.twice);
     // partials: a row's for every piece, or at most 256 tiles' worth
     auto partials = [&](int64_t rows, int64_t span) {
       int64_t n = (span / 512 > 1 ? span / 512 : 1) * rows * q.ldh;
       if (n > int64_t(256) * kTile * kTile) n = int64_t(256) * kTile * kTile;
       return 4 * (n < rows * q.ldh ? rows * q.ldh : n);
     };
-    q.off_dx = p.dx != nullptr ? take(partials(p.N, q.chunk)) : 0;
+    q.off_dx = p.dx != nullptr ? take(partials(int64_t(p.N) << q.twice, q.chunk)) : 0;
     // few tiles under many rows (8192 x 64 x 1000 bf16: 155 us for four blocks, 20 us in pieces)
     q.split_w = int64_t(ceil_div(q.chunk, kTile)) * ceil_div(p.D, kTile) <= 128 && p.N >= 1024;
     q.off_dw = p.dw != nullptr && q.split_w ? take(partials(q.chunk, p.N)) : 0;
@@ -1899,6 +1929,7 @@ int pack_hidden(hipStream_t st, const Head& p, const Plan& q) {
   a.rows = p.N;
   a.cols = p.D;
   a.ld = q.ldh;
+  a.twice = q.twice;
   return pack_any(st, p.dtype, a);
 }
 
@@ -1941,6 +1972,7 @@ GemmArgs logits_args(const Head& p, const Plan& q, const Operand& w, int v0, int
   a.v0 = v0;
   a.picked = p.stats + int64_t(2) * p.N;
   a.share = 1.f - p.smooth;
+  a.twice = q.twice;
   return a;
 }
 
@@ -2075,7 +2107,7 @@ int det_vocab_head_backward(void* stream, const DetVocabHead* pp) {
     a.ldg = ldg;
     if (held) {
       const HeldArgs h = {p.e + int64_t(2) * q.planes * v0, p.tops + v0 / 128, q.held, p.rows, a.top, a.log_s, row_w, g_scale, a.c, a.smooth_v, a.share, a.words, v0,
-                          a.colsum, a.G, a.g_plane, ldg};
+                          a.colsum, a.G, a.g_plane, ldg, q.twice};
       const dim3 hg(static_cast<unsigned>(ldg / 64) * ceil_div(p.N, kTile));
       if (p.dtype == kF32) hipLaunchKernelGGL(held_kernel<kF32>, hg, dim3(256), 0, st, h);
       else if (p.dtype == kBF16) hipLaunchKernelGGL(held_kernel<kBF16>, hg, dim3(256), 0, st, h);
@@ -2085,12 +2117,12 @@ int det_vocab_head_backward(void* stream, const DetVocabHead* pp) {
     }
     if (p.index != nullptr) {
       ScatterArgs s = {p.rows, list, p.index, p.index_ld, p.wide, p.K, v0, nv, f16, q.planes, ldg, picked,
-                       picked + int64_t(p.N) * p.K, a.top, a.log_s, row_w, g_scale, a.c, a.G, a.g_plane};
+                       picked + int64_t(p.N) * p.K, a.top, a.log_s, row_w, g_scale, a.c, a.G, a.g_plane, q.twice};
       const int64_t sb = (int64_t(p.N) * p.K + 255) / 256;
       hipLaunchKernelGGL(scatter_kernel, dim3(sb < 8192 ? static_cast<unsigned>(sb) : 8192u), dim3(256), 0, st, s);
       if (cs != nullptr)
         hipLaunchKernelGGL(colsum_kernel, dim3(ceil_div(ldg, 256), q.csplits), dim3(256), 0, st, a.G, a.g_plane, q.planes, f16, ldg,
-                           p.rows, cs);
+                           p.rows, q.twice, cs);
     }
     const Operand G = {a.G, a.g_plane, ldg};
     if (cs != nullptr)
@@ -2103,7 +2135,8 @@ int det_vocab_head_backward(void* stream, const DetVocabHead* pp) {
       d.B = w;
       d.m_dyn = p.rows;
       d.info = p.rows;
-      d.M = p.N;
+      d.twice = q.twice;
+      d.M = p.N << q.twice;
       d.N = p.D;
       d.K = nv;
       d.chunk = q.chunk;
@@ -2119,16 +2152,17 @@ int det_vocab_head_backward(void* stream, const DetVocabHead* pp) {
       d.B = Operand{p.hidden, int64_t(p.N) * q.ldh, q.ldh};
       d.k_dyn = p.rows;
       d.info = p.rows;
+      d.twice = q.twice;
       d.M = nv;
       d.N = p.D;
-      d.K = p.N;
+      d.K = p.N << q.twice;
       d.out = static_cast<char*>(p.dw) + int64_t(v0) * p.D * es;
       if (q.split_w) {
         d.out32 = reinterpret_cast<float*>(ws + q.off_dw);
         d.ldo = q.ldh;
         DET_TRY((gemm<true, true, kPartial>(st, p.dtype, d)));
         hipLaunchKernelGGL(sum_kernel, dim3(nv, ceil_div(p.D, 1024) < 64 ? ceil_div(p.D, 1024) : 64), dim3(256), 0, st, d.out32, 0,
-                           d.ldo, p.rows, nullptr, alpha, q.planes, d.out, p.dtype, p.D);
+                           d.ldo, p.rows, nullptr, 0, alpha, q.planes, d.out, p.dtype, p.D);
       } else {
         d.cut = 1;
         d.ldo = p.D;
@@ -2139,7 +2173,7 @@ int det_vocab_head_backward(void* stream, const DetVocabHead* pp) {
   }
   if (p.dx != nullptr)
     hipLaunchKernelGGL(sum_kernel, dim3(p.N, ceil_div(p.D, 1024) < 64 ? ceil_div(p.D, 1024) : 64), dim3(256), 0, st,
-                       reinterpret_cast<const float*>(ws + q.off_dx), q.chunk, int64_t(q.ldh), p.rows, list + p.N, alpha, q.planes,
+                       reinterpret_cast<const float*>(ws + q.off_dx), q.chunk, int64_t(q.ldh), p.rows, list + p.N, q.twice, alpha, q.planes,
                        p.dx, p.dtype, p.D);
   return static_cast<int>(hipGetLastError());
 }

@@ -12,8 +12,8 @@ Tolerances, elementwise, from the roundings that the kernels make (u: half a ste
     2^-22 (4 + |teacher / T|) covers both directions;
   * the p of held words comes from exponentials that 16-bit operands hold to 2^-12 of themselves and 2^-31 of
     their tile's largest (hold_bits);
-  * G = p - share - eps / V is rounded to the operands' type once (fp32: two planes, 2^-22; fp16 also
-    2^-38 absolutely), then summed in fp32 over V (dx) or N (dw, db) terms;
+  * G = p - share - eps / V is rounded to the operands' type once (fp32: two planes, 2^-22; up to 128 rows of 16
+    bits: two rows each, the square of one's; fp16 also 2^-38 absolutely), then summed in fp32 over V (dx) or N (dw, db) terms;
   * a result is rounded to its type once.
 """
 import math
@@ -33,7 +33,7 @@ NAMES = ("dx", "dweight", "dbias")
 
 
 def _definition(z, target, teacher, index, ignore, smooth, heat, reduction, gout):
-    """(loss, G, A): the loss, its derivative by z, and the magnitudes that G is a difference of."""
+    """(loss, G, A, P): the loss, its derivative by z, the magnitudes that G is a difference of, and p's part of them."""
     n, v = z.shape
     q = torch.zeros_like(z)
     if target is not None:
@@ -57,7 +57,8 @@ def _definition(z, target, teacher, index, ignore, smooth, heat, reduction, gout
     up = (each * gout.double() * heat)[:, None]
     loss = rows if reduction == "none" else (rows * each).sum()
     zero = torch.zeros_like(z)  # an ignored row's p may be anything
-    return loss, torch.where(kept[:, None], up * (logp.exp() - q), zero), torch.where(kept[:, None], up.abs() * (logp.exp() + q), zero)
+    return loss, torch.where(kept[:, None], up * (logp.exp() - q), zero), torch.where(kept[:, None], up.abs() * (logp.exp() + q), zero), (
+        torch.where(kept[:, None], up.abs() * logp.exp(), zero))
 
 
 def _near(got, ref, bound, name):
@@ -104,7 +105,7 @@ def _check_head(x, w, b, got=None, **kw):
     if b is not None:
         z = z + b.double()
         size = size + b.double().abs()
-    ref, G, A = _definition(z, gout=gout, **args)
+    ref, G, A, P = _definition(z, gout=gout, **args)
     heat = args["heat"]
     product = d * 2.0 ** -24 + (2.0 ** -21 if dt == torch.float32 else 0.0)
     E = (2 * product * size.amax(1) + 3 * 2.0 ** -24 * (z / heat).abs().amax(1) * 1.5) / heat + _sum_error(v)  # [n]
@@ -117,9 +118,11 @@ def _check_head(x, w, b, got=None, **kw):
         row_bound.mean() if args["reduction"] == "mean" else row_bound.sum()) + 2.0 ** -22 * ref.abs()
     _near(loss, ref, bound, "loss")
     u_g = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -22}[dt]
+    if n <= 128 and dt != torch.float32:
+        u_g = u_g ** 2  # two rows of G each
     step = 0.0 if dt == torch.bfloat16 else 2.0 ** -38 * (gout.abs().max().item() * heat)
-    held = 0.0 if dt == torch.float32 else 2.0 ** -12
-    err = A * (u_g + held + E)[:, None] + 2.0 ** -19 * held * A.amax(1, keepdim=True) + step if A.numel() else A
+    held = 0.0 if dt == torch.float32 or kw.get("hold_bytes") == 0 else 2.0 ** -12
+    err = A * (u_g + E)[:, None] + held * (P + 2.0 ** -19 * P.amax(1, keepdim=True)) + step if A.numel() else A
     err = err * (A.sum(1, keepdim=True) > 0)
     split = 2.0 ** -21 if dt == torch.float32 else 0.0  # the two planes of w or x, and the lo lo
     bounds = (err @ w64.abs() + (v * 2.0 ** -24 + split) * (A @ w64.abs()), err.t() @ x64.abs() + (n * 2.0 ** -24 + split) * (A.t() @ x64.abs()),
@@ -195,7 +198,7 @@ def _check_logits(z, teacher, index, heat=1.0, reduction="mean", gout=None):
     loss = loss.detach()
     v = z.shape[1]
     z64 = z.double()
-    ref, G, A = _definition(z64, None, teacher, index.long(), -100, 0.0, heat, reduction, gout)
+    ref, G, A, _ = _definition(z64, None, teacher, index.long(), -100, 0.0, heat, reduction, gout)
     top = torch.where(torch.isfinite(z64), z64.abs(), torch.zeros_like(z64)).amax(1) / heat
     E = 3 * 2.0 ** -24 * 1.5 * top + _sum_error(v)
     rows = heat * heat * (2 * E + 2.0 ** -22 * (1 + top) + _share_error(teacher, heat))
@@ -558,7 +561,7 @@ def test_offsets_past_32_bits(gpu):
     rows = torch.tensor([0, 1, 16776, 16777, 16999], device=gpu)  # 16777 * 128000 is the first row past 2^31
     got = z.grad[rows]
     z.grad = None
-    _, G, A = _definition(z.detach()[rows].double(), None, teacher[rows], index[rows], -100, 0.0, 1.0, "none", torch.ones(5, device=gpu))
+    _, G, A, _ = _definition(z.detach()[rows].double(), None, teacher[rows], index[rows], -100, 0.0, 1.0, "none", torch.ones(5, device=gpu))
     _near(got, G, A * 2.0 ** -14 + 1.01 * U[torch.bfloat16] * G.abs(), "dlogits")
     del z, got
     v, d = 530000, 4096  # 2.2e9 weights
