@@ -37,6 +37,7 @@
 // 5e-7 of the gradients' size, an fp32 product by 1.8e-6).
 #include <hip/hip_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 
 namespace {
@@ -1751,8 +1752,14 @@ int ceil_div(int64_t x, int64_t a) { return static_cast<int>((x + a - 1) / a); }
 
 template <bool F16, int PL, bool ACOL, bool BCOL, int EPI>
 int launch_gemm(hipStream_t st, const GemmArgs& a) {
-  const void* fn = reinterpret_cast<const void*>(&gemm_kernel<F16, PL, ACOL, BCOL, EPI>);
-  const hipError_t e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, kGemmSmem);
+  static std::atomic<uint64_t> set{0};  // the devices whose kernel has its LDS size
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  if (e == hipSuccess && (dev > 63 || !(set.load(std::memory_order_relaxed) >> dev & 1))) {
+    const void* fn = reinterpret_cast<const void*>(&gemm_kernel<F16, PL, ACOL, BCOL, EPI>);
+    e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, kGemmSmem);
+    if (e == hipSuccess && dev < 64) set.fetch_or(uint64_t(1) << dev, std::memory_order_relaxed);
+  }
   if (e != hipSuccess) return static_cast<int>(e);
   int64_t tiles = static_cast<int64_t>(ceil_div(a.M, kTile)) * ceil_div(a.N, kTile);
   tiles += 128;                                     // cut ones of the last round

@@ -27,6 +27,7 @@ from typing import Any, Optional
 
 import torch
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 
 from determined_1_amd.ops import _lib
 from determined_1_amd.ops.arena import landing_buffer
@@ -75,14 +76,26 @@ def _buffer(nbytes: int, like: torch.Tensor, what: str) -> torch.Tensor:
 
 def _on(t: torch.Tensor):
     """The tensor's device as the current one (a kernel is launched on the current device)."""
-    return _null() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+    return _null() if t.device.index == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
+
+
+def _traced(*ts: Optional[torch.Tensor]) -> bool:
+    """Whether autograd has to see the call (forward mode: to refuse it)."""
+    return forward_ad._current_level >= 0 or (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts))
+
+
+def _once(fn):
+    """``once_differentiable`` without its cost (5 us a call) where no second derivative can be asked for."""
+    guarded = torch.autograd.function.once_differentiable(fn)
+    return staticmethod(lambda ctx, gout: (guarded if torch.is_grad_enabled() else fn)(ctx, gout))
 
 
 class _Head(torch.autograd.Function):
     """x [N, D], weight [V, D]: unit last strides; target [N], or index and teacher [N, K]."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias, target, teacher, index, opts):  # type: ignore[override]
+    def run(x, weight, bias, target, teacher, index, opts):
+        """(loss, what the backward pass needs, the call)"""
         ignore, smooth, heat, reduction, hold_bytes = opts
         p = _HeadParams()
         p.N, p.D = x.shape
@@ -106,12 +119,15 @@ class _Head(torch.autograd.Function):
         p.kept_bytes, p.ws_bytes = kept.numel(), ws.numel()
         with _on(x):
             _lib.check(lib.det_vocab_head_forward(_stream(x), ref), "det_vocab_head_forward")
-        ctx.save_for_backward(x, weight, bias, target, teacher, index, kept)
-        ctx.params = p
-        return loss
+        return loss, kept, p
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    def forward(ctx, x, weight, bias, target, teacher, index, opts):  # type: ignore[override]
+        loss, kept, ctx.params = _Head.run(x, weight, bias, target, teacher, index, opts)
+        ctx.save_for_backward(x, weight, bias, target, teacher, index, kept)
+        return loss
+
+    @_once
     def backward(ctx, gout):  # type: ignore[override]
         x, weight, bias, target, teacher, index, kept = ctx.saved_tensors
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
@@ -122,14 +138,14 @@ class _Head(torch.autograd.Function):
         if index is not None:
             p.index, p.teacher, p.index_ld, p.teacher_ld = index.data_ptr(), teacher.data_ptr(), index.stride(0), teacher.stride(0)
         gout = gout.float().contiguous()
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
+        dx = torch.empty_like(x, memory_format=torch.contiguous_format) if need_x else None
         dw = db = None
         if need_w:
             dw = landing_buffer(weight)
             if dw is None or dw.dtype != weight.dtype or not dw.is_contiguous() or dw.shape != weight.shape:
-                dw = torch.empty(weight.shape, dtype=weight.dtype, device=weight.device)
+                dw = torch.empty_like(weight, memory_format=torch.contiguous_format)
         if need_b:
-            db = torch.empty(bias.shape, dtype=bias.dtype, device=bias.device)
+            db = torch.empty_like(bias)
         p.dx, p.dw, p.db, p.gout = _ptr(dx), _ptr(dw), _ptr(db), gout.data_ptr()
         ref, lib = ctypes.byref(p), _lib.get_lib()
         ws = _buffer(lib.det_vocab_head_bytes(ref, 2), x, "vocab_loss")
@@ -143,7 +159,8 @@ class _Logits(torch.autograd.Function):
     """logits [N, V], teacher and index [N, K]: unit last strides."""
 
     @staticmethod
-    def forward(ctx, z, teacher, index, heat, reduction):  # type: ignore[override]
+    def run(z, teacher, index, heat, reduction):
+        """(loss, what the backward pass needs, the call)"""
         p = _LogitParams()
         p.N, p.V = z.shape
         p.z, p.index, p.teacher, p.K = z.data_ptr(), index.data_ptr(), teacher.data_ptr(), index.shape[1]
@@ -156,12 +173,15 @@ class _Logits(torch.autograd.Function):
         p.loss, p.kept, p.kept_bytes = loss.data_ptr(), kept.data_ptr(), kept.numel()
         with _on(z):
             _lib.check(lib.det_vocab_logits_forward(_stream(z), ref), "det_vocab_logits_forward")
-        ctx.save_for_backward(z, teacher, index, kept)
-        ctx.params = p
-        return loss
+        return loss, kept, p
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    def forward(ctx, z, teacher, index, heat, reduction):  # type: ignore[override]
+        loss, kept, ctx.params = _Logits.run(z, teacher, index, heat, reduction)
+        ctx.save_for_backward(z, teacher, index, kept)
+        return loss
+
+    @_once
     def backward(ctx, gout):  # type: ignore[override]
         z, teacher, index, kept = ctx.saved_tensors
         p = _LogitParams.from_buffer_copy(ctx.params)
@@ -169,7 +189,7 @@ class _Logits(torch.autograd.Function):
         p.z, p.index, p.teacher, p.kept = z.data_ptr(), index.data_ptr(), teacher.data_ptr(), kept.data_ptr()
         p.z_ld, p.index_ld, p.teacher_ld = z.stride(0), index.stride(0), teacher.stride(0)
         gout = gout.float().contiguous()
-        dz = torch.empty(z.shape, dtype=z.dtype, device=z.device)
+        dz = torch.empty_like(z, memory_format=torch.contiguous_format)
         p.gout, p.dz, p.dz_ld = gout.data_ptr(), dz.data_ptr(), dz.stride(0)
         with _on(z):
             _lib.check(_lib.get_lib().det_vocab_logits_backward(_stream(z), ctypes.byref(p)), "det_vocab_logits_backward")
@@ -310,10 +330,11 @@ def _linear(x, weight, bias, target, teacher, index, opts, lead) -> torch.Tensor
             weight = weight.contiguous()
         if bias is not None and bias.stride(0) != 1:
             bias = bias.contiguous()
-        if not torch.is_grad_enabled() or not (x2.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
-            opts = (*opts[:4], 0)  # no backward pass to hold anything for
-        with torch.autocast("cuda", enabled=False) if ac else _null():
-            loss = _Head.apply(x2, weight, bias, target, teacher, index, opts)
+        if not _traced(x2, weight, bias):
+            loss = _Head.run(x2, weight, bias, target, teacher, index, (*opts[:4], 0))[0]  # nothing to hold anything for
+        else:
+            with torch.autocast("cuda", enabled=False) if ac else _null():
+                loss = _Head.apply(x2, weight, bias, target, teacher, index, opts)
     return loss if opts[3] != "none" or len(lead) == 1 else loss.reshape(lead)
 
 
@@ -381,5 +402,5 @@ def topk_distill(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ind
     if logits.device.type == "cpu":
         loss = _plain_distill(_wide(z), teacher, index, heat, reduction)
     else:
-        loss = _Logits.apply(z, teacher, index, heat, reduction)
+        loss = _Logits.apply(z, teacher, index, heat, reduction) if _traced(z) else _Logits.run(z, teacher, index, heat, reduction)[0]
     return loss if reduction != "none" or len(lead) == 1 else loss.reshape(lead)

@@ -770,6 +770,25 @@ def test_trial_eager_and_replayed(gpu, monkeypatch):
     assert abs(got["1"][1] - got["0"][1]) <= 1e-4 * abs(got["0"][1])
 
 
+def test_second_and_forward_derivatives_are_refused(gpu):
+    from torch.autograd import forward_ad
+
+    x, w, b, g = _tensors(gpu, 9, 16, 50, torch.float32)
+    t = torch.randint(0, 50, (9,), generator=g, device=gpu)
+    teacher, index = _lists(gpu, g, 9, 50, 3)
+    for call in (lambda x: linear_cross_entropy(x, w, t, b), lambda x: linear_topk_distill(x, w, teacher, index, b),
+                 lambda x: topk_distill(x, teacher, index % 16)):
+        leaf = x.detach().requires_grad_(True)
+        first, = torch.autograd.grad(call(leaf), leaf)
+        again, = torch.autograd.grad(call(leaf), leaf, create_graph=True)
+        assert torch.equal(first, again)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(again.sum(), leaf)
+        with forward_ad.dual_level():
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                call(forward_ad.make_dual(x, torch.ones_like(x)))
+
+
 def test_backward_twice(gpu):
     x, w, b, g = _tensors(gpu, 70, 100, 300, torch.float32)
     t = torch.randint(0, 300, (70,), generator=g, device=gpu)
