@@ -1006,22 +1006,18 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Place& at, un
 #pragma unroll
       for (int j = 0; j < FN; ++j) acc[i][j] *= alpha;
     if constexpr (PL == 1) {
-      const bool wide = (g.ldo & 7) == 0 && (reinterpret_cast<uintptr_t>(g.out) & 15) == 0;
       tile_to_lds<F16, 1>(acc, smem, row0, col0);
       __syncthreads();
       const u16* ct = reinterpret_cast<const u16*>(smem);
       u16* out = static_cast<u16*>(g.out);
-      if (wide) {
-        for (int q = tid; q < kTile * (BN / 8); q += kThreads) {
-          const int row = q / (BN / 8), cc = (q % (BN / 8)) * 8;
-          if (m0 + row < M && n0 + cc < g.N)
-            *reinterpret_cast<us8*>(out + (m0 + row) * g.ldo + n0 + cc) = *reinterpret_cast<const us8*>(ct + row * kLdc + cc);
-        }
-      } else {
-        for (int q = tid; q < kTile * BN; q += kThreads) {
-          const int row = q / BN, cc = q % BN;
-          if (m0 + row < M && n0 + cc < g.N) out[(m0 + row) * g.ldo + n0 + cc] = ct[row * kLdc + cc];
-        }
+      // 16-byte stores need no alignment here, so rows of any width take them
+      for (int q = tid; q < kTile * (BN / 8); q += kThreads) {
+        const int row = q / (BN / 8), cc = (q % (BN / 8)) * 8, left = g.N - n0 - cc;
+        if (m0 + row >= M) continue;
+        u16* o = out + (m0 + row) * g.ldo + n0 + cc;
+        if (left >= 8) __builtin_memcpy(o, ct + row * kLdc + cc, 16);
+        else
+          for (int e = 0; e < left; ++e) o[e] = ct[row * kLdc + cc + e];
       }
     } else {
       float* ct = reinterpret_cast<float*>(smem);  // half the rows at a time
@@ -1034,9 +1030,13 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Place& at, un
 #pragma unroll
             for (int j = 0; j < FN; ++j) *reinterpret_cast<f32x4*>(ct + (fr + i * 16) * kLdc32 + col0 + j * 16) = acc[i][j];
         __syncthreads();
-        for (int q = tid; q < 128 * BN; q += kThreads) {
-          const int row = q / BN, cc = q % BN;
-          if (m0 + half * 128 + row < M && n0 + cc < g.N) out[(m0 + half * 128 + row) * g.ldo + n0 + cc] = ct[row * kLdc32 + cc];
+        for (int q = tid; q < 128 * (BN / 4); q += kThreads) {
+          const int row = q / (BN / 4), cc = (q % (BN / 4)) * 4, left = g.N - n0 - cc;
+          if (m0 + half * 128 + row >= M) continue;
+          float* o = out + (m0 + half * 128 + row) * g.ldo + n0 + cc;
+          if (left >= 4) __builtin_memcpy(o, ct + row * kLdc32 + cc, 16);
+          else
+            for (int e = 0; e < left; ++e) o[e] = ct[row * kLdc32 + cc + e];
         }
         __syncthreads();
       }
@@ -1443,7 +1443,6 @@ __global__ void __launch_bounds__(256) sum_kernel(const float* part, int span, i
   float a = alpha();
   if (planes == 2) a *= pow2(-scale_exp(static_cast<uint32_t>(info[pos != nullptr ? 2 : 1])));
   const int64_t stride = count * ldo, out = static_cast<int64_t>(n) * D;
-  const bool wide = (D & 3) == 0 && (reinterpret_cast<uintptr_t>(dx) & 15) == 0;
   for (int d = (blockIdx.y * 256 + threadIdx.x) * 4; d < D; d += gridDim.y * 1024) {
     f32x4 t = f32x4{0.f, 0.f, 0.f, 0.f};
     const float* p = part + at * ldo + d;
@@ -1453,15 +1452,15 @@ __global__ void __launch_bounds__(256) sum_kernel(const float* part, int span, i
 #pragma unroll 4
       for (int s = 0; s < splits; ++s) t += *reinterpret_cast<const f32x4*>(p + info[0] * ldo + s * stride);
     t *= a;
-    if (wide) {
+    if (d + 4 <= D) {  // (wide stores need no alignment)
       if (dt == kF32) {
-        *reinterpret_cast<f32x4*>(static_cast<float*>(dx) + out + d) = t;
+        __builtin_memcpy(static_cast<float*>(dx) + out + d, &t, 16);
       } else {
         typedef __attribute__((ext_vector_type(4))) u16 us4;
         us4 o;
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] = dt == kBF16 ? f2bf(t[e]) : f2h(t[e]);
-        *reinterpret_cast<us4*>(static_cast<u16*>(dx) + out + d) = o;
+        __builtin_memcpy(static_cast<u16*>(dx) + out + d, &o, 8);
       }
     } else {
 #pragma unroll
