@@ -15,7 +15,7 @@
 // adds the K listed logits, dot products of their own.  Backward: the vocabulary is walked in chunks; per
 // chunk G is written to a workspace, and two more products read it.  G comes from the tile's exponentials,
 // which the forward held in 16 bits as far as the caller's bound goes (2 GiB unless it says otherwise), and past
-// that from the product once more, in its epilogue.  What bounds it, 8192 x 4096 x 128000 bf16 in 22.2 ms: the
+// that from the product once more, in its epilogue.  What bounds it, 8192 x 4096 x 128000 bf16 in 22.1 ms: the
 // matrix units, 1.23 PFLOP/s over the three products (logits 6.8 ms, G w 6.9, G^T h 7.4; G from 2 GB of
 // exponentials 0.8, where the product again takes 6.7); for few rows the reads of w (one row against
 // 128000 x 4096: 5.3 TB/s).
@@ -34,7 +34,7 @@
 // each operand is held to 2^-23 of itself (2^-39 of the tensor's largest value at worst) and the
 // dropped lo lo is below 2^-22 of its product, the size of one fp32 rounding, at a third of the matrix
 // units' 16-bit rate instead of the sixteenth that their fp32 instructions have (2240 x 850 x 10000: off by
-// 5e-7 of the gradients' size, an fp32 product by 1.8e-6).
+// 5e-7 of the gradients' size, an fp32 product by 1.9e-6).
 #include <hip/hip_runtime.h>
 
 #include <atomic>
@@ -894,7 +894,9 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Place& at, un
           u16* out = static_cast<u16*>(g.E) + g.v0 + n0;
           for (int q = tid; q < kTile * (BN / 8); q += kThreads) {
             const int row = q / (BN / 8), cc = (q % (BN / 8)) * 8;
-            if (m0 + row < M) *reinterpret_cast<us8*>(out + static_cast<int64_t>(m0 + row) * g.held + cc) = *reinterpret_cast<const us8*>(ct + row * kLdc + cc);
+            if (m0 + row < M)
+              *reinterpret_cast<us8*>(out + static_cast<int64_t>(m0 + row) * g.held + cc) =
+                  *reinterpret_cast<const us8*>(ct + row * kLdc + cc);
           }
         } else {
           float* ct = reinterpret_cast<float*>(smem);  // half the rows at a time
@@ -2112,8 +2114,8 @@ int det_vocab_head_backward(void* stream, const DetVocabHead* pp) {
     a.g_plane = int64_t(p.N) * ldg;
     a.ldg = ldg;
     if (held) {
-      const HeldArgs h = {p.e + int64_t(2) * q.planes * v0, p.tops + v0 / 128, q.held, p.rows, a.top, a.log_s, row_w, g_scale, a.c, a.smooth_v, a.share, a.words, v0,
-                          a.colsum, a.G, a.g_plane, ldg, q.twice};
+      const HeldArgs h = {p.e + int64_t(2) * q.planes * v0, p.tops + v0 / 128, q.held, p.rows, a.top, a.log_s, row_w, g_scale, a.c,
+                          a.smooth_v, a.share, a.words, v0, a.colsum, a.G, a.g_plane, ldg, q.twice};
       const dim3 hg(static_cast<unsigned>(ldg / 64) * ceil_div(p.N, kTile));
       if (p.dtype == kF32) hipLaunchKernelGGL(held_kernel<kF32>, hg, dim3(256), 0, st, h);
       else if (p.dtype == kBF16) hipLaunchKernelGGL(held_kernel<kBF16>, hg, dim3(256), 0, st, h);
