@@ -22,7 +22,7 @@ def pytest_configure(config):
         # what xdist's own pytest_cmdline_main derives from ``-n`` (it has run by now)
         config.option.numprocesses = workers
         if getattr(config.option, "dist", "no") == "no":
-            config.option.dist = "load"
+            config.option.dist = "loadfile"  # a module's tests share its fixtures and go in order
         config.option.tx = ["popen"] * workers
 
 
