@@ -1124,16 +1124,21 @@ __device__ __forceinline__ float diverge(float q, float t, float tt, float tl, f
   return q * (((t - tt) * inv_t - tl * kLn2) - ((z - top) * inv_t - log_s * kLn2));
 }
 
-// one target a row: a wave each (8192 rows of 1000 parts in 13 us)
+// one target a row: a wave each (8192 rows of 1000 parts in 18 us, one row in 5)
 __global__ void __launch_bounds__(256) finish_target_kernel(FinishArgs a) {
   const int lane = threadIdx.x & 63, count = a.info[0];
   for (int row = blockIdx.x * 4 + (threadIdx.x >> 6); row < count; row += gridDim.x * 4) {
     float m = kNegInf, s = 0.f, sz = 0.f;
     const int64_t at = static_cast<int64_t>(row) * a.parts;
-    for (int t = lane; t < a.parts; t += 64) {
-      const float2 v = a.part[at + t];
-      join(m, s, v.x, v.y, kLog2e);
-      if (a.part_z != nullptr) sz += a.part_z[at + t];
+    for (int t = lane; t < a.parts; t += 512) {  // eight loads on their way at a time
+      float2 v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = t + e * 64 < a.parts ? a.part[at + t + e * 64] : make_float2(kNegInf, 0.f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) join(m, s, v[e].x, v[e].y, kLog2e);
+      if (a.part_z != nullptr)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sz += t + e * 64 < a.parts ? a.part_z[at + t + e * 64] : 0.f;
     }
     join_lanes(m, s, 64, kLog2e);
     if (a.part_z != nullptr) sz = sum_lanes(sz);
