@@ -39,6 +39,7 @@
 
 #include <atomic>
 #include <cstdint>
+#include <type_traits>
 
 namespace {
 
@@ -747,40 +748,50 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Place& at, un
   }
   phase_barrier();
   if (wr == 1) phase_barrier();
-  for (int t = 0; t < nk; ++t) {
-    read_a(t, 0);
-    read_b(t, 0);
-    if (t + 1 < nk) {
-      group(2, t + 1);
-      wait_vmcnt<kAfterA>();
-    } else {
-      wait_vmcnt<0>();
+  // A tile's last rows: 64-row quadrants behind them take no reads and no products (a row of 4096 against 128000
+  // words 235 to 180 us; the conditions cost full tiles 2 to 7 %, so these have a loop without).
+  auto stages = [&](auto all) {
+    const int left = M - m0 - wr * 128;
+    const bool upper = all || left > 0, lower = all || left > 64;
+    for (int t = 0; t < nk; ++t) {
+      if (upper) {
+        read_a(t, 0);
+        read_b(t, 0);
+      }
+      if (t + 1 < nk) {
+        group(2, t + 1);
+        wait_vmcnt<kAfterA>();
+      } else {
+        wait_vmcnt<0>();
+      }
+      phase_barrier();
+      wait_lgkm0();
+      if (upper) mfma(0, 0);
+      phase_barrier();
+      if (lower) read_a(t, 4);
+      if (upper) read_b(t, JH);
+      if (t + 1 < nk) group(3, t + 1);
+      phase_barrier();
+      wait_lgkm0();
+      if (upper) mfma(0, JH);
+      phase_barrier();
+      if (t + 2 < nk) group(0, t + 2);
+      phase_barrier();
+      if (lower) mfma(4, JH);
+      phase_barrier();
+      if (t + 2 < nk) {
+        group(1, t + 2);
+        wait_vmcnt<kAfterB>();
+      } else {
+        wait_vmcnt<kRest>();
+      }
+      phase_barrier();
+      if (lower) mfma(4, 0);
+      phase_barrier();
     }
-    phase_barrier();
-    wait_lgkm0();
-    mfma(0, 0);
-    phase_barrier();
-    read_a(t, 4);
-    read_b(t, JH);
-    if (t + 1 < nk) group(3, t + 1);
-    phase_barrier();
-    wait_lgkm0();
-    mfma(0, JH);
-    phase_barrier();
-    if (t + 2 < nk) group(0, t + 2);
-    phase_barrier();
-    mfma(4, JH);
-    phase_barrier();
-    if (t + 2 < nk) {
-      group(1, t + 2);
-      wait_vmcnt<kAfterB>();
-    } else {
-      wait_vmcnt<kRest>();
-    }
-    phase_barrier();
-    mfma(4, 0);
-    phase_barrier();
-  }
+  };
+  if (M - m0 > 192) stages(std::true_type{});
+  else stages(std::false_type{});
   if (wr == 0) phase_barrier();
   __syncthreads();
 
@@ -798,6 +809,7 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Place& at, un
       float* red = reinterpret_cast<float*>(smem);  // [3][4 column waves][256 rows]
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
+        if (m0 + wr * 128 + i * 16 >= M) break;  // nothing of the 16 rows' is read
         float m = kNegInf, s = 0.f, sz = 0.f;
 #pragma unroll
         for (int j = 0; j < FN; ++j)
