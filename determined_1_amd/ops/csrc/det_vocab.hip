@@ -366,6 +366,7 @@ struct GemmArgs {
   const int* k_dyn;  // length of the sum (null: K)
   int twice;         // rows of G are two: kGrad writes both, kPartial and kOut read twice as many as m_dyn or k_dyn says
   int M, N, K;
+  int least;                // kPartial: the shortest piece
   int chunk;                // kPartial of words: the longest K of the pass, which the splits are made for
   int cut;                  // whether the last round's tiles may be cut in two
   const int* info;          // scales of fp32 operands
@@ -405,11 +406,13 @@ struct GemmArgs {
   Alpha alpha;
 };
 
-// Few tiles: their sum (over a chunk's words for G w, over the kept rows for G^T h) is cut until a block
-// runs on every CU (one fills a CU), no piece under 512 long.  The length of a piece, a multiple of 64.
-__host__ __device__ inline int split_length(int tiles, int span) {
+// Few tiles: their sum (over a chunk's words for G w, over the kept rows for G^T h, over D for logits) is cut
+// until a block runs on every CU (one fills a CU), no piece under `least` long.  The length of a piece, a
+// multiple of 64.
+constexpr int kPiece = 512, kLogitPiece = 256;
+__host__ __device__ inline int split_length(int tiles, int span, int least) {
   int splits = tiles < 256 ? 256 / tiles : 1;
-  const int most = span / 512 > 1 ? span / 512 : 1;
+  const int most = span / least > 1 ? span / least : 1;
   if (splits > most) splits = most;
   return ((span + splits - 1) / splits + 63) / 64 * 64;
 }
@@ -541,7 +544,7 @@ __device__ __forceinline__ int gemm_blocks(const GemmArgs& g, int epi) {
   if (epi == kPartial && tiles < 256) {
     const int span = g.k_dyn != nullptr ? sum_of(g) : g.chunk;
     if (tiles == 0 || span == 0) return 0;
-    const int len = split_length(tiles, span);
+    const int len = split_length(tiles, span, g.least);
     return tiles * ((span + len - 1) / len);
   }
   const int last = tiles & 255;
@@ -558,7 +561,7 @@ __device__ __forceinline__ Place gemm_place(const GemmArgs& g, int epi, int bid,
   at.half = at.lone = false;
   int tile, side = 0;
   if (epi == kPartial && tiles < 256) {
-    const int len = split_length(tiles, g.k_dyn != nullptr ? K : g.chunk);
+    const int len = split_length(tiles, g.k_dyn != nullptr ? K : g.chunk, g.least);
     tile = xcd_remap(bid, blocks);
     at.split = tile / tiles;  // the tiles of one piece, which share its words, stay together
     tile -= at.split * tiles;
@@ -1076,6 +1079,62 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(GemmArgs g) {
 }
 
 
+// The statistics of few tiles of logits, whose sums over D came in pieces (kPartial, of g.chunk): what kStats'
+// epilogue does, a wave for 256 words of a row.  Bound by reading the pieces (482 x 2738, ten of them: 53 MB from
+// the caches in 11 us).
+__global__ void __launch_bounds__(256) pieces_kernel(GemmArgs g, int planes) {
+  const int M = *g.m_dyn, ntn = (g.N + kTile - 1) / kTile, lane = threadIdx.x & 63;
+  if (M == 0) return;
+  const int len = split_length((M + kTile - 1) / kTile * ntn, g.chunk, g.least), splits = (g.chunk + len - 1) / len;
+  const float zs = planes == 1 ? 1.f : pow2(-scale_exp(static_cast<uint32_t>(g.info[1]))) * pow2(-scale_exp(static_cast<uint32_t>(g.info[2])));
+  const int64_t units = static_cast<int64_t>(M) * ntn, stride = M * g.ldo;
+  for (int64_t unit = blockIdx.x * 4ll + (threadIdx.x >> 6); unit < units; unit += gridDim.x * 4ll) {
+    const int row = static_cast<int>(unit / ntn), tile = static_cast<int>(unit - static_cast<int64_t>(row) * ntn);
+    const int col = tile * kTile + lane * 4;
+    const float* p = g.out32 + row * g.ldo + col;
+    f32x4 z = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s) z += *reinterpret_cast<const f32x4*>(p + s * stride);
+    float m = kNegInf, sum = 0.f, sz = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const bool there = col + e < g.N;
+      z[e] = there ? z[e] * zs + (g.bias != nullptr ? load_any(g.bias, col + e, g.bias_dt) : 0.f) : kNegInf;
+      if (there) sz += z[e] * g.inv_v;
+      m = fmaxf(m, z[e]);
+    }
+    m = max_lanes(m);
+    const float ref = m == kNegInf ? 0.f : m;
+    const int word = g.words != nullptr ? g.words[row] - col : -1;
+    f32x4 x;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (word == e) g.picked[row] = z[e];
+      x[e] = exp2_((z[e] - ref) * g.c);
+      sum += x[e];
+    }
+    sum = sum_lanes(sum);
+    if (g.part_z != nullptr) sz = sum_lanes(sz);
+    if (lane < 2) {
+      const int64_t to = static_cast<int64_t>(row) * g.parts + tile * 2 + lane;
+      g.part[to] = lane == 0 ? make_float2(m, sum) : make_float2(kNegInf, 0.f);
+      if (g.part_z != nullptr) g.part_z[to] = lane == 0 ? sz : 0.f;
+      if (g.E != nullptr) g.tops[static_cast<int64_t>(row) * (g.held / 128) + tile * 2 + lane] = m;
+    }
+    if (g.E == nullptr) continue;
+    const int64_t at = static_cast<int64_t>(row) * g.held + col;
+    if (planes == 2) {
+      *reinterpret_cast<f32x4*>(static_cast<float*>(g.E) + at) = x;
+    } else {
+      typedef __attribute__((ext_vector_type(4))) u16 us4;
+      us4 v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = hold_bits(x[e]);
+      *reinterpret_cast<us4*>(static_cast<u16*>(g.E) + at) = v;
+    }
+  }
+}
+
 // ------------------------------------------------------------------------------------------------
 // Joining a row's tiles, its K picked logits, its loss.  One wave a row (cross entropy) or four (lists).
 // ------------------------------------------------------------------------------------------------
@@ -1456,7 +1515,7 @@ __global__ void __launch_bounds__(256) sum_kernel(const float* part, int span, i
   int splits = 0;
   if (pos == nullptr) span = info[0];
   if (at >= 0 && span > 0) {
-    const int len = split_length(tiles, span);
+    const int len = split_length(tiles, span, kPiece);
     splits = (span + len - 1) / len;
   }
   float a = alpha();
@@ -1814,9 +1873,9 @@ namespace {
 // What both directions lay out in the workspace.
 struct Plan {
   int planes, ldh, chunk, nchunks, parts, csplits, held, twice;
-  bool pack_w, keep_w, split_w;
+  bool pack_w, keep_w, split_w, split_z;
   int64_t off_rows_info, off_h, off_e, off_tops, off_kw, kept;  // in `kept`
-  int64_t off_w, off_flag, off_part, off_partz, off_rows, off_roww, off_alpha, off_g, off_dx, off_dw, off_cs, total;
+  int64_t off_w, off_z, off_flag, off_part, off_partz, off_rows, off_roww, off_alpha, off_g, off_dx, off_dw, off_cs, total;
 };
 
 constexpr int64_t kChunkBytes = int64_t(512) << 20;  // G of one chunk, and the packed weights of one
@@ -1868,26 +1927,32 @@ Plan plan(const DetVocabHead& p, bool backward) {
     at += up(bytes, 256);
     return o;
   };
+  // partial sums of rows x width: one for every piece of a sum of `span`, or at most 256 tiles' worth
+  auto partials = [](int64_t rows, int64_t width, int64_t span, int least) {
+    int64_t n = (span / least > 1 ? span / least : 1) * rows * width;
+    if (n > int64_t(256) * kTile * kTile) n = int64_t(256) * kTile * kTile;
+    return 4 * (n < rows * width ? rows * width : n);
+  };
   q.off_w = q.pack_w && !q.keep_w ? take(int64_t(2) * q.planes * q.chunk * q.ldh) : 0;
   if (!backward) {
     q.off_flag = take(p.N);
     q.off_part = take(int64_t(8) * p.N * q.parts);
+    // few tiles of a wide model, whose stages would follow each other on few CUs: 482 x 2752 x 2738 fp32 93 us, in
+    // pieces 35 and 11 to join them; one row of 4096 against 32000 words 56, and 38 and 5; but a forward pass of
+    // 300 x 768 x 8000 36 and in pieces 50, of 500 x 2048 x 14000 fp32 160 and 173: there their traffic costs more
+    const int64_t tiles = int64_t(ceil_div(p.N, kTile)) * ceil_div(p.V, kTile);
+    q.split_z = q.nchunks == 1 && p.D >= 1024 && (tiles <= 64 || (tiles <= 128 && p.N <= 64));
+    q.off_z = q.split_z ? take(partials(p.N, up(p.V, kTile), q.ldh, kLogitPiece)) : 0;
     q.off_partz = p.smooth != 0.f ? take(int64_t(4) * p.N * q.parts) : 0;
     q.off_rows = take(int64_t(8) * p.N);
   } else {
     q.off_roww = take(int64_t(4) * p.N);
     q.off_alpha = take(4);
     q.off_g = take((int64_t(2) * q.planes * p.N * q.chunk) << q.twice);
-    // partials: a row's for every piece, or at most 256 tiles' worth
-    auto partials = [&](int64_t rows, int64_t span) {
-      int64_t n = (span / 512 > 1 ? span / 512 : 1) * rows * q.ldh;
-      if (n > int64_t(256) * kTile * kTile) n = int64_t(256) * kTile * kTile;
-      return 4 * (n < rows * q.ldh ? rows * q.ldh : n);
-    };
-    q.off_dx = p.dx != nullptr ? take(partials(int64_t(p.N) << q.twice, q.chunk)) : 0;
+    q.off_dx = p.dx != nullptr ? take(partials(int64_t(p.N) << q.twice, q.ldh, q.chunk, kPiece)) : 0;
     // few tiles under many rows (8192 x 64 x 1000 bf16: 155 us for four blocks, 20 us in pieces)
     q.split_w = int64_t(ceil_div(q.chunk, kTile)) * ceil_div(p.D, kTile) <= 128 && p.N >= 1024;
-    q.off_dw = p.dw != nullptr && q.split_w ? take(partials(q.chunk, p.N)) : 0;
+    q.off_dw = p.dw != nullptr && q.split_w ? take(partials(q.chunk, q.ldh, p.N, kPiece)) : 0;
     // column sums: from the product's tiles for one target a row, from G for lists (which change it)
     q.csplits = p.index == nullptr ? ceil_div(p.N, kTile) : p.N > 2048 ? 32 : ceil_div(p.N, 64);
     q.off_cs = p.db != nullptr ? take(int64_t(4) * q.csplits * q.chunk) : 0;
@@ -2044,7 +2109,18 @@ int det_vocab_head_forward(void* stream, const DetVocabHead* pp) {
     a.E = q.held > 0 ? p.e : nullptr;
     a.tops = p.tops;
     a.held = q.held;
-    DET_TRY((gemm<false, false, kStats>(st, p.dtype, a)));
+    if (q.split_z) {
+      a.twice = 0;
+      a.chunk = a.K;
+      a.least = kLogitPiece;
+      a.out32 = reinterpret_cast<float*>(ws + q.off_z);
+      a.ldo = up(p.V, kTile);
+      DET_TRY((gemm<false, false, kPartial>(st, p.dtype, a)));
+      const int64_t pb = (int64_t(p.N) * ceil_div(p.V, kTile) + 3) / 4;
+      hipLaunchKernelGGL(pieces_kernel, dim3(pb < 8192 ? static_cast<unsigned>(pb) : 8192u), dim3(256), 0, st, a, q.planes);
+    } else {
+      DET_TRY((gemm<false, false, kStats>(st, p.dtype, a)));
+    }
   }
   FinishArgs f = {};
   f.x = p.x;
@@ -2161,6 +2237,7 @@ int det_vocab_head_backward(void* stream, const DetVocabHead* pp) {
       d.m_dyn = p.rows;
       d.info = p.rows;
       d.twice = q.twice;
+      d.least = kPiece;
       d.M = p.N << q.twice;
       d.N = p.D;
       d.K = nv;
@@ -2178,6 +2255,7 @@ int det_vocab_head_backward(void* stream, const DetVocabHead* pp) {
       d.k_dyn = p.rows;
       d.info = p.rows;
       d.twice = q.twice;
+      d.least = kPiece;
       d.M = nv;
       d.N = p.D;
       d.K = p.N << q.twice;

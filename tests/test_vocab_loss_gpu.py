@@ -597,6 +597,30 @@ def _check_words(x, w, t):
     assert (dw[t].double() - refw).abs().max().item() <= 2.0 ** -7 * refw.abs().max().item()
 
 
+@pytest.mark.parametrize("hold_bytes", [0, vocab_loss.HOLD_BYTES])
+@pytest.mark.parametrize("n,d,v", [(1, 1024, 1), (1, 2350, 7148), (2, 1600, 385), (70, 1500, 4001), (300, 2047, 2000), (513, 1024, 3700), (33, 1032, 25000)])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32])
+def test_few_tiles_of_a_wide_model(gpu, n, d, v, dt, hold_bytes):
+    """Logits whose sums come in pieces: targets that are ignored and masked words, smoothing, a list."""
+    x, w, b, g = _tensors(gpu, n, d, v, dt)
+    t = torch.randint(0, v, (n,), generator=g, device=gpu)
+    t[2::3] = -100
+    _check_head(x, w, b, target=t, smooth=0.1, reduction="sum", hold_bytes=hold_bytes)
+    if v > 300:
+        low = b.float()
+        low[256:290] = torch.finfo(torch.float32).min
+        loss, _, _ = _run_head(x, w, low, target=torch.full((n,), 255, device=gpu), reduction="none", hold_bytes=hold_bytes)
+        z = (x.double() @ w.double().t() + b.double())
+        z[:, 256:290] = -math.inf
+        ref = torch.logsumexp(z, 1) - z[:, 255]
+        # a logit's error, of d products and for fp32 of the planes, twice, and the sum's
+        size = (x.double().abs() @ w.double().abs().t() + b.double().abs()).amax(1)
+        bound = 2 * (d * 2.0 ** -24 + 2.0 ** -21) * size + 3 * 2.0 ** -23 * size + _sum_error(v)
+        _near(loss, ref, bound + 2.0 ** -22 * ref.abs(), "masked loss")
+    teacher, index = _lists(gpu, g, n, v, min(v, 5))
+    _check_head(x, w, b, teacher=teacher, index=index, heat=2.0, hold_bytes=hold_bytes)
+
+
 @pytest.mark.parametrize("reduction", ["mean", "none"])
 @pytest.mark.parametrize("kind", ["target", "list"])
 @pytest.mark.parametrize("n,d,v", [(1, 8, 7), (300, 129, 1111), (513, 64, 641)])
