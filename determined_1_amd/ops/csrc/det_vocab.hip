@@ -18,7 +18,7 @@
 // that from the product once more, in its epilogue.  What bounds it, 8192 x 4096 x 128000 bf16 in 22.1 ms: the
 // matrix units, 1.23 PFLOP/s over the three products (logits 6.8 ms, G w 6.9, G^T h 7.4; G from 2 GB of
 // exponentials 0.8, where the product again takes 6.7); for few rows the reads of w (one row against
-// 128000 x 4096: 5.3 TB/s).
+// 128000 x 4096: 6.0 TB/s).
 //
 // Rows without a target are dropped before the products (an ordered list of the kept ones, made on the
 // device; tiles past its end return), so a masked-language-model step with 15 % targets costs 15 %.
@@ -751,8 +751,9 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Place& at, un
   }
   phase_barrier();
   if (wr == 1) phase_barrier();
-  // A tile's last rows: 64-row quadrants behind them take no reads and no products (a row of 4096 against 128000
-  // words 235 to 180 us; the conditions cost full tiles 2 to 7 %, so these have a loop without).
+  // Up to 128 rows left: 64-row quadrants behind the last one take no reads and no products (a row of 4096 against
+  // 128000 words 235 to 180 us).  The conditions cost full tiles 2 to 7 % and a tile of 192 rows 2 %, so these have
+  // a loop without.
   auto stages = [&](auto all) {
     const int left = M - m0 - wr * 128;
     const bool upper = all || left > 0, lower = all || left > 64;
@@ -793,7 +794,7 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Place& at, un
       phase_barrier();
     }
   };
-  if (M - m0 > 192) stages(std::true_type{});
+  if (M - m0 > 128) stages(std::true_type{});
   else stages(std::false_type{});
   if (wr == 0) phase_barrier();
   __syncthreads();
