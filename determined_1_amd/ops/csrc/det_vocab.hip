@@ -228,12 +228,13 @@ __global__ void __launch_bounds__(1024) rows_kernel(RowArgs a) {
 }
 
 // The largest finite magnitudes of the hidden states and the weights (fp32), as bits: blocks below
-// x_blocks go over x.  One atomic a block (eight thousand, one a wave, took 65 us of a 75 us launch); a
-// maximum does not depend on their order.
+// x_blocks go over x, its kept rows alone: what an ignored one holds must not decide their scale.  One atomic a
+// block (eight thousand, one a wave, took 65 us of a 75 us launch); a maximum does not depend on their order.
 struct Matrix {
   const float* p;
   int64_t ld;
   int rows, cols;
+  const int *list, *count;  // the rows that count, and how many (null: all)
 };
 
 __global__ void __launch_bounds__(256) absmax_kernel(Matrix x, Matrix w, int x_blocks, int* info) {
@@ -247,7 +248,7 @@ __global__ void __launch_bounds__(256) absmax_kernel(Matrix x, Matrix w, int x_b
     if (b < 0x7F800000u && b > m) m = b;
   };
   const int64_t all = static_cast<int64_t>(a.rows) * a.cols;
-  if (a.ld == a.cols && (reinterpret_cast<uintptr_t>(a.p) & 15) == 0) {
+  if (a.list == nullptr && a.ld == a.cols && (reinterpret_cast<uintptr_t>(a.p) & 15) == 0) {
 #pragma unroll 4
     for (int64_t i = block * 256 + threadIdx.x; i < all / 4; i += blocks * 256) {
       const f32x4 v = reinterpret_cast<const f32x4*>(a.p)[i];
@@ -256,8 +257,12 @@ __global__ void __launch_bounds__(256) absmax_kernel(Matrix x, Matrix w, int x_b
     }
     if (block == 0 && threadIdx.x < (all & 3)) take(a.p[all - 1 - threadIdx.x]);
   } else {
-    for (int64_t r = block * 4 + (threadIdx.x >> 6); r < a.rows; r += blocks * 4)
-      for (int c = threadIdx.x & 63; c < a.cols; c += 64) take(a.p[r * a.ld + c]);
+    const int rows = a.list != nullptr ? *a.count : a.rows;
+    for (int64_t r = block * 4 + (threadIdx.x >> 6); r < rows; r += blocks * 4) {
+      const float* p = a.p + (a.list != nullptr ? a.list[r] : r) * a.ld;
+#pragma unroll 4
+      for (int c = threadIdx.x & 63; c < a.cols; c += 64) take(p[c]);
+    }
   }
   for (int o = 1; o < 64; o <<= 1) {
     const uint32_t v = __shfl_xor(m, o, 64);
@@ -2094,8 +2099,8 @@ int det_vocab_head_forward(void* stream, const DetVocabHead* pp) {
   hipLaunchKernelGGL(rows_kernel, dim3(1), dim3(1024), 0, st, r);
   if (p.dtype == kF32) {
     const int xb = p.N < 512 ? ceil_div(p.N, 4) : 128, wb = p.V < 2048 ? ceil_div(p.V, 4) : 512;
-    hipLaunchKernelGGL(absmax_kernel, dim3(xb + wb), dim3(256), 0, st, Matrix{static_cast<const float*>(p.x), p.x_ld, p.N, p.D},
-                       Matrix{static_cast<const float*>(p.w), p.w_ld, p.V, p.D}, xb, p.rows);
+    hipLaunchKernelGGL(absmax_kernel, dim3(xb + wb), dim3(256), 0, st, Matrix{static_cast<const float*>(p.x), p.x_ld, p.N, p.D, list, p.rows},
+                       Matrix{static_cast<const float*>(p.w), p.w_ld, p.V, p.D, nullptr, nullptr}, xb, p.rows);
   }
   DET_TRY(static_cast<int>(hipGetLastError()));
   DET_TRY(pack_hidden(st, p, q));
