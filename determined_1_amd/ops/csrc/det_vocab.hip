@@ -121,13 +121,10 @@ __device__ __forceinline__ float max_lanes(float v) {
   return v;
 }
 
-// the power of two that brings a tensor's largest finite magnitude (its bits) to [2^14, 2^15), and its inverse
-__device__ __forceinline__ int scale_exp(uint32_t bits) {
-  if (bits == 0) return 0;
-  int e = 14 - (static_cast<int>(bits >> 23) - 127);
-  return e > 60 ? 60 : e < -100 ? -100 : e;
-}
-__device__ __forceinline__ float pow2(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
+// the exponent of the power of two that brings a tensor's largest finite magnitude (its bits) to [2^14, 2^15): from
+// -113 to 141, so that the power itself may be out of range and is applied by ldexp
+__device__ __forceinline__ int scale_exp(uint32_t bits) { return bits == 0 ? 0 : 141 - static_cast<int>(bits >> 23); }
+__device__ __forceinline__ float times_pow2(float v, int e) { return __builtin_ldexpf(v, e); }
 
 __device__ __forceinline__ int64_t load_index(const void* p, int64_t i, int wide) {
   return wide ? static_cast<const int64_t*>(p)[i] : static_cast<const int32_t*>(p)[i];
@@ -310,7 +307,7 @@ __global__ void __launch_bounds__(256) pack_kernel(PackArgs a) {
   typedef typename Elem<DT>::type T;
   const int rows = a.count != nullptr ? *a.count : a.rows;
   const int chunks = a.ld >> 3;
-  const float s = DT == kF32 ? pow2(scale_exp(static_cast<uint32_t>(*a.absmax))) : 1.f;
+  const int scale = DT == kF32 ? scale_exp(static_cast<uint32_t>(*a.absmax)) : 0;
   // a thread per eight columns, whatever the width
   const int64_t all = static_cast<int64_t>(rows) * chunks, step = gridDim.x * 256ll;
   for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < all; i += step) {
@@ -322,7 +319,7 @@ __global__ void __launch_bounds__(256) pack_kernel(PackArgs a) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       if constexpr (DT == kF32) {
-        const float x = v[e] * s;
+        const float x = times_pow2(v[e], scale);
         hi[e] = f2h(x);
         lo[e] = f2h(x - h2f(hi[e]));
       } else {
@@ -809,7 +806,8 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Place& at, un
   // wc * 16 FN + j * 16 + fch * 4 + r.  A row's reduction is 4 FN values in registers and two lane steps.
   const int row0 = wr * 128 + fr, col0 = wc * (FN * 16) + fch * 4;
   if constexpr (EPI == kStats || EPI == kGrad) {
-    const float zs = PL == 1 ? 1.f : pow2(-scale_exp(static_cast<uint32_t>(g.info[1]))) * pow2(-scale_exp(static_cast<uint32_t>(g.info[2])));
+    const int unscale = PL == 1 ? 0 : -scale_exp(static_cast<uint32_t>(g.info[1])) - scale_exp(static_cast<uint32_t>(g.info[2]));
+    auto logit = [&](float sum, float b) { return (PL == 1 ? sum : times_pow2(sum, unscale)) + b; };
     const float c = g.c;
     f32x4 bias[4];
 #pragma unroll
@@ -824,7 +822,7 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Place& at, un
         for (int j = 0; j < FN; ++j)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            acc[i][j][r] = acc[i][j][r] * zs + bias[j][r];
+            acc[i][j][r] = logit(acc[i][j][r], bias[j][r]);
             m = fmaxf(m, acc[i][j][r]);
           }
         if (g.words != nullptr) {
@@ -950,7 +948,7 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Place& at, un
         for (int j = 0; j < FN; ++j)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float p = exp2_(fmaf(acc[i][j][r] * zs + bias[j][r] - top, c, -l));
+            const float p = exp2_(fmaf(logit(acc[i][j][r], bias[j][r]) - top, c, -l));
             acc[i][j][r] = ok ? w * (p - g.smooth_v) : 0.f;
           }
         if (g.words != nullptr) {
@@ -1022,12 +1020,14 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Place& at, un
       }
     }
   } else {
-    float alpha = g.alpha();
-    if (PL == 2) alpha *= pow2(-scale_exp(static_cast<uint32_t>(g.info[1])));
+    const float alpha = g.alpha();
+    const int unscale = PL == 1 ? 0 : -scale_exp(static_cast<uint32_t>(g.info[1]));
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
-      for (int j = 0; j < FN; ++j) acc[i][j] *= alpha;
+      for (int j = 0; j < FN; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[i][j][r] = PL == 1 ? acc[i][j][r] * alpha : times_pow2(acc[i][j][r] * alpha, unscale);
     if constexpr (PL == 1) {
       tile_to_lds<F16, 1>(acc, smem, row0, col0);
       __syncthreads();
@@ -1092,7 +1092,7 @@ __global__ void __launch_bounds__(256) pieces_kernel(GemmArgs g, int planes) {
   const int M = *g.m_dyn, ntn = (g.N + kTile - 1) / kTile, lane = threadIdx.x & 63;
   if (M == 0) return;
   const int len = split_length((M + kTile - 1) / kTile * ntn, g.chunk, g.least), splits = (g.chunk + len - 1) / len;
-  const float zs = planes == 1 ? 1.f : pow2(-scale_exp(static_cast<uint32_t>(g.info[1]))) * pow2(-scale_exp(static_cast<uint32_t>(g.info[2])));
+  const int unscale = planes == 1 ? 0 : -scale_exp(static_cast<uint32_t>(g.info[1])) - scale_exp(static_cast<uint32_t>(g.info[2]));
   const int64_t units = static_cast<int64_t>(M) * ntn, stride = M * g.ldo;
   for (int64_t unit = blockIdx.x * 4ll + (threadIdx.x >> 6); unit < units; unit += gridDim.x * 4ll) {
     const int row = static_cast<int>(unit / ntn), tile = static_cast<int>(unit - static_cast<int64_t>(row) * ntn);
@@ -1105,7 +1105,7 @@ __global__ void __launch_bounds__(256) pieces_kernel(GemmArgs g, int planes) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const bool there = col + e < g.N;
-      z[e] = there ? z[e] * zs + (g.bias != nullptr ? load_any(g.bias, col + e, g.bias_dt) : 0.f) : kNegInf;
+      z[e] = there ? times_pow2(z[e], unscale) + (g.bias != nullptr ? load_any(g.bias, col + e, g.bias_dt) : 0.f) : kNegInf;
       if (there) sz += z[e] * g.inv_v;
       m = fmaxf(m, z[e]);
     }
@@ -1524,8 +1524,8 @@ __global__ void __launch_bounds__(256) sum_kernel(const float* part, int span, i
     const int len = split_length(tiles, span, kPiece);
     splits = (span + len - 1) / len;
   }
-  float a = alpha();
-  if (planes == 2) a *= pow2(-scale_exp(static_cast<uint32_t>(info[pos != nullptr ? 2 : 1])));
+  const float a = alpha();
+  const int unscale = planes == 2 ? -scale_exp(static_cast<uint32_t>(info[pos != nullptr ? 2 : 1])) : 0;
   const int64_t stride = count * ldo, out = static_cast<int64_t>(n) * D;
   for (int d = (blockIdx.y * 256 + threadIdx.x) * 4; d < D; d += gridDim.y * 1024) {
     f32x4 t = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -1535,7 +1535,8 @@ __global__ void __launch_bounds__(256) sum_kernel(const float* part, int span, i
     if (twice)
 #pragma unroll 4
       for (int s = 0; s < splits; ++s) t += *reinterpret_cast<const f32x4*>(p + info[0] * ldo + s * stride);
-    t *= a;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) t[e] = times_pow2(t[e] * a, unscale);
     if (d + 4 <= D) {  // (wide stores need no alignment)
       if (dt == kF32) {
         __builtin_memcpy(static_cast<float*>(dx) + out + d, &t, 16);

@@ -41,3 +41,26 @@ def test_what_an_ignored_row_holds_does_not_matter(gpu, dt, kind, junk):
     loss, grads, _ = _run_head(x, w, b, **kw)
     assert torch.isfinite(ref) and ref.item() > 0
     _same((loss, *grads), (ref, *ref_grads))
+
+
+@pytest.mark.parametrize("hold_bytes", [0, vocab_loss.HOLD_BYTES])
+@pytest.mark.parametrize("d", [64, 1024])
+@pytest.mark.parametrize("power", [-118, -100, 40, 100, 118])
+def test_fp32_operands_of_any_magnitude(gpu, power, d, hold_bytes):
+    """x 2^k and W 2^-k: the same logits, and gradients of the same digits."""
+    g = torch.Generator(device=gpu).manual_seed(7)
+    n, v = 150, 600
+    x = torch.randint(-16, 17, (n, d), generator=g, device=gpu).float() / 16  # (no entry becomes a denormal)
+    w = torch.randint(-16, 17, (v, d), generator=g, device=gpu).float() / 16
+    b = torch.randn(v, generator=g, device=gpu)
+    t = torch.randint(0, v, (n,), generator=g, device=gpu)
+    t[::5] = -100
+    teacher, index = _lists(gpu, g, n, v, 4)
+    for kw in (dict(target=t, reduction="sum"), dict(teacher=teacher, index=index, heat=2.0, reduction="sum")):
+        ref, (dx0, dw0, db0), _ = _run_head(x, w, b, hold_bytes=hold_bytes, **kw)
+        s = 2.0 ** power
+        loss, (dx, dw, db), _ = _run_head(x * s, w / s, b, hold_bytes=hold_bytes, **kw)
+        _same((loss, db), (ref, db0))
+        # a gradient's own step is 2^-149 at least
+        assert (dx.double() * s - dx0.double()).abs().max().item() <= 2.0 ** -149 * s
+        assert (dw.double() / s - dw0.double()).abs().max().item() <= 2.0 ** -149 / s
