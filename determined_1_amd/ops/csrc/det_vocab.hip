@@ -351,7 +351,8 @@ struct Alpha {
   int mean;
   __device__ __forceinline__ float operator()() const {
     const int count = info[0];
-    return *p * scale / (mean && count > 0 ? static_cast<float>(count) : 1.f);
+    if (count == 0) return 0.f;  // no row's gradient, whatever the derivative is
+    return *p * scale / (mean ? static_cast<float>(count) : 1.f);
   }
 };
 
@@ -1524,7 +1525,7 @@ __global__ void __launch_bounds__(256) sum_kernel(const float* part, int span, i
     const int len = split_length(tiles, span, kPiece);
     splits = (span + len - 1) / len;
   }
-  const float a = alpha();
+  const float a = at >= 0 ? alpha() : 0.f;  // (a row that does not count: zeros, whatever the derivative is)
   const int unscale = planes == 2 ? -scale_exp(static_cast<uint32_t>(info[pos != nullptr ? 2 : 1])) : 0;
   const int64_t stride = count * ldo, out = static_cast<int64_t>(n) * D;
   for (int d = (blockIdx.y * 256 + threadIdx.x) * 4; d < D; d += gridDim.y * 1024) {

@@ -64,3 +64,20 @@ def test_fp32_operands_of_any_magnitude(gpu, power, d, hold_bytes):
         # a gradient's own step is 2^-149 at least
         assert (dx.double() * s - dx0.double()).abs().max().item() <= 2.0 ** -149 * s
         assert (dw.double() / s - dw0.double()).abs().max().item() <= 2.0 ** -149 / s
+
+
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("dt", TYPES)
+def test_an_ignored_row_has_no_gradient_whatever_comes_in(gpu, dt, reduction, bad):
+    x, w, b, g = _tensors(gpu, 300, 64, 700, dt)
+    t = torch.randint(0, 700, (300,), generator=g, device=gpu)
+    t[::3] = -100
+    gout = torch.full((300,) if reduction == "none" else (), bad, device=gpu)
+    _, (dx, _, _), _ = _run_head(x, w, b, target=t, reduction=reduction, gout=gout)
+    assert not dx[::3].any() and not torch.isfinite(dx[1::3]).any()
+    _, grads, _ = _run_head(x, w, b, target=torch.full_like(t, -100), reduction=reduction, gout=gout)
+    assert not any(a.any() for a in grads)
+    teacher, index = _lists(gpu, g, 300, 700, 5)
+    _, grads, _ = _run_head(x, w, b, teacher=teacher, index=index * 0 - 1, reduction=reduction, gout=gout)
+    assert not any(a.any() for a in grads)
