@@ -1335,8 +1335,9 @@ __global__ void __launch_bounds__(1024) reduce_kernel(const double* rows, const 
 }
 
 // ------------------------------------------------------------------------------------------------
-// Backward of losses by row: row_w[c] = g_n / max |g| times 2^kGExp for fp16 G, *top = max |g|.  (A mean
-// and a sum have one weight for all, and need none of this.)
+// Backward of losses by row: row_w[c] = g_n / max |g| times 2^kGExp for fp16 G, *top = max |g|, over the rows
+// whose g is finite: one that is not keeps its own, and spoils no other row.  (A mean and a sum have one weight for
+// all, and need none of this.)
 // ------------------------------------------------------------------------------------------------
 struct WeightArgs {
   const float* g;  // [N]
@@ -1345,23 +1346,25 @@ struct WeightArgs {
   float g_scale;
 };
 
+__device__ __forceinline__ bool finite(float v) { return (__float_as_uint(v) & 0x7F800000u) != 0x7F800000u; }
+
 __global__ void __launch_bounds__(1024) weights_kernel(WeightArgs a) {
   __shared__ float part[16];
   const int count = a.info[0];
   float top = 0.f;
-  bool nan = false;
   for (int c = threadIdx.x; c < count; c += 1024) {
     const float g = fabsf(a.g[a.list[c]]);
-    nan |= g != g;
-    top = fmaxf(top, g);
+    if (finite(g)) top = fmaxf(top, g);
   }
-  if (nan) top = __builtin_huge_valf();
   top = max_lanes(top);
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
   __syncthreads();
   top = part[0];
   for (int w = 1; w < 16; ++w) top = fmaxf(top, part[w]);
-  for (int c = threadIdx.x; c < count; c += 1024) a.row_w[c] = top == 0.f ? 0.f : a.g[a.list[c]] / top * a.g_scale;
+  for (int c = threadIdx.x; c < count; c += 1024) {
+    const float g = a.g[a.list[c]];
+    a.row_w[c] = !finite(g) ? g : top == 0.f ? 0.f : g / top * a.g_scale;
+  }
   if (threadIdx.x == 0) *a.top = top;
 }
 

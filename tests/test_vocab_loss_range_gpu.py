@@ -66,6 +66,36 @@ def test_fp32_operands_of_any_magnitude(gpu, power, d, hold_bytes):
         assert (dw.double() / s - dw0.double()).abs().max().item() <= 2.0 ** -149 / s
 
 
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("kind", ["target", "list"])
+@pytest.mark.parametrize("n", [40, 300])
+@pytest.mark.parametrize("dt", TYPES)
+def test_a_derivative_that_is_not_finite_spoils_its_row_alone(gpu, dt, n, kind, bad):
+    x, w, b, g = _tensors(gpu, n, 64, 700, dt)
+    t = torch.randint(0, 700, (n,), generator=g, device=gpu)
+    t[::4] = -100
+    teacher, index = _lists(gpu, g, n, 700, 5)
+    index[::4] = -1
+    kw = dict(target=t) if kind == "target" else dict(teacher=teacher, index=index, heat=2.0)
+    gout = torch.randn(n, generator=g, device=gpu)
+    gout[5] = 0.0
+    _, (ref, _, _), _ = _run_head(x, w, b, reduction="none", gout=gout, **kw)
+    gout[5] = bad
+    gout[8] = math.nan  # of an ignored row: nothing
+    _, (dx, dw, db), _ = _run_head(x, w, b, reduction="none", gout=gout, **kw)
+    others = torch.arange(n, device=gpu) != 5
+    _same((dx[others],), (ref[others],))
+    assert not torch.isfinite(dx[5]).any() and not torch.isfinite(dw).any() and not torch.isfinite(db).any()
+    gout[5] = 0.0
+    z = torch.randn(n, 700, generator=g, device=gpu).to(dt)
+    leaf = z.requires_grad_(True)
+    (ref,) = torch.autograd.grad(topk_distill(leaf, teacher, index, reduction="none"), leaf, gout)
+    gout[5] = bad
+    (dz,) = torch.autograd.grad(topk_distill(leaf, teacher, index, reduction="none"), leaf, gout)
+    _same((dz[others],), (ref[others],))
+    assert not torch.isfinite(dz[5]).any() and not dz[::4].any()
+
+
 @pytest.mark.parametrize("bad", [math.inf, math.nan])
 @pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
 @pytest.mark.parametrize("dt", TYPES)
