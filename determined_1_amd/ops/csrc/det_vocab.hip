@@ -1456,7 +1456,14 @@ struct ScatterArgs {
   u16* G;
   int64_t g_plane;
   int twice;
+  unsigned long long* listed;  // [nv] sums of shares times their rows' weights, in whole steps, or null
+  double steps;                // steps of a weight g_scale
 };
+
+__global__ void __launch_bounds__(256) clear_kernel(unsigned long long* p, int n) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i < n) p[i] = 0;
+}
 
 __global__ void __launch_bounds__(256) scatter_kernel(ScatterArgs a) {
   const int count = a.info[0];
@@ -1470,6 +1477,9 @@ __global__ void __launch_bounds__(256) scatter_kernel(ScatterArgs a) {
     for (int j = 0; j < a.K; ++j)
       if (load_index(a.index, i0 + j, a.wide) == word) s += share[j];
     const float w = a.row_w != nullptr ? a.row_w[row] : a.g_scale;
+    // integers, whose sum does not depend on their order (a row that is not finite shows in p's part)
+    if (a.listed != nullptr && finite(w * share[k]))
+      atomicAdd(a.listed + (word - a.v0), static_cast<unsigned long long>(__double2ll_rn(static_cast<double>(w) * share[k] * a.steps)));
     const float v = settled(w * (exp2_(fmaf(a.picked[i] - a.top[row], a.c, -a.log_s[row])) - s));
     u16* o = a.G + static_cast<int64_t>(row) * a.ldg + (word - a.v0);
     const u16 hi = a.f16 ? f2h(v) : f2bf(v);
@@ -1479,39 +1489,16 @@ __global__ void __launch_bounds__(256) scatter_kernel(ScatterArgs a) {
   }
 }
 
-// column sums of a chunk's G after the scatter (rows split over blockIdx.y)
-__global__ void __launch_bounds__(256) colsum_kernel(const u16* G, int64_t g_plane, int planes, int f16, int ldg, const int* info,
-                                                     int twice, float* part) {
-  __shared__ float red[8][256 + 8];
-  const int tid = threadIdx.x, cg = tid & 31, rg = tid >> 5;
-  const int col = blockIdx.x * 256 + cg * 8;
-  const int count = info[0] << twice;
-  float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (col < ldg)
-    for (int r = blockIdx.y * 8 + rg; r < count; r += gridDim.y * 8)
-      for (int pl = 0; pl < planes; ++pl) {
-        const us8 v = *reinterpret_cast<const us8*>(G + pl * g_plane + static_cast<int64_t>(r) * ldg + col);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) s[e] += f16 ? h2f(v[e]) : bf2f(v[e]);
-      }
-#pragma unroll
-  for (int e = 0; e < 8; ++e) red[rg][cg * 8 + e] = s[e];
-  __syncthreads();
-  float t = 0.f;
-#pragma unroll
-  for (int w = 0; w < 8; ++w) t += red[w][tid];
-  if (blockIdx.x * 256 + tid < ldg) part[static_cast<int64_t>(blockIdx.y) * ldg + blockIdx.x * 256 + tid] = t;
-}
-
-// the bias gradient from column sums (of `splits` parts, or with 0 one for every tile of kept rows)
-__global__ void __launch_bounds__(256) dbias_kernel(const float* part, int splits, int ldg, int nv, Alpha alpha, void* db, int64_t at,
-                                                    int dt) {
+// the bias gradient: column sums of G before its rounding, one for every tile of kept rows, less the shares of listed words
+__global__ void __launch_bounds__(256) dbias_kernel(const float* part, int ldg, int nv, const unsigned long long* listed, double steps,
+                                                    Alpha alpha, void* db, int64_t at, int dt) {
   const int v = blockIdx.x * 256 + threadIdx.x;
   if (v >= nv) return;
-  if (splits == 0) splits = (alpha.info[0] + kTile - 1) / kTile;
+  const int splits = (alpha.info[0] + kTile - 1) / kTile;
   float t = 0.f;
 #pragma unroll 8
   for (int s = 0; s < splits; ++s) t += part[static_cast<int64_t>(s) * ldg + v];
+  if (listed != nullptr) t = static_cast<float>(t - static_cast<double>(static_cast<long long>(listed[v])) / steps);
   store_any(db, at + v, dt, t * alpha());
 }
 
@@ -1883,10 +1870,10 @@ namespace {
 
 // What both directions lay out in the workspace.
 struct Plan {
-  int planes, ldh, chunk, nchunks, parts, csplits, held, twice;
+  int planes, ldh, chunk, nchunks, parts, held, twice;
   bool pack_w, keep_w, split_w, split_z;
   int64_t off_rows_info, off_h, off_e, off_tops, off_kw, kept;  // in `kept`
-  int64_t off_w, off_z, off_flag, off_part, off_partz, off_rows, off_roww, off_alpha, off_g, off_dx, off_dw, off_cs, total;
+  int64_t off_w, off_z, off_flag, off_part, off_partz, off_rows, off_roww, off_alpha, off_g, off_dx, off_dw, off_cs, off_listed, total;
 };
 
 constexpr int64_t kChunkBytes = int64_t(512) << 20;  // G of one chunk, and the packed weights of one
@@ -1964,9 +1951,8 @@ Plan plan(const DetVocabHead& p, bool backward) {
     // few tiles under many rows (8192 x 64 x 1000 bf16: 155 us for four blocks, 20 us in pieces)
     q.split_w = int64_t(ceil_div(q.chunk, kTile)) * ceil_div(p.D, kTile) <= 128 && p.N >= 1024;
     q.off_dw = p.dw != nullptr && q.split_w ? take(partials(q.chunk, q.ldh, p.N, kPiece)) : 0;
-    // column sums: from the product's tiles for one target a row, from G for lists (which change it)
-    q.csplits = p.index == nullptr ? ceil_div(p.N, kTile) : p.N > 2048 ? 32 : ceil_div(p.N, 64);
-    q.off_cs = p.db != nullptr ? take(int64_t(4) * q.csplits * q.chunk) : 0;
+    q.off_cs = p.db != nullptr ? take(int64_t(4) * ceil_div(p.N, kTile) * q.chunk) : 0;  // G's column sums
+    q.off_listed = p.db != nullptr && p.index != nullptr ? take(int64_t(8) * q.chunk) : 0;
   }
   q.total = at;
   return q;
@@ -2199,6 +2185,10 @@ int det_vocab_head_backward(void* stream, const DetVocabHead* pp) {
     DET_TRY(static_cast<int>(hipGetLastError()));
     alpha.p = top;
   }
+  // a word's listed shares add up to N times the largest weight at most: in steps of 2^-61 N of that, below 2^63
+  unsigned long long* listed = p.db != nullptr && p.index != nullptr ? reinterpret_cast<unsigned long long*>(ws + q.off_listed) : nullptr;
+  double steps = 2305843009213693952.0 / g_scale;  // 2^61
+  for (int64_t n = 1; n < p.N; n *= 2) steps /= 2;
   const int64_t es = p.dtype == kF32 ? 4 : 2;
   for (int c = 0; c < q.nchunks; ++c) {
     const int v0 = c * q.chunk, nv = p.V - v0 < q.chunk ? p.V - v0 : q.chunk;
@@ -2213,7 +2203,7 @@ int det_vocab_head_backward(void* stream, const DetVocabHead* pp) {
     a.row_w = row_w;
     a.g_scale = g_scale;
     a.smooth_v = p.smooth / static_cast<float>(p.V);
-    a.colsum = p.target != nullptr ? cs : nullptr;
+    a.colsum = cs;
     a.G = reinterpret_cast<u16*>(ws + q.off_g);
     a.g_plane = int64_t(p.N) * ldg;
     a.ldg = ldg;
@@ -2229,17 +2219,15 @@ int det_vocab_head_backward(void* stream, const DetVocabHead* pp) {
     }
     if (p.index != nullptr) {
       ScatterArgs s = {p.rows, list, p.index, p.index_ld, p.wide, p.K, v0, nv, f16, q.planes, ldg, picked,
-                       picked + int64_t(p.N) * p.K, a.top, a.log_s, row_w, g_scale, a.c, a.G, a.g_plane, q.twice};
+                       picked + int64_t(p.N) * p.K, a.top, a.log_s, row_w, g_scale, a.c, a.G, a.g_plane, q.twice, listed, steps};
+      if (listed != nullptr) hipLaunchKernelGGL(clear_kernel, dim3(ceil_div(nv, 256)), dim3(256), 0, st, listed, nv);
       const int64_t sb = (int64_t(p.N) * p.K + 255) / 256;
       hipLaunchKernelGGL(scatter_kernel, dim3(sb < 8192 ? static_cast<unsigned>(sb) : 8192u), dim3(256), 0, st, s);
-      if (cs != nullptr)
-        hipLaunchKernelGGL(colsum_kernel, dim3(ceil_div(ldg, 256), q.csplits), dim3(256), 0, st, a.G, a.g_plane, q.planes, f16, ldg,
-                           p.rows, q.twice, cs);
     }
     const Operand G = {a.G, a.g_plane, ldg};
     if (cs != nullptr)
-      hipLaunchKernelGGL(dbias_kernel, dim3(ceil_div(nv, 256)), dim3(256), 0, st, cs, p.target != nullptr ? 0 : q.csplits, ldg, nv, alpha,
-                         p.db, int64_t(v0), p.bias_dt);
+      hipLaunchKernelGGL(dbias_kernel, dim3(ceil_div(nv, 256)), dim3(256), 0, st, cs, ldg, nv, listed, steps, alpha, p.db, int64_t(v0),
+                         p.bias_dt);
     DET_TRY(static_cast<int>(hipGetLastError()));
     if (p.dx != nullptr) {
       GemmArgs d = {};

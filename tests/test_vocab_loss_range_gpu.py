@@ -111,3 +111,31 @@ def test_an_ignored_row_has_no_gradient_whatever_comes_in(gpu, dt, reduction, ba
     teacher, index = _lists(gpu, g, 300, 700, 5)
     _, grads, _ = _run_head(x, w, b, teacher=teacher, index=index * 0 - 1, reduction=reduction, gout=gout)
     assert not any(a.any() for a in grads)
+
+
+@pytest.mark.parametrize("hold_bytes", [0, vocab_loss.HOLD_BYTES])
+@pytest.mark.parametrize("reduction", ["sum", "none"])
+@pytest.mark.parametrize("n,v", [(40, 700), (300, 700), (2100, 300)])
+@pytest.mark.parametrize("dt", TYPES)
+def test_a_lists_bias_gradient_is_summed_in_fp32(gpu, dt, n, v, reduction, hold_bytes):
+    """An fp32 bias beside operands of any type: no rounding of G in its gradient, words in every list and words twice in one."""
+    x, w, b, g = _tensors(gpu, n, 64, v, dt)
+    b = b.float()
+    teacher, index = _lists(gpu, g, n, v, 7)
+    index[:, 0] = 3
+    index[1::2, 2] = index[1::2, 1]
+    index[::5] = -1
+    heat = 2.0
+    gout = torch.randn(n, generator=g, device=gpu) if reduction == "none" else torch.tensor(3.0, device=gpu)
+    _, (_, _, db), _ = _run_head(x, w, b, teacher=teacher, index=index, heat=heat, reduction=reduction, gout=gout, hold_bytes=hold_bytes)
+    z = x.double() @ w.double().t() + b.double()
+    size = x.double().abs() @ w.double().abs().t() + b.double().abs()
+    _, G, A, P = _definition(z, None, teacher, index, -100, 0.0, heat, reduction, gout)
+    product = 64 * 2.0 ** -24 + (2.0 ** -21 if dt == torch.float32 else 0.0)
+    E = (2 * product * size.amax(1) + 3 * 2.0 ** -24 * (z / heat).abs().amax(1) * 1.5) / heat + _sum_error(v) + _share_error(teacher, heat)
+    held = 0.0 if dt == torch.float32 or hold_bytes == 0 else 2.0 ** -12
+    # a share in whole steps of 2^-61 N: 2^-46 and less
+    err = A * E[:, None] + held * (P + 2.0 ** -19 * P.amax(1, keepdim=True)) + 2.0 ** -40 * gout.double().abs().max() * heat
+    _near(db, G.sum(0), 1.01 * err.sum(0) + (n + 4) * 2.0 ** -24 * A.sum(0), "dbias")
+    again = _run_head(x, w, b, teacher=teacher, index=index, heat=heat, reduction=reduction, gout=gout, hold_bytes=hold_bytes)[1][2]
+    assert torch.equal(again, db)
