@@ -277,7 +277,8 @@ __global__ void __launch_bounds__(256) absmax_kernel(Matrix x, Matrix w, int x_b
 // Operands of the products: 16-bit rows, 16-byte aligned, columns past the width zero.  Copies the
 // rows of `list` (or all), and splits fp32 into two fp16 planes.  Bound by memory: 128000 x 4096 fp32 in
 // 0.85 ms, 4.9 TB/s.  The hidden states always (their kept rows move together), weights only if they are
-// fp32, of a width or a row distance that 16 bytes do not divide, or misaligned.
+// fp32, of a width or a row distance that 16 bytes do not divide, or misaligned.  DT kBF16 copies any 16-bit type as
+// bits; kF16 is for rows times a power of two.
 // ------------------------------------------------------------------------------------------------
 struct PackArgs {
   const void* src;
@@ -289,6 +290,7 @@ struct PackArgs {
   int64_t plane;     // elements between the planes
   int rows, cols, ld;  // ld % 8 == 0
   int twice;         // the rows once more behind the last one
+  const int* row_e;  // rows times 2^row_e, or null
 };
 
 // eight elements from any address (16-byte loads need no alignment here), zeros past the row's end
@@ -312,6 +314,7 @@ __global__ void __launch_bounds__(256) pack_kernel(PackArgs a) {
   const int64_t all = static_cast<int64_t>(rows) * chunks, step = gridDim.x * 256ll;
   for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < all; i += step) {
     const int r = static_cast<int>(i / chunks), c = static_cast<int>(i - static_cast<int64_t>(r) * chunks) * 8;
+    const int more = a.row_e != nullptr ? a.row_e[r] : 0;
     const int64_t from = static_cast<int64_t>(a.list != nullptr ? a.list[r] : r) * a.src_ld;
     T v[8];
     load8(static_cast<const T*>(a.src) + from + c, a.cols - c, v);
@@ -319,9 +322,11 @@ __global__ void __launch_bounds__(256) pack_kernel(PackArgs a) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       if constexpr (DT == kF32) {
-        const float x = times_pow2(v[e], scale);
+        const float x = times_pow2(v[e], scale + more);
         hi[e] = f2h(x);
         lo[e] = f2h(x - h2f(hi[e]));
+      } else if constexpr (DT == kF16) {
+        hi[e] = f2h(times_pow2(h2f(v[e]), more));
       } else {
         hi[e] = v[e];
       }
@@ -388,6 +393,7 @@ struct GemmArgs {
   // kGrad: p = 2^(c (z - top) - log2 sum)
   const float *top, *log_s;  // [M]
   const float* row_w;        // [M] (null: g_scale for each)
+  const int* row_e;          // [M] row_w's rows are to be taken times 2^row_e (null: as they are)
   float g_scale;
   float smooth_v;      // eps / V
   float* colsum;       // [tiles of M][ldg] G's column sums, or null
@@ -964,11 +970,17 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Place& at, un
       }
       if (g.colsum != nullptr) {  // before G is rounded
         float* red = reinterpret_cast<float*>(smem);  // [2 row waves][256 columns]
+        float each[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int row = m0 + row0 + i * 16;
+          each[i] = g.row_e != nullptr && row < M ? times_pow2(1.f, g.row_e[row]) : 1.f;
+        }
 #pragma unroll
         for (int j = 0; j < FN; ++j) {
-          f32x4 t = acc[0][j];
+          f32x4 t = acc[0][j] * each[0];
 #pragma unroll
-          for (int i = 1; i < 8; ++i) t += acc[i][j];
+          for (int i = 1; i < 8; ++i) t += acc[i][j] * each[i];
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             t[r] += lane_ror<8>(t[r]);
@@ -1335,14 +1347,19 @@ __global__ void __launch_bounds__(1024) reduce_kernel(const double* rows, const 
 }
 
 // ------------------------------------------------------------------------------------------------
-// Backward of losses by row: row_w[c] = g_n / max |g| times 2^kGExp for fp16 G, *top = max |g|, over the rows
-// whose g is finite: one that is not keeps its own, and spoils no other row.  (A mean and a sum have one weight for
+// Backward of losses by row: row_w[c] 2^row_e[c] = g_n / max |g| times 2^kGExp for fp16 G, *top = max |g|, over the
+// rows whose g is finite: one that is not keeps its own, and spoils no other row.  (A mean and a sum have one weight for
 // all, and need none of this.)
+// G in fp16 has its smallest step at 2^-38.  A row whose weight is below 2^-8 of the largest would lose its bits
+// there, so its row_w is taken back to 2^-8..2^-7 and row_e says how far: G w is multiplied by it at the end, and for
+// G^T h it goes into h, whose rows are packed once more (to 2^-25 of the largest weight for fp16, 2^-39 of the
+// largest h for fp32: what a row of a far smaller weight gives to a sum over rows).  bf16 has fp32's range and needs none.
 // ------------------------------------------------------------------------------------------------
 struct WeightArgs {
   const float* g;  // [N]
   const int *info, *list;
   float *row_w, *top;
+  int* row_e;      // null: zeros
   float g_scale;
 };
 
@@ -1363,7 +1380,12 @@ __global__ void __launch_bounds__(1024) weights_kernel(WeightArgs a) {
   for (int w = 1; w < 16; ++w) top = fmaxf(top, part[w]);
   for (int c = threadIdx.x; c < count; c += 1024) {
     const float g = a.g[a.list[c]];
-    a.row_w[c] = !finite(g) ? g : top == 0.f ? 0.f : g / top * a.g_scale;
+    int e = 0;
+    if (a.row_e != nullptr) {
+      if (finite(g) && g != 0.f) e = __builtin_amdgcn_frexp_expf(g) - __builtin_amdgcn_frexp_expf(top) + 8;
+      a.row_e[c] = e = e < 0 ? e : 0;
+    }
+    a.row_w[c] = !finite(g) ? g : top == 0.f ? 0.f : times_pow2(g, -e) / top * a.g_scale;
   }
   if (threadIdx.x == 0) *a.top = top;
 }
@@ -1381,6 +1403,7 @@ struct HeldArgs {
   int held;       // (a multiple of 256)
   const int* info;
   const float *top, *log_s, *row_w;
+  const int* row_e;
   float g_scale, c, smooth_v, share;
   const int* words;  // one target a row (null for lists)
   int v0;
@@ -1420,11 +1443,12 @@ __global__ void __launch_bounds__(256) held_kernel(HeldArgs a) {
     const float tile = a.tops[static_cast<int64_t>(row) * (a.held / 128) + col / 128];
     const float f = exp2_(fmaf(tile - a.top[row], a.c, -a.log_s[row]));
     const int word = a.words != nullptr ? a.words[row] - a.v0 - col : -1;
+    const float each = a.row_e != nullptr ? times_pow2(1.f, a.row_e[row]) : 1.f;
     us8 hi, lo;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       g[k] = settled(w * (fmaf(g[k], f, -a.smooth_v) - (word == k ? a.share : 0.f)));
-      sums[k] += g[k];
+      sums[k] += g[k] * each;
       hi[k] = DT == kBF16 ? f2bf(g[k]) : f2h(g[k]);
       lo[k] = DT == kBF16 ? f2bf(g[k] - bf2f(hi[k])) : f2h(g[k] - h2f(hi[k]));
     }
@@ -1452,6 +1476,7 @@ struct ScatterArgs {
   int64_t index_ld;
   int wide, K, v0, nv, f16, planes, ldg;
   const float *picked, *share, *top, *log_s, *row_w;
+  const int* row_e;
   float g_scale, c;
   u16* G;
   int64_t g_plane;
@@ -1479,7 +1504,8 @@ __global__ void __launch_bounds__(256) scatter_kernel(ScatterArgs a) {
     const float w = a.row_w != nullptr ? a.row_w[row] : a.g_scale;
     // integers, whose sum does not depend on their order (a row that is not finite shows in p's part)
     if (a.listed != nullptr && finite(w * share[k]))
-      atomicAdd(a.listed + (word - a.v0), static_cast<unsigned long long>(__double2ll_rn(static_cast<double>(w) * share[k] * a.steps)));
+      atomicAdd(a.listed + (word - a.v0), static_cast<unsigned long long>(__double2ll_rn(
+                                              __builtin_ldexp(static_cast<double>(w) * share[k] * a.steps, a.row_e != nullptr ? a.row_e[row] : 0))));
     const float v = settled(w * (exp2_(fmaf(a.picked[i] - a.top[row], a.c, -a.log_s[row])) - s));
     u16* o = a.G + static_cast<int64_t>(row) * a.ldg + (word - a.v0);
     const u16 hi = a.f16 ? f2h(v) : f2bf(v);
@@ -1505,7 +1531,7 @@ __global__ void __launch_bounds__(256) dbias_kernel(const float* part, int ldg, 
 // The sum of a row's partials: of dh (pos: a row's place among the kept ones; zeros for the others), or of
 // dw (pos null; rows of words, pieces of the kept rows).  Bound by memory (4608 rows, 28 pieces of 691 kept:
 // 59 MB in 13 us)
-__global__ void __launch_bounds__(256) sum_kernel(const float* part, int span, int64_t ldo, const int* info, const int* pos, int twice,
+__global__ void __launch_bounds__(256) sum_kernel(const float* part, int span, int64_t ldo, const int* info, const int* pos, const int* row_e, int twice,
                                                   Alpha alpha, int planes, void* dx, int dt, int D) {
   const int n = blockIdx.x, at = pos != nullptr ? pos[n] : n, count = pos != nullptr ? info[0] << twice : gridDim.x;
   const int tiles = ((count + kTile - 1) / kTile) * ((D + kTile - 1) / kTile);
@@ -1516,7 +1542,8 @@ __global__ void __launch_bounds__(256) sum_kernel(const float* part, int span, i
     splits = (span + len - 1) / len;
   }
   const float a = at >= 0 ? alpha() : 0.f;  // (a row that does not count: zeros, whatever the derivative is)
-  const int unscale = planes == 2 ? -scale_exp(static_cast<uint32_t>(info[pos != nullptr ? 2 : 1])) : 0;
+  int unscale = planes == 2 ? -scale_exp(static_cast<uint32_t>(info[pos != nullptr ? 2 : 1])) : 0;
+  if (row_e != nullptr && at >= 0) unscale += row_e[at];
   const int64_t stride = count * ldo, out = static_cast<int64_t>(n) * D;
   for (int d = (blockIdx.y * 256 + threadIdx.x) * 4; d < D; d += gridDim.y * 1024) {
     f32x4 t = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -1871,9 +1898,9 @@ namespace {
 // What both directions lay out in the workspace.
 struct Plan {
   int planes, ldh, chunk, nchunks, parts, held, twice;
-  bool pack_w, keep_w, split_w, split_z;
-  int64_t off_rows_info, off_h, off_e, off_tops, off_kw, kept;  // in `kept`
-  int64_t off_w, off_z, off_flag, off_part, off_partz, off_rows, off_roww, off_alpha, off_g, off_dx, off_dw, off_cs, off_listed, total;
+  bool pack_w, keep_w, split_w, split_z, spread;
+  int64_t off_rows_info, off_hidden, off_e, off_tops, off_kw, kept;  // in `kept`
+  int64_t off_w, off_z, off_flag, off_part, off_partz, off_rows, off_roww, off_alpha, off_rowe, off_again, off_g, off_dx, off_dw, off_cs, off_listed, total;
 };
 
 constexpr int64_t kChunkBytes = int64_t(512) << 20;  // G of one chunk, and the packed weights of one
@@ -1888,13 +1915,14 @@ Plan plan(const DetVocabHead& p, bool backward) {
   q.planes = p.dtype == kF32 ? 2 : 1;
   q.ldh = static_cast<int>(up(p.D, 8));
   q.twice = p.dtype != kF32 && p.N <= kFewRows;
+  q.spread = p.dtype != kBF16 && p.reduction == 0;  // rows of any weight, whose G is fp16 (weights_kernel)
   // read as they are: 16-byte rows, and 256 of them within 32-bit offsets
   q.pack_w = p.dtype == kF32 || p.D % 8 != 0 || p.w_ld % 8 != 0 || (reinterpret_cast<uintptr_t>(p.w) & 15) != 0 ||
              p.w_ld > (int64_t(1) << 21);
   const int64_t w_bytes = int64_t(2) * q.planes * p.V * q.ldh, h_bytes = up((int64_t(2) * q.planes * p.N * q.ldh) << q.twice, 256);
   q.keep_w = q.pack_w && w_bytes <= kKeepBytes;
   q.off_rows_info = up(int64_t(8) * p.N * (1 + p.K), 256);
-  q.off_h = q.off_rows_info + up(int64_t(4) * (4 + 3 * int64_t(p.N)), 256);
+  q.off_hidden = q.off_rows_info + up(int64_t(4) * (4 + 3 * int64_t(p.N)), 256);
   auto chunks = [&](bool of_g) {
     int64_t chunk = up(p.V, kTile);
     if (of_g) {
@@ -1914,7 +1942,7 @@ Plan plan(const DetVocabHead& p, bool backward) {
   const int gc = chunks(true);
   const int64_t held = p.hold_bytes / (int64_t(2) * q.planes * p.N) / gc * gc;  // whole chunks of G
   q.held = static_cast<int>(held < up(p.V, gc) ? held : up(p.V, gc));
-  q.off_e = q.off_h + h_bytes;
+  q.off_e = q.off_hidden + h_bytes;
   q.off_tops = q.off_e + int64_t(2) * q.planes * p.N * q.held;
   q.off_kw = q.off_tops + up(int64_t(4) * p.N * (q.held / 128), 256);
   q.kept = q.off_kw + (q.keep_w ? w_bytes : 0);
@@ -1946,6 +1974,8 @@ Plan plan(const DetVocabHead& p, bool backward) {
   } else {
     q.off_roww = take(int64_t(4) * p.N);
     q.off_alpha = take(4);
+    q.off_rowe = q.spread ? take(int64_t(4) * p.N) : 0;
+    q.off_again = q.spread && p.dw != nullptr ? take(h_bytes) : 0;
     q.off_g = take((int64_t(2) * q.planes * p.N * q.chunk) << q.twice);
     q.off_dx = p.dx != nullptr ? take(partials(int64_t(p.N) << q.twice, q.ldh, q.chunk, kPiece)) : 0;
     // few tiles under many rows (8192 x 64 x 1000 bf16: 155 us for four blocks, 20 us in pieces)
@@ -1982,7 +2012,8 @@ int pack(hipStream_t st, const PackArgs& a) {
   return static_cast<int>(hipGetLastError());
 }
 int pack_any(hipStream_t st, int dt, const PackArgs& a) {
-  return dt == kF32 ? pack<kF32>(st, a) : pack<kBF16>(st, a);  // 16-bit types are copied as bits
+  if (dt == kF32) return pack<kF32>(st, a);
+  return dt == kF16 && a.row_e != nullptr ? pack<kF16>(st, a) : pack<kBF16>(st, a);
 }
 
 // The call with its kept parts in place.
@@ -1997,21 +2028,22 @@ struct Head : DetVocabHead {
     char* at = static_cast<char*>(p.kept);
     stats = reinterpret_cast<float*>(at);
     rows = reinterpret_cast<int*>(at + q.off_rows_info);
-    hidden = reinterpret_cast<u16*>(at + q.off_h);
+    hidden = reinterpret_cast<u16*>(at + q.off_hidden);
     e = at + q.off_e;
     tops = reinterpret_cast<float*>(at + q.off_tops);
     weights = reinterpret_cast<u16*>(at + q.off_kw);
   }
 };
 
-int pack_hidden(hipStream_t st, const Head& p, const Plan& q) {
+int pack_hidden(hipStream_t st, const Head& p, const Plan& q, const int* row_e, u16* to) {
   PackArgs a = {};
   a.src = p.x;
   a.src_ld = p.x_ld;
   a.list = p.rows + 4;
   a.count = p.rows;
   a.absmax = p.rows + 1;
-  a.dst = p.hidden;
+  a.dst = to;
+  a.row_e = row_e;
   a.plane = int64_t(p.N) * q.ldh;
   a.rows = p.N;
   a.cols = p.D;
@@ -2094,7 +2126,7 @@ int det_vocab_head_forward(void* stream, const DetVocabHead* pp) {
                        Matrix{static_cast<const float*>(p.w), p.w_ld, p.V, p.D, nullptr, nullptr}, xb, p.rows);
   }
   DET_TRY(static_cast<int>(hipGetLastError()));
-  DET_TRY(pack_hidden(st, p, q));
+  DET_TRY(pack_hidden(st, p, q, nullptr, p.hidden));
   for (int c = 0; c < q.nchunks; ++c) {
     const int v0 = c * q.chunk, nv = p.V - v0 < q.chunk ? p.V - v0 : q.chunk;
     Operand w;
@@ -2178,12 +2210,18 @@ int det_vocab_head_backward(void* stream, const DetVocabHead* pp) {
   const float g_scale = f16 ? static_cast<float>(1 << kGExp) : 1.f;
   Alpha alpha = {static_cast<const float*>(p.gout), p.rows, 1.f / (p.inv_t * g_scale), p.reduction == 1};
   float* row_w = nullptr;
+  int* row_e = q.spread ? reinterpret_cast<int*>(ws + q.off_rowe) : nullptr;
+  u16* hidden = p.hidden;  // as G^T h takes them
   if (p.reduction == 0) {
     row_w = reinterpret_cast<float*>(ws + q.off_roww);
     float* top = reinterpret_cast<float*>(ws + q.off_alpha);
-    hipLaunchKernelGGL(weights_kernel, dim3(1), dim3(1024), 0, st, WeightArgs{alpha.p, p.rows, list, row_w, top, g_scale});
+    hipLaunchKernelGGL(weights_kernel, dim3(1), dim3(1024), 0, st, WeightArgs{alpha.p, p.rows, list, row_w, top, row_e, g_scale});
     DET_TRY(static_cast<int>(hipGetLastError()));
     alpha.p = top;
+  }
+  if (q.spread && p.dw != nullptr) {
+    hidden = reinterpret_cast<u16*>(ws + q.off_again);
+    DET_TRY(pack_hidden(st, p, q, row_e, hidden));
   }
   // a word's listed shares add up to N times the largest weight at most: in steps of 2^-61 N of that, below 2^63
   unsigned long long* listed = p.db != nullptr && p.index != nullptr ? reinterpret_cast<unsigned long long*>(ws + q.off_listed) : nullptr;
@@ -2201,6 +2239,7 @@ int det_vocab_head_backward(void* stream, const DetVocabHead* pp) {
     a.top = p.stats;
     a.log_s = p.stats + p.N;
     a.row_w = row_w;
+    a.row_e = row_e;
     a.g_scale = g_scale;
     a.smooth_v = p.smooth / static_cast<float>(p.V);
     a.colsum = cs;
@@ -2208,7 +2247,7 @@ int det_vocab_head_backward(void* stream, const DetVocabHead* pp) {
     a.g_plane = int64_t(p.N) * ldg;
     a.ldg = ldg;
     if (held) {
-      const HeldArgs h = {p.e + int64_t(2) * q.planes * v0, p.tops + v0 / 128, q.held, p.rows, a.top, a.log_s, row_w, g_scale, a.c,
+      const HeldArgs h = {p.e + int64_t(2) * q.planes * v0, p.tops + v0 / 128, q.held, p.rows, a.top, a.log_s, row_w, row_e, g_scale, a.c,
                           a.smooth_v, a.share, a.words, v0, a.colsum, a.G, a.g_plane, ldg, q.twice};
       const dim3 hg(static_cast<unsigned>(ldg / 64) * ceil_div(p.N, kTile));
       if (p.dtype == kF32) hipLaunchKernelGGL(held_kernel<kF32>, hg, dim3(256), 0, st, h);
@@ -2219,7 +2258,8 @@ int det_vocab_head_backward(void* stream, const DetVocabHead* pp) {
     }
     if (p.index != nullptr) {
       ScatterArgs s = {p.rows, list, p.index, p.index_ld, p.wide, p.K, v0, nv, f16, q.planes, ldg, picked,
-                       picked + int64_t(p.N) * p.K, a.top, a.log_s, row_w, g_scale, a.c, a.G, a.g_plane, q.twice, listed, steps};
+                       picked + int64_t(p.N) * p.K, a.top, a.log_s, row_w, row_e, g_scale, a.c, a.G, a.g_plane, q.twice, listed,
+                       steps};
       if (listed != nullptr) hipLaunchKernelGGL(clear_kernel, dim3(ceil_div(nv, 256)), dim3(256), 0, st, listed, nv);
       const int64_t sb = (int64_t(p.N) * p.K + 255) / 256;
       hipLaunchKernelGGL(scatter_kernel, dim3(sb < 8192 ? static_cast<unsigned>(sb) : 8192u), dim3(256), 0, st, s);
@@ -2250,7 +2290,7 @@ int det_vocab_head_backward(void* stream, const DetVocabHead* pp) {
     if (p.dw != nullptr) {
       GemmArgs d = {};
       d.A = G;
-      d.B = Operand{p.hidden, int64_t(p.N) * q.ldh, q.ldh};
+      d.B = Operand{hidden, int64_t(p.N) * q.ldh, q.ldh};
       d.k_dyn = p.rows;
       d.info = p.rows;
       d.twice = q.twice;
@@ -2264,7 +2304,7 @@ int det_vocab_head_backward(void* stream, const DetVocabHead* pp) {
         d.ldo = q.ldh;
         DET_TRY((gemm<true, true, kPartial>(st, p.dtype, d)));
         hipLaunchKernelGGL(sum_kernel, dim3(nv, ceil_div(p.D, 1024) < 64 ? ceil_div(p.D, 1024) : 64), dim3(256), 0, st, d.out32, 0,
-                           d.ldo, p.rows, nullptr, 0, alpha, q.planes, d.out, p.dtype, p.D);
+                           d.ldo, p.rows, nullptr, nullptr, 0, alpha, q.planes, d.out, p.dtype, p.D);
       } else {
         d.cut = 1;
         d.ldo = p.D;
@@ -2275,8 +2315,8 @@ int det_vocab_head_backward(void* stream, const DetVocabHead* pp) {
   }
   if (p.dx != nullptr)
     hipLaunchKernelGGL(sum_kernel, dim3(p.N, ceil_div(p.D, 1024) < 64 ? ceil_div(p.D, 1024) : 64), dim3(256), 0, st,
-                       reinterpret_cast<const float*>(ws + q.off_dx), q.chunk, int64_t(q.ldh), p.rows, list + p.N, q.twice, alpha, q.planes,
-                       p.dx, p.dtype, p.D);
+                       reinterpret_cast<const float*>(ws + q.off_dx), q.chunk, int64_t(q.ldh), p.rows, list + p.N, row_e, q.twice, alpha,
+                       q.planes, p.dx, p.dtype, p.D);
   return static_cast<int>(hipGetLastError());
 }
 

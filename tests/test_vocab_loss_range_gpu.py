@@ -66,6 +66,54 @@ def test_fp32_operands_of_any_magnitude(gpu, power, d, hold_bytes):
         assert (dw.double() / s - dw0.double()).abs().max().item() <= 2.0 ** -149 / s
 
 
+@pytest.mark.parametrize("hold_bytes", [0, vocab_loss.HOLD_BYTES])
+@pytest.mark.parametrize("kind", ["target", "list"])
+@pytest.mark.parametrize("n", [40, 300])
+@pytest.mark.parametrize("dt", TYPES)
+def test_rows_of_very_different_weight(gpu, dt, n, kind, hold_bytes):
+    """Incoming derivatives over sixty powers of two: a row's gradient by x depends on its own alone, to its own precision."""
+    d, v = 64, 900
+    x, w, b, g = _tensors(gpu, n, d, v, dt)
+    if kind == "target":
+        kw = dict(target=torch.randint(0, v, (n,), generator=g, device=gpu), smooth=0.1)
+    else:
+        teacher, index = _lists(gpu, g, n, v, 5)
+        kw = dict(teacher=teacher, index=index, heat=2.0)
+    scale = 2.0 ** 12  # (fp16's gradients have their smallest step at 2^-24)
+    gout = torch.exp2(-60 * torch.rand(n, generator=g, device=gpu)) * torch.where(torch.rand(n, generator=g, device=gpu) < 0.5, -scale, scale)
+    gout[3], gout[4], gout[7] = 0.0, scale, 1e-30
+    _, (dx, dw, db), _ = _run_head(x, w, b, reduction="none", gout=gout, hold_bytes=hold_bytes, **kw)
+    args = dict(target=None, teacher=None, index=None, ignore=-100, smooth=0.0, heat=1.0, reduction="none", gout=gout)
+    args.update(kw)
+    x64, w64 = x.double(), w.double()
+    z = x64 @ w64.t() + b.double()
+    size = x64.abs() @ w64.abs().t() + b.double().abs()
+    _, G, A, P = _definition(z, **args)
+    fp32, heat = dt == torch.float32, args["heat"]
+    product = d * 2.0 ** -24 + (2.0 ** -21 if fp32 else 0.0)
+    E = (2 * product * size.amax(1) + 3 * 2.0 ** -24 * (z / heat).abs().amax(1) * 1.5) / heat + _sum_error(v)
+    if kind == "list":
+        E = E + _share_error(teacher, heat)
+    u_g = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -22}[dt]
+    if n <= 128 and not fp32:
+        u_g = u_g ** 2
+    held = 0.0 if fp32 or hold_bytes == 0 else 2.0 ** -12
+    # G is held to 2^-39 at least where its row's weight is 1, and that weight to 2^-8 at least
+    step = 0.0 if dt == torch.bfloat16 else 2.0 ** -31 * gout.double().abs()[:, None] * heat
+    err = A * (u_g + E)[:, None] + held * (P + 2.0 ** -19 * P.amax(1, keepdim=True)) + step
+    split = 2.0 ** -21 if fp32 else 0.0
+    _near(dx, G @ w64, 1.01 * (err @ w64.abs() + (v * 2.0 ** -24 + split) * (A @ w64.abs())) + 1.01 * U[dt] * (G @ w64).abs() + TINY[dt], "dx")
+    # where a row's weight is below 2^-8 of the largest, its x takes what is missing, and G stays below 2^-7 of a row's of
+    # weight 1: fp16 holds such an x to 2^-25, fp32's planes hold every x to 2^-39 of the largest
+    floor = {torch.bfloat16: 0.0, torch.float16: 2.0 ** -25, torch.float32: 2.0 ** -39 * x64.abs().max().item()}[dt]
+    weight = gout.double().abs()[:, None]
+    unit = torch.where(weight > 0, A / weight.clamp(min=1e-300), torch.zeros_like(A))
+    loose = (unit * torch.where(weight < scale * 2.0 ** -8, torch.full_like(weight, scale * 2.0 ** -7), weight)).sum(0) * floor
+    _near(dw, G.t() @ x64, 1.01 * (err.t() @ x64.abs() + (n * 2.0 ** -24 + split) * (A.t() @ x64.abs()) + loose[:, None])
+          + 1.01 * U[dt] * (G.t() @ x64).abs() + TINY[dt], "dweight")
+    _near(db, G.sum(0), 1.01 * (err.sum(0) + n * 2.0 ** -24 * A.sum(0)) + 1.01 * U[dt] * G.sum(0).abs() + TINY[dt], "dbias")
+
+
 @pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
 @pytest.mark.parametrize("kind", ["target", "list"])
 @pytest.mark.parametrize("n", [40, 300])
