@@ -225,13 +225,15 @@ __global__ void __launch_bounds__(1024) rows_kernel(RowArgs a) {
 }
 
 // The largest finite magnitudes of the hidden states and the weights (fp32), as bits: blocks below
-// x_blocks go over x, its kept rows alone: what an ignored one holds must not decide their scale.  One atomic a
-// block (eight thousand, one a wave, took 65 us of a 75 us launch); a maximum does not depend on their order.
+// x_blocks go over x, its kept rows alone (what an ignored one holds must not decide their scale), and leave each
+// row's as well.  One atomic a block (eight thousand, one a wave, took 65 us of a 75 us launch); a maximum does not
+// depend on their order.
 struct Matrix {
   const float* p;
   int64_t ld;
   int rows, cols;
   const int *list, *count;  // the rows that count, and how many (null: all)
+  int* each;                // their magnitudes, with a list
 };
 
 __global__ void __launch_bounds__(256) absmax_kernel(Matrix x, Matrix w, int x_blocks, int* info) {
@@ -244,6 +246,13 @@ __global__ void __launch_bounds__(256) absmax_kernel(Matrix x, Matrix w, int x_b
     const uint32_t b = __float_as_uint(f) & 0x7FFFFFFFu;
     if (b < 0x7F800000u && b > m) m = b;
   };
+  auto most = [](uint32_t v) {
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint32_t u = __shfl_xor(v, o, 64);
+      v = u > v ? u : v;
+    }
+    return v;
+  };
   const int64_t all = static_cast<int64_t>(a.rows) * a.cols;
   if (a.list == nullptr && a.ld == a.cols && (reinterpret_cast<uintptr_t>(a.p) & 15) == 0) {
 #pragma unroll 4
@@ -255,16 +264,21 @@ __global__ void __launch_bounds__(256) absmax_kernel(Matrix x, Matrix w, int x_b
     if (block == 0 && threadIdx.x < (all & 3)) take(a.p[all - 1 - threadIdx.x]);
   } else {
     const int rows = a.list != nullptr ? *a.count : a.rows;
+    uint32_t all_rows = 0;
     for (int64_t r = block * 4 + (threadIdx.x >> 6); r < rows; r += blocks * 4) {
       const float* p = a.p + (a.list != nullptr ? a.list[r] : r) * a.ld;
+      m = 0;
 #pragma unroll 4
       for (int c = threadIdx.x & 63; c < a.cols; c += 64) take(p[c]);
+      if (a.list != nullptr) {
+        m = most(m);
+        if ((threadIdx.x & 63) == 0) a.each[r] = static_cast<int>(m);
+      }
+      all_rows = m > all_rows ? m : all_rows;
     }
+    m = all_rows;
   }
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint32_t v = __shfl_xor(m, o, 64);
-    m = v > m ? v : m;
-  }
+  m = most(m);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
   __syncthreads();
   if (threadIdx.x == 0) {
@@ -285,7 +299,8 @@ struct PackArgs {
   int64_t src_ld;
   const int* list;   // null: rows as they are
   const int* count;  // null: `rows`
-  const int* absmax; // fp32
+  const int* absmax; // fp32: the largest magnitude that the scale is for,
+  const int* each;   // or each row's
   u16* dst;
   int64_t plane;     // elements between the planes
   int rows, cols, ld;  // ld % 8 == 0
@@ -309,13 +324,13 @@ __global__ void __launch_bounds__(256) pack_kernel(PackArgs a) {
   typedef typename Elem<DT>::type T;
   const int rows = a.count != nullptr ? *a.count : a.rows;
   const int chunks = a.ld >> 3;
-  const int scale = DT == kF32 ? scale_exp(static_cast<uint32_t>(*a.absmax)) : 0;
   // a thread per eight columns, whatever the width
   const int64_t all = static_cast<int64_t>(rows) * chunks, step = gridDim.x * 256ll;
   for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < all; i += step) {
     const int r = static_cast<int>(i / chunks), c = static_cast<int>(i - static_cast<int64_t>(r) * chunks) * 8;
     const int more = a.row_e != nullptr ? a.row_e[r] : 0;
     const int64_t from = static_cast<int64_t>(a.list != nullptr ? a.list[r] : r) * a.src_ld;
+    const int scale = DT == kF32 ? scale_exp(static_cast<uint32_t>(a.each != nullptr ? a.each[r] : *a.absmax)) : 0;
     T v[8];
     load8(static_cast<const T*>(a.src) + from + c, a.cols - c, v);
     us8 hi, lo;
@@ -377,7 +392,8 @@ struct GemmArgs {
   int least;                // kPartial: the shortest piece
   int chunk;                // kPartial of words: the longest K of the pass, which the splits are made for
   int cut;                  // whether the last round's tiles may be cut in two
-  const int* info;          // scales of fp32 operands
+  // what the scales of fp32 operands are made of: kStats, kGrad: each row's of A, info[2] for B; kOut: B's
+  const int *info, *bits;
   // kStats, kGrad: z = acc / scales + bias, c = log2(e) / T
   const void* bias;
   int bias_dt;
@@ -430,7 +446,7 @@ constexpr int kTile = 256, kThreads = 512;
 constexpr int kHalf = 16384, kStage = 4 * kHalf;
 constexpr int kLdc = kTile + 16, kLdc32 = kTile + 4;
 constexpr int kSideOff = kTile * kLdc * 2;  // the rows' and words' numbers for the epilogue, behind the tile
-constexpr int kGemmSmem = kSideOff + kTile * 20;
+constexpr int kGemmSmem = kSideOff + kTile * 24;
 static_assert(kSideOff >= 2 * kStage && kSideOff >= 128 * kLdc32 * 4, "the epilogues reuse the stages");
 constexpr unsigned kOOB = 0x80000000u;     // past kRange: the load returns zeros
 constexpr unsigned kRange = 0x7FFFFFF0u;
@@ -684,10 +700,11 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Place& at, un
     return *reinterpret_cast<const s16x8*>(half + s * 8192 + r * 64 + ((fch ^ swz64_row(r)) << 4));
   };
 
-  // what the epilogue needs of each row (maximum, log of the sum, weight, target relative to the tile) and
+  // what the epilogue needs of each row (maximum, log of the sum, weight, target relative to the tile; scale) and
   // word (bias; -inf past the last) goes to LDS ahead of the products: there it would be loads in a row
   f32x4* side_row = reinterpret_cast<f32x4*>(smem + kSideOff);
   float* side_col = reinterpret_cast<float*>(smem + kSideOff + kTile * 16);
+  int* side_e = reinterpret_cast<int*>(smem + kSideOff + kTile * 20);
   if constexpr (EPI == kStats || EPI == kGrad) {
     if (tid < kTile) {
       const int row = m0 + tid;
@@ -700,6 +717,8 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Place& at, un
         }
         if (g.words != nullptr) v[3] = __int_as_float(g.words[row] - g.v0 - n0);
       }
+      if (PL == 2)
+        side_e[tid] = row < M ? -scale_exp(static_cast<uint32_t>(g.bits[row])) - scale_exp(static_cast<uint32_t>(g.info[2])) : 0;
       side_row[tid] = v;
     } else if (tid < kTile + BN) {
       const int col = n0 + tid - kTile;
@@ -813,8 +832,7 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Place& at, un
   // wc * 16 FN + j * 16 + fch * 4 + r.  A row's reduction is 4 FN values in registers and two lane steps.
   const int row0 = wr * 128 + fr, col0 = wc * (FN * 16) + fch * 4;
   if constexpr (EPI == kStats || EPI == kGrad) {
-    const int unscale = PL == 1 ? 0 : -scale_exp(static_cast<uint32_t>(g.info[1])) - scale_exp(static_cast<uint32_t>(g.info[2]));
-    auto logit = [&](float sum, float b) { return (PL == 1 ? sum : times_pow2(sum, unscale)) + b; };
+    auto logit = [&](float sum, float b, int unscale) { return (PL == 1 ? sum : times_pow2(sum, unscale)) + b; };
     const float c = g.c;
     f32x4 bias[4];
 #pragma unroll
@@ -825,11 +843,12 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Place& at, un
       for (int i = 0; i < 8; ++i) {
         if (m0 + wr * 128 + i * 16 >= M) break;  // nothing of the 16 rows' is read
         float m = kNegInf, s = 0.f, sz = 0.f;
+        const int unscale = PL == 2 ? side_e[row0 + i * 16] : 0;
 #pragma unroll
         for (int j = 0; j < FN; ++j)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            acc[i][j][r] = logit(acc[i][j][r], bias[j][r]);
+            acc[i][j][r] = logit(acc[i][j][r], bias[j][r], unscale);
             m = fmaxf(m, acc[i][j][r]);
           }
         if (g.words != nullptr) {
@@ -951,11 +970,12 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Place& at, un
         const bool ok = m0 + row0 + i * 16 < M;
         const f32x4 of = side_row[row0 + i * 16];
         const float top = of[0], l = of[1], w = of[2];
+        const int unscale = PL == 2 ? side_e[row0 + i * 16] : 0;
 #pragma unroll
         for (int j = 0; j < FN; ++j)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float p = exp2_(fmaf(logit(acc[i][j][r], bias[j][r]) - top, c, -l));
+            const float p = exp2_(fmaf(logit(acc[i][j][r], bias[j][r], unscale) - top, c, -l));
             acc[i][j][r] = ok ? w * (p - g.smooth_v) : 0.f;
           }
         if (g.words != nullptr) {
@@ -1034,7 +1054,7 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Place& at, un
     }
   } else {
     const float alpha = g.alpha();
-    const int unscale = PL == 1 ? 0 : -scale_exp(static_cast<uint32_t>(g.info[1]));
+    const int unscale = PL == 1 ? 0 : -scale_exp(static_cast<uint32_t>(*g.bits));
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
@@ -1105,11 +1125,12 @@ __global__ void __launch_bounds__(256) pieces_kernel(GemmArgs g, int planes) {
   const int M = *g.m_dyn, ntn = (g.N + kTile - 1) / kTile, lane = threadIdx.x & 63;
   if (M == 0) return;
   const int len = split_length((M + kTile - 1) / kTile * ntn, g.chunk, g.least), splits = (g.chunk + len - 1) / len;
-  const int unscale = planes == 1 ? 0 : -scale_exp(static_cast<uint32_t>(g.info[1])) - scale_exp(static_cast<uint32_t>(g.info[2]));
+  const int of_words = planes == 1 ? 0 : -scale_exp(static_cast<uint32_t>(g.info[2]));
   const int64_t units = static_cast<int64_t>(M) * ntn, stride = M * g.ldo;
   for (int64_t unit = blockIdx.x * 4ll + (threadIdx.x >> 6); unit < units; unit += gridDim.x * 4ll) {
     const int row = static_cast<int>(unit / ntn), tile = static_cast<int>(unit - static_cast<int64_t>(row) * ntn);
     const int col = tile * kTile + lane * 4;
+    const int unscale = planes == 1 ? 0 : of_words - scale_exp(static_cast<uint32_t>(g.bits[row]));
     const float* p = g.out32 + row * g.ldo + col;
     f32x4 z = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
@@ -1360,6 +1381,8 @@ struct WeightArgs {
   const int *info, *list;
   float *row_w, *top;
   int* row_e;      // null: zeros
+  const int* each; // fp32: the largest magnitude of each row of h; *most: of them times 2^row_e
+  int* most;
   float g_scale;
 };
 
@@ -1368,7 +1391,7 @@ __device__ __forceinline__ bool finite(float v) { return (__float_as_uint(v) & 0
 __global__ void __launch_bounds__(1024) weights_kernel(WeightArgs a) {
   __shared__ float part[16];
   const int count = a.info[0];
-  float top = 0.f;
+  float top = 0.f, most = 0.f;
   for (int c = threadIdx.x; c < count; c += 1024) {
     const float g = fabsf(a.g[a.list[c]]);
     if (finite(g)) top = fmaxf(top, g);
@@ -1386,8 +1409,18 @@ __global__ void __launch_bounds__(1024) weights_kernel(WeightArgs a) {
       a.row_e[c] = e = e < 0 ? e : 0;
     }
     a.row_w[c] = !finite(g) ? g : top == 0.f ? 0.f : times_pow2(g, -e) / top * a.g_scale;
+    if (a.each != nullptr) most = fmaxf(most, times_pow2(__int_as_float(a.each[c]), e));
   }
   if (threadIdx.x == 0) *a.top = top;
+  if (a.each == nullptr) return;
+  most = max_lanes(most);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = most;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 16; ++w) most = fmaxf(most, part[w]);
+    *a.most = __float_as_int(most);
+  }
 }
 
 // the listed words' entries of a chunk's G, from the fp32 logits of the forward pass (a word twice in
@@ -1531,8 +1564,8 @@ __global__ void __launch_bounds__(256) dbias_kernel(const float* part, int ldg, 
 // The sum of a row's partials: of dh (pos: a row's place among the kept ones; zeros for the others), or of
 // dw (pos null; rows of words, pieces of the kept rows).  Bound by memory (4608 rows, 28 pieces of 691 kept:
 // 59 MB in 13 us)
-__global__ void __launch_bounds__(256) sum_kernel(const float* part, int span, int64_t ldo, const int* info, const int* pos, const int* row_e, int twice,
-                                                  Alpha alpha, int planes, void* dx, int dt, int D) {
+__global__ void __launch_bounds__(256) sum_kernel(const float* part, int span, int64_t ldo, const int* info, const int* bits, const int* pos,
+                                                  const int* row_e, int twice, Alpha alpha, int planes, void* dx, int dt, int D) {
   const int n = blockIdx.x, at = pos != nullptr ? pos[n] : n, count = pos != nullptr ? info[0] << twice : gridDim.x;
   const int tiles = ((count + kTile - 1) / kTile) * ((D + kTile - 1) / kTile);
   int splits = 0;
@@ -1542,7 +1575,7 @@ __global__ void __launch_bounds__(256) sum_kernel(const float* part, int span, i
     splits = (span + len - 1) / len;
   }
   const float a = at >= 0 ? alpha() : 0.f;  // (a row that does not count: zeros, whatever the derivative is)
-  int unscale = planes == 2 ? -scale_exp(static_cast<uint32_t>(info[pos != nullptr ? 2 : 1])) : 0;
+  int unscale = planes == 2 ? -scale_exp(static_cast<uint32_t>(*bits)) : 0;
   if (row_e != nullptr && at >= 0) unscale += row_e[at];
   const int64_t stride = count * ldo, out = static_cast<int64_t>(n) * D;
   for (int d = (blockIdx.y * 256 + threadIdx.x) * 4; d < D; d += gridDim.y * 1024) {
@@ -1898,9 +1931,10 @@ namespace {
 // What both directions lay out in the workspace.
 struct Plan {
   int planes, ldh, chunk, nchunks, parts, held, twice;
-  bool pack_w, keep_w, split_w, split_z, spread;
+  bool pack_w, keep_w, split_w, split_z, spread, again;
   int64_t off_rows_info, off_hidden, off_e, off_tops, off_kw, kept;  // in `kept`
-  int64_t off_w, off_z, off_flag, off_part, off_partz, off_rows, off_roww, off_alpha, off_rowe, off_again, off_g, off_dx, off_dw, off_cs, off_listed, total;
+  int64_t off_w, off_z, off_flag, off_part, off_partz, off_rows;                                                     // forward
+  int64_t off_roww, off_alpha, off_rowe, off_most, off_again, off_g, off_dx, off_dw, off_cs, off_listed, total;      // backward
 };
 
 constexpr int64_t kChunkBytes = int64_t(512) << 20;  // G of one chunk, and the packed weights of one
@@ -1916,13 +1950,15 @@ Plan plan(const DetVocabHead& p, bool backward) {
   q.ldh = static_cast<int>(up(p.D, 8));
   q.twice = p.dtype != kF32 && p.N <= kFewRows;
   q.spread = p.dtype != kBF16 && p.reduction == 0;  // rows of any weight, whose G is fp16 (weights_kernel)
+  // G^T h sums over rows, so it takes them under one scale; the logits' have one each
+  q.again = p.dw != nullptr && (p.dtype == kF32 || q.spread);
   // read as they are: 16-byte rows, and 256 of them within 32-bit offsets
   q.pack_w = p.dtype == kF32 || p.D % 8 != 0 || p.w_ld % 8 != 0 || (reinterpret_cast<uintptr_t>(p.w) & 15) != 0 ||
              p.w_ld > (int64_t(1) << 21);
   const int64_t w_bytes = int64_t(2) * q.planes * p.V * q.ldh, h_bytes = up((int64_t(2) * q.planes * p.N * q.ldh) << q.twice, 256);
   q.keep_w = q.pack_w && w_bytes <= kKeepBytes;
   q.off_rows_info = up(int64_t(8) * p.N * (1 + p.K), 256);
-  q.off_hidden = q.off_rows_info + up(int64_t(4) * (4 + 3 * int64_t(p.N)), 256);
+  q.off_hidden = q.off_rows_info + up(int64_t(4) * (4 + 4 * int64_t(p.N)), 256);
   auto chunks = [&](bool of_g) {
     int64_t chunk = up(p.V, kTile);
     if (of_g) {
@@ -1975,7 +2011,8 @@ Plan plan(const DetVocabHead& p, bool backward) {
     q.off_roww = take(int64_t(4) * p.N);
     q.off_alpha = take(4);
     q.off_rowe = q.spread ? take(int64_t(4) * p.N) : 0;
-    q.off_again = q.spread && p.dw != nullptr ? take(h_bytes) : 0;
+    q.off_most = take(4);
+    q.off_again = q.again ? take(h_bytes) : 0;
     q.off_g = take((int64_t(2) * q.planes * p.N * q.chunk) << q.twice);
     q.off_dx = p.dx != nullptr ? take(partials(int64_t(p.N) << q.twice, q.ldh, q.chunk, kPiece)) : 0;
     // few tiles under many rows (8192 x 64 x 1000 bf16: 155 us for four blocks, 20 us in pieces)
@@ -2019,7 +2056,7 @@ int pack_any(hipStream_t st, int dt, const PackArgs& a) {
 // The call with its kept parts in place.
 struct Head : DetVocabHead {
   float* stats;  // [2, N] maxima and log2 of sums, [N, K] picked logits, [N, K] shares
-  int* rows;     // [4 + 3 N]: info, the list of kept rows, each row's place in it, targets
+  int* rows;     // [4 + 4 N]: info, the list of kept rows, each row's place in it, targets, kept rows' magnitudes
   u16* hidden;   // the packed hidden states
   char* e;       // exponentials of the first q.held words' logits
   float* tops;   // their tiles' maxima
@@ -2035,13 +2072,15 @@ struct Head : DetVocabHead {
   }
 };
 
-int pack_hidden(hipStream_t st, const Head& p, const Plan& q, const int* row_e, u16* to) {
+// the kept rows, under a scale each or (absmax) one for all
+int pack_hidden(hipStream_t st, const Head& p, const Plan& q, const int* absmax, const int* row_e, u16* to) {
   PackArgs a = {};
   a.src = p.x;
   a.src_ld = p.x_ld;
   a.list = p.rows + 4;
   a.count = p.rows;
-  a.absmax = p.rows + 1;
+  a.absmax = absmax;
+  a.each = absmax == nullptr ? p.rows + 4 + int64_t(3) * p.N : nullptr;
   a.dst = to;
   a.row_e = row_e;
   a.plane = int64_t(p.N) * q.ldh;
@@ -2079,6 +2118,7 @@ GemmArgs logits_args(const Head& p, const Plan& q, const Operand& w, int v0, int
   a.B = w;
   a.m_dyn = p.rows;
   a.info = p.rows;
+  a.bits = p.rows + 4 + int64_t(3) * p.N;
   a.M = p.N;
   a.N = nv;
   a.K = q.ldh;
@@ -2122,11 +2162,12 @@ int det_vocab_head_forward(void* stream, const DetVocabHead* pp) {
   hipLaunchKernelGGL(rows_kernel, dim3(1), dim3(1024), 0, st, r);
   if (p.dtype == kF32) {
     const int xb = p.N < 512 ? ceil_div(p.N, 4) : 128, wb = p.V < 2048 ? ceil_div(p.V, 4) : 512;
-    hipLaunchKernelGGL(absmax_kernel, dim3(xb + wb), dim3(256), 0, st, Matrix{static_cast<const float*>(p.x), p.x_ld, p.N, p.D, list, p.rows},
-                       Matrix{static_cast<const float*>(p.w), p.w_ld, p.V, p.D, nullptr, nullptr}, xb, p.rows);
+    hipLaunchKernelGGL(absmax_kernel, dim3(xb + wb), dim3(256), 0, st,
+                       Matrix{static_cast<const float*>(p.x), p.x_ld, p.N, p.D, list, p.rows, list + int64_t(3) * p.N},
+                       Matrix{static_cast<const float*>(p.w), p.w_ld, p.V, p.D, nullptr, nullptr, nullptr}, xb, p.rows);
   }
   DET_TRY(static_cast<int>(hipGetLastError()));
-  DET_TRY(pack_hidden(st, p, q, nullptr, p.hidden));
+  DET_TRY(pack_hidden(st, p, q, nullptr, nullptr, p.hidden));
   for (int c = 0; c < q.nchunks; ++c) {
     const int v0 = c * q.chunk, nv = p.V - v0 < q.chunk ? p.V - v0 : q.chunk;
     Operand w;
@@ -2211,17 +2252,21 @@ int det_vocab_head_backward(void* stream, const DetVocabHead* pp) {
   Alpha alpha = {static_cast<const float*>(p.gout), p.rows, 1.f / (p.inv_t * g_scale), p.reduction == 1};
   float* row_w = nullptr;
   int* row_e = q.spread ? reinterpret_cast<int*>(ws + q.off_rowe) : nullptr;
-  u16* hidden = p.hidden;  // as G^T h takes them
+  u16* hidden = p.hidden;        // as G^T h takes them,
+  const int* bits = p.rows + 1;  // and what their scale is made of (fp32)
   if (p.reduction == 0) {
     row_w = reinterpret_cast<float*>(ws + q.off_roww);
     float* top = reinterpret_cast<float*>(ws + q.off_alpha);
-    hipLaunchKernelGGL(weights_kernel, dim3(1), dim3(1024), 0, st, WeightArgs{alpha.p, p.rows, list, row_w, top, row_e, g_scale});
+    int* most = reinterpret_cast<int*>(ws + q.off_most);
+    bits = most;
+    hipLaunchKernelGGL(weights_kernel, dim3(1), dim3(1024), 0, st,
+                       WeightArgs{alpha.p, p.rows, list, row_w, top, row_e, p.dtype == kF32 ? list + int64_t(3) * p.N : nullptr, most, g_scale});
     DET_TRY(static_cast<int>(hipGetLastError()));
     alpha.p = top;
   }
-  if (q.spread && p.dw != nullptr) {
+  if (q.again) {
     hidden = reinterpret_cast<u16*>(ws + q.off_again);
-    DET_TRY(pack_hidden(st, p, q, row_e, hidden));
+    DET_TRY(pack_hidden(st, p, q, bits, row_e, hidden));
   }
   // a word's listed shares add up to N times the largest weight at most: in steps of 2^-61 N of that, below 2^63
   unsigned long long* listed = p.db != nullptr && p.index != nullptr ? reinterpret_cast<unsigned long long*>(ws + q.off_listed) : nullptr;
@@ -2293,6 +2338,7 @@ int det_vocab_head_backward(void* stream, const DetVocabHead* pp) {
       d.B = Operand{hidden, int64_t(p.N) * q.ldh, q.ldh};
       d.k_dyn = p.rows;
       d.info = p.rows;
+      d.bits = bits;
       d.twice = q.twice;
       d.least = kPiece;
       d.M = nv;
@@ -2304,7 +2350,7 @@ int det_vocab_head_backward(void* stream, const DetVocabHead* pp) {
         d.ldo = q.ldh;
         DET_TRY((gemm<true, true, kPartial>(st, p.dtype, d)));
         hipLaunchKernelGGL(sum_kernel, dim3(nv, ceil_div(p.D, 1024) < 64 ? ceil_div(p.D, 1024) : 64), dim3(256), 0, st, d.out32, 0,
-                           d.ldo, p.rows, nullptr, nullptr, 0, alpha, q.planes, d.out, p.dtype, p.D);
+                           d.ldo, p.rows, bits, nullptr, nullptr, 0, alpha, q.planes, d.out, p.dtype, p.D);
       } else {
         d.cut = 1;
         d.ldo = p.D;
@@ -2315,8 +2361,8 @@ int det_vocab_head_backward(void* stream, const DetVocabHead* pp) {
   }
   if (p.dx != nullptr)
     hipLaunchKernelGGL(sum_kernel, dim3(p.N, ceil_div(p.D, 1024) < 64 ? ceil_div(p.D, 1024) : 64), dim3(256), 0, st,
-                       reinterpret_cast<const float*>(ws + q.off_dx), q.chunk, int64_t(q.ldh), p.rows, list + p.N, row_e, q.twice, alpha,
-                       q.planes, p.dx, p.dtype, p.D);
+                       reinterpret_cast<const float*>(ws + q.off_dx), q.chunk, int64_t(q.ldh), p.rows, p.rows + 2, list + p.N, row_e, q.twice,
+                       alpha, q.planes, p.dx, p.dtype, p.D);
   return static_cast<int>(hipGetLastError());
 }
 

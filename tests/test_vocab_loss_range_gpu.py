@@ -67,6 +67,24 @@ def test_fp32_operands_of_any_magnitude(gpu, power, d, hold_bytes):
 
 
 @pytest.mark.parametrize("hold_bytes", [0, vocab_loss.HOLD_BYTES])
+@pytest.mark.parametrize("d", [64, 1024])
+@pytest.mark.parametrize("times", [1e8, 1e30, 1e-8, 1e-30])
+def test_a_row_far_larger_than_the_others(gpu, times, d, hold_bytes):
+    """A kept row decides nothing of the other rows' losses and gradients by x."""
+    x, w, b, g = _tensors(gpu, 300, d, 700, torch.float32)
+    t = torch.randint(0, 700, (300,), generator=g, device=gpu)
+    teacher, index = _lists(gpu, g, 300, 700, 5)
+    others = torch.arange(300, device=gpu) != 5
+    far = x.clone()
+    far[5] *= times
+    for kw in (dict(target=t), dict(teacher=teacher, index=index)):
+        ref, (ref_dx, _, _), _ = _run_head(x, w, b, reduction="none", hold_bytes=hold_bytes, **kw)
+        loss, (dx, dw, db), _ = _run_head(far, w, b, reduction="none", hold_bytes=hold_bytes, **kw)
+        assert torch.isfinite(loss).all() and all(torch.isfinite(a).all() for a in (dx, dw, db))
+        _same((loss[others], dx[others]), (ref[others], ref_dx[others]))
+
+
+@pytest.mark.parametrize("hold_bytes", [0, vocab_loss.HOLD_BYTES])
 @pytest.mark.parametrize("kind", ["target", "list"])
 @pytest.mark.parametrize("n", [40, 300])
 @pytest.mark.parametrize("dt", TYPES)
