@@ -226,7 +226,7 @@ __global__ void __launch_bounds__(1024) rows_kernel(RowArgs a) {
 
 // The largest finite magnitudes of the hidden states and the weights (fp32), as bits: blocks below
 // x_blocks go over x, its kept rows alone (what an ignored one holds must not decide their scale), and leave each
-// row's as well.  One atomic a block (eight thousand, one a wave, took 65 us of a 75 us launch); a maximum does not
+// row's as well; of the weights, words that a bias of -inf takes out do not count either.  One atomic a block (eight thousand, one a wave, took 65 us of a 75 us launch); a maximum does not
 // depend on their order.
 struct Matrix {
   const float* p;
@@ -234,7 +234,13 @@ struct Matrix {
   int rows, cols;
   const int *list, *count;  // the rows that count, and how many (null: all)
   int* each;                // their magnitudes, with a list
+  const void* bias;         // the weights': null or [rows]
+  int bias_dt;
 };
+
+// a word that its bias takes out: z is -inf whatever its row of the weights holds
+__device__ __forceinline__ bool masked(const void* bias, int64_t word, int dt) { return bias != nullptr && load_any(bias, word, dt) == kNegInf; }
+
 
 __global__ void __launch_bounds__(256) absmax_kernel(Matrix x, Matrix w, int x_blocks, int* info) {
   __shared__ uint32_t red[4];
@@ -254,7 +260,7 @@ __global__ void __launch_bounds__(256) absmax_kernel(Matrix x, Matrix w, int x_b
     return v;
   };
   const int64_t all = static_cast<int64_t>(a.rows) * a.cols;
-  if (a.list == nullptr && a.ld == a.cols && (reinterpret_cast<uintptr_t>(a.p) & 15) == 0) {
+  if (a.list == nullptr && a.bias == nullptr && a.ld == a.cols && (reinterpret_cast<uintptr_t>(a.p) & 15) == 0) {
 #pragma unroll 4
     for (int64_t i = block * 256 + threadIdx.x; i < all / 4; i += blocks * 256) {
       const f32x4 v = reinterpret_cast<const f32x4*>(a.p)[i];
@@ -266,10 +272,18 @@ __global__ void __launch_bounds__(256) absmax_kernel(Matrix x, Matrix w, int x_b
     const int rows = a.list != nullptr ? *a.count : a.rows;
     uint32_t all_rows = 0;
     for (int64_t r = block * 4 + (threadIdx.x >> 6); r < rows; r += blocks * 4) {
+      if (masked(a.bias, r, a.bias_dt)) continue;
       const float* p = a.p + (a.list != nullptr ? a.list[r] : r) * a.ld;
+      const int fours = (reinterpret_cast<uintptr_t>(p) & 15) == 0 ? a.cols / 4 : 0;
       m = 0;
 #pragma unroll 4
-      for (int c = threadIdx.x & 63; c < a.cols; c += 64) take(p[c]);
+      for (int c = threadIdx.x & 63; c < fours; c += 64) {
+        const f32x4 v = reinterpret_cast<const f32x4*>(p)[c];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) take(v[e]);
+      }
+#pragma unroll 4
+      for (int c = fours * 4 + (threadIdx.x & 63); c < a.cols; c += 64) take(p[c]);
       if (a.list != nullptr) {
         m = most(m);
         if ((threadIdx.x & 63) == 0) a.each[r] = static_cast<int>(m);
@@ -306,6 +320,8 @@ struct PackArgs {
   int rows, cols, ld;  // ld % 8 == 0
   int twice;         // the rows once more behind the last one
   const int* row_e;  // rows times 2^row_e, or null
+  const void* bias;  // words (fp32) that it takes out are zeros, or null
+  int bias_dt;
 };
 
 // eight elements from any address (16-byte loads need no alignment here), zeros past the row's end
@@ -332,7 +348,7 @@ __global__ void __launch_bounds__(256) pack_kernel(PackArgs a) {
     const int64_t from = static_cast<int64_t>(a.list != nullptr ? a.list[r] : r) * a.src_ld;
     const int scale = DT == kF32 ? scale_exp(static_cast<uint32_t>(a.each != nullptr ? a.each[r] : *a.absmax)) : 0;
     T v[8];
-    load8(static_cast<const T*>(a.src) + from + c, a.cols - c, v);
+    load8(static_cast<const T*>(a.src) + from + c, DT == kF32 && masked(a.bias, r, a.bias_dt) ? 0 : a.cols - c, v);
     us8 hi, lo;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -2101,6 +2117,8 @@ int weight_operand(hipStream_t st, const Head& p, const Plan& q, char* ws, int v
   }
   PackArgs a = {};
   a.src = q.keep_w ? p.w : src;
+  if (p.bias != nullptr) a.bias = static_cast<const char*>(p.bias) + (q.keep_w ? 0 : int64_t(v0) * (p.bias_dt == kF32 ? 4 : 2));
+  a.bias_dt = p.bias_dt;
   a.src_ld = p.w_ld;
   a.absmax = p.rows + 2;
   a.dst = q.keep_w ? p.weights : reinterpret_cast<u16*>(ws + q.off_w);
@@ -2161,10 +2179,10 @@ int det_vocab_head_forward(void* stream, const DetVocabHead* pp) {
   if (p.index != nullptr) hipLaunchKernelGGL(list_flags_kernel, dim3(ceil_div(p.N, 4)), dim3(256), 0, st, r);
   hipLaunchKernelGGL(rows_kernel, dim3(1), dim3(1024), 0, st, r);
   if (p.dtype == kF32) {
-    const int xb = p.N < 512 ? ceil_div(p.N, 4) : 128, wb = p.V < 2048 ? ceil_div(p.V, 4) : 512;
+    const int xb = p.N < 512 ? ceil_div(p.N, 4) : 128, wb = p.V < 4096 ? ceil_div(p.V, 4) : p.bias == nullptr ? 512 : 1024;
     hipLaunchKernelGGL(absmax_kernel, dim3(xb + wb), dim3(256), 0, st,
-                       Matrix{static_cast<const float*>(p.x), p.x_ld, p.N, p.D, list, p.rows, list + int64_t(3) * p.N},
-                       Matrix{static_cast<const float*>(p.w), p.w_ld, p.V, p.D, nullptr, nullptr, nullptr}, xb, p.rows);
+                       Matrix{static_cast<const float*>(p.x), p.x_ld, p.N, p.D, list, p.rows, list + int64_t(3) * p.N, nullptr, 0},
+                       Matrix{static_cast<const float*>(p.w), p.w_ld, p.V, p.D, nullptr, nullptr, nullptr, p.bias, p.bias_dt}, xb, p.rows);
   }
   DET_TRY(static_cast<int>(hipGetLastError()));
   DET_TRY(pack_hidden(st, p, q, nullptr, nullptr, p.hidden));

@@ -84,6 +84,27 @@ def test_a_row_far_larger_than_the_others(gpu, times, d, hold_bytes):
         _same((loss[others], dx[others]), (ref[others], ref_dx[others]))
 
 
+@pytest.mark.parametrize("d", [64, 1024])
+@pytest.mark.parametrize("dt", TYPES)
+def test_what_a_masked_word_weighs_does_not_matter(gpu, dt, d):
+    """Words that a bias of -inf takes out (a padded vocabulary), with whatever their rows of W hold."""
+    x, w, b, g = _tensors(gpu, 200, d, 700, dt)
+    out = torch.zeros(700, dtype=torch.bool, device=gpu)
+    out[650:] = out[100:110] = True
+    b = b.float().masked_fill(out, -math.inf)
+    t = torch.randint(120, 640, (200,), generator=g, device=gpu)
+    teacher, index = _lists(gpu, g, 200, 500, 5)
+    w[out] = 0
+    for kw in (dict(target=t), dict(teacher=teacher, index=index + 120, heat=2.0)):
+        for junk in (1e4, 1e20, 1e30):
+            clean, wild = w.clone(), w.clone()
+            wild[out] = min(junk, torch.finfo(dt).max)
+            ref, ref_grads, _ = _run_head(x, clean, b, **kw)
+            loss, grads, _ = _run_head(x, wild, b, **kw)
+            assert torch.isfinite(ref)
+            _same((loss, *grads), (ref, *ref_grads))
+
+
 @pytest.mark.parametrize("hold_bytes", [0, vocab_loss.HOLD_BYTES])
 @pytest.mark.parametrize("kind", ["target", "list"])
 @pytest.mark.parametrize("n", [40, 300])
