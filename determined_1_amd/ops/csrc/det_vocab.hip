@@ -416,7 +416,8 @@ struct GemmArgs {
   float c;
   float2* part;   // kStats [M][parts], 128 columns each: maximum and sum
   // kStats: the first `held` words' exponentials below the tile's maximum (null: none), and the maxima
-  void* E;        // [M][held], 11-bit numbers or fp32
+  void* E;        // [M][held], 11-bit numbers, or fp32 if exact
+  int exact;
   float* tops;    // [M][held / 128]
   int held;       // (a multiple of 256)
   float* part_z;  // sum of z / V, or null
@@ -939,7 +940,7 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Place& at, un
           for (int j = 0; j < FN; ++j) acc[i][j] *= f;
         }
         __syncthreads();
-        if constexpr (PL == 1) {
+        if (PL == 1 && !g.exact) {
           typedef __attribute__((ext_vector_type(4))) u16 us4;
           u16* ct = reinterpret_cast<u16*>(smem);
 #pragma unroll
@@ -1179,7 +1180,7 @@ __global__ void __launch_bounds__(256) pieces_kernel(GemmArgs g, int planes) {
     }
     if (g.E == nullptr) continue;
     const int64_t at = static_cast<int64_t>(row) * g.held + col;
-    if (planes == 2) {
+    if (g.exact) {
       *reinterpret_cast<f32x4*>(static_cast<float*>(g.E) + at) = x;
     } else {
       typedef __attribute__((ext_vector_type(4))) u16 us4;
@@ -1462,7 +1463,7 @@ struct HeldArgs {
   int ldg, twice;
 };
 
-template <int DT>
+template <int DT, bool EXACT>
 __global__ void __launch_bounds__(256) held_kernel(HeldArgs a) {
   constexpr bool kF = DT == kF32;
   const int M = a.info[0], tid = threadIdx.x, across = a.ldg / 64, down = static_cast<int>(blockIdx.x) / across;
@@ -1475,7 +1476,7 @@ __global__ void __launch_bounds__(256) held_kernel(HeldArgs a) {
     if (row >= M) continue;
     const int64_t at = static_cast<int64_t>(row) * a.held + col;
     float g[8];
-    if constexpr (kF) {
+    if constexpr (EXACT) {
       const f32x4* e = reinterpret_cast<const f32x4*>(static_cast<const float*>(a.E) + at);
       const f32x4 lo = __builtin_nontemporal_load(e), hi = __builtin_nontemporal_load(e + 1);
 #pragma unroll
@@ -1946,7 +1947,7 @@ namespace {
 
 // What both directions lay out in the workspace.
 struct Plan {
-  int planes, ldh, chunk, nchunks, parts, held, twice;
+  int planes, ldh, chunk, nchunks, parts, held, exact, twice;
   bool pack_w, keep_w, split_w, split_z, spread, again;
   int64_t off_rows_info, off_hidden, off_e, off_tops, off_kw, kept;  // in `kept`
   int64_t off_w, off_z, off_flag, off_part, off_partz, off_rows;                                                     // forward
@@ -1992,10 +1993,14 @@ Plan plan(const DetVocabHead& p, bool backward) {
   q.chunk = chunks(backward);
   q.nchunks = ceil_div(p.V, q.chunk);
   const int gc = chunks(true);
-  const int64_t held = p.hold_bytes / (int64_t(2) * q.planes * p.N) / gc * gc;  // whole chunks of G
+  // Exponentials are held in fp32 for fp32 operands and with label smoothing, where G is the difference of p and
+  // eps / V: near the optimum, where they are equal, 11 bits of p would be few of G's.
+  q.exact = p.dtype == kF32 || p.smooth != 0.f;
+  const int64_t e_bytes = (q.exact ? 4 : 2) * int64_t(p.N);  // a word's
+  const int64_t held = p.hold_bytes / e_bytes / gc * gc;  // whole chunks of G
   q.held = static_cast<int>(held < up(p.V, gc) ? held : up(p.V, gc));
   q.off_e = q.off_hidden + h_bytes;
-  q.off_tops = q.off_e + int64_t(2) * q.planes * p.N * q.held;
+  q.off_tops = q.off_e + e_bytes * q.held;
   q.off_kw = q.off_tops + up(int64_t(4) * p.N * (q.held / 128), 256);
   q.kept = q.off_kw + (q.keep_w ? w_bytes : 0);
   q.parts = 2 * ceil_div(p.V, kTile);
@@ -2197,6 +2202,7 @@ int det_vocab_head_forward(void* stream, const DetVocabHead* pp) {
     a.E = q.held > 0 ? p.e : nullptr;
     a.tops = p.tops;
     a.held = q.held;
+    a.exact = q.exact;
     if (q.split_z) {
       a.twice = 0;
       a.chunk = a.K;
@@ -2310,12 +2316,14 @@ int det_vocab_head_backward(void* stream, const DetVocabHead* pp) {
     a.g_plane = int64_t(p.N) * ldg;
     a.ldg = ldg;
     if (held) {
-      const HeldArgs h = {p.e + int64_t(2) * q.planes * v0, p.tops + v0 / 128, q.held, p.rows, a.top, a.log_s, row_w, row_e, g_scale, a.c,
+      const HeldArgs h = {p.e + int64_t(q.exact ? 4 : 2) * v0, p.tops + v0 / 128, q.held, p.rows, a.top, a.log_s, row_w, row_e, g_scale, a.c,
                           a.smooth_v, a.share, a.words, v0, a.colsum, a.G, a.g_plane, ldg, q.twice};
       const dim3 hg(static_cast<unsigned>(ldg / 64) * ceil_div(p.N, kTile));
-      if (p.dtype == kF32) hipLaunchKernelGGL(held_kernel<kF32>, hg, dim3(256), 0, st, h);
-      else if (p.dtype == kBF16) hipLaunchKernelGGL(held_kernel<kBF16>, hg, dim3(256), 0, st, h);
-      else hipLaunchKernelGGL(held_kernel<kF16>, hg, dim3(256), 0, st, h);
+      if (p.dtype == kF32) hipLaunchKernelGGL((held_kernel<kF32, true>), hg, dim3(256), 0, st, h);
+      else if (p.dtype == kBF16 && q.exact) hipLaunchKernelGGL((held_kernel<kBF16, true>), hg, dim3(256), 0, st, h);
+      else if (p.dtype == kBF16) hipLaunchKernelGGL((held_kernel<kBF16, false>), hg, dim3(256), 0, st, h);
+      else if (q.exact) hipLaunchKernelGGL((held_kernel<kF16, true>), hg, dim3(256), 0, st, h);
+      else hipLaunchKernelGGL((held_kernel<kF16, false>), hg, dim3(256), 0, st, h);
     } else {
       DET_TRY((gemm<false, false, kGrad>(st, p.dtype, a)));
     }

@@ -11,13 +11,14 @@ into the gradients of ``x`` and ``W``.  It makes a chunk from exponentials that 
 chunks as ``hold_bytes`` has room for, and from the logits computed again past those.  Rows that are
 ignored cost nothing.  Losses are fp32; sums, softmax statistics and gradients are accumulated in fp32; a
 chunk's logit gradient is held in the operands' type (fp32: two fp16 planes, 22 bits), exponentials in 16
-bits with a step of 2^-11 (fp32: as they are).
+bits with a step of 2^-11 down to 2^-31 of a tile's largest (for fp32 operands and with label smoothing: in
+fp32; with ``hold_bytes=0`` none are).
 
 GPU tensors (bf16, fp16, fp32) always run on the kernels; what those do not cover is refused.  CPU
 tensors run the plain composite below.  The kernels are differentiable once.
 
-Memory of a ``linear_`` call: between forward and backward at most ``hold_bytes`` (2 or, for fp32, 4 bytes a
-logit) and two percent more, the kept rows of ``x`` once more, 8 K bytes a row, and weights that had to be packed
+Memory of a ``linear_`` call: between forward and backward at most ``hold_bytes`` (2 or, where they are fp32, 4
+bytes a logit) and two percent more, the kept rows of ``x`` once more, 8 K bytes a row, and weights that had to be packed
 (fp32, or rows that 16 bytes do not divide) up to 4 GiB of them; in the backward 512 MiB for a chunk's logit
 gradient and fp32 sums of ``x``'s gradient.  Under ``torch.no_grad()`` none of these exponentials.
 """

@@ -226,3 +226,35 @@ def test_a_lists_bias_gradient_is_summed_in_fp32(gpu, dt, n, v, reduction, hold_
     _near(db, G.sum(0), 1.01 * err.sum(0) + (n + 4) * 2.0 ** -24 * A.sum(0), "dbias")
     again = _run_head(x, w, b, teacher=teacher, index=index, heat=heat, reduction=reduction, gout=gout, hold_bytes=hold_bytes)[1][2]
     assert torch.equal(again, db)
+
+
+@pytest.mark.parametrize("hold_bytes", [0, vocab_loss.HOLD_BYTES])
+@pytest.mark.parametrize("n", [100, 300])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+def test_smoothing_near_its_optimum(gpu, dt, n, hold_bytes):
+    """p near eps / V, of which G is the difference: G to its type's precision, not to that of p.
+
+    G's entries are off by u_g |G| and, each for itself, by p times the logit's error and 2^-20 (the exponent's rounding at
+    11, the exponential's and a product's); besides, all p of a row are off together (its sum, its logarithm).  A matrix of
+    errors moves dx by at most its Frobenius norm times W's largest singular value, an error of a whole row by that error
+    times sum_v p w_v."""
+    d, v = 64, 2000
+    x, w, _, g = _tensors(gpu, n, d, v, dt, bias=False)
+    x = (x.float() * 0.001).to(dt)  # logits of 0.0015: p is 1 / V times 1 +- 0.0015
+    t = torch.randint(0, v, (n,), generator=g, device=gpu)
+    gout = torch.tensor(2.0 ** 10, device=gpu)
+    _, (dx, dw), _ = _run_head(x, w, None, target=t, smooth=1.0, reduction="sum", gout=gout, hold_bytes=hold_bytes)
+    x64, w64 = x.double(), w.double()
+    z = x64 @ w64.t()
+    _, G, _, P = _definition(z, t, None, None, -100, 1.0, 1.0, "sum", gout)
+    each = 2 * d * 2.0 ** -24 * (x64.abs() @ w64.abs().t()).amax(1) + 2.0 ** -20
+    row = _sum_error(v) + 3 * 2.0 ** -24 * 1.5 * (math.log2(v) + z.abs().amax(1))
+    off = U[dt] ** (2 if n <= 128 else 1) * G.abs() + each[:, None] * P + (0.0 if dt == torch.bfloat16 else 2.0 ** -39 * 2.0 ** 10)
+    whole = row[:, None] * P
+    for got, ref, err in ((dx, G @ w64, off.norm() * torch.linalg.matrix_norm(w64, 2) + (row[:, None] * (P @ w64)).norm()
+                           + v * 2.0 ** -24 * (G.abs() @ w64.abs()).norm()),
+                          (dw, G.t() @ x64, (off.norm() + whole.norm()) * torch.linalg.matrix_norm(x64, 2)
+                           + n * 2.0 ** -24 * (G.abs().t() @ x64.abs()).norm())):
+        bound = 1.01 * (err + U[dt] * ref.norm()).item() + TINY[dt] * ref.numel() ** 0.5
+        error = (got.double() - ref).norm().item()
+        assert error <= bound, f"{error / bound:.2f} times the bound"
