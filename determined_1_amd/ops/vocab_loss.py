@@ -304,8 +304,8 @@ def _bytes(what: str, hold_bytes: int) -> int:
 
 
 def _empty(reduction: str, lead: torch.Size, *ts: Optional[torch.Tensor]) -> torch.Tensor:
-    """The loss of no rows: 0, with gradients of zeros."""
-    zero = sum((t * 0).sum().float() for t in ts if t is not None)
+    """The loss of no rows: 0, with gradients of zeros, whatever the tensors hold."""
+    zero = sum(_wide(t.narrow(0, 0, 0)).sum() for t in ts if t is not None)
     return zero if reduction != "none" else zero.expand(lead)
 
 
