@@ -228,7 +228,10 @@ def _plain_ce(z: torch.Tensor, target: torch.Tensor, ignore: int, smooth: float,
     kept = target != ignore
     z = torch.where(kept[:, None], z, torch.zeros_like(z))
     logp = F.log_softmax(z, dim=1)
-    rows = -(1.0 - smooth) * _pick(logp, target[:, None], kept[:, None])[:, 0]
+    picked = _pick(logp, target[:, None], kept[:, None])[:, 0]
+    if smooth == 1.0:  # the target does not count, not even one of logit -inf
+        picked = torch.where(picked.isnan(), picked, torch.zeros_like(picked))
+    rows = -(1.0 - smooth) * picked
     if smooth:
         rows = rows - smooth * logp.mean(dim=1)
     return _reduce(rows, kept, reduction)

@@ -25,3 +25,13 @@ def test_no_rows_are_zero_whatever_the_weights_hold(junk):
             assert torch.equal(grad, torch.zeros_like(leaf))
     assert linear_cross_entropy(x[:0].bfloat16(), w.detach().bfloat16(), none).dtype == torch.float32
     assert topk_distill(x[:0].bfloat16(), x[:0, :2], none[:, None].expand(0, 2)).dtype == torch.float32
+
+
+def test_a_masked_target_that_does_not_count():
+    """With a label smoothing of 1 the target has no share, so a masked one makes the loss infinite as any masked word
+    does, and not NaN; one outside the vocabulary is NaN all the same."""
+    x, w, b = _head()
+    b[4] = -math.inf
+    t = torch.tensor([4, 1, 2, 4, 11, 5, 6])
+    loss = linear_cross_entropy(x, w, t, b, label_smoothing=1.0, reduction="none")
+    assert loss.isnan().tolist() == [False] * 4 + [True] + [False] * 2 and (loss[:4] == math.inf).all()
