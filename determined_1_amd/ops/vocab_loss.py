@@ -363,7 +363,10 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
         _refuse(what, f"target is {target.dtype}: int32 or int64 expected", TypeError)
     if not 0.0 <= label_smoothing <= 1.0:
         _refuse(what, f"label_smoothing {label_smoothing} is not within [0, 1]")
-    opts = (int(ignore_index), float(label_smoothing), 1.0, reduction, _bytes(what, hold_bytes))
+    ignore = int(ignore_index)
+    if not -2 ** 63 <= ignore < 2 ** 63:
+        _refuse(what, f"ignore_index {ignore_index} is not of 64 bits")
+    opts = (ignore, float(label_smoothing), 1.0, reduction, _bytes(what, hold_bytes))
     return _linear(x, weight, bias, target, None, None, opts, lead)
 
 

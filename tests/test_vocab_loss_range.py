@@ -35,3 +35,11 @@ def test_a_masked_target_that_does_not_count():
     t = torch.tensor([4, 1, 2, 4, 11, 5, 6])
     loss = linear_cross_entropy(x, w, t, b, label_smoothing=1.0, reduction="none")
     assert loss.isnan().tolist() == [False] * 4 + [True] + [False] * 2 and (loss[:4] == math.inf).all()
+
+
+@pytest.mark.parametrize("ignore", [2 ** 63, -2 ** 63 - 1, 2 ** 64 - 100])
+def test_an_index_that_no_target_can_hold_is_refused(ignore):
+    x, w, _ = _head()
+    with pytest.raises(ValueError, match="linear_cross_entropy"):
+        linear_cross_entropy(x, w, torch.arange(7), ignore_index=ignore)
+    assert linear_cross_entropy(x, w, torch.arange(7), ignore_index=-2 ** 63).item() > 0
