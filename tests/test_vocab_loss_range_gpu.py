@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from determined_1_amd.ops import vocab_loss
-from determined_1_amd.ops.vocab_loss import topk_distill
+from determined_1_amd.ops.vocab_loss import linear_cross_entropy, linear_topk_distill, topk_distill
 from tests.test_vocab_loss_gpu import TINY, U, _definition, _lists, _near, _run_head, _share_error, _sum_error, _tensors
 
 pytestmark = pytest.mark.gpu
@@ -258,3 +258,134 @@ def test_smoothing_near_its_optimum(gpu, dt, n, hold_bytes):
         bound = 1.01 * (err + U[dt] * ref.norm()).item() + TINY[dt] * ref.numel() ** 0.5
         error = (got.double() - ref).norm().item()
         assert error <= bound, f"{error / bound:.2f} times the bound"
+
+
+def test_the_gradient_is_the_slope_along_itself(gpu):
+    """Each gradient against the differences of losses along it: (f(a + h u) - f(a - h u)) / 2 h = |grad| for u = grad / |grad|.
+
+    The third derivative of a row's loss along u is the third central moment of z' under p (over T^2 for a list, times T^2), at
+    most R^3 / (6 sqrt 3) for z' of range R / T; the two losses are off by 2^-21 of themselves each."""
+    n, d, v = 50, 96, 400
+    x, w, b, g = _tensors(gpu, n, d, v, torch.float32)
+    t = torch.randint(0, v, (n,), generator=g, device=gpu)
+    t[::4] = -100
+    teacher, index = _lists(gpu, g, n, v, 10)
+    for kw in (dict(target=t, smooth=0.1), dict(teacher=teacher, index=index, heat=2.0)):
+        loss, grads, _ = _run_head(x, w, b, **kw)
+        heat = kw.get("heat", 1.0)
+        for i in range(3):
+            size = grads[i].double().norm().item()
+            u = (grads[i].double() / size).float()
+            h = 2.0 ** -4
+            ends = []
+            for s in (h, -h):
+                args = [x, w, b]
+                args[i] = args[i] + s * u
+                ends.append(_run_head(*args, **kw)[0].item())
+            slope = (ends[0] - ends[1]) / (2 * h)
+            move = (u.double() @ w.double().t() if i == 0 else x.double() @ u.double().t() if i == 1 else u.double().expand(n, v)) / heat
+            reach = (move.amax(1) - move.amin(1)) ** 3 * heat * heat
+            tol = h * h / 6 * reach.max().item() / (6 * 3 ** 0.5) + 2.0 ** -21 * abs(loss.item()) / h + 2.0 ** -12 * size
+            assert tol < 0.1 * size, (i, tol / size)  # (or it would show nothing)
+            assert abs(slope - size) <= tol, (i, slope, size, tol)
+
+
+def test_a_weight_past_32_bits_elementwise(gpu):
+    """dx and rows of dweight of a weight of more than 2^31 entries, each against its own bound."""
+    v, d = 530000, 4096
+    g = torch.Generator(device=gpu).manual_seed(2)
+    w = torch.empty(v, d, dtype=torch.bfloat16, device=gpu).normal_(std=0.02, generator=g)
+    x = torch.randn(3, d, generator=g, device=gpu).bfloat16()
+    t = torch.tensor([0, 524288, v - 1], device=gpu)
+    loss, (dx, dw), gout = _run_head(x, w, None, target=t, reduction="none")
+    x64 = x.double()
+    z = torch.cat([x64 @ part.double().t() for part in w.split(20000)], 1)
+    size = torch.cat([x64.abs() @ part.double().abs().t() for part in w.split(20000)], 1).amax(1)
+    ref, G, A, P = _definition(z, t, None, None, -100, 0.0, 1.0, "none", gout)
+    E = 2 * d * 2.0 ** -24 * size + 3 * 2.0 ** -24 * z.abs().amax(1) * 1.5 + _sum_error(v)
+    _near(loss, ref, 2 * E + 2.0 ** -22 * (1 + z.abs().amax(1)) + 2.0 ** -22 * ref.abs(), "loss")
+    # three rows: G is two 16-bit rows each
+    err = A * (2.0 ** -16 + E)[:, None] + 2.0 ** -12 * (P + 2.0 ** -19 * P.amax(1, keepdim=True))
+    sums = [0.0, 0.0]
+    for i in range(0, v, 20000):
+        part = w[i:i + 20000].double()
+        sums[0] = sums[0] + G[:, i:i + 20000] @ part
+        sums[1] = sums[1] + err[:, i:i + 20000] @ part.abs() + v * 2.0 ** -24 * (A[:, i:i + 20000] @ part.abs())
+    _near(dx, sums[0], 1.01 * sums[1] + 1.01 * 2.0 ** -8 * sums[0].abs() + TINY[torch.bfloat16], "dx")
+    rows = torch.cat([t, torch.tensor([1, 262143, 262144, 500000, v - 2], device=gpu)])
+    r = G[:, rows].t() @ x64
+    bound = err[:, rows].t() @ x64.abs() + 3 * 2.0 ** -24 * (A[:, rows].t() @ x64.abs())
+    _near(dw[rows], r, 1.01 * bound + 1.01 * 2.0 ** -8 * r.abs() + TINY[torch.bfloat16], "dweight")
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.float32])
+def test_captured_steps_of_weighted_rows(gpu, dt):
+    """Row weights, smoothing and a list with a bias in one captured step: replays are the eager step's bits."""
+    n, d, v = 200, 72, 1000
+    x, w, b, g = _tensors(gpu, n, d, v, dt)
+    t = torch.randint(0, v, (n,), generator=g, device=gpu)
+    teacher, index = _lists(gpu, g, n, v, 5)
+    weight = torch.ones(n, device=gpu)
+
+    def step(leaves):
+        xl, wl, bl = leaves
+        loss = ((linear_cross_entropy(xl, wl, t, bl, label_smoothing=0.1, reduction="none") * weight).sum()
+                + (linear_topk_distill(xl, wl, teacher, index, bl, temperature=2.0, reduction="none") * weight).sum()
+                + linear_topk_distill(xl, wl, teacher, index, bl))
+        return (loss.detach(),) + torch.autograd.grad(loss, leaves)
+
+    def fresh():
+        return [a.detach().clone().requires_grad_(True) for a in (x, w, b)]
+
+    static = fresh()
+    s = torch.cuda.Stream(gpu)
+    s.wait_stream(torch.cuda.current_stream(gpu))
+    with torch.cuda.stream(s):
+        step(static)
+    torch.cuda.current_stream(gpu).wait_stream(s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(static)
+    for i in range(4):
+        x.copy_(torch.randn(n, d, generator=g, device=gpu) * 10.0 ** i)
+        weight.copy_(torch.exp2(-20 * torch.rand(n, generator=g, device=gpu)))
+        t[: 50 * i] = -100
+        index[i] = -1
+        ref = step(fresh())
+        torch.cuda.synchronize()
+        with torch.no_grad():
+            static[0].copy_(x)
+        graph.replay()
+        torch.cuda.synchronize()
+        _same(out, ref)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+def test_weighted_rows_in_chunks(gpu, dt):
+    """Row weights and a list's bias gradient over more than one chunk of the vocabulary: as over one."""
+    n, d, v = 1500, 40, 300000
+    x, w, b, g = _tensors(gpu, n, d, v, dt)
+    teacher, index = _lists(gpu, g, n, v, 6)
+    index[:, 0], index[:, 1] = 150007, 150008
+    weight = torch.exp2(-30 * torch.rand(n, generator=g, device=gpu))
+    weight[7] = 1.0
+    _, (dx, dw, db), _ = _run_head(x, w, b, teacher=teacher, index=index, reduction="none", gout=weight)
+    # the largest row, and one of a weight of 2^-15 or less, alone
+    small = int(((weight < 2.0 ** -15) & (weight > 2.0 ** -25)).nonzero()[0])
+    for row in (7, small):
+        one, (dx1, _, _), _ = _run_head(x[row:row + 1], w, b, teacher=teacher[row:row + 1], index=index[row:row + 1], reduction="none",
+                                        gout=weight[row:row + 1])
+        size = dx1.double().norm().item()
+        # G to u of itself (one row alone: twice as many bits), held to 2^-12 or not, and dx's own rounding on either side
+        tol = (2 * U[dt] + (0.0 if dt == torch.float32 else 2.0 ** -12 + U[dt]) + 2.0 ** -14) * size + TINY[dt] * d ** 0.5
+        assert (dx[row].double() - dx1[0].double()).norm().item() <= tol, (row, size)
+    words = torch.tensor([150007, 150008], device=gpu)
+    z = x.double() @ w[words].double().t() + b[words].double()
+    lse = torch.cat([torch.logsumexp(x[i:i + 100].double() @ w.double().t() + b.double(), 1) for i in range(0, n, 100)])
+    p = torch.exp(z - lse[:, None])
+    share = torch.softmax(teacher.double(), 1)
+    share = torch.stack([(share * (index == wd)).sum(1) for wd in words.tolist()], 1)
+    ref = (weight.double()[:, None] * (p - share)).sum(0)
+    size = (weight.double()[:, None] * (p + share)).sum(0)
+    assert ((db[words].double() - ref).abs() <= 2.0 ** -12 * size + 1.01 * U[dt] * ref.abs() + TINY[dt]).all()
