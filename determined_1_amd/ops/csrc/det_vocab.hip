@@ -242,6 +242,18 @@ struct Matrix {
 __device__ __forceinline__ bool masked(const void* bias, int64_t word, int dt) { return bias != nullptr && load_any(bias, word, dt) == kNegInf; }
 
 
+// four values from any address (16-byte loads need no alignment here), zeros past the row's end
+__device__ __forceinline__ f32x4 load4(const float* p, int there) {
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  if (there >= 4) {
+    __builtin_memcpy(&v, p, sizeof(v));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 3; ++e) v[e] = e < there ? p[e] : 0.f;
+  }
+  return v;
+}
+
 __global__ void __launch_bounds__(256) absmax_kernel(Matrix x, Matrix w, int x_blocks, int* info) {
   __shared__ uint32_t red[4];
   const bool isx = blockIdx.x < static_cast<unsigned>(x_blocks);
@@ -268,26 +280,35 @@ __global__ void __launch_bounds__(256) absmax_kernel(Matrix x, Matrix w, int x_b
       for (int e = 0; e < 4; ++e) take(v[e]);
     }
     if (block == 0 && threadIdx.x < (all & 3)) take(a.p[all - 1 - threadIdx.x]);
-  } else {
-    const int rows = a.list != nullptr ? *a.count : a.rows;
+  } else if (a.list == nullptr) {  // four rows of a block on their way at a time
+    for (int64_t r0 = block * 4; r0 < a.rows; r0 += blocks * 4) {
+      bool there[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) there[q] = r0 + q < a.rows && !masked(a.bias, r0 + q, a.bias_dt);
+      for (int c = threadIdx.x * 4; c < a.cols; c += 1024) {
+        f32x4 v[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] = there[q] ? load4(a.p + (r0 + q) * a.ld + c, a.cols - c) : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) take(v[q][e]);
+      }
+    }
+  } else {  // a row a wave
+    const int rows = *a.count;
     uint32_t all_rows = 0;
     for (int64_t r = block * 4 + (threadIdx.x >> 6); r < rows; r += blocks * 4) {
-      if (masked(a.bias, r, a.bias_dt)) continue;
-      const float* p = a.p + (a.list != nullptr ? a.list[r] : r) * a.ld;
-      const int fours = (reinterpret_cast<uintptr_t>(p) & 15) == 0 ? a.cols / 4 : 0;
+      const float* p = a.p + a.list[r] * a.ld;
       m = 0;
 #pragma unroll 4
-      for (int c = threadIdx.x & 63; c < fours; c += 64) {
-        const f32x4 v = reinterpret_cast<const f32x4*>(p)[c];
+      for (int c = (threadIdx.x & 63) * 4; c < a.cols; c += 256) {
+        const f32x4 v = load4(p + c, a.cols - c);
 #pragma unroll
         for (int e = 0; e < 4; ++e) take(v[e]);
       }
-#pragma unroll 4
-      for (int c = fours * 4 + (threadIdx.x & 63); c < a.cols; c += 64) take(p[c]);
-      if (a.list != nullptr) {
-        m = most(m);
-        if ((threadIdx.x & 63) == 0) a.each[r] = static_cast<int>(m);
-      }
+      m = most(m);
+      if ((threadIdx.x & 63) == 0) a.each[r] = static_cast<int>(m);
       all_rows = m > all_rows ? m : all_rows;
     }
     m = all_rows;
@@ -2184,7 +2205,7 @@ int det_vocab_head_forward(void* stream, const DetVocabHead* pp) {
   if (p.index != nullptr) hipLaunchKernelGGL(list_flags_kernel, dim3(ceil_div(p.N, 4)), dim3(256), 0, st, r);
   hipLaunchKernelGGL(rows_kernel, dim3(1), dim3(1024), 0, st, r);
   if (p.dtype == kF32) {
-    const int xb = p.N < 512 ? ceil_div(p.N, 4) : 128, wb = p.V < 4096 ? ceil_div(p.V, 4) : p.bias == nullptr ? 512 : 1024;
+    const int xb = p.N < 1024 ? ceil_div(p.N, 4) : 256, wb = p.V < 2048 ? ceil_div(p.V, 4) : 512;
     hipLaunchKernelGGL(absmax_kernel, dim3(xb + wb), dim3(256), 0, st,
                        Matrix{static_cast<const float*>(p.x), p.x_ld, p.N, p.D, list, p.rows, list + int64_t(3) * p.N, nullptr, 0},
                        Matrix{static_cast<const float*>(p.w), p.w_ld, p.V, p.D, nullptr, nullptr, nullptr, p.bias, p.bias_dt}, xb, p.rows);
