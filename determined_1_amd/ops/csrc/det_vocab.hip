@@ -14,9 +14,9 @@
 // sum of exponentials per row (and hands out the target's logit); a joining pass per row, which for lists
 // adds the K listed logits, dot products of their own.  Backward: the vocabulary is walked in chunks; per
 // chunk G is written to a workspace, and two more products read it.  G comes from the tile's exponentials,
-// which the forward held in 16 bits as far as the caller's bound goes (2 GiB unless it says otherwise), and past
-// that from the product once more, in its epilogue.  What bounds it, 8192 x 4096 x 128000 bf16 in 22.1 ms: the
-// matrix units, 1.23 PFLOP/s over the three products (logits 6.8 ms, G w 6.9, G^T h 7.4; G from 2 GB of
+// which the forward held (hold_bits; with smoothing and for fp32 in fp32) as far as the caller's bound goes (2 GiB
+// unless it says otherwise), and past that from the product once more, in its epilogue.  What bounds it, 8192 x 4096 x 128000 bf16 in 22.1 ms: the
+// matrix units, 1.23 PFLOP/s over the three products (logits 6.8 ms, G w 6.8, G^T h 7.2; G from 2 GB of
 // exponentials 0.8, where the product again takes 6.7); for few rows the reads of w (one row against
 // 128000 x 4096: 6.0 TB/s).
 //
@@ -25,16 +25,17 @@
 //
 // G is held in the operands' 16 bits, which the matrix units take: each entry is off by at most half a step
 // (bf16 2^-8), at random, so gradients of many rows are off by about as much as their own rounding once more
-// (bf16 2048 x 2048 x 32000: 0.0024 against 0.0017 of their size).  With few rows one entry of one row can
+// (bf16 2048 x 2048 x 32000: 0.0023 against 0.0017 of their size).  With few rows one entry of one row can
 // decide: there G is two 16-bit rows each, the second what the first one's rounding took, which only fills
-// what is left of a tile.  Everything else is fp32.
+// what is left of a tile.  A bias gradient comes from G before its rounding.  Everything else is fp32.
 //
-// fp32 operands become two fp16 planes each, x s = hi + lo with s a power of two that puts the tensor's
-// largest finite magnitude at 2^14..2^15, and a product is hi hi + hi lo + lo hi in fp32 accumulators:
-// each operand is held to 2^-23 of itself (2^-39 of the tensor's largest value at worst) and the
-// dropped lo lo is below 2^-22 of its product, the size of one fp32 rounding, at a third of the matrix
-// units' 16-bit rate instead of the sixteenth that their fp32 instructions have (2240 x 850 x 10000: off by
-// 5e-7 of the gradients' size, an fp32 product by 1.9e-6).
+// fp32 operands become two fp16 planes each, x s = hi + lo with s a power of two that puts the largest finite
+// magnitude at 2^14..2^15: of each row of h in the logits, of all kept rows in G^T h, of all words in w, those that a
+// bias of -inf takes out not among them.  A product is hi hi + hi lo + lo hi in fp32 accumulators: each operand is
+// held to 2^-23 of itself, or 2^-39 of that largest magnitude where that is more (entries of w, or of h for dw, more
+// than 2^16 below it lose bits that an fp32 product keeps), and the dropped lo lo is below 2^-22 of its product, the
+// size of one fp32 rounding, at a third of the matrix units' 16-bit rate instead of the sixteenth that their fp32
+// instructions have (2240 x 850 x 10000: off by 5e-7 of the gradients' size, an fp32 product by 1.8e-6).
 #include <hip/hip_runtime.h>
 
 #include <atomic>
@@ -227,7 +228,7 @@ __global__ void __launch_bounds__(1024) rows_kernel(RowArgs a) {
 // The largest finite magnitudes of the hidden states and the weights (fp32), as bits: blocks below
 // x_blocks go over x, its kept rows alone (what an ignored one holds must not decide their scale), and leave each
 // row's as well; of the weights, words that a bias of -inf takes out do not count either.  One atomic a block (eight thousand, one a wave, took 65 us of a 75 us launch); a maximum does not
-// depend on their order.
+// depend on their order.  Bound by the read of w (333 x 768 against 30522 words: 94 MB in 30 us, 3.1 TB/s).
 struct Matrix {
   const float* p;
   int64_t ld;
@@ -818,7 +819,7 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, const Place& at, un
   phase_barrier();
   if (wr == 1) phase_barrier();
   // Up to 128 rows left: 64-row quadrants behind the last one take no reads and no products (a row of 4096 against
-  // 128000 words 235 to 180 us).  The conditions cost full tiles 2 to 7 % and a tile of 192 rows 2 %, so these have
+  // 128000 words 235 to 173 us).  The conditions cost full tiles 2 to 7 % and a tile of 192 rows 2 %, so these have
   // a loop without.
   auto stages = [&](auto all) {
     const int left = M - m0 - wr * 128;
@@ -1461,8 +1462,6 @@ __global__ void __launch_bounds__(1024) weights_kernel(WeightArgs a) {
   }
 }
 
-// the listed words' entries of a chunk's G, from the fp32 logits of the forward pass (a word twice in
-// a list: its shares add up, and each of its entries writes the same value)
 // ------------------------------------------------------------------------------------------------
 // G of the words whose exponentials the forward pass left: w (e 2^(c (the tile's maximum - top) - log2 sum) -
 // eps / V), minus the target's share; as the product's epilogue writes it.  A block has 256 rows of 64
@@ -1541,6 +1540,10 @@ __global__ void __launch_bounds__(256) held_kernel(HeldArgs a) {
   }
 }
 
+// The listed words' entries of a chunk's G, from the fp32 logits of the forward pass (a word twice in a list: its
+// shares add up, and each of its entries writes the same value), and their part of the bias gradient.  Each entry goes
+// over its row's list for that, so the work grows with K^2: 2048 lists of 64 in 16 us, a step of them with K = 1024
+// takes 3.2 ms where K = 64 takes 0.82.
 struct ScatterArgs {
   const int *info, *list;
   const void* index;
@@ -1854,7 +1857,7 @@ __global__ void __launch_bounds__(1024) logit_reduce_kernel(LogitArgs a, int fin
 
 // The gradient: one read, one write, then the listed words of the segment once more, from the fp32
 // arithmetic (a word's entries add up their shares and write the same value).  Bound by memory: 4096 x 128000
-// bf16 in 427 us, 4.9 TB/s.  The last rows come first, since the forward pass has left them in the caches; a
+// bf16 in 430 us, 4.9 TB/s.  The last rows come first, since the forward pass has left them in the caches; a
 // gradient that they cannot hold is written past them (the step of 4096 x 128000 bf16 667 -> 627 us).
 template <int DT>
 __global__ void __launch_bounds__(256) logit_grad_kernel(LogitArgs a) {
@@ -2320,7 +2323,7 @@ int det_vocab_head_backward(void* stream, const DetVocabHead* pp) {
   const int64_t es = p.dtype == kF32 ? 4 : 2;
   for (int c = 0; c < q.nchunks; ++c) {
     const int v0 = c * q.chunk, nv = p.V - v0 < q.chunk ? p.V - v0 : q.chunk;
-    const int ldg = static_cast<int>(up(nv, 64));  // columns past nv are zero
+    const int ldg = static_cast<int>(up(nv, 64));  // columns past nv hold -w eps / V; what they meet is fetched as zeros
     const bool held = v0 < q.held;
     Operand w = {};
     if (!held || p.dx != nullptr) DET_TRY(weight_operand(st, p, q, ws, v0, nv, false, &w));

@@ -17,10 +17,16 @@ fp32; with ``hold_bytes=0`` none are).
 GPU tensors (bf16, fp16, fp32) always run on the kernels; what those do not cover is refused.  CPU
 tensors run the plain composite below.  The kernels are differentiable once.
 
+fp32 operands are multiplied as two fp16 planes each, under a power of two: a row's own for ``x`` in the logits,
+one for all words of ``W`` (those that a bias of -inf takes out do not count), one for all kept rows of ``x``
+in ``W``'s gradient.  Entries more than 2^16 below the largest under the same scale are held to 2^-39 of that
+one instead of 2^-23 of themselves.
+
 Memory of a ``linear_`` call: between forward and backward at most ``hold_bytes`` (2 or, where they are fp32, 4
 bytes a logit) and two percent more, the kept rows of ``x`` once more, 8 K bytes a row, and weights that had to be packed
 (fp32, or rows that 16 bytes do not divide) up to 4 GiB of them; in the backward 512 MiB for a chunk's logit
-gradient and fp32 sums of ``x``'s gradient.  Under ``torch.no_grad()`` none of these exponentials.
+gradient, fp32 sums of ``x``'s gradient, and for fp32, and fp16 with ``reduction="none"``, the kept rows of ``x``
+again.  Under ``torch.no_grad()`` none of these exponentials.
 """
 import ctypes
 import math
@@ -350,7 +356,9 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     x [..., D], weight [V, D], bias [V] (x's type or fp32), target [...] int32 or int64.  Rows whose target is
     ``ignore_index`` have loss 0, no gradient, and take no work; a mean over none of them is 0.  A target
     outside the vocabulary gives its row (and a mean or sum) a NaN loss and NaN gradients: nothing is read
-    out of bounds, and no host check waits for the GPU.  With ``reduction="none"`` under ``torch.no_grad()``
+    out of bounds, and no host check waits for the GPU.  With ``reduction="none"`` each row's gradient by x has
+    the precision of its own incoming derivative, however small beside the others, and one that is not finite
+    spoils its own row (and the gradients that sum over rows).  With ``reduction="none"`` under ``torch.no_grad()``
     it scores tokens: the loss [...] is each target's negative log-probability.  ``hold_bytes`` bounds what a
     call holds of its logits' exponentials for its backward pass; 0 recomputes all of them there."""
     what = "linear_cross_entropy"
@@ -375,8 +383,9 @@ def linear_topk_distill(x: torch.Tensor, weight: torch.Tensor, teacher_logits: t
                         hold_bytes: int = HOLD_BYTES) -> torch.Tensor:
     """``topk_distill(F.linear(x, weight, bias), teacher_logits, teacher_index, ...)`` without the logits.
 
-    x [..., D], weight [V, D], bias [V]; the lists [..., K] as in ``topk_distill``; ``hold_bytes`` as in
-    ``linear_cross_entropy``."""
+    x [..., D], weight [V, D], bias [V]; the lists [..., K] as in ``topk_distill``, of up to a few hundred words (a
+    step of 2,048 rows of 2,048 against 32,000 words: 0.8 ms for K = 64, 1.2 for 256, 3.2 for 1,024, 23 for
+    4,096); ``hold_bytes`` and rows with ``reduction="none"`` as in ``linear_cross_entropy``."""
     what = "linear_topk_distill"
     _check_common(what, reduction, x, weight, teacher_logits, teacher_index, bias)
     _check_head(what, x, weight, bias)
@@ -395,7 +404,9 @@ def topk_distill(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ind
     indices), no gradient for them.  Entries with a negative index or a logit of -inf are absent, so lists
     may be of any length up to K; a row without an entry has loss 0 and no gradient and does not count in a
     mean; a mean over none is 0.  A word that is listed twice has the sum of its shares.  An index past the
-    vocabulary gives its row a NaN loss and NaN gradients."""
+    vocabulary gives its row a NaN loss and NaN gradients.  Meant for lists of up to a few hundred words: the
+    gradient's work on a list grows with K^2 (2,048 rows of 32,000 bf16 logits: 0.1 ms for K up to 256, 0.4 ms for
+    1,024, 5 ms for 4,096)."""
     what = "topk_distill"
     _check_common(what, reduction, logits, teacher_logits, teacher_index)
     if logits.dim() < 1 or logits.shape[-1] == 0:
