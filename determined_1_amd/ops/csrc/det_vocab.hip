@@ -15,10 +15,10 @@
 // adds the K listed logits, dot products of their own.  Backward: the vocabulary is walked in chunks; per
 // chunk G is written to a workspace, and two more products read it.  G comes from the tile's exponentials,
 // which the forward held (hold_bits; with smoothing and for fp32 in fp32) as far as the caller's bound goes (2 GiB
-// unless it says otherwise), and past that from the product once more, in its epilogue.  What bounds it, 8192 x 4096 x 128000 bf16 in 22.1 ms: the
-// matrix units, 1.23 PFLOP/s over the three products (logits 6.8 ms, G w 6.8, G^T h 7.2; G from 2 GB of
-// exponentials 0.8, where the product again takes 6.7); for few rows the reads of w (one row against
-// 128000 x 4096: 6.0 TB/s).
+// unless it says otherwise), and past that from the product once more, in its epilogue.  What bounds it, 8192 x 4096
+// x 128000 bf16 in 22.3 ms: the matrix units, 1.24 PFLOP/s over the three products (logits 6.8 ms, G w 6.8, G^T h
+// 7.2; G from 2 GB of exponentials 0.8, where the product again takes 6.7); for few rows the reads of w (one row
+// against 128000 x 4096: 6.0 TB/s).
 //
 // Rows without a target are dropped before the products (an ordered list of the kept ones, made on the
 // device; tiles past its end return), so a masked-language-model step with 15 % targets costs 15 %.
@@ -227,8 +227,9 @@ __global__ void __launch_bounds__(1024) rows_kernel(RowArgs a) {
 
 // The largest finite magnitudes of the hidden states and the weights (fp32), as bits: blocks below
 // x_blocks go over x, its kept rows alone (what an ignored one holds must not decide their scale), and leave each
-// row's as well; of the weights, words that a bias of -inf takes out do not count either.  One atomic a block (eight thousand, one a wave, took 65 us of a 75 us launch); a maximum does not
-// depend on their order.  Bound by the read of w (333 x 768 against 30522 words: 94 MB in 30 us, 3.1 TB/s).
+// row's as well; of the weights, words that a bias of -inf takes out do not count either.  One atomic a block (eight
+// thousand, one a wave, took 65 us of a 75 us launch); a maximum does not depend on their order.  Bound by the
+// read of w (333 x 768 against 30522 words: 94 MB in 30 us, 3.1 TB/s).
 struct Matrix {
   const float* p;
   int64_t ld;
@@ -241,7 +242,6 @@ struct Matrix {
 
 // a word that its bias takes out: z is -inf whatever its row of the weights holds
 __device__ __forceinline__ bool masked(const void* bias, int64_t word, int dt) { return bias != nullptr && load_any(bias, word, dt) == kNegInf; }
-
 
 // four values from any address (16-byte loads need no alignment here), zeros past the row's end
 __device__ __forceinline__ f32x4 load4(const float* p, int there) {
@@ -1974,8 +1974,8 @@ struct Plan {
   int planes, ldh, chunk, nchunks, parts, held, exact, twice;
   bool pack_w, keep_w, split_w, split_z, spread, again;
   int64_t off_rows_info, off_hidden, off_e, off_tops, off_kw, kept;  // in `kept`
-  int64_t off_w, off_z, off_flag, off_part, off_partz, off_rows;                                                     // forward
-  int64_t off_roww, off_alpha, off_rowe, off_most, off_again, off_g, off_dx, off_dw, off_cs, off_listed, total;      // backward
+  int64_t off_w, off_z, off_flag, off_part, off_partz, off_rows;  // forward
+  int64_t off_roww, off_alpha, off_rowe, off_most, off_again, off_g, off_dx, off_dw, off_cs, off_listed, total;  // backward
 };
 
 constexpr int64_t kChunkBytes = int64_t(512) << 20;  // G of one chunk, and the packed weights of one
